@@ -391,6 +391,55 @@ int gnn_trimul_relayout(const gnn_trimul_relayout_args* args, void* stream) {
   return hip_status((hipError_t)rc, "trimul_relayout");
 }
 
+static bool known_dtype(int32_t t) { return t == GNN_BF16 || t == GNN_F16 || t == GNN_F32; }
+
+// Shapes, types and row addresses shared by the LayerNorm's two directions
+static int check_layer_norm(int64_t rows, int64_t K, int32_t dtype, int32_t param_dtype, const void* params) {
+  if (rows < 1 || K < 1) return set_error(GNN_ERR_ARG, "layer_norm: rows and K must be positive");
+  if (!known_dtype(dtype)) return set_error(GNN_ERR_ARG, "layer_norm: unknown dtype");
+  if (params && param_dtype != dtype && param_dtype != GNN_F32)
+    return set_error(GNN_ERR_ARG, "layer_norm: parameters must be in the rows' dtype or fp32");
+  return GNN_OK;
+}
+static int check_layer_norm_rows(const void* p, int64_t rows, int64_t inner, int64_t outer, int64_t stride, int32_t dtype) {
+  if (inner < 1 || inner > rows || outer < 0 || stride < 0)
+    return set_error(GNN_ERR_ARG, "layer_norm: inner rows must be in 1 .. rows and strides not negative");
+  if (!aligned(p, dtype == GNN_F32 ? 4 : 2))
+    return set_error(GNN_ERR_ARG, "layer_norm: tensors must be aligned to their elements");
+  return GNN_OK;
+}
+
+int gnn_layer_norm_fwd(const gnn_layer_norm_fwd_args* args, void* stream) {
+  if (!args) return set_error(GNN_ERR_ARG, "layer_norm: args is NULL");
+  const gnn_layer_norm_fwd_args& a = *args;
+  if (!a.x || !a.y) return set_error(GNN_ERR_ARG, "layer_norm: x and y are required");
+  if (!a.mean != !a.rstd) return set_error(GNN_ERR_ARG, "layer_norm: mean and rstd are written together");
+  if (int rc = check_layer_norm(a.rows, a.K, a.dtype, a.param_dtype, a.weight ? a.weight : a.bias)) return rc;
+  if (int rc = check_layer_norm_rows(a.x, a.rows, a.x_inner, a.x_outer_stride, a.x_stride, a.dtype)) return rc;
+  int rc = layer_norm_fwd(a, (hipStream_t)stream);
+  if (rc < 0) return rc;
+  return hip_status((hipError_t)rc, "layer_norm");
+}
+
+int64_t gnn_layer_norm_bwd_parts(int64_t rows, int64_t K, int32_t dtype) {
+  return rows < 1 || K < 1 ? 0 : layer_norm_bwd_parts(rows, K, dtype);
+}
+
+int gnn_layer_norm_bwd(const gnn_layer_norm_bwd_args* args, void* stream) {
+  if (!args) return set_error(GNN_ERR_ARG, "layer_norm backward: args is NULL");
+  const gnn_layer_norm_bwd_args& a = *args;
+  if (!a.x || !a.dy || !a.mean || !a.rstd || (!a.dx && !a.partial))
+    return set_error(GNN_ERR_ARG, "layer_norm backward: x, dy, mean, rstd and one of dx and partial are required");
+  if (a.parts < 1 || a.parts >= ((int64_t)1 << 31))
+    return set_error(GNN_ERR_ARG, "layer_norm backward: parts must be positive and fit a grid");
+  if (int rc = check_layer_norm(a.rows, a.K, a.dtype, a.param_dtype, a.weight)) return rc;
+  if (int rc = check_layer_norm_rows(a.x, a.rows, a.x_inner, a.x_outer_stride, a.x_stride, a.dtype)) return rc;
+  if (int rc = check_layer_norm_rows(a.dy, a.rows, a.dy_inner, a.dy_outer_stride, a.dy_stride, a.dtype)) return rc;
+  int rc = layer_norm_bwd(a, (hipStream_t)stream);
+  if (rc < 0) return rc;
+  return hip_status((hipError_t)rc, "layer_norm backward");
+}
+
 const char* gnn_last_error(void) { return g_last_error.c_str(); }
 
 const char* gnn_version(void) { return "0.1.0 gfx950"; }

@@ -392,6 +392,59 @@ class ReduceArgs(ctypes.Structure):
     _fields_ = [("seg", ReduceSegment * REDUCE_MAX), ("count", ctypes.c_int64)]
 
 
+class LayerNormFwdArgs(ctypes.Structure):
+    """Mirror of ``gnn_layer_norm_fwd_args``."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("y", ctypes.c_void_p),
+        ("mean", ctypes.c_void_p),
+        ("rstd", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("K", ctypes.c_int64),
+        ("x_inner", ctypes.c_int64),
+        ("x_outer_stride", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64),
+        ("eps", ctypes.c_float),
+        ("dtype", ctypes.c_int32),
+        ("param_dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+pack_layer_norm_fwd = packer(LayerNormFwdArgs)
+
+
+class LayerNormBwdArgs(ctypes.Structure):
+    """Mirror of ``gnn_layer_norm_bwd_args``."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("dy", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("mean", ctypes.c_void_p),
+        ("rstd", ctypes.c_void_p),
+        ("dx", ctypes.c_void_p),
+        ("partial", ctypes.c_void_p),
+        ("parts", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+        ("K", ctypes.c_int64),
+        ("x_inner", ctypes.c_int64),
+        ("x_outer_stride", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64),
+        ("dy_inner", ctypes.c_int64),
+        ("dy_outer_stride", ctypes.c_int64),
+        ("dy_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("param_dtype", ctypes.c_int32),
+    ]
+
+
+pack_layer_norm_bwd = packer(LayerNormBwdArgs)
+
+
 RELAYOUT_PLANES_TO_PIXELS, RELAYOUT_PIXELS_TO_BLOCKED, RELAYOUT_PIXELS_TO_PLANES = 0, 1, 2
 
 _SIGNATURES = {
@@ -424,6 +477,9 @@ _SIGNATURES = {
     "gnn_rows_product_slices": (ctypes.c_int64, [ctypes.POINTER(RowsProductArgs)]),
     "gnn_rows_product": (ctypes.c_int, [ctypes.POINTER(RowsProductArgs), ctypes.c_void_p]),
     "gnn_reduce_parts": (ctypes.c_int, [ctypes.POINTER(ReduceArgs), ctypes.c_void_p]),
+    "gnn_layer_norm_fwd": (ctypes.c_int, [ctypes.POINTER(LayerNormFwdArgs), ctypes.c_void_p]),
+    "gnn_layer_norm_bwd_parts": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32]),
+    "gnn_layer_norm_bwd": (ctypes.c_int, [ctypes.POINTER(LayerNormBwdArgs), ctypes.c_void_p]),
     "gnn_last_error": (ctypes.c_char_p, []),
     "gnn_version": (ctypes.c_char_p, []),
 }

@@ -19,7 +19,7 @@ from typing import Optional
 
 import torch
 
-__all__ = ["triangle_attention_fwd", "trimul_fwd", "attention_pair_bias_fwd", "eager_ok"]
+__all__ = ["triangle_attention_fwd", "trimul_fwd", "attention_pair_bias_fwd", "layer_norm_fwd", "eager_ok"]
 
 
 _PLAIN_TYPES = (torch.Tensor, torch.nn.Parameter)  # Parameter disables __torch_function__
@@ -145,3 +145,23 @@ def _attention_pair_bias_fwd_fake(s, q, k, v, z, proj_g_weight, proj_o_weight, p
     if z_is_projected:
         return out, z.new_empty((0,))
     return out, z.new_empty((z.shape[0], H, U, k.shape[2]))
+
+
+def layer_norm_fwd_impl(
+    x: torch.Tensor,
+    weight: Optional[torch.Tensor],
+    bias: Optional[torch.Tensor],
+    eps: float,
+) -> torch.Tensor:
+    """``[..., C]`` in any strides; returns a fresh contiguous tensor of x's shape and dtype."""
+    from .triangle._kernels.layer_norm import layer_norm_hip
+
+    return layer_norm_hip(x, weight, bias, eps)
+
+
+layer_norm_fwd = torch.library.custom_op("gnn_amd::layer_norm_fwd", layer_norm_fwd_impl, mutates_args=())
+
+
+@layer_norm_fwd.register_fake
+def _layer_norm_fwd_fake(x, weight, bias, eps):
+    return x.new_empty(x.shape)

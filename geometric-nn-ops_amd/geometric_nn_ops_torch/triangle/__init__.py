@@ -1,11 +1,13 @@
 """Triangle (protein-folding) ops (reference geometric_nn_ops_torch/triangle/__init__.py:6-14)."""
 
 from ._attention_pair_bias import attention_pair_bias
+from ._layer_norm import layer_norm
 from ._triattn import triangle_attention
 from ._trimul import triangle_multiplicative_update
 
 __all__ = [
     "attention_pair_bias",
+    "layer_norm",
     "triangle_attention",
     "triangle_multiplicative_update",
 ]

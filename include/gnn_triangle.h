@@ -572,6 +572,50 @@ typedef struct gnn_reduce_args {
 } gnn_reduce_args;
 int gnn_reduce_parts(const gnn_reduce_args* args, void* stream);
 
+/* LayerNorm over rows of K <= 16384 elements (any width and alignment of the rows):
+ *   y = (x - mean) rstd weight + bias,  rstd = 1 / sqrt(var + eps), statistics in fp32.
+ * Row r of x starts at (r / x_inner) x_outer_stride + (r % x_inner) x_stride elements (x_inner =
+ * rows: one stride); y is dense. weight / bias: [K] in param_dtype (the rows' dtype or GNN_F32), or
+ * NULL. mean / rstd: fp32 [rows], written where not NULL (both or neither), for the backward. The
+ * reference runs F.layer_norm (triangle/_reference/trimul.py:85, 94). */
+typedef struct gnn_layer_norm_fwd_args {
+  const void* x;
+  const void* weight;
+  const void* bias;
+  void* y;
+  float* mean;
+  float* rstd;
+  int64_t rows, K;
+  int64_t x_inner, x_outer_stride, x_stride;
+  float eps;
+  int32_t dtype;       /* enum gnn_dtype of x and y */
+  int32_t param_dtype; /* enum gnn_dtype of weight and bias */
+  int32_t reserved;
+} gnn_layer_norm_fwd_args;
+int gnn_layer_norm_fwd(const gnn_layer_norm_fwd_args* args, void* stream);
+
+/* Its backward: dx (dense, or NULL) and, where partial is not NULL, fp32 [parts][2][K]: partial sums of
+ * the weight's and the bias's gradient, to be added with gnn_reduce_parts. parts is the number of
+ * workgroups, gnn_layer_norm_bwd_parts(rows, K, dtype) the best one for the current device. dy is
+ * addressed as x is. */
+typedef struct gnn_layer_norm_bwd_args {
+  const void* x;
+  const void* dy;
+  const void* weight;
+  const float* mean;
+  const float* rstd;
+  void* dx;
+  float* partial;
+  int64_t parts;
+  int64_t rows, K;
+  int64_t x_inner, x_outer_stride, x_stride;
+  int64_t dy_inner, dy_outer_stride, dy_stride;
+  int32_t dtype;
+  int32_t param_dtype;
+} gnn_layer_norm_bwd_args;
+int64_t gnn_layer_norm_bwd_parts(int64_t rows, int64_t K, int32_t dtype);
+int gnn_layer_norm_bwd(const gnn_layer_norm_bwd_args* args, void* stream);
+
 /* Message for the last failing call on this thread ("" if none). */
 const char* gnn_last_error(void);
 
