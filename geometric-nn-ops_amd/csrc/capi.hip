@@ -440,6 +440,59 @@ int gnn_layer_norm_bwd(const gnn_layer_norm_bwd_args* args, void* stream) {
   return hip_status((hipError_t)rc, "layer_norm backward");
 }
 
+static int check_relpos(const gnn_relpos_args* args) {
+  if (!args) return set_error(GNN_ERR_ARG, "relative_position_bias: args is NULL");
+  const gnn_relpos_args& a = *args;
+  if (!known_dtype(a.dtype)) return set_error(GNN_ERR_ARG, "relative_position_bias: unknown dtype");
+  if (a.pos_bytes != 4 && a.pos_bytes != 8)
+    return set_error(GNN_ERR_ARG, "relative_position_bias: positions must have 4 or 8 bytes");
+  const int64_t most = INT32_MAX;
+  if (a.B < 1 || a.U < 1 || a.V < 1 || a.H < 1 || a.buckets < 1 || a.B > most || a.U > most || a.V > most - 4096 ||
+      a.H > most || a.V * a.H > most - 4096 || a.buckets > most / a.H)
+    return set_error(GNN_ERR_ARG, "relative_position_bias: B, U, V, H and buckets must be positive, V H below 2^31");
+  if (a.max_distance < 1 || a.max_distance > (1 << 30))
+    return set_error(GNN_ERR_ARG, "relative_position_bias: max_distance must be in 1 .. 2^30");
+  if (!a.log_spacing) {
+    if (a.buckets != (a.two_sided ? 2 : 1) * a.max_distance + 1)
+      return set_error(GNN_ERR_ARG, "relative_position_bias: clip needs 2 max_distance + 1 buckets, one-sided max_distance + 1");
+    return GNN_OK;
+  }
+  const int64_t n = a.buckets / (a.two_sided ? 2 : 1), near = n / 2, m = n - near;
+  if (n < 2 || (a.two_sided && a.buckets % 2) || a.max_distance <= near)
+    return set_error(GNN_ERR_ARG, "relative_position_bias: log needs 2 buckets a side or more and a max_distance above half of them");
+  if (m > GNN_RELPOS_MAX_BORDERS)
+    return set_error(GNN_ERR_UNSUPPORTED, "relative_position_bias: more than 256 logarithmic buckets a side");
+  if (m > 1 && !a.border) return set_error(GNN_ERR_ARG, "relative_position_bias: log needs its borders");
+  for (int64_t k = 0; k + 1 < m; ++k)
+    if (a.border[k] < (k ? a.border[k - 1] : near) || a.border[k] > a.max_distance)
+      return set_error(GNN_ERR_ARG, "relative_position_bias: borders must ascend and not pass max_distance");
+  return GNN_OK;
+}
+
+int gnn_relpos_fwd(const gnn_relpos_args* args, void* stream) {
+  if (int rc = check_relpos(args)) return rc;
+  if (!args->table || !args->query_pos || !args->key_pos || !args->out)
+    return set_error(GNN_ERR_ARG, "relative_position_bias: table, positions and out are required");
+  if (!aligned(args->out, args->dtype == GNN_F32 ? 4 : 2))
+    return set_error(GNN_ERR_ARG, "relative_position_bias: out must be aligned to its elements");
+  int rc = relpos(*args, false, (hipStream_t)stream);
+  if (rc < 0) return rc;
+  return hip_status((hipError_t)rc, "relative_position_bias");
+}
+
+int64_t gnn_relpos_parts(const gnn_relpos_args* args) { return check_relpos(args) ? 0 : relpos_parts(*args); }
+
+int gnn_relpos_bwd(const gnn_relpos_args* args, void* stream) {
+  if (int rc = check_relpos(args)) return rc;
+  if (!args->query_pos || !args->key_pos || !args->dout || !args->partial || args->parts < 1)
+    return set_error(GNN_ERR_ARG, "relative_position_bias backward: positions, dout, partial and parts are required");
+  if (!aligned(args->dout, args->dtype == GNN_F32 ? 4 : 2))
+    return set_error(GNN_ERR_ARG, "relative_position_bias backward: dout must be aligned to its elements");
+  int rc = relpos(*args, true, (hipStream_t)stream);
+  if (rc < 0) return rc;
+  return hip_status((hipError_t)rc, "relative_position_bias backward");
+}
+
 const char* gnn_last_error(void) { return g_last_error.c_str(); }
 
 const char* gnn_version(void) { return "0.1.0 gfx950"; }

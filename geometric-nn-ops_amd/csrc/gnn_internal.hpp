@@ -64,6 +64,8 @@ int64_t rows_product_slices(const gnn_rows_product_args& a);
 int rows_product(const gnn_rows_product_args& a, hipStream_t stream);
 int reduce_parts(const gnn_reduce_args& a, hipStream_t stream);
 
+int relpos(const gnn_relpos_args& a, bool backward, hipStream_t stream);
+int64_t relpos_parts(const gnn_relpos_args& a);
 int layer_norm_fwd(const gnn_layer_norm_fwd_args& a, hipStream_t stream);
 int64_t layer_norm_bwd_parts(int64_t rows, int64_t K, int32_t dtype);
 int layer_norm_bwd(const gnn_layer_norm_bwd_args& a, hipStream_t stream);

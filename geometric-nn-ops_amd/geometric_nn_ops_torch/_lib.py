@@ -392,6 +392,39 @@ class ReduceArgs(ctypes.Structure):
     _fields_ = [("seg", ReduceSegment * REDUCE_MAX), ("count", ctypes.c_int64)]
 
 
+class RelposArgs(ctypes.Structure):
+    """Mirror of ``gnn_relpos_args``."""
+
+    _fields_ = [
+        ("table", ctypes.c_void_p),
+        ("query_pos", ctypes.c_void_p),
+        ("key_pos", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("dout", ctypes.c_void_p),
+        ("partial", ctypes.c_void_p),
+        ("border", ctypes.c_void_p),
+        ("parts", ctypes.c_int64),
+        ("query_stride", ctypes.c_int64),
+        ("key_stride", ctypes.c_int64),
+        ("stride", I64x3),
+        ("B", ctypes.c_int64),
+        ("U", ctypes.c_int64),
+        ("V", ctypes.c_int64),
+        ("H", ctypes.c_int64),
+        ("buckets", ctypes.c_int64),
+        ("max_distance", ctypes.c_int64),
+        ("log_spacing", ctypes.c_int32),
+        ("two_sided", ctypes.c_int32),
+        ("channels_last", ctypes.c_int32),
+        ("pos_bytes", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+pack_relpos = packer(RelposArgs)
+
+
 class LayerNormFwdArgs(ctypes.Structure):
     """Mirror of ``gnn_layer_norm_fwd_args``."""
 
@@ -480,6 +513,9 @@ _SIGNATURES = {
     "gnn_layer_norm_fwd": (ctypes.c_int, [ctypes.POINTER(LayerNormFwdArgs), ctypes.c_void_p]),
     "gnn_layer_norm_bwd_parts": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32]),
     "gnn_layer_norm_bwd": (ctypes.c_int, [ctypes.POINTER(LayerNormBwdArgs), ctypes.c_void_p]),
+    "gnn_relpos_fwd": (ctypes.c_int, [ctypes.POINTER(RelposArgs), ctypes.c_void_p]),
+    "gnn_relpos_parts": (ctypes.c_int64, [ctypes.POINTER(RelposArgs)]),
+    "gnn_relpos_bwd": (ctypes.c_int, [ctypes.POINTER(RelposArgs), ctypes.c_void_p]),
     "gnn_last_error": (ctypes.c_char_p, []),
     "gnn_version": (ctypes.c_char_p, []),
 }

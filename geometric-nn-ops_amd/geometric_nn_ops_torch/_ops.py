@@ -19,7 +19,8 @@ from typing import Optional
 
 import torch
 
-__all__ = ["triangle_attention_fwd", "trimul_fwd", "attention_pair_bias_fwd", "layer_norm_fwd", "eager_ok"]
+__all__ = ["triangle_attention_fwd", "trimul_fwd", "attention_pair_bias_fwd", "layer_norm_fwd",
+           "relative_position_bias_fwd", "eager_ok"]
 
 
 _PLAIN_TYPES = (torch.Tensor, torch.nn.Parameter)  # Parameter disables __torch_function__
@@ -165,3 +166,32 @@ layer_norm_fwd = torch.library.custom_op("gnn_amd::layer_norm_fwd", layer_norm_f
 @layer_norm_fwd.register_fake
 def _layer_norm_fwd_fake(x, weight, bias, eps):
     return x.new_empty(x.shape)
+
+
+def relative_position_bias_fwd_impl(
+    weight: torch.Tensor,
+    query_pos: torch.Tensor,
+    key_pos: torch.Tensor,
+    max_distance: int,
+    spacing: str,
+    bidirectional: bool,
+    channels_last: bool,
+) -> torch.Tensor:
+    """``weight [buckets, H]``, positions ``[B, U]`` / ``[B, V]``; returns ``[B, H, U, V]`` with a row pitch
+    rounded up to 8, or the contiguous ``[B, U, V, H]``."""
+    from .triangle._kernels.relative_position import relative_position_bias_hip
+
+    return relative_position_bias_hip(weight, query_pos, key_pos, max_distance, spacing, bidirectional, channels_last)
+
+
+relative_position_bias_fwd = torch.library.custom_op("gnn_amd::relative_position_bias_fwd",
+                                                     relative_position_bias_fwd_impl, mutates_args=())
+
+
+@relative_position_bias_fwd.register_fake
+def _relative_position_bias_fwd_fake(weight, query_pos, key_pos, max_distance, spacing, bidirectional, channels_last):
+    B, U = query_pos.shape
+    V, H = key_pos.shape[1], weight.shape[1]
+    if channels_last:
+        return weight.new_empty((B, U, V, H))
+    return weight.new_empty((B, H, U, (V + 7) // 8 * 8))[..., :V]

@@ -2,12 +2,14 @@
 
 from ._attention_pair_bias import attention_pair_bias
 from ._layer_norm import layer_norm
+from ._relative_position import relative_position_bias
 from ._triattn import triangle_attention
 from ._trimul import triangle_multiplicative_update
 
 __all__ = [
     "attention_pair_bias",
     "layer_norm",
+    "relative_position_bias",
     "triangle_attention",
     "triangle_multiplicative_update",
 ]

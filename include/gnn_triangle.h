@@ -616,6 +616,42 @@ typedef struct gnn_layer_norm_bwd_args {
 int64_t gnn_layer_norm_bwd_parts(int64_t rows, int64_t K, int32_t dtype);
 int gnn_layer_norm_bwd(const gnn_layer_norm_bwd_args* args, void* stream);
 
+/* Learned bias by buckets of the distance between keys and queries, forward:
+ *   out[b, h, i, j] (channels_last: out[b, i, j, h]) = table[bucket(key_pos[b, j] - query_pos[b, i])][h]
+ * and backward: dtable[t][h] = sum over the (b, i, j) of bucket t of dout[b, h, i, j], as fp32 partial sums
+ * [parts][buckets][H] to be added with gnn_reduce_parts; parts as gnn_relpos_parts returns it (any from 1
+ * on is right). With D = max_distance and a = key_pos - query_pos:
+ *   clip, two-sided: clamp(a, -D, D) + D (2 D + 1 buckets); one-sided: clamp(-a, 0, D) (D + 1 buckets);
+ *   log: n buckets a side (buckets / 2 where two-sided, those of keys ahead, a > 0, in the second half),
+ *     near = n / 2 of them for distances d < near, bucket near + k from the least d on with
+ *     d >= near (D / near)^(k / (n - near)); border[k - 1] is that d, for k = 1 .. n - near - 1 (a host array
+ *     read during the call), ascending and not above D. One-sided: d = max(-a, 0).
+ * table: [buckets][H] dense; positions of pos_bytes 4 or 8, unit stride, batches query_stride / key_stride
+ * apart; out / dout: strides {b, h, i} with unit stride over the keys, channels_last {b, unused, i} with
+ * dense [V][H] rows. The reference has no such op (its callers build the bias themselves). */
+#define GNN_RELPOS_MAX_BORDERS 256
+typedef struct gnn_relpos_args {
+  const void* table;
+  const void* query_pos;
+  const void* key_pos;
+  void* out;
+  const void* dout;
+  float* partial;
+  const int32_t* border;
+  int64_t parts;
+  int64_t query_stride, key_stride;
+  int64_t stride[3];
+  int64_t B, U, V, H;
+  int64_t buckets, max_distance;
+  int32_t log_spacing, two_sided, channels_last;
+  int32_t pos_bytes;
+  int32_t dtype; /* enum gnn_dtype of table, out and dout */
+  int32_t reserved;
+} gnn_relpos_args;
+int gnn_relpos_fwd(const gnn_relpos_args* args, void* stream);
+int64_t gnn_relpos_parts(const gnn_relpos_args* args);
+int gnn_relpos_bwd(const gnn_relpos_args* args, void* stream);
+
 /* Message for the last failing call on this thread ("" if none). */
 const char* gnn_last_error(void);
 
