@@ -493,6 +493,47 @@ int gnn_relpos_bwd(const gnn_relpos_args* args, void* stream) {
   return hip_status((hipError_t)rc, "relative_position_bias backward");
 }
 
+int gnn_linear(const gnn_linear_args* args, void* stream) {
+  if (!args) return set_error(GNN_ERR_ARG, "fused_linear: args is NULL");
+  const gnn_linear_args& a = *args;
+  if (!a.x || !a.w || !a.out || (a.dz && !a.side))
+    return set_error(GNN_ERR_ARG, "fused_linear: x, w, out and, for dz, the output gradient are required");
+  if (!known_dtype(a.dtype)) return set_error(GNN_ERR_ARG, "fused_linear: unknown dtype");
+  if (a.precision != GNN_PREC_IEEE && a.precision != GNN_PREC_BF16X3)
+    return set_error(GNN_ERR_ARG, "fused_linear: unknown precision");
+  if (a.activation < GNN_ACT_NONE || a.activation > GNN_ACT_SIGMOID)
+    return set_error(GNN_ERR_ARG, "fused_linear: unknown activation");
+  const int64_t most = (int64_t)1 << 30;
+  if (a.M < 1 || a.I < 1 || a.O < 1 || a.I > most || a.O > most || a.out_cols < a.O || a.out_cols > most)
+    return set_error(GNN_ERR_ARG, "fused_linear: M, I and O must be positive, I and out_cols at most 2^30, out_cols at least O");
+  const int64_t e = a.dtype == GNN_F32 ? 4 : 2;
+  if (!aligned(a.x, 16) || !aligned(a.w, 16) || (a.I * e) % 16 || (a.x_ld * e) % 16 || (a.w_ld * e) % 16)
+    return set_error(GNN_ERR_ARG, "fused_linear: rows of x and w must be 16-byte aligned and multiples of 16 bytes");
+  if (a.x_ld < 0 || a.w_ld < a.I || (a.side && a.side_ld < 0) || a.out_ld < a.out_cols)
+    return set_error(GNN_ERR_ARG, "fused_linear: row pitches must cover their rows");
+  if (!aligned(a.bias, e) || !aligned(a.side, e) || !aligned(a.out, e))
+    return set_error(GNN_ERR_ARG, "fused_linear: tensors must be aligned to their elements");
+  int rc = linear(a, (hipStream_t)stream);
+  if (rc < 0) return rc;
+  return hip_status((hipError_t)rc, "fused_linear");
+}
+
+int64_t gnn_column_sums_parts(int64_t M, int64_t O) { return M < 1 || O < 1 ? 0 : column_sums_parts(M, O); }
+
+int gnn_column_sums(const gnn_column_sums_args* args, void* stream) {
+  if (!args) return set_error(GNN_ERR_ARG, "column_sums: args is NULL");
+  const gnn_column_sums_args& a = *args;
+  if (!a.d || !a.partial) return set_error(GNN_ERR_ARG, "column_sums: d and partial are required");
+  if (!known_dtype(a.dtype)) return set_error(GNN_ERR_ARG, "column_sums: unknown dtype");
+  if (a.M < 1 || a.O < 1 || a.O > (1 << 24) || a.parts < 1 || a.parts >= ((int64_t)1 << 31) || a.ld < 0)
+    return set_error(GNN_ERR_ARG, "column_sums: M, O and parts must be positive, O at most 2^24");
+  if (!aligned(a.d, a.dtype == GNN_F32 ? 4 : 2))
+    return set_error(GNN_ERR_ARG, "column_sums: d must be aligned to its elements");
+  int rc = column_sums(a, (hipStream_t)stream);
+  if (rc < 0) return rc;
+  return hip_status((hipError_t)rc, "column_sums");
+}
+
 const char* gnn_last_error(void) { return g_last_error.c_str(); }
 
 const char* gnn_version(void) { return "0.1.0 gfx950"; }

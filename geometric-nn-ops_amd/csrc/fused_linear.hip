@@ -1,0 +1,366 @@
+// A linear layer with its epilogue in one pass, y = act(x W^T + b) + r for rows x [M, I] and W [O, I], and
+// the products of its backward:
+//   z = x W^T + b, dz = dy act'(z), dx = dz W, dW = dz^T x, db = sum over the rows of dz, dr = dy.
+//
+// The backward forms z again from x and W instead of keeping it: in 16 bits, z would put a second rounding
+// under every gradient, and in fp32 it would cost 4 M O bytes written and read.
+//
+// linear_kernel. BM x BN output tiles, the contraction in stages of 128 bytes a row, both operands moved by
+// global_load_lds into LDS (STAGES of them in flight) with the 16-byte chunks of row r XOR-swizzled by r % 8,
+// so that the fragment reads of 8 rows hit 8 bank groups. The products are formed transposed (W's rows as the
+// rows of the 32x32 MFMA tile): a lane then holds one row of x and, once v_permlane32_swap has exchanged the
+// halves of neighbouring register groups, 8 consecutive outputs of it, which take bias, activation and
+// residual in fp32, round once and leave as one 16-byte store (two in fp32). Workgroups that share rows of x
+// follow each other on one XCD, whose L2 then serves x.
+#include <algorithm>
+
+#include "gnn_common.hpp"
+#include "gnn_internal.hpp"
+
+namespace gnn {
+
+namespace {
+
+typedef __attribute__((address_space(3))) void lds_void_t;
+
+__device__ __attribute__((aligned(16))) const uint32_t zero_chunk[4] = {0u, 0u, 0u, 0u};
+
+// s_waitcnt vmcnt(VM) expcnt(7) lgkmcnt(0)
+template <int VM>
+__device__ __forceinline__ void wait_vm_lgkm0() {
+  static_assert(VM >= 0 && VM < 64, "vmcnt immediate");
+  __builtin_amdgcn_s_waitcnt(0x070 | (VM & 15) | ((VM >> 4) << 14));
+}
+
+// ---- activations ------------------------------------------------------------------------
+// 16-bit results: exp2 and rcp of the hardware (1 ulp each) and, for the normal distribution, Abramowitz and
+// Stegun 7.1.26: erfc(u) = t (a1 + t (a2 + ...)) exp(-u^2), t = 1 / (1 + 0.3275911 u), off by at most 1.5e-7;
+// both are far below half a step of fp16 (2.4e-4). fp32: the library's functions and full divisions.
+template <bool F32>
+__device__ __forceinline__ float sigmoid(float z) {
+  if constexpr (F32) return 1.0f / (1.0f + expf(-z));
+  return __builtin_amdgcn_rcpf(1.0f + fast_exp2(-1.4426950408889634f * z));
+}
+
+// Phi(z), and z phi(z) where the slope needs it
+template <bool F32>
+__device__ __forceinline__ float normal_cdf(float z, float& z_pdf) {
+  if constexpr (F32) {
+    z_pdf = z * 0.3989422804014327f * expf(-0.5f * z * z);
+    return 0.5f * erfcf(-0.7071067811865476f * z);
+  }
+  const float e = fast_exp2(-0.7213475204444817f * z * z);  // exp(-z^2 / 2)
+  const float u = 0.7071067811865476f * fabsf(z);
+  const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * u);
+  const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  const float tail = 0.5f * p * e;  // Phi(-|z|)
+  z_pdf = z * 0.3989422804014327f * e;
+  return z < 0.f ? tail : 1.0f - tail;
+}
+
+template <bool F32>
+__device__ __forceinline__ float activate(int act, float z) {
+  float unused;
+  switch (act) {
+    case GNN_ACT_RELU: return z < 0.f ? 0.f : z;
+    case GNN_ACT_GELU: return z * normal_cdf<F32>(z, unused);
+    case GNN_ACT_SILU: return z * sigmoid<F32>(z);
+    case GNN_ACT_SIGMOID: return sigmoid<F32>(z);
+    default: return z;
+  }
+}
+template <bool F32>
+__device__ __forceinline__ float slope(int act, float z) {
+  switch (act) {
+    case GNN_ACT_RELU: return z <= 0.f ? 0.f : 1.f;
+    case GNN_ACT_GELU: {
+      float z_pdf;
+      const float cdf = normal_cdf<F32>(z, z_pdf);
+      return cdf + z_pdf;
+    }
+    case GNN_ACT_SILU: {
+      const float s = sigmoid<F32>(z);
+      return s * (1.0f + z * (1.0f - s));
+    }
+    case GNN_ACT_SIGMOID: {
+      const float s = sigmoid<F32>(z);
+      return s * (1.0f - s);
+    }
+    default: return 1.f;
+  }
+}
+
+// ---- tiles --------------------------------------------------------------------------------
+struct LinArgs {
+  const void* x;
+  const void* w;
+  const void* bias;
+  const void* side;  // residual, or dy
+  void* out;
+  int64_t M;
+  int64_t x_ld, w_ld, side_ld, out_ld;
+  int I, O;      // contraction (a multiple of 8; 4 in fp32), outputs
+  int out_cols;  // columns written, zeros from O on
+  int act;
+  bool dz;  // out = side * act'(z) instead of act(z) + side
+};
+
+// 8 consecutive elements at any element's address, the first `left` of them
+template <typename T>
+__device__ __forceinline__ f32x8 load8_any(const T* p, int left) {
+  typedef typename TypeOps<T>::V8 V8;
+  typedef V8 VU __attribute__((aligned(sizeof(T))));
+  if (left >= 8) {
+    const V8 v = *(const __attribute__((address_space(1))) VU*)p;
+    return TypeOps<T>::to_f32(v);
+  }
+  f32x8 v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = e < left ? (float)p[e] : 0.f;
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store8_any(T* p, const f32x8& v, int left) {
+  typedef typename TypeOps<T>::V8 V8;
+  typedef V8 VU __attribute__((aligned(sizeof(T))));
+  const V8 o = TypeOps<T>::from_f32(v);
+  if (left >= 8) {
+    *(__attribute__((address_space(1))) VU*)p = o;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < left) p[e] = o[e];
+}
+
+// The 8 consecutive rows (of the transposed product: outputs) 16 t + 8 g + (0 .. 7) of a lane's column
+__device__ __forceinline__ f32x8 swapped8(const f32x16& acc, int t) {
+  f32x8 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[8 * t + i]), __float_as_uint(acc[8 * t + 4 + i]),
+                                                    false, false);
+    v[i] = __uint_as_float(s[0]);
+    v[4 + i] = __uint_as_float(s[1]);
+  }
+  return v;
+}
+
+// Bias, activation and residual (or the slope of dy) on 8 outputs n .. n + 7 of row m, and their store
+template <typename T>
+__device__ __forceinline__ void finish8(const LinArgs& a, const f32x8& z0, const f32x8& b, int64_t m, int n) {
+  constexpr bool F32 = sizeof(T) == 4;
+  const int left = a.O - n;
+  f32x8 z = z0 + b;
+  if (a.dz) {
+    const f32x8 dy = load8_any((const T*)a.side + m * a.side_ld + n, left);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] = dy[e] * slope<F32>(a.act, z[e]);
+  } else {
+    if (a.act)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[e] = activate<F32>(a.act, z[e]);
+    if (a.side) z += load8_any((const T*)a.side + m * a.side_ld + n, left);
+  }
+  if (left < 8)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] = e < left ? z[e] : 0.f;
+  store8_any((T*)a.out + m * a.out_ld + n, z, a.out_cols - n);
+}
+
+// GM x GN waves of 32 X rows x 32 Y outputs
+template <typename T, int GM_, int GN_, int X_, int Y_, int STAGES_>
+struct Tile {
+  static constexpr int GM = GM_, GN = GN_, X = X_, Y = Y_, STAGES = STAGES_;
+  static constexpr int BM = 32 * GM * X, BN = 32 * GN * Y;
+  static constexpr int NW = GM * GN, NT = 64 * NW;
+  static constexpr int BK = 128 / (int)sizeof(T);  // elements of a row a stage
+  static constexpr int EPC = 16 / (int)sizeof(T);  // elements a chunk
+  static constexpr int QA = BM / 8 / NW, QB = BN / 8 / NW;  // DMA instructions a wave and stage
+  static constexpr int STAGE = (BM + BN) * 128;
+  static constexpr int LDS = STAGES * STAGE;
+  static_assert(QA * 8 * NW == BM && QB * 8 * NW == BN, "DMA split");
+  static_assert(STAGES == 2, "waits below");
+};
+
+template <typename T, int PREC, typename Cfg>
+__global__ __launch_bounds__(Cfg::NT, Cfg::LDS <= (80 << 10) ? 2 * Cfg::NW / 4 : Cfg::NW / 4) void linear_kernel(
+    const LinArgs a) {
+  typedef typename TypeOps<T>::V8 V8;
+  __shared__ __align__(16) unsigned char smem[Cfg::LDS];
+  const int ntn = (a.out_cols + Cfg::BN - 1) / Cfg::BN;
+  const uint32_t w = xcd_remap(blockIdx.x, gridDim.x);
+  const int n0 = (int)(w % (uint32_t)ntn) * Cfg::BN;
+  const int64_t m0 = (int64_t)(w / (uint32_t)ntn) * Cfg::BM;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l32 = lane & 31, g = lane >> 5;
+  const int wm = wave / Cfg::GN, wn = wave % Cfg::GN;
+
+  // DMA: an instruction moves 8 rows of 128 bytes; lane -> row lane / 8, stored chunk lane % 8, which holds
+  // the row's chunk (lane % 8) ^ (row % 8). Rows past the end repeat the last one (never stored), chunks
+  // past the contraction's end are zeros in both operands.
+  const int drow = lane >> 3, dchunk = (lane & 7) ^ drow;
+  const T* xsrc[Cfg::QA];
+  const T* wsrc[Cfg::QB];
+#pragma unroll
+  for (int q = 0; q < Cfg::QA; ++q)
+    xsrc[q] = (const T*)a.x + min(m0 + 8 * (Cfg::QA * wave + q) + drow, a.M - 1) * a.x_ld + dchunk * Cfg::EPC;
+#pragma unroll
+  for (int q = 0; q < Cfg::QB; ++q)
+    wsrc[q] = (const T*)a.w + (int64_t)min(n0 + 8 * (Cfg::QB * wave + q) + drow, a.O - 1) * a.w_ld + dchunk * Cfg::EPC;
+  const int nkt = (a.I + Cfg::BK - 1) / Cfg::BK;
+  auto issue = [&](int kt) {
+    unsigned char* st = smem + (kt % Cfg::STAGES) * Cfg::STAGE;
+    const int k0 = kt * Cfg::BK;
+    const bool in = k0 + dchunk * Cfg::EPC < a.I;
+#pragma unroll
+    for (int q = 0; q < Cfg::QA; ++q)
+      __builtin_amdgcn_global_load_lds(in ? (const void*)(xsrc[q] + k0) : (const void*)zero_chunk,
+                                       (lds_void_t*)(st + (Cfg::QA * wave + q) * 1024), 16, 0, 0);
+#pragma unroll
+    for (int q = 0; q < Cfg::QB; ++q)
+      __builtin_amdgcn_global_load_lds(in ? (const void*)(wsrc[q] + k0) : (const void*)zero_chunk,
+                                       (lds_void_t*)(st + Cfg::BM * 128 + (Cfg::QB * wave + q) * 1024), 16, 0, 0);
+  };
+  // 8 elements kk * 16 + 8 g of a row
+  auto frag = [&](const unsigned char* base, int r, int kk) -> V8 {
+    const unsigned char* row = base + r * 128;
+    if constexpr (sizeof(T) == 2) {
+      return *reinterpret_cast<const V8*>(row + (((2 * kk + g) ^ (r & 7)) << 4));
+    } else {
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(row + (((4 * kk + 2 * g) ^ (r & 7)) << 4));
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(row + (((4 * kk + 2 * g + 1) ^ (r & 7)) << 4));
+      return V8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    }
+  };
+
+  f32x16 acc[Cfg::X][Cfg::Y];
+#pragma unroll
+  for (int x = 0; x < Cfg::X; ++x)
+#pragma unroll
+    for (int y = 0; y < Cfg::Y; ++y)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
+
+#pragma unroll
+  for (int s = 0; s < Cfg::STAGES; ++s)
+    if (s < nkt) issue(s);
+  for (int kt = 0; kt < nkt; ++kt) {
+    // this wave's DMA of stage kt has landed; after the barrier every wave's has
+    if (kt + 1 < nkt)
+      wait_vm_lgkm0<Cfg::QA + Cfg::QB>();
+    else
+      wait_vm_lgkm0<0>();
+    asm volatile("s_barrier" ::: "memory");
+    const unsigned char* sx = smem + (kt % Cfg::STAGES) * Cfg::STAGE;
+    const unsigned char* sw = sx + Cfg::BM * 128;
+    constexpr int KS = Cfg::BK / 16;
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) {
+      V8 xf[Cfg::X], wf[Cfg::Y];
+#pragma unroll
+      for (int x = 0; x < Cfg::X; ++x) xf[x] = frag(sx, 32 * (Cfg::X * wm + x) + l32, kk);
+#pragma unroll
+      for (int y = 0; y < Cfg::Y; ++y) wf[y] = frag(sw, 32 * (Cfg::Y * wn + y) + l32, kk);
+#pragma unroll
+      for (int x = 0; x < Cfg::X; ++x)
+#pragma unroll
+        for (int y = 0; y < Cfg::Y; ++y) Mma<T, PREC>::step(acc[x][y], wf[y], xf[x]);
+    }
+    if (kt + Cfg::STAGES < nkt) {
+      // every wave's reads of the stage have returned: its buffer takes the stage after the next
+      wait_vm_lgkm0<Cfg::QA + Cfg::QB>();
+      asm volatile("s_barrier" ::: "memory");
+      issue(kt + Cfg::STAGES);
+    }
+  }
+
+#pragma unroll
+  for (int y = 0; y < Cfg::Y; ++y)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int n = n0 + 32 * (Cfg::Y * wn + y) + 16 * t + 8 * g;
+      f32x8 b = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (a.bias && n < a.O) b = load8_any((const T*)a.bias + n, a.O - n);
+#pragma unroll
+      for (int x = 0; x < Cfg::X; ++x) {
+        const f32x8 z = swapped8(acc[x][y], t);  // every lane takes part in the swap
+        const int64_t m = m0 + 32 * (Cfg::X * wm + x) + l32;
+        if (m < a.M && n < a.out_cols) finish8<T>(a, z, b, m, n);
+      }
+    }
+}
+
+template <typename T, int PREC, typename Cfg>
+int launch(const LinArgs& a, hipStream_t st) {
+  const int64_t tiles = (a.M + Cfg::BM - 1) / Cfg::BM * ((a.out_cols + Cfg::BN - 1) / Cfg::BN);
+  if (tiles >= ((int64_t)1 << 31)) return set_error(GNN_ERR_UNSUPPORTED, "fused_linear: grid too large");
+  hipLaunchKernelGGL((linear_kernel<T, PREC, Cfg>), dim3((uint32_t)tiles), dim3(Cfg::NT), 0, st, a);
+  return (int)hipGetLastError();
+}
+
+template <typename T, int PREC>
+int run(const LinArgs& a, hipStream_t st) {
+  return launch<T, PREC, Tile<T, 2, 2, 2, 2, 2>>(a, st);
+}
+
+// ---- column sums ---------------------------------------------------------------------------
+// partial[part][n] = sum of d[m][n] over the rows m of a part: 32 lanes of 8 columns, 8 rows a turn
+template <typename T>
+__global__ __launch_bounds__(256) void column_sums_kernel(const T* d, int64_t ld, int64_t M, int O, int64_t rows,
+                                                          float* partial) {
+  __shared__ float sum[8][32 * 8 + 8];
+  const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
+  const int n = (blockIdx.y * 32 + c) * 8;
+  f32x8 s = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const int64_t m1 = min(M, (int64_t)(blockIdx.x + 1) * rows);
+  if (n < O)
+    for (int64_t m = (int64_t)blockIdx.x * rows + r; m < m1; m += 8) s += load8_any(d + m * ld + n, O - n);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum[r][c * 8 + e] = s[e];
+  __syncthreads();
+  const int col = blockIdx.y * 256 + threadIdx.x;
+  if (col >= O) return;
+  float t = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) t += sum[k][threadIdx.x];
+  partial[(int64_t)blockIdx.x * O + col] = t;
+}
+
+}  // namespace
+
+int linear(const gnn_linear_args& g, hipStream_t st) {
+  LinArgs a{};
+  a.x = g.x, a.w = g.w, a.bias = g.bias, a.side = g.side, a.out = g.out;
+  a.M = g.M, a.x_ld = g.x_ld, a.w_ld = g.w_ld, a.side_ld = g.side_ld, a.out_ld = g.out_ld;
+  a.I = (int)g.I, a.O = (int)g.O, a.out_cols = (int)g.out_cols, a.act = g.activation, a.dz = g.dz != 0;
+  switch (g.dtype) {
+    case GNN_BF16: return run<bf16, PREC_NATIVE>(a, st);
+    case GNN_F16: return run<f16, PREC_NATIVE>(a, st);
+    default: return g.precision == GNN_PREC_BF16X3 ? run<float, PREC_BF16X3>(a, st) : run<float, PREC_IEEE>(a, st);
+  }
+}
+
+int64_t column_sums_parts(int64_t M, int64_t O) {
+  const int64_t tiles = (O + 255) / 256;
+  return std::max<int64_t>(1, std::min<int64_t>((M + 63) / 64, 4 * (int64_t)compute_units() / tiles));
+}
+
+int column_sums(const gnn_column_sums_args& a, hipStream_t st) {
+  const int64_t rows = (a.M + a.parts - 1) / a.parts;
+  const dim3 grid((uint32_t)a.parts, (uint32_t)((a.O + 255) / 256)), blk(256);
+  switch (a.dtype) {
+    case GNN_BF16:
+      hipLaunchKernelGGL(column_sums_kernel<bf16>, grid, blk, 0, st, (const bf16*)a.d, a.ld, a.M, (int)a.O, rows, a.partial);
+      break;
+    case GNN_F16:
+      hipLaunchKernelGGL(column_sums_kernel<f16>, grid, blk, 0, st, (const f16*)a.d, a.ld, a.M, (int)a.O, rows, a.partial);
+      break;
+    default:
+      hipLaunchKernelGGL(column_sums_kernel<float>, grid, blk, 0, st, (const float*)a.d, a.ld, a.M, (int)a.O, rows,
+                         a.partial);
+      break;
+  }
+  return (int)hipGetLastError();
+}
+
+}  // namespace gnn

@@ -392,6 +392,51 @@ class ReduceArgs(ctypes.Structure):
     _fields_ = [("seg", ReduceSegment * REDUCE_MAX), ("count", ctypes.c_int64)]
 
 
+class LinearArgs(ctypes.Structure):
+    """Mirror of ``gnn_linear_args``."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("w", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("side", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("M", ctypes.c_int64),
+        ("I", ctypes.c_int64),
+        ("O", ctypes.c_int64),
+        ("out_cols", ctypes.c_int64),
+        ("x_ld", ctypes.c_int64),
+        ("w_ld", ctypes.c_int64),
+        ("side_ld", ctypes.c_int64),
+        ("out_ld", ctypes.c_int64),
+        ("activation", ctypes.c_int32),
+        ("dz", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("precision", ctypes.c_int32),
+    ]
+
+
+pack_linear = packer(LinearArgs)
+
+
+class ColumnSumsArgs(ctypes.Structure):
+    """Mirror of ``gnn_column_sums_args``."""
+
+    _fields_ = [
+        ("d", ctypes.c_void_p),
+        ("partial", ctypes.c_void_p),
+        ("M", ctypes.c_int64),
+        ("O", ctypes.c_int64),
+        ("ld", ctypes.c_int64),
+        ("parts", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+pack_column_sums = packer(ColumnSumsArgs)
+
+
 class RelposArgs(ctypes.Structure):
     """Mirror of ``gnn_relpos_args``."""
 
@@ -516,6 +561,9 @@ _SIGNATURES = {
     "gnn_relpos_fwd": (ctypes.c_int, [ctypes.POINTER(RelposArgs), ctypes.c_void_p]),
     "gnn_relpos_parts": (ctypes.c_int64, [ctypes.POINTER(RelposArgs)]),
     "gnn_relpos_bwd": (ctypes.c_int, [ctypes.POINTER(RelposArgs), ctypes.c_void_p]),
+    "gnn_linear": (ctypes.c_int, [ctypes.POINTER(LinearArgs), ctypes.c_void_p]),
+    "gnn_column_sums_parts": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64]),
+    "gnn_column_sums": (ctypes.c_int, [ctypes.POINTER(ColumnSumsArgs), ctypes.c_void_p]),
     "gnn_last_error": (ctypes.c_char_p, []),
     "gnn_version": (ctypes.c_char_p, []),
 }

@@ -20,7 +20,7 @@ from typing import Optional
 import torch
 
 __all__ = ["triangle_attention_fwd", "trimul_fwd", "attention_pair_bias_fwd", "layer_norm_fwd",
-           "relative_position_bias_fwd", "eager_ok"]
+           "relative_position_bias_fwd", "fused_linear_fwd", "eager_ok"]
 
 
 _PLAIN_TYPES = (torch.Tensor, torch.nn.Parameter)  # Parameter disables __torch_function__
@@ -195,3 +195,26 @@ def _relative_position_bias_fwd_fake(weight, query_pos, key_pos, max_distance, s
     if channels_last:
         return weight.new_empty((B, U, V, H))
     return weight.new_empty((B, H, U, (V + 7) // 8 * 8))[..., :V]
+
+
+def fused_linear_fwd_impl(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    bias: Optional[torch.Tensor],
+    activation: Optional[str],
+    residual: Optional[torch.Tensor],
+) -> torch.Tensor:
+    """``x [..., I]``, ``weight [O, I]``; returns a fresh contiguous ``[..., O]`` tensor of x's dtype."""
+    from . import _precision
+    from .triangle._kernels.fused_linear import fused_linear_hip
+
+    precision = _precision.matmul_precision(fp32_operands=x.dtype == torch.float32)
+    return fused_linear_hip(x, weight, bias, activation, residual, precision=precision)
+
+
+fused_linear_fwd = torch.library.custom_op("gnn_amd::fused_linear_fwd", fused_linear_fwd_impl, mutates_args=())
+
+
+@fused_linear_fwd.register_fake
+def _fused_linear_fwd_fake(x, weight, bias, activation, residual):
+    return x.new_empty((*x.shape[:-1], weight.shape[0]))

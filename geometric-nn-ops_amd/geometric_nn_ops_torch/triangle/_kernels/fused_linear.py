@@ -1,0 +1,114 @@
+"""Host side of the HIP linear layer with its epilogue: ``fused_linear_hip`` and the gradients,
+``fused_linear_bwd_hip``.
+
+The kernels read x and the weight in 16-byte chunks of rows: rows of another alignment, and widths that are
+no multiple of 8, are copied once into padded rows. Results, residuals and output gradients are read and
+written in place at any alignment."""
+
+import torch
+import torch.nn.functional as F
+
+from ... import _lib
+from .trimul import reduce_parts_hip, rows_products_hip
+
+ACTIVATION_CODE = {None: 0, "relu": 1, "gelu": 2, "silu": 3, "sigmoid": 4}
+MAX_WIDTH = 1 << 20
+
+
+def supports(weight: torch.Tensor) -> bool:
+    """Whether the HIP kernels cover these widths (dtype handled by the caller)."""
+    return 1 <= weight.shape[0] <= MAX_WIDTH and 1 <= weight.shape[1] <= MAX_WIDTH
+
+
+def _chunked(t: torch.Tensor) -> torch.Tensor:
+    """``[R, C]`` rows of 16-byte chunks: C padded with zeros to a multiple of 8."""
+    c = t.shape[1]
+    if c % 8:
+        return F.pad(t, (0, 8 - c % 8))
+    if t.shape[0] == 1 and t.stride(1) == 1:
+        t = t.as_strided((1, c), (c, 1))  # one row: its pitch says nothing
+    if t.stride(1) == 1 and t.stride(0) >= c and t.stride(0) * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _unit(t: torch.Tensor) -> torch.Tensor:
+    """``[R, C]`` with unit stride in a row, at any pitch and alignment."""
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _pitch(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _linear(x, w, bias, side, outputs, activation, precision, *, dz=False, pad=False):
+    """One kernel over chunked rows ``x [M, K]`` and ``w [>= outputs, K]``; ``[M, outputs]``, with ``pad`` in
+    rows of a multiple of 8 columns, zeros behind."""
+    M, K = x.shape
+    cols = (outputs + 7) // 8 * 8 if pad else outputs
+    out = torch.empty((M, cols), device=x.device, dtype=x.dtype)
+    a = _lib.LinearArgs()
+    _lib.pack_linear(
+        a, 0, x.data_ptr(), w.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if side is None else side.data_ptr(),
+        out.data_ptr(), M, K, outputs, cols, _pitch(x), _pitch(w), 0 if side is None else _pitch(side), cols,
+        ACTIVATION_CODE[activation], dz, _lib.DTYPE_CODE[x.dtype], _lib.PRECISION_CODE[precision])
+    _lib.call("gnn_linear", a, x.device)
+    return out
+
+
+def fused_linear_hip(x, weight, bias=None, activation=None, residual=None, *, precision):
+    """``act(x weight^T + bias) + residual``, fresh and contiguous."""
+    O, I = weight.shape
+    shape = (*x.shape[:-1], O)
+    M = x.numel() // I
+    if not M:
+        return torch.empty(shape, device=x.device, dtype=x.dtype)
+    side = None if residual is None else _unit(residual.reshape(M, O))
+    bias = None if bias is None else bias.contiguous()
+    return _linear(_chunked(x.reshape(M, I)), _chunked(weight), bias, side, O, activation, precision).view(shape)
+
+
+def _column_sums(d, outputs):
+    """fp32 partial sums ``[parts, outputs]`` over the rows of ``d``."""
+    parts = _lib.load().gnn_column_sums_parts(d.shape[0], outputs)
+    part = torch.empty((parts, outputs), device=d.device, dtype=torch.float32)
+    a = _lib.ColumnSumsArgs()
+    _lib.pack_column_sums(a, 0, d.data_ptr(), part.data_ptr(), d.shape[0], outputs, _pitch(d), parts,
+                          _lib.DTYPE_CODE[d.dtype], 0)
+    _lib.call("gnn_column_sums", a, d.device)
+    return part
+
+
+def fused_linear_bwd_hip(x, weight, bias, activation, dy, *, precision, need_x=True, need_w=True, need_b=True):
+    """``(dx, dweight, dbias)``, None where not needed. The activation's input is formed again from x and the
+    weight (in fp32); its gradient dz is rounded to x's dtype once, as the operand of the products."""
+    O, I = weight.shape
+    M = x.numel() // I
+    if not M:
+        grads = (x, weight, weight[:, 0])
+        return tuple(torch.zeros(t.shape, device=x.device, dtype=x.dtype) if need else None
+                     for t, need in zip(grads, (need_x, need_w, need_b)))
+    dx = dw = db = None
+    x2 = _chunked(x.reshape(M, I))
+    dz = _unit(dy.reshape(M, O))
+    if activation is not None:
+        dz = _linear(x2, _chunked(weight), None if bias is None else bias.contiguous(), dz, O, activation, precision,
+                     dz=True, pad=True)
+    elif need_x or need_w:
+        dz = _chunked(dz)
+    if need_x:
+        dx = _linear(dz, _chunked(weight.t()), None, None, I, None, precision).view(x.shape)
+    segments = []
+    if need_w:
+        (part,) = rows_products_hip([(dz, x2)])
+        dw = torch.empty(part.shape[1:], device=x.device, dtype=x.dtype)
+        segments.append((part, 0, dw.numel(), dw))
+    if need_b:
+        db = torch.empty((O,), device=x.device, dtype=x.dtype)
+        segments.append((_column_sums(dz, O), 0, O, db))
+    if segments:
+        reduce_parts_hip(segments, x.device)
+    if need_w and dw.shape != weight.shape:
+        dw = dw[:O, :I].contiguous()
+    return dx, dw, db

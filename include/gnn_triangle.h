@@ -652,6 +652,47 @@ int gnn_relpos_fwd(const gnn_relpos_args* args, void* stream);
 int64_t gnn_relpos_parts(const gnn_relpos_args* args);
 int gnn_relpos_bwd(const gnn_relpos_args* args, void* stream);
 
+/* A linear layer with its epilogue, out = act(x w^T + bias) + side, or with `dz` set the gradient that goes
+ * into its products, out = side * act'(x w^T + bias) (side = dy then). x: rows of I elements, x_ld apart;
+ * w: [O] rows of I, w_ld apart; both 16-byte aligned with I and the pitches multiples of 16 bytes (pad with
+ * zeros). bias: [O] or NULL. side: rows of O, side_ld apart, or NULL without dz; out: rows of out_cols >= O
+ * columns, out_ld apart, zeros from column O on; any alignment of their elements. All in dtype; products and
+ * epilogue in fp32, one rounding. precision: fp32 products (GNN_PREC_IEEE or GNN_PREC_BF16X3). The reference
+ * runs F.linear and separate elementwise ops (triangle/_reference/trimul.py:86-97). */
+enum gnn_activation {
+  GNN_ACT_NONE = 0,
+  GNN_ACT_RELU = 1,
+  GNN_ACT_GELU = 2, /* z Phi(z), the exact form */
+  GNN_ACT_SILU = 3,
+  GNN_ACT_SIGMOID = 4
+};
+typedef struct gnn_linear_args {
+  const void* x;
+  const void* w;
+  const void* bias;
+  const void* side;
+  void* out;
+  int64_t M, I, O, out_cols;
+  int64_t x_ld, w_ld, side_ld, out_ld;
+  int32_t activation; /* enum gnn_activation */
+  int32_t dz;
+  int32_t dtype;
+  int32_t precision;
+} gnn_linear_args;
+int gnn_linear(const gnn_linear_args* args, void* stream);
+
+/* Sums over the rows of d [M, O] (pitch ld), as fp32 partial sums [parts][O] to be added with
+ * gnn_reduce_parts; parts as gnn_column_sums_parts(M, O) returns it (any from 1 on is right). */
+typedef struct gnn_column_sums_args {
+  const void* d;
+  float* partial;
+  int64_t M, O, ld, parts;
+  int32_t dtype;
+  int32_t reserved;
+} gnn_column_sums_args;
+int64_t gnn_column_sums_parts(int64_t M, int64_t O);
+int gnn_column_sums(const gnn_column_sums_args* args, void* stream);
+
 /* Message for the last failing call on this thread ("" if none). */
 const char* gnn_last_error(void);
 

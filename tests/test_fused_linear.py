@@ -1,0 +1,143 @@
+"""fused_linear on a CPU-only host: the torch path and its gradients, the refusals, the rows that the
+kernels are given, and the C entry points' argument errors."""
+
+import ctypes
+import pathlib
+import subprocess
+
+import pytest
+import torch
+
+from geometric_nn_ops_torch import _lib
+from geometric_nn_ops_torch.triangle import fused_linear
+from geometric_nn_ops_torch.triangle._kernels import fused_linear as _hip
+
+ACTS = [None, "relu", "gelu", "silu", "sigmoid"]
+
+
+def _formula(z, act):
+    if act == "relu":
+        return z.clamp(min=0)
+    if act == "gelu":
+        return z * torch.special.ndtr(z)
+    if act == "silu":
+        return z / (1 + (-z).exp())
+    return 1 / (1 + (-z).exp()) if act == "sigmoid" else z
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16])
+def test_torch_path(act, dtype):
+    g = torch.Generator().manual_seed(1)
+    x, w, b, r = (torch.randn(*s, generator=g).to(dtype) for s in ((2, 3, 7), (5, 7), (5,), (2, 3, 5)))
+    want = _formula(x.double() @ w.double().t() + b.double(), act) + r.double()
+    got = fused_linear(x, w, b, act, r)
+    assert got.dtype == dtype and got.shape == (2, 3, 5)
+    tol = {torch.float32: 1e-6, torch.float64: 1e-14, torch.bfloat16: 2.0 ** -8}[dtype]
+    assert ((got.double() - want).abs() <= tol * (1 + want.abs())).all()
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_torch_path_gradients(act):
+    g = torch.Generator().manual_seed(2)
+    args = [torch.randn(*s, generator=g, dtype=torch.float64, requires_grad=True)
+            for s in ((4, 6), (3, 6), (3,), (4, 3))]
+    assert torch.autograd.gradcheck(lambda x, w, b, r: fused_linear(x, w, b, act, r), args)
+
+
+def test_refusals():
+    x, w = torch.zeros(2, 3, 8), torch.zeros(5, 8)
+    with pytest.raises(ValueError, match=r"weight must have shape \[outputs, 8\]"):
+        fused_linear(x, w.t())
+    with pytest.raises(ValueError, match="weight must have shape"):
+        fused_linear(x, torch.zeros(0, 8))
+    with pytest.raises(ValueError, match="weight must have shape"):
+        fused_linear(x, torch.zeros(8))
+    with pytest.raises(ValueError, match="activation must be one of"):
+        fused_linear(x, w, activation="tanh")
+    with pytest.raises(ValueError, match="bias must have shape"):
+        fused_linear(x, w, torch.zeros(8))
+    with pytest.raises(ValueError, match="residual must have shape"):
+        fused_linear(x, w, residual=torch.zeros(5))
+    with pytest.raises(ValueError, match="bias must be torch.float32 like x"):
+        fused_linear(x, w, torch.zeros(5).half())
+    with pytest.raises(ValueError, match="weight must be torch.float32 like x"):
+        fused_linear(x, w.bfloat16())
+    with pytest.raises(ValueError, match="residual is on meta"):
+        fused_linear(x, w, residual=torch.zeros(2, 3, 5, device="meta"))
+    with pytest.raises(ValueError, match="floating-point"):
+        fused_linear(x.long(), w)
+    with pytest.raises(ValueError, match="floating-point"):
+        fused_linear(torch.tensor(1.0), w)
+
+
+def test_chunked_rows():
+    base = torch.arange(4 * 64, dtype=torch.bfloat16).reshape(4, 64)
+    for t, same in ((base, True), (base[:, 8:24], True), (base[:, 4:20], False), (base[:, :13], False),
+                    (base.t()[:8, :2].t(), True), (base[:, ::4], False), (base[:1].expand(3, 64), False), (base[1:2, 16:24], True),
+                    (torch.arange(66, dtype=torch.bfloat16)[2:].view(1, 64), False)):
+        c = _hip._chunked(t)
+        assert torch.equal(c[:, :t.shape[1]], t) and not c[:, t.shape[1]:].any()
+        assert c.shape[1] % 8 == 0 and c.stride(1) == 1 and c.stride(0) % 8 == 0 and c.data_ptr() % 16 == 0
+        assert c.stride(0) >= c.shape[1]
+        assert (c.data_ptr() == t.data_ptr()) == same
+
+
+def test_argument_errors():
+    lib = _lib.load()
+    assert lib.gnn_linear(None, None) == _lib.GNN_ERR_ARG
+    a = _lib.LinearArgs()
+
+    def refused(text, fn=lib.gnn_linear, args=a):
+        assert fn(ctypes.byref(args), None) == _lib.GNN_ERR_ARG
+        assert text in lib.gnn_last_error(), lib.gnn_last_error()
+
+    refused(b"required")
+    a.x = a.w = a.out = 4096
+    a.dz = 1
+    refused(b"required")
+    a.dz, a.dtype = 0, 9
+    refused(b"dtype")
+    a.dtype, a.precision = _lib.GNN_BF16, 5
+    refused(b"precision")
+    a.precision, a.activation = 0, 5
+    refused(b"activation")
+    a.activation = 0
+    refused(b"positive")
+    a.M, a.I, a.O, a.out_cols = 4, 12, 5, 4
+    refused(b"out_cols")
+    a.out_cols = 5
+    refused(b"16 bytes")
+    a.I = a.x_ld = 16
+    a.w_ld = 8
+    refused(b"pitches")
+    a.w_ld, a.out_ld = 16, 4
+    refused(b"pitches")
+    a.out_ld, a.out = 5, 4097
+    refused(b"aligned")
+    a.out, a.x = 4096, 4104
+    refused(b"16-byte")
+
+    assert lib.gnn_column_sums(None, None) == _lib.GNN_ERR_ARG
+    assert lib.gnn_column_sums_parts(0, 5) == 0 and lib.gnn_column_sums_parts(1, 5) == 1
+    c = _lib.ColumnSumsArgs()
+    refused(b"required", lib.gnn_column_sums, c)
+    c.d = c.partial = 4096
+    refused(b"positive", lib.gnn_column_sums, c)
+    c.M, c.O, c.parts, c.dtype = 4, 5, 1, _lib.GNN_BF16
+    c.d = 4097
+    refused(b"aligned", lib.gnn_column_sums, c)
+
+
+def test_args_match_the_c_layout(tmp_path):
+    root = pathlib.Path(__file__).resolve().parent.parent
+    structs = {"gnn_linear_args": _lib.LinearArgs, "gnn_column_sums_args": _lib.ColumnSumsArgs}
+    body = "".join(f'printf("%zu\\n", sizeof({s}));' + "".join(
+        f'printf("%zu\\n", offsetof({s}, {f[0]}));' for f in c._fields_) for s, c in structs.items())
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "gnn_triangle.h"\nint main(void) {' + body +
+                   "return 0;}")
+    subprocess.run(["gcc", "-std=c11", f"-I{root / 'include'}", str(src), "-o", str(tmp_path / "layout")], check=True)
+    out = subprocess.run([str(tmp_path / "layout")], capture_output=True, text=True, check=True).stdout.split()
+    want = [v for c in structs.values() for v in (ctypes.sizeof(c), *(getattr(c, f[0]).offset for f in c._fields_))]
+    assert [int(v) for v in out] == want
