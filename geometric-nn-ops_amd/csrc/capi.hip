@@ -509,14 +509,18 @@ int gnn_linear(const gnn_linear_args* args, void* stream) {
   const int64_t e = a.dtype == GNN_F32 ? 4 : 2;
   if (!aligned(a.x, 16) || !aligned(a.w, 16) || (a.I * e) % 16 || (a.x_ld * e) % 16 || (a.w_ld * e) % 16)
     return set_error(GNN_ERR_ARG, "fused_linear: rows of x and w must be 16-byte aligned and multiples of 16 bytes");
-  if (a.x_ld < 0 || a.w_ld < a.I || (a.side && a.side_ld < 0) || a.out_ld < a.out_cols)
+  if (a.x_ld < 0 || a.w_ld < (a.w_transposed ? a.O : a.I) || (a.side && a.side_ld < 0) || a.out_ld < a.out_cols)
     return set_error(GNN_ERR_ARG, "fused_linear: row pitches must cover their rows");
   if (!aligned(a.bias, e) || !aligned(a.side, e) || !aligned(a.out, e))
     return set_error(GNN_ERR_ARG, "fused_linear: tensors must be aligned to their elements");
+  if (a.w_transposed && !linear_takes_transposed(a))
+    return set_error(GNN_ERR_UNSUPPORTED, "fused_linear: this call does not take a transposed weight");
   int rc = linear(a, (hipStream_t)stream);
   if (rc < 0) return rc;
   return hip_status((hipError_t)rc, "fused_linear");
 }
+
+int gnn_linear_takes_transposed(const gnn_linear_args* args) { return args && linear_takes_transposed(*args) ? 1 : 0; }
 
 int64_t gnn_column_sums_parts(int64_t M, int64_t O) { return M < 1 || O < 1 ? 0 : column_sums_parts(M, O); }
 

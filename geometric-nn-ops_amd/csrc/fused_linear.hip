@@ -8,164 +8,24 @@
 // linear_kernel. BM x BN output tiles, the contraction in stages of 128 bytes a row, both operands moved by
 // global_load_lds into LDS (STAGES of them in flight) with the 16-byte chunks of row r XOR-swizzled by r % 8,
 // so that the fragment reads of 8 rows hit 8 bank groups. The products are formed transposed (W's rows as the
-// rows of the 32x32 MFMA tile): a lane then holds one row of x and, once v_permlane32_swap has exchanged the
-// halves of neighbouring register groups, 8 consecutive outputs of it, which take bias, activation and
-// residual in fp32, round once and leave as one 16-byte store (two in fp32). Workgroups that share rows of x
+// rows of the 32x32 MFMA tile, in an order that leaves a lane 8 consecutive outputs of one row of x): these
+// take bias, activation and residual in fp32, round once and leave as one 16-byte store (two in fp32). Workgroups that share rows of x
 // follow each other on one XCD, whose L2 then serves x.
 #include <algorithm>
 
-#include "gnn_common.hpp"
-#include "gnn_internal.hpp"
+#include "linear_common.hpp"
 
 namespace gnn {
 
 namespace {
 
-typedef __attribute__((address_space(3))) void lds_void_t;
-
-__device__ __attribute__((aligned(16))) const uint32_t zero_chunk[4] = {0u, 0u, 0u, 0u};
+using namespace lin;
 
 // s_waitcnt vmcnt(VM) expcnt(7) lgkmcnt(0)
 template <int VM>
 __device__ __forceinline__ void wait_vm_lgkm0() {
   static_assert(VM >= 0 && VM < 64, "vmcnt immediate");
   __builtin_amdgcn_s_waitcnt(0x070 | (VM & 15) | ((VM >> 4) << 14));
-}
-
-// ---- activations ------------------------------------------------------------------------
-// 16-bit results: exp2 and rcp of the hardware (1 ulp each) and, for the normal distribution, Abramowitz and
-// Stegun 7.1.26: erfc(u) = t (a1 + t (a2 + ...)) exp(-u^2), t = 1 / (1 + 0.3275911 u), off by at most 1.5e-7;
-// both are far below half a step of fp16 (2.4e-4). fp32: the library's functions and full divisions.
-template <bool F32>
-__device__ __forceinline__ float sigmoid(float z) {
-  if constexpr (F32) return 1.0f / (1.0f + expf(-z));
-  return __builtin_amdgcn_rcpf(1.0f + fast_exp2(-1.4426950408889634f * z));
-}
-
-// Phi(z), and z phi(z) where the slope needs it
-template <bool F32>
-__device__ __forceinline__ float normal_cdf(float z, float& z_pdf) {
-  if constexpr (F32) {
-    z_pdf = z * 0.3989422804014327f * expf(-0.5f * z * z);
-    return 0.5f * erfcf(-0.7071067811865476f * z);
-  }
-  const float e = fast_exp2(-0.7213475204444817f * z * z);  // exp(-z^2 / 2)
-  const float u = 0.7071067811865476f * fabsf(z);
-  const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * u);
-  const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-  const float tail = 0.5f * p * e;  // Phi(-|z|)
-  z_pdf = z * 0.3989422804014327f * e;
-  return z < 0.f ? tail : 1.0f - tail;
-}
-
-template <bool F32>
-__device__ __forceinline__ float activate(int act, float z) {
-  float unused;
-  switch (act) {
-    case GNN_ACT_RELU: return z < 0.f ? 0.f : z;
-    case GNN_ACT_GELU: return z * normal_cdf<F32>(z, unused);
-    case GNN_ACT_SILU: return z * sigmoid<F32>(z);
-    case GNN_ACT_SIGMOID: return sigmoid<F32>(z);
-    default: return z;
-  }
-}
-template <bool F32>
-__device__ __forceinline__ float slope(int act, float z) {
-  switch (act) {
-    case GNN_ACT_RELU: return z <= 0.f ? 0.f : 1.f;
-    case GNN_ACT_GELU: {
-      float z_pdf;
-      const float cdf = normal_cdf<F32>(z, z_pdf);
-      return cdf + z_pdf;
-    }
-    case GNN_ACT_SILU: {
-      const float s = sigmoid<F32>(z);
-      return s * (1.0f + z * (1.0f - s));
-    }
-    case GNN_ACT_SIGMOID: {
-      const float s = sigmoid<F32>(z);
-      return s * (1.0f - s);
-    }
-    default: return 1.f;
-  }
-}
-
-// ---- tiles --------------------------------------------------------------------------------
-struct LinArgs {
-  const void* x;
-  const void* w;
-  const void* bias;
-  const void* side;  // residual, or dy
-  void* out;
-  int64_t M;
-  int64_t x_ld, w_ld, side_ld, out_ld;
-  int I, O;      // contraction (a multiple of 8; 4 in fp32), outputs
-  int out_cols;  // columns written, zeros from O on
-  int act;
-  bool dz;  // out = side * act'(z) instead of act(z) + side
-};
-
-// 8 consecutive elements at any element's address, the first `left` of them
-template <typename T>
-__device__ __forceinline__ f32x8 load8_any(const T* p, int left) {
-  typedef typename TypeOps<T>::V8 V8;
-  typedef V8 VU __attribute__((aligned(sizeof(T))));
-  if (left >= 8) {
-    const V8 v = *(const __attribute__((address_space(1))) VU*)p;
-    return TypeOps<T>::to_f32(v);
-  }
-  f32x8 v;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = e < left ? (float)p[e] : 0.f;
-  return v;
-}
-template <typename T>
-__device__ __forceinline__ void store8_any(T* p, const f32x8& v, int left) {
-  typedef typename TypeOps<T>::V8 V8;
-  typedef V8 VU __attribute__((aligned(sizeof(T))));
-  const V8 o = TypeOps<T>::from_f32(v);
-  if (left >= 8) {
-    *(__attribute__((address_space(1))) VU*)p = o;
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (e < left) p[e] = o[e];
-}
-
-// The 8 consecutive rows (of the transposed product: outputs) 16 t + 8 g + (0 .. 7) of a lane's column
-__device__ __forceinline__ f32x8 swapped8(const f32x16& acc, int t) {
-  f32x8 v;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[8 * t + i]), __float_as_uint(acc[8 * t + 4 + i]),
-                                                    false, false);
-    v[i] = __uint_as_float(s[0]);
-    v[4 + i] = __uint_as_float(s[1]);
-  }
-  return v;
-}
-
-// Bias, activation and residual (or the slope of dy) on 8 outputs n .. n + 7 of row m, and their store
-template <typename T>
-__device__ __forceinline__ void finish8(const LinArgs& a, const f32x8& z0, const f32x8& b, int64_t m, int n) {
-  constexpr bool F32 = sizeof(T) == 4;
-  const int left = a.O - n;
-  f32x8 z = z0 + b;
-  if (a.dz) {
-    const f32x8 dy = load8_any((const T*)a.side + m * a.side_ld + n, left);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) z[e] = dy[e] * slope<F32>(a.act, z[e]);
-  } else {
-    if (a.act)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] = activate<F32>(a.act, z[e]);
-    if (a.side) z += load8_any((const T*)a.side + m * a.side_ld + n, left);
-  }
-  if (left < 8)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) z[e] = e < left ? z[e] : 0.f;
-  store8_any((T*)a.out + m * a.out_ld + n, z, a.out_cols - n);
 }
 
 // GM x GN waves of 32 X rows x 32 Y outputs
@@ -206,7 +66,11 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::LDS <= (80 << 10) ? 2 * Cfg::NW / 4 :
     xsrc[q] = (const T*)a.x + min(m0 + 8 * (Cfg::QA * wave + q) + drow, a.M - 1) * a.x_ld + dchunk * Cfg::EPC;
 #pragma unroll
   for (int q = 0; q < Cfg::QB; ++q)
-    wsrc[q] = (const T*)a.w + (int64_t)min(n0 + 8 * (Cfg::QB * wave + q) + drow, a.O - 1) * a.w_ld + dchunk * Cfg::EPC;
+    {
+    // tiles of 32 rows hold the outputs in tile_output's order
+    const int r = 8 * (Cfg::QB * wave + q) + drow, n = n0 + (r & ~31) + tile_output(r & 31);
+    wsrc[q] = (const T*)a.w + (int64_t)min(n, a.O - 1) * a.w_ld + dchunk * Cfg::EPC;
+  }
   const int nkt = (a.I + Cfg::BK - 1) / Cfg::BK;
   auto issue = [&](int kt) {
     unsigned char* st = smem + (kt % Cfg::STAGES) * Cfg::STAGE;
@@ -283,9 +147,8 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::LDS <= (80 << 10) ? 2 * Cfg::NW / 4 :
       if (a.bias && n < a.O) b = load8_any((const T*)a.bias + n, a.O - n);
 #pragma unroll
       for (int x = 0; x < Cfg::X; ++x) {
-        const f32x8 z = swapped8(acc[x][y], t);  // every lane takes part in the swap
         const int64_t m = m0 + 32 * (Cfg::X * wm + x) + l32;
-        if (m < a.M && n < a.out_cols) finish8<T>(a, z, b, m, n);
+        if (m < a.M && n < a.out_cols) finish8<T>(a, outputs8(acc[x][y], t), b, m, n);
       }
     }
 }
@@ -328,7 +191,10 @@ __global__ __launch_bounds__(256) void column_sums_kernel(const T* d, int64_t ld
 
 }  // namespace
 
+bool linear_takes_transposed(const gnn_linear_args& g) { return linear_resident_applicable(g); }
+
 int linear(const gnn_linear_args& g, hipStream_t st) {
+  if (linear_resident_applicable(g)) return linear_resident(g, st);
   LinArgs a{};
   a.x = g.x, a.w = g.w, a.bias = g.bias, a.side = g.side, a.out = g.out;
   a.M = g.M, a.x_ld = g.x_ld, a.w_ld = g.w_ld, a.side_ld = g.side_ld, a.out_ld = g.out_ld;

@@ -1,0 +1,183 @@
+// What the linear layer's kernels share: activations and their slopes, the arguments, and the epilogue of 8
+// consecutive outputs of a row.
+#pragma once
+
+#include "gnn_common.hpp"
+#include "gnn_internal.hpp"
+
+namespace gnn {
+namespace lin {
+
+typedef __attribute__((address_space(3))) void lds_void_t;
+
+// Source of the chunks that a DMA fills with zeros
+__device__ __attribute__((aligned(16))) const uint32_t zero_chunk[4] = {0u, 0u, 0u, 0u};
+
+// ---- activations ------------------------------------------------------------------------
+// 16-bit results: exp2 and rcp of the hardware (1 ulp each) and, for the normal distribution, Abramowitz and
+// Stegun 7.1.26: erfc(u) = t (a1 + t (a2 + ...)) exp(-u^2), t = 1 / (1 + 0.3275911 u), off by at most 1.5e-7;
+// both are far below half a step of fp16 (2.4e-4). fp32: the library's functions and full divisions.
+template <bool F32>
+__device__ __forceinline__ float sigmoid(float z) {
+  if constexpr (F32) return 1.0f / (1.0f + expf(-z));
+  return __builtin_amdgcn_rcpf(1.0f + fast_exp2(-1.4426950408889634f * z));
+}
+
+// Phi(z), and z phi(z) where the slope needs it
+template <bool F32>
+__device__ __forceinline__ float normal_cdf(float z, float& z_pdf) {
+  if constexpr (F32) {
+    z_pdf = z * 0.3989422804014327f * expf(-0.5f * z * z);
+    return 0.5f * erfcf(-0.7071067811865476f * z);
+  }
+  const float e = fast_exp2(-0.7213475204444817f * z * z);  // exp(-z^2 / 2)
+  const float u = 0.7071067811865476f * fabsf(z);
+  const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * u);
+  const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  const float tail = 0.5f * p * e;  // Phi(-|z|)
+  z_pdf = z * 0.3989422804014327f * e;
+  return z < 0.f ? tail : 1.0f - tail;
+}
+
+template <bool F32, int ACT>
+__device__ __forceinline__ float activate(float z) {
+  float unused;
+  if constexpr (ACT == GNN_ACT_RELU) return __builtin_elementwise_maximum(z, 0.f);  // NaN stays
+  if constexpr (ACT == GNN_ACT_GELU) return z * normal_cdf<F32>(z, unused);
+  if constexpr (ACT == GNN_ACT_SILU) return z * sigmoid<F32>(z);
+  if constexpr (ACT == GNN_ACT_SIGMOID) return sigmoid<F32>(z);
+  return z;
+}
+template <bool F32, int ACT>
+__device__ __forceinline__ float slope(float z) {
+  if constexpr (ACT == GNN_ACT_RELU) return z <= 0.f ? 0.f : 1.f;
+  if constexpr (ACT == GNN_ACT_GELU) {
+    float z_pdf;
+    const float cdf = normal_cdf<F32>(z, z_pdf);
+    return cdf + z_pdf;
+  }
+  if constexpr (ACT == GNN_ACT_SILU) {
+    const float s = sigmoid<F32>(z);
+    return s * (1.0f + z * (1.0f - s));
+  }
+  if constexpr (ACT == GNN_ACT_SIGMOID) {
+    const float s = sigmoid<F32>(z);
+    return s * (1.0f - s);
+  }
+  return 1.f;
+}
+
+// A vector of values at once: one uniform branch (16 of them, one an element, took longer than the products)
+template <bool F32, int ACT, typename V>
+__device__ __forceinline__ void activate_all(V& z) {
+#pragma unroll
+  for (int e = 0; e < (int)(sizeof(V) / sizeof(float)); ++e) z[e] = activate<F32, ACT>(z[e]);
+}
+template <bool F32, typename V>
+__device__ __forceinline__ void activate_all(int act, V& z) {
+  switch (act) {
+    case GNN_ACT_RELU: activate_all<F32, GNN_ACT_RELU>(z); break;
+    case GNN_ACT_GELU: activate_all<F32, GNN_ACT_GELU>(z); break;
+    case GNN_ACT_SILU: activate_all<F32, GNN_ACT_SILU>(z); break;
+    case GNN_ACT_SIGMOID: activate_all<F32, GNN_ACT_SIGMOID>(z); break;
+    default: break;
+  }
+}
+template <bool F32, int ACT, typename V>
+__device__ __forceinline__ void slope_all(V& z) {
+#pragma unroll
+  for (int e = 0; e < (int)(sizeof(V) / sizeof(float)); ++e) z[e] = slope<F32, ACT>(z[e]);
+}
+template <bool F32, typename V>
+__device__ __forceinline__ void slope_all(int act, V& z) {
+  switch (act) {
+    case GNN_ACT_RELU: slope_all<F32, GNN_ACT_RELU>(z); break;
+    case GNN_ACT_GELU: slope_all<F32, GNN_ACT_GELU>(z); break;
+    case GNN_ACT_SILU: slope_all<F32, GNN_ACT_SILU>(z); break;
+    case GNN_ACT_SIGMOID: slope_all<F32, GNN_ACT_SIGMOID>(z); break;
+    default: slope_all<F32, GNN_ACT_NONE>(z); break;
+  }
+}
+
+// ---- arguments and epilogue ---------------------------------------------------------------
+struct LinArgs {
+  const void* x;
+  const void* w;
+  const void* bias;
+  const void* side;  // residual, or dy
+  void* out;
+  int64_t M;
+  int64_t x_ld, w_ld, side_ld, out_ld;
+  int I, O;      // contraction (a multiple of 8; 4 in fp32), outputs
+  int out_cols;  // columns written, zeros from O on
+  int act;
+  bool dz;  // out = side * act'(z) instead of act(z) + side
+};
+
+// 8 consecutive elements at any element's address, the first `left` of them
+template <typename T>
+__device__ __forceinline__ f32x8 load8_any(const T* p, int left) {
+  typedef typename TypeOps<T>::V8 V8;
+  typedef V8 VU __attribute__((aligned(sizeof(T))));
+  if (left >= 8) {
+    const V8 v = *(const __attribute__((address_space(1))) VU*)p;
+    return TypeOps<T>::to_f32(v);
+  }
+  f32x8 v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = e < left ? (float)p[e] : 0.f;
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store8_any(T* p, const f32x8& v, int left) {
+  typedef typename TypeOps<T>::V8 V8;
+  typedef V8 VU __attribute__((aligned(sizeof(T))));
+  const V8 o = TypeOps<T>::from_f32(v);
+  if (left >= 8) {
+    *(__attribute__((address_space(1))) VU*)p = o;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < left) p[e] = o[e];
+}
+
+// The 32x32 accumulator has rows 8 q + 4 g + i (q = r / 4, i = r % 4) in a lane. Tile row r of the transposed
+// product takes output tile_output(r), so that a lane's 8 registers 8 t .. 8 t + 7 are the 8 consecutive
+// outputs 16 t + 8 g + (0 .. 7), and tile_row is the other way round. (Exchanging the halves of natural tiles
+// with v_permlane32_swap took 8 more instructions a tile.)
+__host__ __device__ constexpr int tile_output(int r) { return (r & 16) | (r & 4) << 1 | (r & 8) >> 1 | (r & 3); }
+__host__ __device__ constexpr int tile_row(int n) { return (n & 16) | (n & 8) >> 1 | (n & 4) << 1 | (n & 3); }
+__device__ __forceinline__ f32x8 outputs8(const f32x16& acc, int t) {
+  f32x8 v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = acc[8 * t + e];
+  return v;
+}
+
+// Bias, activation and residual (or the slope of dy) on 8 outputs n .. n + 7 of row m, and their store
+template <typename T>
+__device__ __forceinline__ void finish8(const LinArgs& a, const f32x8& z0, const f32x8& b, int64_t m, int n) {
+  constexpr bool F32 = sizeof(T) == 4;
+  const int left = a.O - n;
+  f32x8 z = z0 + b;
+  if (a.dz) {
+    slope_all<F32>(a.act, z);
+    z *= load8_any((const T*)a.side + m * a.side_ld + n, left);
+  } else {
+    activate_all<F32>(a.act, z);
+    if (a.side) z += load8_any((const T*)a.side + m * a.side_ld + n, left);
+  }
+  if (left < 8)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] = e < left ? z[e] : 0.f;
+  store8_any((T*)a.out + m * a.out_ld + n, z, a.out_cols - n);
+}
+
+}  // namespace lin
+
+// Kernels that keep the whole weight in LDS (16-bit types, many rows); false where a call is not theirs.
+bool linear_resident_applicable(const gnn_linear_args& a);
+int linear_resident(const gnn_linear_args& a, hipStream_t stream);
+
+}  // namespace gnn

@@ -411,8 +411,10 @@ class LinearArgs(ctypes.Structure):
         ("out_ld", ctypes.c_int64),
         ("activation", ctypes.c_int32),
         ("dz", ctypes.c_int32),
+        ("w_transposed", ctypes.c_int32),
         ("dtype", ctypes.c_int32),
         ("precision", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
     ]
 
 
@@ -561,6 +563,7 @@ _SIGNATURES = {
     "gnn_relpos_fwd": (ctypes.c_int, [ctypes.POINTER(RelposArgs), ctypes.c_void_p]),
     "gnn_relpos_parts": (ctypes.c_int64, [ctypes.POINTER(RelposArgs)]),
     "gnn_relpos_bwd": (ctypes.c_int, [ctypes.POINTER(RelposArgs), ctypes.c_void_p]),
+    "gnn_linear_takes_transposed": (ctypes.c_int, [ctypes.POINTER(LinearArgs)]),
     "gnn_linear": (ctypes.c_int, [ctypes.POINTER(LinearArgs), ctypes.c_void_p]),
     "gnn_column_sums_parts": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64]),
     "gnn_column_sums": (ctypes.c_int, [ctypes.POINTER(ColumnSumsArgs), ctypes.c_void_p]),

@@ -5,6 +5,8 @@ The kernels read x and the weight in 16-byte chunks of rows: rows of another ali
 no multiple of 8, are copied once into padded rows. Results, residuals and output gradients are read and
 written in place at any alignment."""
 
+import ctypes
+
 import torch
 import torch.nn.functional as F
 
@@ -42,9 +44,9 @@ def _pitch(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _linear(x, w, bias, side, outputs, activation, precision, *, dz=False, pad=False):
-    """One kernel over chunked rows ``x [M, K]`` and ``w [>= outputs, K]``; ``[M, outputs]``, with ``pad`` in
-    rows of a multiple of 8 columns, zeros behind."""
+def _linear(x, w, bias, side, outputs, activation, precision, *, dz=False, pad=False, transposed=False):
+    """One kernel over chunked rows ``x [M, K]`` and ``w [>= outputs, K]`` (``transposed``: ``[K, >= outputs]``);
+    ``[M, outputs]``, with ``pad`` in rows of a multiple of 8 columns, zeros behind."""
     M, K = x.shape
     cols = (outputs + 7) // 8 * 8 if pad else outputs
     out = torch.empty((M, cols), device=x.device, dtype=x.dtype)
@@ -52,7 +54,10 @@ def _linear(x, w, bias, side, outputs, activation, precision, *, dz=False, pad=F
     _lib.pack_linear(
         a, 0, x.data_ptr(), w.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if side is None else side.data_ptr(),
         out.data_ptr(), M, K, outputs, cols, _pitch(x), _pitch(w), 0 if side is None else _pitch(side), cols,
-        ACTIVATION_CODE[activation], dz, _lib.DTYPE_CODE[x.dtype], _lib.PRECISION_CODE[precision])
+        ACTIVATION_CODE[activation], dz, transposed, _lib.DTYPE_CODE[x.dtype], _lib.PRECISION_CODE[precision], 0)
+    if transposed and not _lib.load().gnn_linear_takes_transposed(ctypes.byref(a)):
+        w = _chunked(w[:, :outputs].t())
+        a.w, a.w_ld, a.w_transposed = w.data_ptr(), _pitch(w), 0
     _lib.call("gnn_linear", a, x.device)
     return out
 
@@ -91,14 +96,15 @@ def fused_linear_bwd_hip(x, weight, bias, activation, dy, *, precision, need_x=T
                      for t, need in zip(grads, (need_x, need_w, need_b)))
     dx = dw = db = None
     x2 = _chunked(x.reshape(M, I))
+    w2 = _chunked(weight)
     dz = _unit(dy.reshape(M, O))
     if activation is not None:
-        dz = _linear(x2, _chunked(weight), None if bias is None else bias.contiguous(), dz, O, activation, precision,
+        dz = _linear(x2, w2, None if bias is None else bias.contiguous(), dz, O, activation, precision,
                      dz=True, pad=True)
     elif need_x or need_w:
         dz = _chunked(dz)
     if need_x:
-        dx = _linear(dz, _chunked(weight.t()), None, None, I, None, precision).view(x.shape)
+        dx = _linear(dz, w2, None, None, I, None, precision, transposed=True).view(x.shape)
     segments = []
     if need_w:
         (part,) = rows_products_hip([(dz, x2)])

@@ -676,9 +676,14 @@ typedef struct gnn_linear_args {
   int64_t x_ld, w_ld, side_ld, out_ld;
   int32_t activation; /* enum gnn_activation */
   int32_t dz;
+  int32_t w_transposed;
   int32_t dtype;
   int32_t precision;
+  int32_t reserved;
 } gnn_linear_args;
+/* Whether this call could read w transposed, [I] rows of O (w_ld apart, O a multiple of 8): the input gradient's
+ * product takes the weight as it is then. gnn_linear refuses w_transposed where this is 0. */
+int gnn_linear_takes_transposed(const gnn_linear_args* args);
 int gnn_linear(const gnn_linear_args* args, void* stream);
 
 /* Sums over the rows of d [M, O] (pitch ld), as fp32 partial sums [parts][O] to be added with

@@ -19,9 +19,10 @@ def assert_within(name, got, want, slack):
     """``|got - want| <= half a step of got's type * |want| + slack``, elementwise; ``want`` and ``slack``
     float64. The smallest step of the type counts where values fall below its normal range."""
     assert got.shape == want.shape, f"{name}: {tuple(got.shape)} != {tuple(want.shape)}"
-    d = (got.double().cpu() - want.cpu()).abs()
+    got, slack = got.to(want.device), slack.to(want.device)
+    d = (got.double() - want).abs()
     info = torch.finfo(got.dtype)
-    bound = half_step(got.dtype) * want.abs().cpu() * (1 + 4 * U) + slack.cpu() * (1 + half_step(got.dtype))
+    bound = half_step(got.dtype) * want.abs() * (1 + 4 * U) + slack * (1 + half_step(got.dtype))
     bound = bound + info.tiny * info.eps
     bad = ~(d <= bound)
     if bad.any():

@@ -132,6 +132,41 @@ def test_forward_and_gradients(m, i, o, dtype):
         _run(m, i, o, dtype, act, (m + o) % 3 != 0, (m + i) % 2 == 0, seed=m + i + o)
 
 
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=IDS[:2])
+@pytest.mark.parametrize("m,i,o", [(32768, 128, 512), (32791, 40, 72), (40001, 256, 200), (33000, 512, 128), (33333, 400, 24),
+                                   (36865, 64, 1024), (33001, 136, 264), (35000, 576, 96), (33000, 16, 8),
+                                   (131072, 128, 128)])
+def test_many_rows(m, i, o, dtype):
+    """The pixels of a pair tensor, where the weight stays in LDS, in every direction of the layer."""
+    act = ACTS[(m + i + o) % 5]
+    for bias, residual in ((True, False), (False, True)):
+        x, w, b, r, dy = (None if t is None else t.to(DEV) for t in _inputs(m, i, o, dtype, bias, residual, seed=o))
+        exact = _exact(x, w, b, r, act, dy)
+        leaves = {n: t.clone().requires_grad_() for n, t in (("x", x), ("w", w), ("b", b)) if t is not None}
+        y = fused_linear(leaves["x"], leaves["w"], leaves.get("b"), act, r)
+        grads = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)))
+        assert_within(f"y {act}", y.detach(), *exact[0])
+        for n, (want, slack) in zip("xwb", exact[1:]):
+            if n in grads:
+                assert_within(f"d{n} {act}", grads[n], want, slack)
+
+
+def test_many_rows_leave_what_lies_behind():
+    """Rows behind the last one of a result inside a larger buffer stay as they were, and so do columns."""
+    from geometric_nn_ops_torch import _lib
+
+    m, i, o = 32768 + 5, 64, 40
+    x, w, _, _, _ = (None if t is None else t.to(DEV) for t in _inputs(m, i, o, torch.bfloat16, False, False))
+    out = torch.full((m + 40, o + 8), 7.0, device=DEV, dtype=torch.bfloat16)
+    a = _lib.LinearArgs()
+    _lib.pack_linear(a, 0, x.data_ptr(), w.data_ptr(), 0, 0, out.data_ptr(), m, i, o, o, i, i, 0, o + 8, 0, 0, 0,
+                     _lib.GNN_BF16, 0, 0)
+    _lib.call("gnn_linear", a, x.device)
+    want, slack = _exact(x, w, None, None, None)[0]
+    assert_within("y", out[:m, :o], want, slack)
+    assert (out[m:] == 7).all() and (out[:, o:] == 7).all()
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("act", ACTS)
 def test_every_activation(act, dtype):
