@@ -496,7 +496,7 @@ int gnn_relpos_bwd(const gnn_relpos_args* args, void* stream) {
 int gnn_linear(const gnn_linear_args* args, void* stream) {
   if (!args) return set_error(GNN_ERR_ARG, "fused_linear: args is NULL");
   const gnn_linear_args& a = *args;
-  if (!a.x || !a.w || !a.out || (a.dz && !a.side))
+  if (!a.x || !a.w || (!a.out && !a.dx) || (a.dz && !a.side))
     return set_error(GNN_ERR_ARG, "fused_linear: x, w, out and, for dz, the output gradient are required");
   if (!known_dtype(a.dtype)) return set_error(GNN_ERR_ARG, "fused_linear: unknown dtype");
   if (a.precision != GNN_PREC_IEEE && a.precision != GNN_PREC_BF16X3)
@@ -513,12 +513,16 @@ int gnn_linear(const gnn_linear_args* args, void* stream) {
     return set_error(GNN_ERR_ARG, "fused_linear: row pitches must cover their rows");
   if (!aligned(a.bias, e) || !aligned(a.side, e) || !aligned(a.out, e))
     return set_error(GNN_ERR_ARG, "fused_linear: tensors must be aligned to their elements");
+  if (a.dx && !linear_takes_dx(a))
+    return set_error(GNN_ERR_UNSUPPORTED, "fused_linear: this call does not take dx");
   if (a.w_transposed && !linear_takes_transposed(a))
     return set_error(GNN_ERR_UNSUPPORTED, "fused_linear: this call does not take a transposed weight");
   int rc = linear(a, (hipStream_t)stream);
   if (rc < 0) return rc;
   return hip_status((hipError_t)rc, "fused_linear");
 }
+
+int gnn_linear_takes_dx(const gnn_linear_args* args) { return args && args->dx && linear_takes_dx(*args) ? 1 : 0; }
 
 int gnn_linear_takes_transposed(const gnn_linear_args* args) { return args && linear_takes_transposed(*args) ? 1 : 0; }
 

@@ -191,6 +191,8 @@ __global__ __launch_bounds__(256) void column_sums_kernel(const T* d, int64_t ld
 
 }  // namespace
 
+bool linear_takes_dx(const gnn_linear_args& g) { return linear_resident_takes_dx(g); }
+
 bool linear_takes_transposed(const gnn_linear_args& g) { return linear_resident_applicable(g); }
 
 int linear(const gnn_linear_args& g, hipStream_t st) {

@@ -66,6 +66,7 @@ int reduce_parts(const gnn_reduce_args& a, hipStream_t stream);
 
 int linear(const gnn_linear_args& a, hipStream_t stream);
 bool linear_takes_transposed(const gnn_linear_args& a);
+bool linear_takes_dx(const gnn_linear_args& a);
 int64_t column_sums_parts(int64_t M, int64_t O);
 int column_sums(const gnn_column_sums_args& a, hipStream_t stream);
 int relpos(const gnn_relpos_args& a, bool backward, hipStream_t stream);

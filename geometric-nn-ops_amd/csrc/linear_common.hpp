@@ -112,6 +112,8 @@ struct LinArgs {
   int out_cols;  // columns written, zeros from O on
   int act;
   bool dz;  // out = side * act'(z) instead of act(z) + side
+  void* dx;  // with dz, or NULL: out W
+  int64_t dx_ld;
 };
 
 // 8 consecutive elements at any element's address, the first `left` of them
@@ -178,6 +180,7 @@ __device__ __forceinline__ void finish8(const LinArgs& a, const f32x8& z0, const
 
 // Kernels that keep the whole weight in LDS (16-bit types, many rows); false where a call is not theirs.
 bool linear_resident_applicable(const gnn_linear_args& a);
+bool linear_resident_takes_dx(const gnn_linear_args& a);
 int linear_resident(const gnn_linear_args& a, hipStream_t stream);
 
 }  // namespace gnn

@@ -26,8 +26,8 @@ using namespace lin;
 #ifndef GNN_RS_NT
 #define GNN_RS_NT 512
 #endif
-#ifndef GNN_RS_UNROLL
-#define GNN_RS_UNROLL 2
+#ifndef GNN_BWD_AHEAD
+#define GNN_BWD_AHEAD 4
 #endif
 constexpr int RS_LDS = 144 << 10;         // the weight and the bias, beside 2 KB a wave
 constexpr int64_t RS_MIN_ROWS = 1 << 15;  // below, filling LDS costs more than it saves
@@ -239,16 +239,16 @@ __global__ __launch_bounds__(NT, NT / 256) void linear_rows_kernel(const LinArgs
   for (; grp < groups; grp += step) {
     const auto srs = rows_rsrc<T>(a.side, grp * 32, a.M, a.side_ld, a.O);
     const auto ors = rows_rsrc<T>(a.out, grp * 32, a.M, a.out_ld, a.O);
-    u32x4_t side[2][2];  // of this pair of tiles
-    if (SIDE) {
-      sm.load(side[0], srs, 0);
-      sm.load(side[1], srs, 32);
-    }
+    u32x4_t side[2][2][2];  // of this pair of tiles and the next
+    auto load_side = [&](u32x4_t (&s)[2][2], int y) {
+      sm.load(s[0], srs, 32 * y);
+      sm.load(s[1], srs, 32 * (y + 1));
+    };
     // tiles by twos, whose 128-byte lines are stored at once
-    for (int y = 0; y < nb; y += 2) {
+    auto pair = [&](int y, u32x4_t (&s)[2][2]) {
       u32x4_t o[2][2];
       f32x16 ahead = tile(y + 1);  // zeros past the last: the weight's rows are padded to pairs
-      finish(acc, side[0], o[0]);
+      finish(acc, s[0], o[0]);
       acc = ahead;
       if (y + 2 < nb) {
         ahead = tile(y + 2);
@@ -258,14 +258,153 @@ __global__ __launch_bounds__(NT, NT / 256) void linear_rows_kernel(const LinArgs
         if (AHEAD) load_rows(next, grp + 2 * step);
         ahead = tile(0);
       }
-      finish(acc, side[1], o[1]);
+      finish(acc, s[1], o[1]);
       acc = ahead;
       om.store(o[0], ors, 32 * y);
       om.store(o[1], ors, 32 * (y + 1));
-      if (SIDE) {
-        sm.load(side[0], srs, 32 * (y + 2));
-        sm.load(side[1], srs, 32 * (y + 3));
+      if (SIDE) load_side(s, y + 4);
+    };
+    if (SIDE) {
+      load_side(side[0], 0);
+      load_side(side[1], 2);
+    }
+    for (int y = 0; y < nb; y += 4) {
+      pair(y, side[0]);
+      if (y + 2 < nb) pair(y + 2, side[1]);
+    }
+  }
+}
+
+// The activation's gradient and the input's in one pass: dz = dy act'(z) is written for the weight's gradient,
+// and goes on from the registers into dx = dz W. A tile of dz, 8 consecutive outputs a lane, is an operand
+// fragment of that product as it stands; W's columns for it come from the same LDS image by ds_read_b64_tr_b16
+// (4 rows of 16 columns each), the columns in tile_output's order again. Beside dz kept and read back, this
+// saves the read of dz and a launch.
+template <typename T, int KS, int ACT, int NT>
+__global__ __launch_bounds__(NT, NT / 256) void linear_rows_bwd_kernel(const LinArgs a, int) {
+  typedef typename TypeOps<T>::V8 V8;
+  typedef typename TypeOps<T>::V4 V4;
+  typedef short v4i16 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
+  extern __shared__ __align__(16) unsigned char smem[];
+  constexpr int ROWB = 32 * KS, KB = KS / 2;
+  const int nb = (a.O + 31) / 32;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
+  unsigned char* const weight = smem + NT / 64 * TURN;
+  fill_weight<T, NT>(weight, a, false, 64 * ((nb + 1) / 2), ROWB);
+  const float* bias = (const float*)(weight + 64 * ((nb + 1) / 2) * ROWB);
+  __syncthreads();
+  const Turn turn(smem + wave * TURN, lane);
+  const MemOrder xm(a.x_ld, a.I, lane), sm(a.side_ld, a.O, lane), om(a.out_ld, a.O, lane), dm(a.dx_ld, a.I, lane);
+  const int64_t groups = (a.M + 31) / 32, step = (int64_t)gridDim.x * (NT / 64);
+  const unsigned char* wrow[KS];
+#pragma unroll
+  for (int kk = 0; kk < KS; ++kk) wrow[kk] = weight + l32 * ROWB + (((2 * kk + g) ^ (l32 & 7)) << 4);
+  // transposed reads: row 4 g + q (and 8 further), 4 columns of the 32 of block kb
+  const unsigned char* wcol[KB];
+  {
+    const int row = 4 * g + ((lane & 15) >> 2), m = lane & 3;
+    const int col = 16 * ((lane >> 4) & 1) + 4 * (2 * (m & 1) + (m >> 1));
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+      wcol[kb] = weight + row * ROWB + (((4 * kb + (col >> 3)) ^ row) << 4) + 2 * (col & 7);
+  }
+  auto column8 = [&](int kb, int row) {
+    V4 v[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+      v[b] = __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                        (lds_v4i16*)(__attribute__((address_space(3))) const unsigned char*)(
+                                            wcol[kb] + (row + 8 * b) * ROWB)));
+    return __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  auto load_rows = [&](u32x4_t (&x)[KS / 2][2], int64_t grp) {
+    const auto r = rows_rsrc<T>(a.x, grp * 32, a.M, a.x_ld, a.I);
+#pragma unroll
+    for (int p = 0; p < KS / 2; ++p) xm.load(x[p], r, 32 * p);
+  };
+  u32x4_t next[KS / 2][2], x[KS / 2][2];
+  auto turn_rows = [&]() {
+#pragma unroll
+    for (int p = 0; p < KS / 2; ++p) {
+      Turn::put(turn.to_mem, next[p]);
+      Turn::get(turn.to_rows, x[p]);
+    }
+  };
+  auto tile = [&](int y) {
+    f32x16 acc = bias_tile(bias + 32 * y, g);
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk)
+      Mma<T, PREC_NATIVE>::step(acc, *reinterpret_cast<const V8*>(wrow[kk] + y * 32 * ROWB),
+                                __builtin_bit_cast(V8, x[kk / 2][kk % 2]));
+    return acc;
+  };
+  constexpr bool AHEAD = KS <= GNN_BWD_AHEAD;  // beside the sums of dx, 8 steps leave no registers for the next rows
+  int64_t grp = (int64_t)blockIdx.x * (NT / 64) + wave;
+  load_rows(next, grp);
+  turn_rows();
+  f32x16 acc = tile(0);
+  for (; grp < groups; grp += step) {
+    const auto srs = rows_rsrc<T>(a.side, grp * 32, a.M, a.side_ld, a.O);
+    const auto ors = rows_rsrc<T>(a.out, grp * 32, a.out ? a.M : 0, a.out_ld, a.O);
+    const auto drs = rows_rsrc<T>(a.dx, grp * 32, a.M, a.dx_ld, a.I);
+    f32x16 dx[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dx[kb][r] = 0.f;
+    u32x4_t side[2][2][2];
+    auto load_side = [&](u32x4_t (&s)[2][2], int y) {
+      sm.load(s[0], srs, 32 * y);
+      sm.load(s[1], srs, 32 * (y + 1));
+    };
+    auto finish = [&](const f32x16& z, const u32x4_t (&side)[2], u32x4_t (&o)[2], int y) {
+      u32x4_t s[2];
+      Turn::put(turn.to_mem, side);
+      Turn::get(turn.to_rows, s);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) o[t] = finish16<T, EPI_DZ, ACT>(outputs8(z, t), s[t]);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+          Mma<T, PREC_NATIVE>::step(dx[kb], column8(kb, 32 * y + 16 * t), __builtin_bit_cast(V8, o[t]));
+      Turn::put(turn.to_rows, o);
+      Turn::get(turn.to_mem, o);
+    };
+    auto pair = [&](int y, u32x4_t (&s)[2][2]) {
+      u32x4_t o[2][2];
+      f32x16 ahead = tile(y + 1);
+      finish(acc, s[0], o[0], y);
+      acc = ahead;
+      if (y + 2 < nb) {
+        ahead = tile(y + 2);
+      } else {
+        if (!AHEAD) load_rows(next, grp + step);
+        turn_rows();
+        ahead = tile(0);
       }
+      finish(acc, s[1], o[1], y + 1);
+      acc = ahead;
+      om.store(o[0], ors, 32 * y);
+      om.store(o[1], ors, 32 * (y + 1));
+      load_side(s, y + 4);
+    };
+    load_side(side[0], 0);
+    load_side(side[1], 2);
+    if (AHEAD) load_rows(next, grp + step);
+    for (int y = 0; y < nb; y += 4) {
+      pair(y, side[0]);
+      if (y + 2 < nb) pair(y + 2, side[1]);
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      u32x4_t o[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) o[t] = finish16<T, EPI_ACT, GNN_ACT_NONE>(outputs8(dx[kb], t), o[t]);
+      Turn::put(turn.to_rows, o);
+      Turn::get(turn.to_mem, o);
+      dm.store(o, drs, 32 * kb);
     }
   }
 }
@@ -374,6 +513,15 @@ Kernel rows_kernel(int act) {
   }
 }
 
+int launch_fn(Kernel fn, int nt, const LinArgs& a, const Form& f, int transposed, hipStream_t st) {
+  const size_t lds = f.lds + nt / 64 * TURN;
+  if (lds > 64 * 1024) (void)hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  const int64_t groups = (a.M + 31) / 32;
+  const int64_t grid = std::min<int64_t>((groups + nt / 64 - 1) / (nt / 64), persistent_grid((const void*)fn, nt, lds));
+  hipLaunchKernelGGL(fn, dim3((uint32_t)grid), dim3(nt), lds, st, a, transposed);
+  return (int)hipGetLastError();
+}
+
 template <typename T, int EPI>
 int launch(const LinArgs& a, const Form& f, int transposed, hipStream_t st) {
   Kernel fn = nullptr;
@@ -387,17 +535,24 @@ int launch(const LinArgs& a, const Form& f, int transposed, hipStream_t st) {
     case 3: fn = linear_outputs_kernel<T, 3, EPI, 512>; break;
     default: fn = linear_outputs_kernel<T, 4, EPI, 512>; break;
   }
-  const size_t lds = f.lds + nt / 64 * TURN;
-  if (lds > 64 * 1024) (void)hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-  const int64_t groups = (a.M + 31) / 32;
-  const int64_t grid = std::min<int64_t>((groups + nt / 64 - 1) / (nt / 64), persistent_grid((const void*)fn, nt, lds));
-  hipLaunchKernelGGL(fn, dim3((uint32_t)grid), dim3(nt), lds, st, a, transposed);
-  return (int)hipGetLastError();
+  return launch_fn(fn, nt, a, f, transposed, st);
+}
+
+template <typename T, int KS, int NT>
+Kernel rows_bwd_kernel(int act) {
+  switch (act) {
+    case GNN_ACT_RELU: return linear_rows_bwd_kernel<T, KS, GNN_ACT_RELU, NT>;
+    case GNN_ACT_GELU: return linear_rows_bwd_kernel<T, KS, GNN_ACT_GELU, NT>;
+    case GNN_ACT_SILU: return linear_rows_bwd_kernel<T, KS, GNN_ACT_SILU, NT>;
+    default: return linear_rows_bwd_kernel<T, KS, GNN_ACT_SIGMOID, NT>;
+  }
 }
 
 template <typename T>
 int launch(const LinArgs& a, int transposed, hipStream_t st) {
   const Form f = form_for(a.I, a.O);
+  if (a.dx)
+    return launch_fn(f.ks == 4 ? rows_bwd_kernel<T, 4, 512>(a.act) : rows_bwd_kernel<T, 8, 512>(a.act), 512, a, f, 0, st);
   if (a.dz) return launch<T, EPI_DZ>(a, f, transposed, st);
   return a.side ? launch<T, EPI_ADD>(a, f, transposed, st) : launch<T, EPI_ACT>(a, f, transposed, st);
 }
@@ -410,8 +565,16 @@ bool linear_resident_applicable(const gnn_linear_args& a) {
          rows16(a.out, a.out_ld) && (!a.side || rows16(a.side, a.side_ld)) && form_for(a.I, a.O).lds != 0;
 }
 
+bool linear_resident_takes_dx(const gnn_linear_args& a) {
+  auto rows16 = [](const void* p, int64_t ld) { return ((uintptr_t)p % 16) == 0 && ld % 8 == 0 && ld < (1 << 24); };
+  const Form f = form_for(a.I, a.O);
+  return linear_resident_applicable(a) && (f.ks == 4 || f.ks == 8) && a.dz && a.activation != GNN_ACT_NONE &&
+         !a.w_transposed && rows16(a.dx, a.dx_ld);
+}
+
 int linear_resident(const gnn_linear_args& g, hipStream_t st) {
   LinArgs a{};
+  a.dx = g.dx, a.dx_ld = g.dx_ld;
   a.x = g.x, a.w = g.w, a.bias = g.bias, a.side = g.side, a.out = g.out;
   a.M = g.M, a.x_ld = g.x_ld, a.w_ld = g.w_ld, a.side_ld = g.side_ld, a.out_ld = g.out_ld;
   a.I = (int)g.I, a.O = (int)g.O, a.out_cols = (int)g.out_cols, a.act = g.activation, a.dz = g.dz != 0;

@@ -409,6 +409,8 @@ class LinearArgs(ctypes.Structure):
         ("w_ld", ctypes.c_int64),
         ("side_ld", ctypes.c_int64),
         ("out_ld", ctypes.c_int64),
+        ("dx", ctypes.c_void_p),
+        ("dx_ld", ctypes.c_int64),
         ("activation", ctypes.c_int32),
         ("dz", ctypes.c_int32),
         ("w_transposed", ctypes.c_int32),
@@ -563,6 +565,7 @@ _SIGNATURES = {
     "gnn_relpos_fwd": (ctypes.c_int, [ctypes.POINTER(RelposArgs), ctypes.c_void_p]),
     "gnn_relpos_parts": (ctypes.c_int64, [ctypes.POINTER(RelposArgs)]),
     "gnn_relpos_bwd": (ctypes.c_int, [ctypes.POINTER(RelposArgs), ctypes.c_void_p]),
+    "gnn_linear_takes_dx": (ctypes.c_int, [ctypes.POINTER(LinearArgs)]),
     "gnn_linear_takes_transposed": (ctypes.c_int, [ctypes.POINTER(LinearArgs)]),
     "gnn_linear": (ctypes.c_int, [ctypes.POINTER(LinearArgs), ctypes.c_void_p]),
     "gnn_column_sums_parts": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64]),

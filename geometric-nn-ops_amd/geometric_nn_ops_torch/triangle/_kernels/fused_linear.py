@@ -44,22 +44,30 @@ def _pitch(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _linear(x, w, bias, side, outputs, activation, precision, *, dz=False, pad=False, transposed=False):
+def _linear(x, w, bias, side, outputs, activation, precision, *, dz=False, pad=False, transposed=False,
+            want_dx=False):
     """One kernel over chunked rows ``x [M, K]`` and ``w [>= outputs, K]`` (``transposed``: ``[K, >= outputs]``);
-    ``[M, outputs]``, with ``pad`` in rows of a multiple of 8 columns, zeros behind."""
+    ``[M, outputs]``, with ``pad`` in rows of a multiple of 8 columns, zeros behind. With ``dz`` ``(out, dx)``,
+    dx None unless it is wanted and the kernel forms ``dx = out w`` in the same pass."""
     M, K = x.shape
     cols = (outputs + 7) // 8 * 8 if pad else outputs
     out = torch.empty((M, cols), device=x.device, dtype=x.dtype)
     a = _lib.LinearArgs()
     _lib.pack_linear(
         a, 0, x.data_ptr(), w.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if side is None else side.data_ptr(),
-        out.data_ptr(), M, K, outputs, cols, _pitch(x), _pitch(w), 0 if side is None else _pitch(side), cols,
+        out.data_ptr(), M, K, outputs, cols, _pitch(x), _pitch(w), 0 if side is None else _pitch(side), cols, 0, 0,
         ACTIVATION_CODE[activation], dz, transposed, _lib.DTYPE_CODE[x.dtype], _lib.PRECISION_CODE[precision], 0)
     if transposed and not _lib.load().gnn_linear_takes_transposed(ctypes.byref(a)):
         w = _chunked(w[:, :outputs].t())
         a.w, a.w_ld, a.w_transposed = w.data_ptr(), _pitch(w), 0
+    dx = None
+    if want_dx:
+        dx = torch.empty((M, K), device=x.device, dtype=x.dtype)
+        a.dx, a.dx_ld = dx.data_ptr(), K
+        if not _lib.load().gnn_linear_takes_dx(ctypes.byref(a)):
+            dx, a.dx = None, None
     _lib.call("gnn_linear", a, x.device)
-    return out
+    return (out, dx) if dz else out
 
 
 def fused_linear_hip(x, weight, bias=None, activation=None, residual=None, *, precision):
@@ -99,12 +107,14 @@ def fused_linear_bwd_hip(x, weight, bias, activation, dy, *, precision, need_x=T
     w2 = _chunked(weight)
     dz = _unit(dy.reshape(M, O))
     if activation is not None:
-        dz = _linear(x2, w2, None if bias is None else bias.contiguous(), dz, O, activation, precision,
-                     dz=True, pad=True)
+        b = None if bias is None else bias.contiguous()
+        dz, dx = _linear(x2, w2, b, dz, O, activation, precision, dz=True, pad=True, want_dx=need_x and I % 8 == 0)
     elif need_x or need_w:
         dz = _chunked(dz)
     if need_x:
-        dx = _linear(dz, w2, None, None, I, None, precision, transposed=True).view(x.shape)
+        if dx is None:
+            dx = _linear(dz, w2, None, None, I, None, precision, transposed=True)
+        dx = dx.view(x.shape)
     segments = []
     if need_w:
         (part,) = rows_products_hip([(dz, x2)])

@@ -674,6 +674,8 @@ typedef struct gnn_linear_args {
   void* out;
   int64_t M, I, O, out_cols;
   int64_t x_ld, w_ld, side_ld, out_ld;
+  void* dx;      /* with dz: the input's gradient out w, [M] rows of I, dx_ld apart, in the same pass; or NULL */
+  int64_t dx_ld;
   int32_t activation; /* enum gnn_activation */
   int32_t dz;
   int32_t w_transposed;
@@ -684,6 +686,9 @@ typedef struct gnn_linear_args {
 /* Whether this call could read w transposed, [I] rows of O (w_ld apart, O a multiple of 8): the input gradient's
  * product takes the weight as it is then. gnn_linear refuses w_transposed where this is 0. */
 int gnn_linear_takes_transposed(const gnn_linear_args* args);
+/* Whether this call, with dx and dx_ld set, could write dx too; gnn_linear refuses dx where this is 0. out may
+ * be NULL then. */
+int gnn_linear_takes_dx(const gnn_linear_args* args);
 int gnn_linear(const gnn_linear_args* args, void* stream);
 
 /* Sums over the rows of d [M, O] (pitch ld), as fp32 partial sums [parts][O] to be added with

@@ -159,8 +159,8 @@ def test_many_rows_leave_what_lies_behind():
     x, w, _, _, _ = (None if t is None else t.to(DEV) for t in _inputs(m, i, o, torch.bfloat16, False, False))
     out = torch.full((m + 40, o + 8), 7.0, device=DEV, dtype=torch.bfloat16)
     a = _lib.LinearArgs()
-    _lib.pack_linear(a, 0, x.data_ptr(), w.data_ptr(), 0, 0, out.data_ptr(), m, i, o, o, i, i, 0, o + 8, 0, 0, 0,
-                     _lib.GNN_BF16, 0, 0)
+    a.x, a.w, a.out = x.data_ptr(), w.data_ptr(), out.data_ptr()
+    a.M, a.I, a.O, a.out_cols, a.x_ld, a.w_ld, a.out_ld, a.dtype = m, i, o, o, i, i, o + 8, _lib.GNN_BF16
     _lib.call("gnn_linear", a, x.device)
     want, slack = _exact(x, w, None, None, None)[0]
     assert_within("y", out[:m, :o], want, slack)
