@@ -344,7 +344,15 @@ int64_t gnn_rows_product_slices(const gnn_rows_product_args* args) {
 
 int gnn_rows_product(const gnn_rows_product_args* args, void* stream) {
   if (int rc = check_rows_product(args, true)) return rc;
-  int rc = rows_product(*args, (hipStream_t)stream);
+  int rc = rows_product(*args, nullptr, (hipStream_t)stream);
+  if (rc < 0) return rc;
+  return hip_status((hipError_t)rc, "rows_product");
+}
+
+int gnn_rows_product_sums(const gnn_rows_product_args* args, float* sums, void* stream) {
+  if (int rc = check_rows_product(args, true)) return rc;
+  if (!sums || !aligned(sums, 4)) return set_error(GNN_ERR_ARG, "rows_product: sums is required, aligned to its elements");
+  int rc = rows_product(*args, sums, (hipStream_t)stream);
   if (rc < 0) return rc;
   return hip_status((hipError_t)rc, "rows_product");
 }

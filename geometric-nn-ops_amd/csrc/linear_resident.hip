@@ -26,9 +26,6 @@ using namespace lin;
 #ifndef GNN_RS_NT
 #define GNN_RS_NT 512
 #endif
-#ifndef GNN_BWD_AHEAD
-#define GNN_BWD_AHEAD 4
-#endif
 constexpr int RS_LDS = 144 << 10;         // the weight and the bias, beside 2 KB a wave
 constexpr int64_t RS_MIN_ROWS = 1 << 15;  // below, filling LDS costs more than it saves
 
@@ -323,11 +320,11 @@ __global__ __launch_bounds__(NT, NT / 256) void linear_rows_bwd_kernel(const Lin
 #pragma unroll
     for (int p = 0; p < KS / 2; ++p) xm.load(x[p], r, 32 * p);
   };
-  u32x4_t next[KS / 2][2], x[KS / 2][2];
+  u32x4_t x[KS / 2][2];
   auto turn_rows = [&]() {
 #pragma unroll
     for (int p = 0; p < KS / 2; ++p) {
-      Turn::put(turn.to_mem, next[p]);
+      Turn::put(turn.to_mem, x[p]);
       Turn::get(turn.to_rows, x[p]);
     }
   };
@@ -339,12 +336,12 @@ __global__ __launch_bounds__(NT, NT / 256) void linear_rows_bwd_kernel(const Lin
                                 __builtin_bit_cast(V8, x[kk / 2][kk % 2]));
     return acc;
   };
-  constexpr bool AHEAD = KS <= GNN_BWD_AHEAD;  // beside the sums of dx, 8 steps leave no registers for the next rows
-  int64_t grp = (int64_t)blockIdx.x * (NT / 64) + wave;
-  load_rows(next, grp);
-  turn_rows();
-  f32x16 acc = tile(0);
-  for (; grp < groups; grp += step) {
+  // Beside the sums of dx, no registers are left for the next rows or for two tiles at once: holding them
+  // spilled up to 232 bytes a lane (147456 x 128 -> 512, bf16: 133 us with the next rows, 102 with two tiles, 96
+  // without either)
+  for (int64_t grp = (int64_t)blockIdx.x * (NT / 64) + wave; grp < groups; grp += step) {
+    load_rows(x, grp);
+    turn_rows();
     const auto srs = rows_rsrc<T>(a.side, grp * 32, a.M, a.side_ld, a.O);
     const auto ors = rows_rsrc<T>(a.out, grp * 32, a.out ? a.M : 0, a.out_ld, a.O);
     const auto drs = rows_rsrc<T>(a.dx, grp * 32, a.M, a.dx_ld, a.I);
@@ -353,7 +350,7 @@ __global__ __launch_bounds__(NT, NT / 256) void linear_rows_bwd_kernel(const Lin
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) dx[kb][r] = 0.f;
-    u32x4_t side[2][2][2];
+    u32x4_t side[2][2];
     auto load_side = [&](u32x4_t (&s)[2][2], int y) {
       sm.load(s[0], srs, 32 * y);
       sm.load(s[1], srs, 32 * (y + 1));
@@ -374,29 +371,14 @@ __global__ __launch_bounds__(NT, NT / 256) void linear_rows_bwd_kernel(const Lin
     };
     auto pair = [&](int y, u32x4_t (&s)[2][2]) {
       u32x4_t o[2][2];
-      f32x16 ahead = tile(y + 1);
-      finish(acc, s[0], o[0], y);
-      acc = ahead;
-      if (y + 2 < nb) {
-        ahead = tile(y + 2);
-      } else {
-        if (!AHEAD) load_rows(next, grp + step);
-        turn_rows();
-        ahead = tile(0);
-      }
-      finish(acc, s[1], o[1], y + 1);
-      acc = ahead;
+      finish(tile(y), s[0], o[0], y);
+      finish(tile(y + 1), s[1], o[1], y + 1);
       om.store(o[0], ors, 32 * y);
       om.store(o[1], ors, 32 * (y + 1));
-      load_side(s, y + 4);
+      load_side(s, y + 2);
     };
-    load_side(side[0], 0);
-    load_side(side[1], 2);
-    if (AHEAD) load_rows(next, grp + step);
-    for (int y = 0; y < nb; y += 4) {
-      pair(y, side[0]);
-      if (y + 2 < nb) pair(y + 2, side[1]);
-    }
+    load_side(side, 0);
+    for (int y = 0; y < nb; y += 2) pair(y, side);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       u32x4_t o[2];

@@ -98,8 +98,12 @@ struct RowsProductGrid {
   int64_t rps;                   // rows per slice
 };
 
-template <typename T>
-__global__ __launch_bounds__(RP_NT, RP_WGS) void rows_product_kernel(const gnn_rows_product_args a, const RowsProductGrid G) {
+// SUMS: the first product's column sums of d beside it, sums[slice][O]: on the matrix unit as one more product,
+// with ones, of the fragments that the first 128 columns of t already hold in registers (fp32: added up there),
+// in the waves of their first half. A pass of its own over d took 23 us of 151 MB.
+template <typename T, bool SUMS>
+__global__ __launch_bounds__(RP_NT, RP_WGS) void rows_product_kernel(const gnn_rows_product_args a, const RowsProductGrid G,
+                                                                    float* sums) {
   typedef RowsProduct<T> Cfg;
   __shared__ __align__(16) unsigned char smem[Cfg::LDS];
   const uint32_t w = xcd_remap(blockIdx.x, gridDim.x);
@@ -146,6 +150,14 @@ __global__ __launch_bounds__(RP_NT, RP_WGS) void rows_product_kernel(const gnn_r
     for (int y = 0; y < 2; ++y)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[x][y][r] = odd[x][y][r] = 0.f;
+
+  const bool summing = SUMS && pi == 0 && i0 == 0 && wn == 0;  // uniform in a wave
+  f32x16 sum16[2];
+  float sum32[2] = {0.f, 0.f};
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sum16[x][r] = 0.f;
 
 #pragma unroll
   for (int st = 0; st < Cfg::STAGES - 1; ++st)
@@ -194,6 +206,14 @@ __global__ __launch_bounds__(RP_NT, RP_WGS) void rows_product_kernel(const gnn_r
         for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int y = 0; y < 2; ++y) Mma<T, PREC_NATIVE>::step(acc[x][y], xf[kk][x], yf[kk][y]);
+      if (summing) {
+        const f32x8 one = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+        const V8 ones = TypeOps<T>::from_f32(one);
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) Mma<T, PREC_NATIVE>::step(sum16[x], xf[kk][x], ones);
+      }
     } else {
       // rows 2 kk + g: column 32 b + l32; the 128-byte block b of an odd row sits in the other half
       const int off = g * Cfg::ROWB + 4 * l32;
@@ -218,6 +238,33 @@ __global__ __launch_bounds__(RP_NT, RP_WGS) void rows_product_kernel(const gnn_r
             f32x16& s = kk % 2 ? odd[x][y] : acc[x][y];
             s = __builtin_amdgcn_mfma_f32_32x32x2f32(xf[kk][x], yf[kk][y], s, 0, 0, 0);
           }
+      if (summing) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {  // a stage's rows in a tree of their own
+          float s = 0.f;
+#pragma unroll
+          for (int kk = 0; kk < KS; ++kk) s += xf[kk][x];
+          sum32[x] += s;
+        }
+      }
+    }
+  }
+
+  if (summing) {
+    float* out = sums + slice * O;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int o = o0 + 64 * wm + 32 * x;
+      if constexpr (sizeof(T) == 4) {  // rows of one parity a lane half, column l32
+        const float s = pair_sum(sum32[x]);
+        if (g == 0 && o + l32 < O) out[o + l32] = s;
+      } else if (l32 == 0) {  // every column of the product holds the sums
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int n = o + 8 * (r / 4) + 4 * g + (r % 4);
+          if (n < O) out[n] = sum16[x][r];
+        }
+      }
     }
   }
 
@@ -324,17 +371,22 @@ int64_t rows_product_slices(const gnn_rows_product_args& a) {
   return (a.rows + G.rps - 1) / G.rps;
 }
 
-int rows_product(const gnn_rows_product_args& a, hipStream_t st) {
+template <bool SUMS>
+static int rows_product(const gnn_rows_product_args& a, float* sums, hipStream_t st) {
   const RowsProductGrid G = rows_product_grid(a);
   const int64_t nblk = (a.rows + G.rps - 1) / G.rps * G.total;
   if (nblk >= ((int64_t)1 << 31)) return set_error(GNN_ERR_UNSUPPORTED, "rows_product: grid too large");
   const dim3 grid((uint32_t)nblk), blk(RP_NT);
   switch (a.dtype) {
-    case GNN_BF16: hipLaunchKernelGGL(rows_product_kernel<bf16>, grid, blk, 0, st, a, G); break;
-    case GNN_F16: hipLaunchKernelGGL(rows_product_kernel<f16>, grid, blk, 0, st, a, G); break;
-    default: hipLaunchKernelGGL(rows_product_kernel<float>, grid, blk, 0, st, a, G); break;
+    case GNN_BF16: hipLaunchKernelGGL((rows_product_kernel<bf16, SUMS>), grid, blk, 0, st, a, G, sums); break;
+    case GNN_F16: hipLaunchKernelGGL((rows_product_kernel<f16, SUMS>), grid, blk, 0, st, a, G, sums); break;
+    default: hipLaunchKernelGGL((rows_product_kernel<float, SUMS>), grid, blk, 0, st, a, G, sums); break;
   }
   return (int)hipGetLastError();
+}
+
+int rows_product(const gnn_rows_product_args& a, float* sums, hipStream_t st) {
+  return sums ? rows_product<true>(a, sums, st) : rows_product<false>(a, nullptr, st);
 }
 
 int reduce_parts(const gnn_reduce_args& a, hipStream_t st) {

@@ -11,7 +11,7 @@ import torch
 import torch.nn.functional as F
 
 from ... import _lib
-from .trimul import reduce_parts_hip, rows_products_hip
+from .trimul import reduce_parts_hip
 
 ACTIVATION_CODE = {None: 0, "relu": 1, "gelu": 2, "silu": 3, "sigmoid": 4}
 MAX_WIDTH = 1 << 20
@@ -82,6 +82,26 @@ def fused_linear_hip(x, weight, bias=None, activation=None, residual=None, *, pr
     return _linear(_chunked(x.reshape(M, I)), _chunked(weight), bias, side, O, activation, precision).view(shape)
 
 
+def _weight_grad(dz, x, sums):
+    """fp32 partial sums of ``dz^T x`` and, with ``sums``, of dz's columns, over the same slices of rows."""
+    lib = _lib.load()
+    a = _lib.RowsProductArgs()
+    a.rows, a.count, a.dtype = dz.shape[0], 1, _lib.DTYPE_CODE[dz.dtype]
+    p, (O, I) = a.p[0], (dz.shape[1], x.shape[1])
+    p.d, p.t, p.d_ld, p.t_ld, p.O, p.I = dz.data_ptr(), x.data_ptr(), _pitch(dz), _pitch(x), O, I
+    slices = lib.gnn_rows_product_slices(ctypes.byref(a))
+    # that count depends on the device current here, the launch must not: pin its split
+    a.slice_rows = (-(-a.rows // slices) + 31) // 32 * 32
+    part = torch.empty((slices, O, I), device=dz.device, dtype=torch.float32)
+    p.partial = part.data_ptr()
+    if not sums:
+        _lib.call("gnn_rows_product", a, dz.device)
+        return part, None
+    sum_part = torch.empty((slices, O), device=dz.device, dtype=torch.float32)
+    _lib.call("gnn_rows_product_sums", a, dz.device, sum_part.data_ptr())
+    return part, sum_part
+
+
 def _column_sums(d, outputs):
     """fp32 partial sums ``[parts, outputs]`` over the rows of ``d``."""
     parts = _lib.load().gnn_column_sums_parts(d.shape[0], outputs)
@@ -117,12 +137,12 @@ def fused_linear_bwd_hip(x, weight, bias, activation, dy, *, precision, need_x=T
         dx = dx.view(x.shape)
     segments = []
     if need_w:
-        (part,) = rows_products_hip([(dz, x2)])
+        part, sum_part = _weight_grad(dz, x2, need_b)
         dw = torch.empty(part.shape[1:], device=x.device, dtype=x.dtype)
         segments.append((part, 0, dw.numel(), dw))
     if need_b:
         db = torch.empty((O,), device=x.device, dtype=x.dtype)
-        segments.append((_column_sums(dz, O), 0, O, db))
+        segments.append((sum_part if need_w else _column_sums(dz, O), 0, O, db))
     if segments:
         reduce_parts_hip(segments, x.device)
     if need_w and dw.shape != weight.shape:

@@ -553,6 +553,9 @@ typedef struct gnn_rows_product_args {
  * _reference/trimul.py:86-97); the reference has no kernel for them. */
 int64_t gnn_rows_product_slices(const gnn_rows_product_args* args);
 int gnn_rows_product(const gnn_rows_product_args* args, void* stream);
+/* The same, and the sums of the first product's d over the rows (a bias's gradient), as fp32 partial sums
+ * [slices][O]. */
+int gnn_rows_product_sums(const gnn_rows_product_args* args, float* sums, void* stream);
 
 /* dst[e] = sum over p < parts of src[p * stride + e] (e < n), in a fixed order, for up to
  * GNN_REDUCE_MAX segments in one launch; dst is in the segment's dtype. Adds the partials that

@@ -141,3 +141,34 @@ def test_args_match_the_c_layout(tmp_path):
     out = subprocess.run([str(tmp_path / "layout")], capture_output=True, text=True, check=True).stdout.split()
     want = [v for c in structs.values() for v in (ctypes.sizeof(c), *(getattr(c, f[0]).offset for f in c._fields_))]
     assert [int(v) for v in out] == want
+
+
+def test_product_with_sums_refuses_missing_sums():
+    lib = _lib.load()
+    a = _lib.RowsProductArgs()
+    a.rows, a.count, a.dtype = 64, 1, _lib.GNN_BF16
+    p = a.p[0]
+    p.d, p.t, p.partial, p.d_ld, p.t_ld, p.O, p.I = 4096, 8192, 4096, 32, 16, 32, 16
+    assert lib.gnn_rows_product_sums(None, None, None) == _lib.GNN_ERR_ARG
+    assert lib.gnn_rows_product_sums(ctypes.byref(a), None, None) == _lib.GNN_ERR_ARG
+    assert b"sums" in lib.gnn_last_error()
+    assert lib.gnn_rows_product_sums(ctypes.byref(a), 4098, None) == _lib.GNN_ERR_ARG
+
+
+def test_calls_that_take_a_transposed_weight_or_dx():
+    lib = _lib.load()
+    a = _lib.LinearArgs()
+    a.x = a.w = a.out = a.side = 4096
+    a.M, a.I, a.O, a.out_cols, a.x_ld, a.w_ld, a.side_ld, a.out_ld = 1 << 16, 128, 512, 512, 128, 128, 512, 512
+    a.dtype, a.dz, a.activation, a.dx, a.dx_ld = _lib.GNN_BF16, 1, 1, 4096, 128
+    assert lib.gnn_linear_takes_dx(ctypes.byref(a)) == 1 and lib.gnn_linear_takes_transposed(ctypes.byref(a)) == 1
+    for name, value in (("M", 64), ("dtype", _lib.GNN_F32), ("I", 512), ("dx", 4098), ("O", 516), ("activation", 0)):
+        was = getattr(a, name)
+        setattr(a, name, value)
+        assert lib.gnn_linear_takes_dx(ctypes.byref(a)) == 0, name
+        if name != "O" and name != "I":
+            assert lib.gnn_linear(ctypes.byref(a), None) in (_lib.GNN_ERR_ARG, _lib.GNN_ERR_UNSUPPORTED)
+        setattr(a, name, was)
+    a.M, a.dx, a.w_transposed, a.w_ld = 64, None, 1, 512
+    assert lib.gnn_linear(ctypes.byref(a), None) == _lib.GNN_ERR_UNSUPPORTED
+    assert b"transposed" in lib.gnn_last_error()
