@@ -458,8 +458,8 @@ static int check_relpos(const gnn_relpos_args* args) {
   if (a.B < 1 || a.U < 1 || a.V < 1 || a.H < 1 || a.buckets < 1 || a.B > most || a.U > most || a.V > most - 4096 ||
       a.H > most || a.V * a.H > most - 4096 || a.buckets > most / a.H)
     return set_error(GNN_ERR_ARG, "relative_position_bias: B, U, V, H and buckets must be positive, V H below 2^31");
-  if (a.max_distance < 1 || a.max_distance > (1 << 30))
-    return set_error(GNN_ERR_ARG, "relative_position_bias: max_distance must be in 1 .. 2^30");
+  if (a.max_distance < 1 || a.max_distance > (1 << 28))
+    return set_error(GNN_ERR_ARG, "relative_position_bias: max_distance must be in 1 .. 2^28");
   if (!a.log_spacing) {
     if (a.buckets != (a.two_sided ? 2 : 1) * a.max_distance + 1)
       return set_error(GNN_ERR_ARG, "relative_position_bias: clip needs 2 max_distance + 1 buckets, one-sided max_distance + 1");

@@ -161,9 +161,67 @@ int launch(const LinArgs& a, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
+// ---- few tiles ------------------------------------------------------------------------------
+// Single tokens and short sequences, whose 128 x 128 tiles would leave most CUs idle and whose time is the
+// latency of one pass over the weight: a workgroup takes 32 rows x 32 outputs and its FW_NW waves split the
+// contraction, each reading its fragments straight into registers, FW_AHEAD steps at a time; the partial sums
+// meet in LDS and are added in wave order. (1 x 384 -> 1536, bf16: 5 us; the 128 x 128 tiles took 13.)
+constexpr int FW_NW = 8, FW_NT = 64 * FW_NW, FW_AHEAD = 4;
+constexpr int FW_LD = 20;  // floats a lane's 16 sums take in LDS: 4 more keep the lanes on different banks
+
+template <typename T, int PREC>
+__global__ __launch_bounds__(FW_NT, 2) void linear_few_kernel(const LinArgs a) {
+  typedef typename TypeOps<T>::V8 V8;
+  __shared__ __align__(16) float part[FW_NW][64][FW_LD];
+  const uint32_t ntn = (uint32_t)(a.out_cols + 31) / 32;
+  const int n0 = (int)(blockIdx.x % ntn) * 32, m0 = (int)(blockIdx.x / ntn) * 32;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, g = lane >> 5;
+  // rows past the end repeat the last one; chunks past the contraction are zeros
+  const T* x = (const T*)a.x + min((int64_t)(m0 + l32), a.M - 1) * a.x_ld + 8 * g;
+  const T* w = (const T*)a.w + (int64_t)min(n0 + tile_output(l32), a.O - 1) * a.w_ld + 8 * g;
+  const int steps = (a.I + 15) / 16, each = (steps + FW_NW - 1) / FW_NW;
+  const int k0 = wave * each, k1 = min(steps, k0 + each);
+  f32x16 acc;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+  for (int k = k0; k < k1; k += FW_AHEAD) {
+    V8 xf[FW_AHEAD], wf[FW_AHEAD];
+#pragma unroll
+    for (int u = 0; u < FW_AHEAD; ++u) {
+      const bool in = k + u < k1 && 16 * (k + u) + 8 * g < a.I;
+      xf[u] = in ? load8_global(x + 16 * (k + u)) : zero8<T>();
+      wf[u] = in ? load8_global(w + 16 * (k + u)) : zero8<T>();
+    }
+#pragma unroll
+    for (int u = 0; u < FW_AHEAD; ++u) Mma<T, PREC>::step(acc, wf[u], xf[u]);
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    *reinterpret_cast<f32x4*>(&part[wave][lane][4 * q]) = f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+  __syncthreads();
+  if (threadIdx.x >= 128) return;
+  // 8 outputs 16 t + 8 g of a row a thread
+  const int t = threadIdx.x >> 6, n = n0 + 16 * t + 8 * g;
+  const int64_t m = m0 + l32;
+  if (m >= a.M || n >= a.out_cols) return;
+  f32x8 z = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < FW_NW; ++k) z += *reinterpret_cast<const f32x8*>(&part[k][lane][8 * t]);
+  f32x8 b = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (a.bias && n < a.O) b = load8_any((const T*)a.bias + n, a.O - n);
+  finish8<T>(a, z, b, m, n);
+}
+
 template <typename T, int PREC>
 int run(const LinArgs& a, hipStream_t st) {
-  return launch<T, PREC, Tile<T, 2, 2, 2, 2, 2>>(a, st);
+  typedef Tile<T, 2, 2, 2, 2, 2> Cfg;
+  const int64_t tiles = (a.M + Cfg::BM - 1) / Cfg::BM * ((a.out_cols + Cfg::BN - 1) / Cfg::BN);
+  if (tiles < compute_units() / 2) {
+    const int64_t few = (a.M + 31) / 32 * ((a.out_cols + 31) / 32);
+    hipLaunchKernelGGL((linear_few_kernel<T, PREC>), dim3((uint32_t)few), dim3(FW_NT), 0, st, a);
+    return (int)hipGetLastError();
+  }
+  return launch<T, PREC, Cfg>(a, st);
 }
 
 // ---- column sums ---------------------------------------------------------------------------

@@ -70,6 +70,33 @@ __device__ __forceinline__ int bucket_of(const Buckets& B, const int* border, in
   return B.two_sided && ahead > 0 ? B.n + side : side;
 }
 
+// The differences that lie in bucket t, unclamped: from .. to
+__device__ __forceinline__ void bucket_range(const Buckets& B, const int* border, int t, int& from, int& to) {
+  constexpr int ALL = 0x7fffffff;
+  if (!B.log) {
+    if (B.two_sided) {
+      from = t == 0 ? -ALL : t - B.far;
+      to = t == 2 * B.far ? ALL : t - B.far;
+    } else {
+      to = t == 0 ? ALL : -t;
+      from = t == B.far ? -ALL : -t;
+    }
+    return;
+  }
+  const bool up = B.two_sided && t >= B.n;
+  const int side = up ? t - B.n : t;
+  int d0 = side, d1 = side;  // distances d0 .. d1
+  if (side >= B.near) {
+    d0 = border[side - B.near];
+    d1 = border[side - B.near + 1] - 1;  // beyond every distance for the last bucket
+  }
+  if (side == B.n - 1) d1 = ALL;
+  if (up)
+    from = d0, to = d1;
+  else
+    from = -d1, to = !B.two_sided && side == 0 ? ALL : -d0;
+}
+
 struct RpArgs {
   const void* table;  // [buckets][H]
   const void* qpos;
@@ -127,12 +154,12 @@ __global__ __launch_bounds__(RP_NT) void relpos_fwd_kernel(const RpArgs a) {
   __shared__ int border[GNN_RELPOS_MAX_BORDERS + 2];
   const int nkey = (a.V + RP_NT * E - 1) / (RP_NT * E), nq = (a.U + a.rows - 1) / a.rows,
             nh = (a.H + a.heads - 1) / a.heads;
-  int64_t w = blockIdx.x;
-  const int h0 = (int)(w % nh) * a.heads;
-  w /= nh;
-  const int j = ((int)(w % nkey) * RP_NT + threadIdx.x) * E;
-  w /= nkey;
-  const int i0 = (int)(w % nq) * a.rows, b = (int)(w / nq);
+  uint32_t w = blockIdx.x;
+  const int h0 = (int)(w % (uint32_t)nh) * a.heads;
+  w /= (uint32_t)nh;
+  const int j = ((int)(w % (uint32_t)nkey) * RP_NT + threadIdx.x) * E;
+  w /= (uint32_t)nkey;
+  const int i0 = (int)(w % (uint32_t)nq) * a.rows, b = (int)(w / (uint32_t)nq);
   const int heads = min(a.heads, a.H - h0);
   load_borders(a, border);
   for (int e = threadIdx.x; e < heads * a.buckets; e += RP_NT) {
@@ -162,43 +189,65 @@ __global__ __launch_bounds__(RP_NT) void relpos_fwd_kernel(const RpArgs a) {
 }
 
 // A wave takes one head and a range of queries; its bins are [buckets of this pass][64 lanes]. A lane keeps
-// its 16 bytes of keys over the queries of a sequence, eight of which are read ahead. The group of keys
-// that it reads at once mostly falls into one bucket (see above) and is added as one.
+// its 16 bytes of keys over the queries of a sequence, eight of which are read ahead. Away from the diagonal
+// the group of keys stays in one bucket over many queries: the lane knows the differences that this bucket
+// holds and adds in a register until it is left (4 instructions a query beside the sum; two bucket_of a query
+// took 109 us of 134 MB). Where a group straddles buckets every key is looked up, in a table of all
+// differences where they are few. Differences run in 32 bits from a base that follows the queries.
 constexpr int RP_AHEAD = 8;
+constexpr int RP_LUT_FAR = 1023;           // differences looked up: 2 far + 1 16-bit entries
+constexpr int RP_FAR_BASE = 1 << 28;       // queries this far from the base move it
 template <typename T, typename P>
 __global__ __launch_bounds__(64) void relpos_bwd_kernel(const RpArgs a, int first, int count) {
   typedef typename Pack<T>::V V;
   constexpr int E = 16 / (int)sizeof(T);
   extern __shared__ __align__(16) unsigned char smem[];
   float* bins = (float*)smem;
+  uint16_t* lut = (uint16_t*)(bins + count * 64);
   __shared__ int border[GNN_RELPOS_MAX_BORDERS + 2];
   const int lane = threadIdx.x;
-  const int h = blockIdx.x % a.H, part = blockIdx.x / a.H;
+  const uint32_t h = blockIdx.x % (uint32_t)a.H, part = blockIdx.x / (uint32_t)a.H;
+  const int far = a.bk.far;
   load_borders(a, border);
   for (int t = 0; t < count; ++t) bins[t * 64 + lane] = 0.f;
   __syncthreads();
+  const bool looked_up = far <= RP_LUT_FAR;
+  if (looked_up) {
+    for (int d = lane; d <= 2 * far; d += 64) lut[d] = (uint16_t)bucket_of(a.bk, border, d - far);
+    __syncthreads();
+  }
+  auto bucket = [&](int ahead) {
+    const int d = max(-far, min(far, ahead));
+    return looked_up ? (int)lut[d + far] : bucket_of(a.bk, border, d);
+  };
   // one lane adds to a bin: the order is the program's
   auto add = [&](int t, float x) {
     t -= first;
     if ((unsigned)t < (unsigned)count)
       __hip_atomic_fetch_add(bins + t * 64 + lane, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
   };
-  const int64_t rows = (int64_t)a.B * a.U;
-  const int64_t r1 = min(rows, (int64_t)(part + 1) * a.rows);
-  for (int64_t r0 = (int64_t)part * a.rows; r0 < r1;) {
-    const int b = (int)(r0 / a.U), i0 = (int)(r0 - (int64_t)b * a.U);
-    const int i1 = (int)min<int64_t>(a.U, i0 + (r1 - r0));
+  const int rows = a.B * a.U;
+  const int r1 = min(rows, (int)(part + 1) * a.rows);
+  for (int r0 = (int)part * a.rows; r0 < r1;) {
+    const int b = r0 / a.U, i0 = r0 - b * a.U;
+    const int i1 = min(a.U, i0 + (r1 - r0));
     r0 += i1 - i0;
     const P* kp = (const P*)a.kpos + b * a.k_bstride;
     const P* qp = (const P*)a.qpos + b * a.q_bstride;
     const T* src = (const T*)a.dout + b * a.sb + (int64_t)h * a.sh;
     for (int j = lane * E; j < a.V; j += 64 * E) {
-      P k[E];
+      P base = qp[i0];
+      int k[E], lo, hi;  // from the base, saturated beyond any bucket's border
+      auto rebase = [&]() {
 #pragma unroll
-      for (int e = 0; e < E; ++e) k[e] = kp[min(j + e, a.V - 1)];
-      P lo = k[0], hi = k[0];
+        for (int e = 0; e < E; ++e) k[e] = ahead_of(kp[min(j + e, a.V - 1)], base, 1 << 30);
+        lo = hi = k[0];
 #pragma unroll
-      for (int e = 1; e < E; ++e) lo = min(lo, k[e]), hi = max(hi, k[e]);
+        for (int e = 1; e < E; ++e) lo = min(lo, k[e]), hi = max(hi, k[e]);
+      };
+      rebase();
+      int cur = 0, from = 1, to = 0;  // differences from .. to lie in bucket cur: none so far
+      float sum = 0.f;
       for (int i = i0; i < i1; i += RP_AHEAD) {
         V v[RP_AHEAD];
 #pragma unroll
@@ -207,18 +256,37 @@ __global__ __launch_bounds__(64) void relpos_bwd_kernel(const RpArgs a, int firs
         for (int u = 0; u < RP_AHEAD; ++u) {
           if (i + u >= i1) break;
           const P q = qp[i + u];
-          const int t = bucket_of(a.bk, border, ahead_of(lo, q, a.bk.far));
-          if (t == bucket_of(a.bk, border, ahead_of(hi, q, a.bk.far))) {
-            float s = 0.f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) s += (float)v[u][e];  // zeros past the last key
-            add(t, s);
-          } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e) add(bucket_of(a.bk, border, ahead_of(k[e], q, a.bk.far)), (float)v[u][e]);
+          int dq = ahead_of(q, base, RP_FAR_BASE);
+          if (abs(dq) == RP_FAR_BASE) {  // uniform
+            base = q;
+            dq = 0;
+            rebase();
           }
+          if (lo - dq < from || hi - dq > to) {
+            const int t = bucket(lo - dq);
+            if (cur != t || from > to) {
+              if (sum != 0.f) add(cur, sum);
+              sum = 0.f;
+            }
+            if (t == bucket(hi - dq)) {
+              cur = t;
+              bucket_range(a.bk, border, t, from, to);
+            } else {
+              if (sum != 0.f) add(cur, sum);
+              sum = 0.f;
+              from = 1, to = 0;
+#pragma unroll
+              for (int e = 0; e < E; ++e) add(bucket(k[e] - dq), (float)v[u][e]);
+              continue;
+            }
+          }
+          float s = 0.f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) s += (float)v[u][e];  // zeros past the last key
+          sum += s;
         }
       }
+      if (from <= to) add(cur, sum);
     }
   }
   __syncthreads();
@@ -245,21 +313,19 @@ __global__ __launch_bounds__(RP_NT) void relpos_last_fwd_kernel(const RpArgs a) 
   if (a.heads)
     for (int e = threadIdx.x; e < a.buckets * a.H; e += RP_NT) table[e] = gtable[e];
   __syncthreads();
-  const int64_t len = (int64_t)a.V * a.H;
-  const int64_t rows = (int64_t)a.B * a.U;
+  const int len = a.V * a.H;  // below 2^31, as the number of items is
   const bool whole = a.H % E == 0;
-  const int nseg = (int)((len + RP_NT * E - 1) / (RP_NT * E));
-  const int64_t items = rows * nseg;
-  for (int64_t w = blockIdx.x; w < items; w += gridDim.x) {
-    const int64_t r = w / nseg;
-    const int64_t x = ((w - r * nseg) * RP_NT + threadIdx.x) * E;
+  const uint32_t nseg = (uint32_t)(len + RP_NT * E - 1) / (RP_NT * E), items = (uint32_t)(a.B * a.U) * nseg;
+  for (uint32_t w = blockIdx.x; w < items; w += gridDim.x) {
+    const uint32_t r = w / nseg;
+    const int x = (int)((w - r * nseg) * RP_NT + threadIdx.x) * E;
     if (x >= len) continue;
-    const int b = (int)(r / a.U), i = (int)(r - (int64_t)b * a.U);
+    const int b = (int)(r / (uint32_t)a.U), i = (int)(r - (uint32_t)b * (uint32_t)a.U);
     const P* kp = (const P*)a.kpos + b * a.k_bstride;
     const P q = ((const P*)a.qpos)[b * a.q_bstride + i];
     T* out = (T*)a.out + b * a.sb + i * a.si + x;
     V v;
-    int j = (int)((uint32_t)x / (uint32_t)a.H), c = (int)x - j * a.H;
+    int j = (int)((uint32_t)x / (uint32_t)a.H), c = x - j * a.H;
     int t = bucket_of(a.bk, border, ahead_of(kp[j], q, a.bk.far));
     if (whole) {
       if (a.heads)
@@ -276,7 +342,7 @@ __global__ __launch_bounds__(RP_NT) void relpos_last_fwd_kernel(const RpArgs a) 
         }
       }
     }
-    store_pack(out, v, (int)min<int64_t>(E, len - x));
+    store_pack(out, v, min(E, len - x));
   }
 }
 
@@ -290,25 +356,24 @@ __global__ __launch_bounds__(256) void relpos_last_bwd_kernel(const RpArgs a, in
   typedef V2 V2U __attribute__((aligned(sizeof(T))));
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ int border[GNN_RELPOS_MAX_BORDERS + 2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int nc = (a.H + 127) / 128;
-  const int c0 = (int)(blockIdx.x % nc) * 128, part = blockIdx.x / nc;
+  const int c0 = (int)(blockIdx.x % (uint32_t)nc) * 128, part = blockIdx.x / (uint32_t)nc;
   float* bins = (float*)smem + wave * count * 128;
   load_borders(a, border);
   for (int t = 0; t < 2 * count; ++t) bins[t * 64 + lane] = 0.f;
   __syncthreads();
   const int c = c0 + 2 * lane;
   const bool has0 = c < a.H, has1 = c + 1 < a.H;
-  const int groups = (a.V + 63) / 64;
-  const int64_t items = (int64_t)a.B * a.U * groups;
-  const int64_t w0 = ((int64_t)part * waves + wave) * a.rows, w1 = min(items, w0 + a.rows);
+  const uint32_t groups = (uint32_t)(a.V + 63) / 64, items = (uint32_t)(a.B * a.U) * groups;
+  const uint32_t w0 = min(items, (uint32_t)(part * waves + wave) * (uint32_t)a.rows), w1 = min(items, w0 + (uint32_t)a.rows);
   float2* const mybins = (float2*)bins + lane;
   int cur = -1;
   float2 sum = {0.f, 0.f};
-  for (int64_t w = w0; w < w1; ++w) {
-    const int64_t r = w / groups;
+  for (uint32_t w = w0; w < w1; ++w) {
+    const uint32_t r = w / groups;
     const int j0 = (int)(w - r * groups) * 64;
-    const int b = (int)(r / a.U), i = (int)(r - (int64_t)b * a.U);
+    const int b = (int)(r / (uint32_t)a.U), i = (int)(r - (uint32_t)b * (uint32_t)a.U);
     const P* kp = (const P*)a.kpos + b * a.k_bstride;
     const P q = ((const P*)a.qpos)[b * a.q_bstride + i];
     const T* src = (const T*)a.dout + b * a.sb + i * a.si + c;
@@ -429,7 +494,8 @@ int backward(const gnn_relpos_args& g, hipStream_t st) {
   a.rows = (int)((bwd_items(g) + each - 1) / each);
   for (int first = 0; first < a.buckets; first += bins.count) {
     const int n = std::min(bins.count, a.buckets - first);
-    const size_t lds = (size_t)bins.waves * n * (bins.bytes / bins.count);
+    const size_t lds = (size_t)bins.waves * n * (bins.bytes / bins.count) +
+                       (!g.channels_last && a.bk.far <= RP_LUT_FAR ? 2 * (2 * a.bk.far + 2) : 0);
     if (lds > 64 * 1024)
       (void)hipFuncSetAttribute((const void*)relpos_last_bwd_kernel<T, P>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                 (int)lds);
@@ -453,6 +519,9 @@ int by_dtype(const gnn_relpos_args& g, bool bwd, hipStream_t st) {
 }  // namespace
 
 int relpos(const gnn_relpos_args& g, bool bwd, hipStream_t st) {
+  const int64_t most = (int64_t)1 << 31;
+  if (g.B * g.U >= most || (g.channels_last && g.B * g.U * ((g.V * g.H + 63) / 64 + 1) >= most))
+    return set_error(GNN_ERR_UNSUPPORTED, "relative_position_bias: more than 2^31 rows or pieces of rows");
   if (g.buckets > RP_MAX_BUCKETS)
     return set_error(GNN_ERR_UNSUPPORTED, "relative_position_bias: more than 4096 buckets");
   return g.pos_bytes == 8 ? by_dtype<int64_t>(g, bwd, st) : by_dtype<int32_t>(g, bwd, st);

@@ -17,9 +17,11 @@ MAX_BORDERS = 256  # logarithmic buckets of a side
 def supports(weight, query_pos, key_pos, max_distance, spacing, bidirectional) -> bool:
     """Whether the HIP kernels cover the call (dtype handled by the caller)."""
     buckets, heads = weight.shape
-    if buckets > MAX_BUCKETS or max_distance > 1 << 30:
+    if buckets > MAX_BUCKETS or max_distance > 1 << 28:
         return False
-    if max(key_pos.shape[1] * heads, query_pos.shape[1]) >= (1 << 31) - 4096:
+    # rows, and 64-element pieces of rows, are numbered in 32 bits
+    row, rows = key_pos.shape[1] * heads, query_pos.shape[0] * query_pos.shape[1]
+    if row >= (1 << 31) - 4096 or rows * ((row + 63) // 64 + 1) >= 1 << 31:
         return False
     if spacing == "clip":
         return True
