@@ -28,47 +28,53 @@ __device__ __forceinline__ void wait_vm_lgkm0() {
   __builtin_amdgcn_s_waitcnt(0x070 | (VM & 15) | ((VM >> 4) << 14));
 }
 
-// GM x GN waves of 32 X rows x 32 Y outputs
-template <typename T, int GM_, int GN_, int X_, int Y_, int STAGES_>
+// GM x GN waves of 32 X rows x 32 Y outputs; stages of ROWB bytes of a row
+template <typename T, int GM_, int GN_, int X_, int Y_, int ROWB_, int STAGES_>
 struct Tile {
-  static constexpr int GM = GM_, GN = GN_, X = X_, Y = Y_, STAGES = STAGES_;
+  static constexpr int GM = GM_, GN = GN_, X = X_, Y = Y_, ROWB = ROWB_, STAGES = STAGES_;
   static constexpr int BM = 32 * GM * X, BN = 32 * GN * Y;
   static constexpr int NW = GM * GN, NT = 64 * NW;
-  static constexpr int BK = 128 / (int)sizeof(T);  // elements of a row a stage
-  static constexpr int EPC = 16 / (int)sizeof(T);  // elements a chunk
-  static constexpr int QA = BM / 8 / NW, QB = BN / 8 / NW;  // DMA instructions a wave and stage
-  static constexpr int STAGE = (BM + BN) * 128;
+  static constexpr int BK = ROWB / (int)sizeof(T);  // elements of a row a stage
+  static constexpr int EPC = 16 / (int)sizeof(T);   // elements a chunk
+  static constexpr int CPR = ROWB / 16, RPI = 1024 / ROWB;        // chunks a row, rows a DMA instruction
+  static constexpr int QA = BM / RPI / NW, QB = BN / RPI / NW;    // DMA instructions a wave and stage
+  static constexpr int QPS = QA + QB;
+  static constexpr int STAGE = (BM + BN) * ROWB;
   static constexpr int LDS = STAGES * STAGE;
-  static_assert(QA * 8 * NW == BM && QB * 8 * NW == BN, "DMA split");
-  static_assert(STAGES == 2, "waits below");
+  static constexpr int WGS = (160 << 10) / LDS;  // workgroups a CU
+  static_assert(ROWB == 64 || ROWB == 128, "swizzle");
+  static_assert(QA * RPI * NW == BM && QB * RPI * NW == BN, "DMA split");
+  static_assert(STAGES >= 2 && STAGES <= 4 && NW * 4096 <= LDS, "waits and the epilogue's tiles");
+  // 8 rows read at once hit 8 bank groups: rows of 128 bytes by row % 8, of 64 by (row / 2) % 4
+  static __device__ __forceinline__ int swz(int row, int chunk) {
+    return chunk ^ (ROWB == 128 ? row & 7 : (row >> 1) & 3);
+  }
 };
 
 template <typename T, int PREC, typename Cfg>
-__global__ __launch_bounds__(Cfg::NT, Cfg::LDS <= (80 << 10) ? 2 * Cfg::NW / 4 : Cfg::NW / 4) void linear_kernel(
-    const LinArgs a) {
+__global__ __launch_bounds__(Cfg::NT, Cfg::WGS * Cfg::NW / 4) void linear_kernel(const LinArgs a) {
   typedef typename TypeOps<T>::V8 V8;
   __shared__ __align__(16) unsigned char smem[Cfg::LDS];
-  const int ntn = (a.out_cols + Cfg::BN - 1) / Cfg::BN;
+  const uint32_t ntn = (uint32_t)(a.out_cols + Cfg::BN - 1) / Cfg::BN;
   const uint32_t w = xcd_remap(blockIdx.x, gridDim.x);
-  const int n0 = (int)(w % (uint32_t)ntn) * Cfg::BN;
-  const int64_t m0 = (int64_t)(w / (uint32_t)ntn) * Cfg::BM;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l32 = lane & 31, g = lane >> 5;
+  const int n0 = (int)(w % ntn) * Cfg::BN;
+  const int64_t m0 = (int64_t)(w / ntn) * Cfg::BM;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
   const int wm = wave / Cfg::GN, wn = wave % Cfg::GN;
 
-  // DMA: an instruction moves 8 rows of 128 bytes; lane -> row lane / 8, stored chunk lane % 8, which holds
-  // the row's chunk (lane % 8) ^ (row % 8). Rows past the end repeat the last one (never stored), chunks
-  // past the contraction's end are zeros in both operands.
-  const int drow = lane >> 3, dchunk = (lane & 7) ^ drow;
+  // DMA: an instruction moves RPI rows; lane -> row lane / CPR, stored chunk lane % CPR, which holds the row's
+  // chunk swz(row, lane % CPR). Rows past the end repeat the last one (never stored), chunks past the
+  // contraction's end are zeros in both operands. Tiles of 32 of W's rows are in tile_output's order.
+  const int drow = lane / Cfg::CPR, dchunk = Cfg::swz(drow, lane % Cfg::CPR);
+  static_assert(Cfg::RPI % 8 == 0, "a row's swizzle is its row's within the instruction");
   const T* xsrc[Cfg::QA];
   const T* wsrc[Cfg::QB];
 #pragma unroll
   for (int q = 0; q < Cfg::QA; ++q)
-    xsrc[q] = (const T*)a.x + min(m0 + 8 * (Cfg::QA * wave + q) + drow, a.M - 1) * a.x_ld + dchunk * Cfg::EPC;
+    xsrc[q] = (const T*)a.x + min(m0 + Cfg::RPI * (Cfg::QA * wave + q) + drow, a.M - 1) * a.x_ld + dchunk * Cfg::EPC;
 #pragma unroll
-  for (int q = 0; q < Cfg::QB; ++q)
-    {
-    // tiles of 32 rows hold the outputs in tile_output's order
-    const int r = 8 * (Cfg::QB * wave + q) + drow, n = n0 + (r & ~31) + tile_output(r & 31);
+  for (int q = 0; q < Cfg::QB; ++q) {
+    const int r = Cfg::RPI * (Cfg::QB * wave + q) + drow, n = n0 + (r & ~31) + tile_output(r & 31);
     wsrc[q] = (const T*)a.w + (int64_t)min(n, a.O - 1) * a.w_ld + dchunk * Cfg::EPC;
   }
   const int nkt = (a.I + Cfg::BK - 1) / Cfg::BK;
@@ -83,16 +89,16 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::LDS <= (80 << 10) ? 2 * Cfg::NW / 4 :
 #pragma unroll
     for (int q = 0; q < Cfg::QB; ++q)
       __builtin_amdgcn_global_load_lds(in ? (const void*)(wsrc[q] + k0) : (const void*)zero_chunk,
-                                       (lds_void_t*)(st + Cfg::BM * 128 + (Cfg::QB * wave + q) * 1024), 16, 0, 0);
+                                       (lds_void_t*)(st + Cfg::BM * Cfg::ROWB + (Cfg::QB * wave + q) * 1024), 16, 0, 0);
   };
   // 8 elements kk * 16 + 8 g of a row
   auto frag = [&](const unsigned char* base, int r, int kk) -> V8 {
-    const unsigned char* row = base + r * 128;
+    const unsigned char* row = base + r * Cfg::ROWB;
     if constexpr (sizeof(T) == 2) {
-      return *reinterpret_cast<const V8*>(row + (((2 * kk + g) ^ (r & 7)) << 4));
+      return *reinterpret_cast<const V8*>(row + (Cfg::swz(r, 2 * kk + g) << 4));
     } else {
-      const f32x4 lo = *reinterpret_cast<const f32x4*>(row + (((4 * kk + 2 * g) ^ (r & 7)) << 4));
-      const f32x4 hi = *reinterpret_cast<const f32x4*>(row + (((4 * kk + 2 * g + 1) ^ (r & 7)) << 4));
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(row + (Cfg::swz(r, 4 * kk + 2 * g) << 4));
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(row + (Cfg::swz(r, 4 * kk + 2 * g + 1) << 4));
       return V8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     }
   };
@@ -106,17 +112,22 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::LDS <= (80 << 10) ? 2 * Cfg::NW / 4 :
       for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
 
 #pragma unroll
-  for (int s = 0; s < Cfg::STAGES; ++s)
+  for (int s = 0; s < Cfg::STAGES - 1; ++s)
     if (s < nkt) issue(s);
   for (int kt = 0; kt < nkt; ++kt) {
-    // this wave's DMA of stage kt has landed; after the barrier every wave's has
-    if (kt + 1 < nkt)
-      wait_vm_lgkm0<Cfg::QA + Cfg::QB>();
+    // this wave's DMA of stage kt has landed (the later stages' may be in flight) and its reads of stage kt - 1
+    // have returned; after the barrier every wave's have, and the buffer of stage kt - 1 is free
+    const int ahead = min(Cfg::STAGES - 2, nkt - 1 - kt);
+    if (Cfg::STAGES >= 4 && ahead >= 2)
+      wait_vm_lgkm0<2 * Cfg::QPS>();
+    else if (Cfg::STAGES >= 3 && ahead >= 1)
+      wait_vm_lgkm0<Cfg::QPS>();
     else
       wait_vm_lgkm0<0>();
     asm volatile("s_barrier" ::: "memory");
+    if (kt + Cfg::STAGES - 1 < nkt) issue(kt + Cfg::STAGES - 1);
     const unsigned char* sx = smem + (kt % Cfg::STAGES) * Cfg::STAGE;
-    const unsigned char* sw = sx + Cfg::BM * 128;
+    const unsigned char* sw = sx + Cfg::BM * Cfg::ROWB;
     constexpr int KS = Cfg::BK / 16;
 #pragma unroll
     for (int kk = 0; kk < KS; ++kk) {
@@ -130,32 +141,45 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::LDS <= (80 << 10) ? 2 * Cfg::NW / 4 :
 #pragma unroll
         for (int y = 0; y < Cfg::Y; ++y) Mma<T, PREC>::step(acc[x][y], wf[y], xf[x]);
     }
-    if (kt + Cfg::STAGES < nkt) {
-      // every wave's reads of the stage have returned: its buffer takes the stage after the next
-      wait_vm_lgkm0<Cfg::QA + Cfg::QB>();
-      asm volatile("s_barrier" ::: "memory");
-      issue(kt + Cfg::STAGES);
-    }
   }
 
+  // A lane's sums are one row's: stored like that, neighbouring lanes would write 16 bytes each to different
+  // rows. Every 32 x 32 tile turns through 4 KB of LDS of the wave's own (fp32, 16-byte chunks XOR-swizzled by
+  // row % 8), and is finished with 4 lanes a row.
+  wait_vm_lgkm0<0>();
+  asm volatile("s_barrier" ::: "memory");
+  unsigned char* tile = smem + wave * 4096;
+  auto at = [&](int row, int chunk) { return reinterpret_cast<f32x4*>(tile + row * 128 + ((chunk ^ (row & 7)) << 4)); };
 #pragma unroll
-  for (int y = 0; y < Cfg::Y; ++y)
+  for (int y = 0; y < Cfg::Y; ++y) {
+    const int n = n0 + 32 * (Cfg::Y * wn + y) + 8 * (lane & 3);
+    f32x8 b = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (a.bias && n < a.O) b = load8_any((const T*)a.bias + n, a.O - n);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int n = n0 + 32 * (Cfg::Y * wn + y) + 16 * t + 8 * g;
-      f32x8 b = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (a.bias && n < a.O) b = load8_any((const T*)a.bias + n, a.O - n);
+    for (int x = 0; x < Cfg::X; ++x) {
 #pragma unroll
-      for (int x = 0; x < Cfg::X; ++x) {
-        const int64_t m = m0 + 32 * (Cfg::X * wm + x) + l32;
-        if (m < a.M && n < a.out_cols) finish8<T>(a, outputs8(acc[x][y], t), b, m, n);
+      for (int q = 0; q < 4; ++q)
+        *at(l32, 4 * (q / 2) + 2 * g + q % 2) = f32x4{acc[x][y][4 * q], acc[x][y][4 * q + 1], acc[x][y][4 * q + 2],
+                                                      acc[x][y][4 * q + 3]};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = 16 * i + (lane >> 2);
+        const f32x4 lo = *at(row, 2 * (lane & 3)), hi = *at(row, 2 * (lane & 3) + 1);
+        const int64_t m = m0 + 32 * (Cfg::X * wm + x) + row;
+        if (m < a.M && n < a.out_cols) finish8<T>(a, f32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, b, m, n);
       }
     }
+  }
+}
+
+template <typename Cfg>
+int64_t tiles_of(const LinArgs& a) {
+  return (a.M + Cfg::BM - 1) / Cfg::BM * ((a.out_cols + Cfg::BN - 1) / Cfg::BN);
 }
 
 template <typename T, int PREC, typename Cfg>
 int launch(const LinArgs& a, hipStream_t st) {
-  const int64_t tiles = (a.M + Cfg::BM - 1) / Cfg::BM * ((a.out_cols + Cfg::BN - 1) / Cfg::BN);
+  const int64_t tiles = tiles_of<Cfg>(a);
   if (tiles >= ((int64_t)1 << 31)) return set_error(GNN_ERR_UNSUPPORTED, "fused_linear: grid too large");
   hipLaunchKernelGGL((linear_kernel<T, PREC, Cfg>), dim3((uint32_t)tiles), dim3(Cfg::NT), 0, st, a);
   return (int)hipGetLastError();
@@ -212,16 +236,23 @@ __global__ __launch_bounds__(FW_NT, 2) void linear_few_kernel(const LinArgs a) {
   finish8<T>(a, z, b, m, n);
 }
 
+#ifndef GNN_LIN_FORCE
+#define GNN_LIN_FORCE 0
+#endif
 template <typename T, int PREC>
 int run(const LinArgs& a, hipStream_t st) {
-  typedef Tile<T, 2, 2, 2, 2, 2> Cfg;
-  const int64_t tiles = (a.M + Cfg::BM - 1) / Cfg::BM * ((a.out_cols + Cfg::BN - 1) / Cfg::BN);
-  if (tiles < compute_units() / 2) {
-    const int64_t few = (a.M + 31) / 32 * ((a.out_cols + 31) / 32);
-    hipLaunchKernelGGL((linear_few_kernel<T, PREC>), dim3((uint32_t)few), dim3(FW_NT), 0, st, a);
-    return (int)hipGetLastError();
+  typedef Tile<T, 2, 2, 1, 1, 128, 4> Small;
+  typedef Tile<T, 2, 2, 2, 2, 128, 4> Medium;
+  const int64_t cus = compute_units();
+  if constexpr (sizeof(T) == 2) {
+    typedef Tile<T, 2, 4, 4, 2, 64, 4> Large;
+    if (GNN_LIN_FORCE == 3 || (GNN_LIN_FORCE == 0 && tiles_of<Large>(a) >= cus)) return launch<T, PREC, Large>(a, st);
   }
-  return launch<T, PREC, Cfg>(a, st);
+  if (GNN_LIN_FORCE == 2 || (GNN_LIN_FORCE == 0 && tiles_of<Medium>(a) >= cus)) return launch<T, PREC, Medium>(a, st);
+  if (GNN_LIN_FORCE == 1 || (GNN_LIN_FORCE == 0 && tiles_of<Small>(a) >= cus / 2)) return launch<T, PREC, Small>(a, st);
+  const int64_t few = (a.M + 31) / 32 * ((a.out_cols + 31) / 32);
+  hipLaunchKernelGGL((linear_few_kernel<T, PREC>), dim3((uint32_t)few), dim3(FW_NT), 0, st, a);
+  return (int)hipGetLastError();
 }
 
 // ---- column sums ---------------------------------------------------------------------------
