@@ -5,9 +5,9 @@
 // The backward forms z again from x and W instead of keeping it: in 16 bits, z would put a second rounding
 // under every gradient, and in fp32 it would cost 4 M O bytes written and read.
 //
-// linear_kernel. BM x BN output tiles, the contraction in stages of 128 bytes a row, both operands moved by
-// global_load_lds into LDS (STAGES of them in flight) with the 16-byte chunks of row r XOR-swizzled by r % 8,
-// so that the fragment reads of 8 rows hit 8 bank groups. The products are formed transposed (W's rows as the
+// linear_kernel. BM x BN output tiles, the contraction in stages of 64 or 128 bytes a row, both operands moved by
+// global_load_lds into LDS (STAGES - 1 of them in flight, one barrier a stage) in 16-byte chunks whose order
+// within a row the source addresses permute (chunk_swizzle). The products are formed transposed (W's rows as the
 // rows of the 32x32 MFMA tile, in an order that leaves a lane 8 consecutive outputs of one row of x): these
 // take bias, activation and residual in fp32, round once and leave as one 16-byte store (two in fp32). Workgroups that share rows of x
 // follow each other on one XCD, whose L2 then serves x.
@@ -45,10 +45,7 @@ struct Tile {
   static_assert(ROWB == 64 || ROWB == 128, "swizzle");
   static_assert(QA * RPI * NW == BM && QB * RPI * NW == BN, "DMA split");
   static_assert(STAGES >= 2 && STAGES <= 4 && NW * 4096 <= LDS, "waits and the epilogue's tiles");
-  // 8 rows read at once hit 8 bank groups: rows of 128 bytes by row % 8, of 64 by (row / 2) % 4
-  static __device__ __forceinline__ int swz(int row, int chunk) {
-    return chunk ^ (ROWB == 128 ? row & 7 : (row >> 1) & 3);
-  }
+  static __device__ __forceinline__ int swz(int row, int chunk) { return chunk ^ chunk_swizzle<ROWB>(row); }
 };
 
 template <typename T, int PREC, typename Cfg>
@@ -65,31 +62,35 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::WGS * Cfg::NW / 4) void linear_kernel
   // DMA: an instruction moves RPI rows; lane -> row lane / CPR, stored chunk lane % CPR, which holds the row's
   // chunk swz(row, lane % CPR). Rows past the end repeat the last one (never stored), chunks past the
   // contraction's end are zeros in both operands. Tiles of 32 of W's rows are in tile_output's order.
-  const int drow = lane / Cfg::CPR, dchunk = Cfg::swz(drow, lane % Cfg::CPR);
-  static_assert(Cfg::RPI % 8 == 0, "a row's swizzle is its row's within the instruction");
+  const int drow = lane / Cfg::CPR, dpos = lane % Cfg::CPR;
   const T* xsrc[Cfg::QA];
   const T* wsrc[Cfg::QB];
 #pragma unroll
-  for (int q = 0; q < Cfg::QA; ++q)
-    xsrc[q] = (const T*)a.x + min(m0 + Cfg::RPI * (Cfg::QA * wave + q) + drow, a.M - 1) * a.x_ld + dchunk * Cfg::EPC;
+  for (int q = 0; q < Cfg::QA; ++q) {
+    const int r = Cfg::RPI * (Cfg::QA * wave + q) + drow;
+    xsrc[q] = (const T*)a.x + min(m0 + r, a.M - 1) * a.x_ld;
+  }
 #pragma unroll
   for (int q = 0; q < Cfg::QB; ++q) {
     const int r = Cfg::RPI * (Cfg::QB * wave + q) + drow, n = n0 + (r & ~31) + tile_output(r & 31);
-    wsrc[q] = (const T*)a.w + (int64_t)min(n, a.O - 1) * a.w_ld + dchunk * Cfg::EPC;
+    wsrc[q] = (const T*)a.w + (int64_t)min(n, a.O - 1) * a.w_ld;
   }
   const int nkt = (a.I + Cfg::BK - 1) / Cfg::BK;
   auto issue = [&](int kt) {
     unsigned char* st = smem + (kt % Cfg::STAGES) * Cfg::STAGE;
     const int k0 = kt * Cfg::BK;
-    const bool in = k0 + dchunk * Cfg::EPC < a.I;
 #pragma unroll
-    for (int q = 0; q < Cfg::QA; ++q)
-      __builtin_amdgcn_global_load_lds(in ? (const void*)(xsrc[q] + k0) : (const void*)zero_chunk,
-                                       (lds_void_t*)(st + (Cfg::QA * wave + q) * 1024), 16, 0, 0);
+    for (int q = 0; q < Cfg::QA; ++q) {
+      const int k = k0 + Cfg::swz(Cfg::RPI * (Cfg::QA * wave + q) + drow, dpos) * Cfg::EPC;
+      const void* src = k < a.I ? (const void*)(xsrc[q] + k) : (const void*)zero_chunk;
+      __builtin_amdgcn_global_load_lds(src, (lds_void_t*)(st + (Cfg::QA * wave + q) * 1024), 16, 0, 0);
+    }
 #pragma unroll
-    for (int q = 0; q < Cfg::QB; ++q)
-      __builtin_amdgcn_global_load_lds(in ? (const void*)(wsrc[q] + k0) : (const void*)zero_chunk,
-                                       (lds_void_t*)(st + Cfg::BM * Cfg::ROWB + (Cfg::QB * wave + q) * 1024), 16, 0, 0);
+    for (int q = 0; q < Cfg::QB; ++q) {
+      const int k = k0 + Cfg::swz(Cfg::RPI * (Cfg::QB * wave + q) + drow, dpos) * Cfg::EPC;
+      const void* src = k < a.I ? (const void*)(wsrc[q] + k) : (const void*)zero_chunk;
+      __builtin_amdgcn_global_load_lds(src, (lds_void_t*)(st + Cfg::BM * Cfg::ROWB + (Cfg::QB * wave + q) * 1024), 16, 0, 0);
+    }
   };
   // 8 elements kk * 16 + 8 g of a row
   auto frag = [&](const unsigned char* base, int r, int kk) -> V8 {
@@ -145,11 +146,11 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::WGS * Cfg::NW / 4) void linear_kernel
 
   // A lane's sums are one row's: stored like that, neighbouring lanes would write 16 bytes each to different
   // rows. Every 32 x 32 tile turns through 4 KB of LDS of the wave's own (fp32, 16-byte chunks XOR-swizzled by
-  // row % 8), and is finished with 4 lanes a row.
+  // (row / 2) % 8), and is finished with 4 lanes a row.
   wait_vm_lgkm0<0>();
   asm volatile("s_barrier" ::: "memory");
   unsigned char* tile = smem + wave * 4096;
-  auto at = [&](int row, int chunk) { return reinterpret_cast<f32x4*>(tile + row * 128 + ((chunk ^ (row & 7)) << 4)); };
+  auto at = [&](int row, int chunk) { return reinterpret_cast<f32x4*>(tile + row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4)); };
 #pragma unroll
   for (int y = 0; y < Cfg::Y; ++y) {
     const int n = n0 + 32 * (Cfg::Y * wn + y) + 8 * (lane & 3);

@@ -13,6 +13,17 @@ typedef __attribute__((address_space(3))) void lds_void_t;
 // Source of the chunks that a DMA fills with zeros
 __device__ __attribute__((aligned(16))) const uint32_t zero_chunk[4] = {0u, 0u, 0u, 0u};
 
+// 16-byte chunk c of row r lies at chunk c ^ chunk_swizzle(r) of its row. LDS serves 16 lanes' chunks, 256
+// bytes, at once: the swizzle spreads 16 consecutive rows' chunk c over all of them, whatever a row's bytes
+// (8 rows over 128 bytes, r % 8, left two-fold conflicts), and also 4-chunk blocks of 8 rows, which the
+// transposed reads take.
+template <int ROWB>
+__device__ __forceinline__ int chunk_swizzle(int r) {
+  if constexpr (ROWB == 64) return (r >> 2) & 3;
+  if constexpr (ROWB == 128) return (r & 2) << 1 | ((r >> 2) & 3);
+  return (r & 3) << 2 | ((r >> 2) & 3);
+}
+
 // ---- activations ------------------------------------------------------------------------
 // 16-bit results: exp2 and rcp of the hardware (1 ulp each) and, for the normal distribution, Abramowitz and
 // Stegun 7.1.26: erfc(u) = t (a1 + t (a2 + ...)) exp(-u^2), t = 1 / (1 + 0.3275911 u), off by at most 1.5e-7;

@@ -2,8 +2,8 @@
 // a pair transition and the projections around it, which HBM bounds (128 -> 512 over 512^2 pixels: 336 MB
 // against 34 GFLOP).
 //
-// A workgroup of 8 waves loads the weight into LDS once, rows padded to whole 32x32 tiles with zeros and their
-// 16-byte chunks XOR-swizzled by row % 8 (fragment reads of 8 rows hit 8 bank groups), and stays. From there
+// A workgroup of 8 waves loads the weight into LDS once, rows padded to whole 32x32 tiles with zeros and
+// their 16-byte chunks in chunk_swizzle's order, and stays. From there
 // on every wave works alone, without a barrier: it takes 32 rows at a time (the next ones on their way while it
 // works on these) and multiplies. The products
 // are transposed, as in linear_kernel: a lane ends up with 8 consecutive outputs of one row. Rows and columns
@@ -42,7 +42,8 @@ __device__ __forceinline__ u32x4_t buffer_load16(__amdgpu_buffer_rsrc_t r, uint3
 // W [O][I] (or, transposed, W[n][k] at k ld + n) into rows of rowb bytes, in tiles of 32 in tile_output's order,
 // zeros past I and O; then the bias. As it is stored, the weight comes by global_load_lds, all of it in flight
 // at once (through registers, four loads at a time, this took 10 us more of a 128 KB weight).
-template <typename T, int NT>
+// SW: the rows' bytes, or 256 for any multiple
+template <typename T, int NT, int SW>
 __device__ __forceinline__ void fill_weight(unsigned char* smem, const LinArgs& a, bool transposed, int rows, int rowb) {
   typedef typename TypeOps<T>::V8 V8;
   const int cpr = rowb / 16;
@@ -50,7 +51,7 @@ __device__ __forceinline__ void fill_weight(unsigned char* smem, const LinArgs& 
   if (!transposed) {
     const int lane = threadIdx.x & 63;
     for (int e0 = (threadIdx.x >> 6) * 64; e0 < rows * cpr; e0 += NT) {  // 1 KB an instruction
-      const uint32_t e = e0 + lane, r = e / (uint32_t)cpr, c = (e - r * cpr) ^ (r & 7);
+      const uint32_t e = e0 + lane, r = e / (uint32_t)cpr, c = (e - r * cpr) ^ chunk_swizzle<SW>(r);
       const int n = (r & ~31) + tile_output(r & 31);
       const void* src = n < a.O && 8 * (int)c < a.I ? (const void*)(w + (int64_t)n * a.w_ld + 8 * c) : (const void*)zero_chunk;
       __builtin_amdgcn_global_load_lds(src, (lds_void_t*)(smem + 16 * e0), 16, 0, 0);
@@ -65,7 +66,7 @@ __device__ __forceinline__ void fill_weight(unsigned char* smem, const LinArgs& 
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int r = ((n + i) & ~31) + tile_row((n + i) & 31);
-        *reinterpret_cast<T*>(smem + r * rowb + (((k >> 3) ^ (r & 7)) << 4) + 2 * (k & 7)) = v[i];
+        *reinterpret_cast<T*>(smem + r * rowb + (((k >> 3) ^ chunk_swizzle<SW>(r)) << 4) + 2 * (k & 7)) = v[i];
       }
     }
   }
@@ -78,7 +79,7 @@ __device__ __forceinline__ void fill_weight(unsigned char* smem, const LinArgs& 
 // pipeline up (128 -> 512 over 512^2 rows: 100 us with the stores alone that way, 39 us is what the bytes
 // take). So a wave moves 32 x 64-byte tiles with 4 lanes a row ("memory order": access i of two, lane -> row
 // 16 i + lane / 4, chunk lane % 4) and turns them into or from the products' order (lane -> row lane % 32,
-// chunks 2 t + lane / 32) through 2 KB of LDS of its own, chunks XOR-swizzled by (row / 2) % 4. A wave's LDS
+// chunks 2 t + lane / 32) through 2 KB of LDS of its own, its chunks swizzled too. A wave's LDS
 // accesses stay in order: no wait is needed beyond the data's own.
 constexpr int TURN = 2048;
 struct Turn {
@@ -88,9 +89,9 @@ struct Turn {
     const int r = lane & 31, g = lane >> 5;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      to_rows[k] = tile + r * 64 + (((2 * k + g) ^ ((r >> 1) & 3)) << 4);
+      to_rows[k] = tile + r * 64 + (((2 * k + g) ^ chunk_swizzle<64>(r)) << 4);
       const int m = 16 * k + (lane >> 2);
-      to_mem[k] = tile + m * 64 + (((lane & 3) ^ ((m >> 1) & 3)) << 4);
+      to_mem[k] = tile + m * 64 + (((lane & 3) ^ chunk_swizzle<64>(m)) << 4);
     }
   }
   __device__ __forceinline__ static void put(unsigned char* const (&at)[2], const u32x4_t (&v)[2]) {
@@ -183,7 +184,7 @@ __global__ __launch_bounds__(NT, NT / 256) void linear_rows_kernel(const LinArgs
   const int nb = (a.O + 31) / 32;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
   unsigned char* const weight = smem + NT / 64 * TURN;
-  fill_weight<T, NT>(weight, a, transposed, 64 * ((nb + 1) / 2), ROWB);
+  fill_weight<T, NT, ROWB>(weight, a, transposed, 64 * ((nb + 1) / 2), ROWB);
   const float* bias = (const float*)(weight + 64 * ((nb + 1) / 2) * ROWB);
   __syncthreads();
   const Turn turn(smem + wave * TURN, lane);
@@ -196,7 +197,7 @@ __global__ __launch_bounds__(NT, NT / 256) void linear_rows_kernel(const LinArgs
   };
   const unsigned char* wrow[KS];
 #pragma unroll
-  for (int kk = 0; kk < KS; ++kk) wrow[kk] = weight + l32 * ROWB + (((2 * kk + g) ^ (l32 & 7)) << 4);
+  for (int kk = 0; kk < KS; ++kk) wrow[kk] = weight + l32 * ROWB + (((2 * kk + g) ^ chunk_swizzle<ROWB>(l32)) << 4);
   // The products of a tile run beside the epilogue of the one before it (of the last rows' last tile, where a
   // wave goes on to new rows): tile() starts a tile's sums, finish() ends the ones before.
   u32x4_t next[KS / 2][2], x[KS / 2][2];
@@ -288,7 +289,7 @@ __global__ __launch_bounds__(NT, NT / 256) void linear_rows_bwd_kernel(const Lin
   const int nb = (a.O + 31) / 32;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
   unsigned char* const weight = smem + NT / 64 * TURN;
-  fill_weight<T, NT>(weight, a, false, 64 * ((nb + 1) / 2), ROWB);
+  fill_weight<T, NT, ROWB>(weight, a, false, 64 * ((nb + 1) / 2), ROWB);
   const float* bias = (const float*)(weight + 64 * ((nb + 1) / 2) * ROWB);
   __syncthreads();
   const Turn turn(smem + wave * TURN, lane);
@@ -296,15 +297,18 @@ __global__ __launch_bounds__(NT, NT / 256) void linear_rows_bwd_kernel(const Lin
   const int64_t groups = (a.M + 31) / 32, step = (int64_t)gridDim.x * (NT / 64);
   const unsigned char* wrow[KS];
 #pragma unroll
-  for (int kk = 0; kk < KS; ++kk) wrow[kk] = weight + l32 * ROWB + (((2 * kk + g) ^ (l32 & 7)) << 4);
+  for (int kk = 0; kk < KS; ++kk) wrow[kk] = weight + l32 * ROWB + (((2 * kk + g) ^ chunk_swizzle<ROWB>(l32)) << 4);
   // transposed reads: row 4 g + q (and 8 further), 4 columns of the 32 of block kb
-  const unsigned char* wcol[KB];
+  const unsigned char* wcol[2][KB];
   {
     const int row = 4 * g + ((lane & 15) >> 2), m = lane & 3;
     const int col = 16 * ((lane >> 4) & 1) + 4 * (2 * (m & 1) + (m >> 1));
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
-      wcol[kb] = weight + row * ROWB + (((4 * kb + (col >> 3)) ^ row) << 4) + 2 * (col & 7);
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        wcol[b][kb] = weight + (row + 8 * b) * ROWB + (((4 * kb + (col >> 3)) ^ chunk_swizzle<ROWB>(row + 8 * b)) << 4) +
+                      2 * (col & 7);
   }
   auto column8 = [&](int kb, int row) {
     V4 v[2];
@@ -312,7 +316,7 @@ __global__ __launch_bounds__(NT, NT / 256) void linear_rows_bwd_kernel(const Lin
     for (int b = 0; b < 2; ++b)
       v[b] = __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                         (lds_v4i16*)(__attribute__((address_space(3))) const unsigned char*)(
-                                            wcol[kb] + (row + 8 * b) * ROWB)));
+                                            wcol[b][kb] + row * ROWB)));
     return __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
   };
   auto load_rows = [&](u32x4_t (&x)[KS / 2][2], int64_t grp) {
@@ -401,7 +405,7 @@ __global__ __launch_bounds__(NT, NT / 256) void linear_outputs_kernel(const LinA
   const int nkc = (a.I + 16 * KC - 1) / (16 * KC), rowb = nkc * KC * 32;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
   unsigned char* const weight = smem + NT / 64 * TURN;
-  fill_weight<T, NT>(weight, a, transposed, 32 * YB, rowb);
+  fill_weight<T, NT, 256>(weight, a, transposed, 32 * YB, rowb);
   const float* bias = (const float*)(weight + 32 * YB * rowb);
   __syncthreads();
   const Turn turn(smem + wave * TURN, lane);
@@ -414,7 +418,7 @@ __global__ __launch_bounds__(NT, NT / 256) void linear_outputs_kernel(const LinA
   };
   const unsigned char* wrow[KC];
 #pragma unroll
-  for (int kk = 0; kk < KC; ++kk) wrow[kk] = weight + l32 * rowb + (((2 * kk + g) ^ (l32 & 7)) << 4);
+  for (int kk = 0; kk < KC; ++kk) wrow[kk] = weight + l32 * rowb + (((2 * kk + g) ^ chunk_swizzle<256>(l32)) << 4);
   int64_t grp = (int64_t)blockIdx.x * (NT / 64) + wave;
   u32x4_t next[KC / 2][2];
   load_part(next, grp, 0);
