@@ -48,14 +48,19 @@ struct Tile {
   static __device__ __forceinline__ int swz(int row, int chunk) { return chunk ^ chunk_swizzle<ROWB>(row); }
 };
 
+constexpr int GROUP = 4;
+
 template <typename T, int PREC, typename Cfg>
 __global__ __launch_bounds__(Cfg::NT, Cfg::WGS * Cfg::NW / 4) void linear_kernel(const LinArgs a) {
   typedef typename TypeOps<T>::V8 V8;
   __shared__ __align__(16) unsigned char smem[Cfg::LDS];
+  // Consecutive workgroups of an XCD take a block of GROUP tiles of rows before the next tiles of outputs: the
+  // operands that its L2 fetches at a time are those of about a square of tiles.
   const uint32_t ntn = (uint32_t)(a.out_cols + Cfg::BN - 1) / Cfg::BN;
-  const uint32_t w = xcd_remap(blockIdx.x, gridDim.x);
-  const int n0 = (int)(w % ntn) * Cfg::BN;
-  const int64_t m0 = (int64_t)(w / ntn) * Cfg::BM;
+  const uint32_t w = xcd_remap(blockIdx.x, gridDim.x), group = w / (GROUP * ntn), rest = w % (GROUP * ntn);
+  const uint32_t high = min((uint32_t)GROUP, gridDim.x / ntn - group * GROUP);
+  const int n0 = (int)(rest / high) * Cfg::BN;
+  const int64_t m0 = (int64_t)(group * GROUP + rest % high) * Cfg::BM;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
   const int wm = wave / Cfg::GN, wn = wave % Cfg::GN;
 
@@ -76,20 +81,18 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::WGS * Cfg::NW / 4) void linear_kernel
     wsrc[q] = (const T*)a.w + (int64_t)min(n, a.O - 1) * a.w_ld;
   }
   const int nkt = (a.I + Cfg::BK - 1) / Cfg::BK;
-  auto issue = [&](int kt) {
+  // instructions [q0, q1) of a stage's QPS, x's first
+  auto issue = [&](int kt, int q0, int q1) {
     unsigned char* st = smem + (kt % Cfg::STAGES) * Cfg::STAGE;
     const int k0 = kt * Cfg::BK;
 #pragma unroll
-    for (int q = 0; q < Cfg::QA; ++q) {
-      const int k = k0 + Cfg::swz(Cfg::RPI * (Cfg::QA * wave + q) + drow, dpos) * Cfg::EPC;
-      const void* src = k < a.I ? (const void*)(xsrc[q] + k) : (const void*)zero_chunk;
-      __builtin_amdgcn_global_load_lds(src, (lds_void_t*)(st + (Cfg::QA * wave + q) * 1024), 16, 0, 0);
-    }
-#pragma unroll
-    for (int q = 0; q < Cfg::QB; ++q) {
-      const int k = k0 + Cfg::swz(Cfg::RPI * (Cfg::QB * wave + q) + drow, dpos) * Cfg::EPC;
-      const void* src = k < a.I ? (const void*)(wsrc[q] + k) : (const void*)zero_chunk;
-      __builtin_amdgcn_global_load_lds(src, (lds_void_t*)(st + Cfg::BM * Cfg::ROWB + (Cfg::QB * wave + q) * 1024), 16, 0, 0);
+    for (int q = q0; q < q1; ++q) {
+      const bool is_x = q < Cfg::QA;
+      const int at = is_x ? Cfg::QA * wave + q : Cfg::QB * wave + q - Cfg::QA;
+      const T* src = is_x ? xsrc[is_x ? q : 0] : wsrc[is_x ? 0 : q - Cfg::QA];
+      const int k = k0 + Cfg::swz(Cfg::RPI * at + drow, dpos) * Cfg::EPC;
+      __builtin_amdgcn_global_load_lds(k < a.I ? (const void*)(src + k) : (const void*)zero_chunk,
+                                       (lds_void_t*)(st + (is_x ? 0 : Cfg::BM * Cfg::ROWB) + at * 1024), 16, 0, 0);
     }
   };
   // 8 elements kk * 16 + 8 g of a row
@@ -112,63 +115,81 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::WGS * Cfg::NW / 4) void linear_kernel
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
 
-#pragma unroll
-  for (int s = 0; s < Cfg::STAGES - 1; ++s)
-    if (s < nkt) issue(s);
-  for (int kt = 0; kt < nkt; ++kt) {
-    // this wave's DMA of stage kt has landed (the later stages' may be in flight) and its reads of stage kt - 1
-    // have returned; after the barrier every wave's have, and the buffer of stage kt - 1 is free
-    const int ahead = min(Cfg::STAGES - 2, nkt - 1 - kt);
-    if (Cfg::STAGES >= 4 && ahead >= 2)
-      wait_vm_lgkm0<2 * Cfg::QPS>();
-    else if (Cfg::STAGES >= 3 && ahead >= 1)
-      wait_vm_lgkm0<Cfg::QPS>();
-    else
-      wait_vm_lgkm0<0>();
-    asm volatile("s_barrier" ::: "memory");
-    if (kt + Cfg::STAGES - 1 < nkt) issue(kt + Cfg::STAGES - 1);
+  // A stage's products go in steps of 16 elements; a step begins with the reads of the next step's fragments, over
+  // the stage's end too. With three stages in flight the DMA of the stage after them goes in equal shares beside
+  // the steps' products (4096 x 4096 -> 1024, bf16: 44 us; all at the stage's start 52). With two buffers it has
+  // only until the stage's end to land and goes in the first two steps (4096^3: 142 us; in shares 149). Stages
+  // past the end are zeros.
+  constexpr int KS = Cfg::BK / 16, SHARE = Cfg::QPS / KS;
+  constexpr bool SPREAD = Cfg::STAGES > 2;
+  static_assert(KS % 2 == 0 && SHARE * KS == Cfg::QPS && (SPREAD || KS > 2), "steps");
+  V8 xf[2][Cfg::X], wf[2][Cfg::Y];
+  auto load_frags = [&](int slot, int kt, int kk) {
     const unsigned char* sx = smem + (kt % Cfg::STAGES) * Cfg::STAGE;
     const unsigned char* sw = sx + Cfg::BM * Cfg::ROWB;
-    constexpr int KS = Cfg::BK / 16;
+#pragma unroll
+    for (int y = 0; y < Cfg::Y; ++y) wf[slot][y] = frag(sw, 32 * (Cfg::Y * wn + y) + l32, kk);
+#pragma unroll
+    for (int x = 0; x < Cfg::X; ++x) xf[slot][x] = frag(sx, 32 * (Cfg::X * wm + x) + l32, kk);
+  };
+  // This wave's DMA of a stage has landed (the later stages' may be in flight) and its reads so far have
+  // returned; after the barrier every wave's have, and the buffer of the stage before is free.
+  auto arrive = [&]() {
+    wait_vm_lgkm0<(Cfg::STAGES - 2) * Cfg::QPS>();
+    asm volatile("s_barrier" ::: "memory");
+  };
+#pragma unroll
+  for (int s = 0; s < Cfg::STAGES - 1; ++s) issue(s, 0, Cfg::QPS);
+  arrive();
+  load_frags(0, 0, 0);
+  if (SPREAD) issue(Cfg::STAGES - 1, 0, SHARE);
+  for (int kt = 0; kt < nkt; ++kt) {
+    const int next = kt + Cfg::STAGES - 1;
 #pragma unroll
     for (int kk = 0; kk < KS; ++kk) {
-      V8 xf[Cfg::X], wf[Cfg::Y];
-#pragma unroll
-      for (int x = 0; x < Cfg::X; ++x) xf[x] = frag(sx, 32 * (Cfg::X * wm + x) + l32, kk);
-#pragma unroll
-      for (int y = 0; y < Cfg::Y; ++y) wf[y] = frag(sw, 32 * (Cfg::Y * wn + y) + l32, kk);
+      const bool last = kk + 1 == KS;
+      if (last) arrive();
+      load_frags((kk + 1) & 1, last ? kt + 1 : kt, last ? 0 : kk + 1);
+      if (SPREAD)
+        issue(last ? next + 1 : next, last ? 0 : (kk + 1) * SHARE, last ? SHARE : (kk + 2) * SHARE);
+      else if (kk < 2)
+        issue(next, kk * Cfg::QPS / 2, (kk + 1) * Cfg::QPS / 2);
 #pragma unroll
       for (int x = 0; x < Cfg::X; ++x)
 #pragma unroll
-        for (int y = 0; y < Cfg::Y; ++y) Mma<T, PREC>::step(acc[x][y], wf[y], xf[x]);
+        for (int y = 0; y < Cfg::Y; ++y) Mma<T, PREC>::step(acc[x][y], wf[kk & 1][y], xf[kk & 1][x]);
     }
   }
 
   // A lane's sums are one row's: stored like that, neighbouring lanes would write 16 bytes each to different
   // rows. Every 32 x 32 tile turns through 4 KB of LDS of the wave's own (fp32, 16-byte chunks XOR-swizzled by
-  // (row / 2) % 8), and is finished with 4 lanes a row.
+  // (row / 2) % 8), and is finished with 4 lanes a row; as many tiles at a time as fit.
   wait_vm_lgkm0<0>();
   asm volatile("s_barrier" ::: "memory");
-  unsigned char* tile = smem + wave * 4096;
-  auto at = [&](int row, int chunk) { return reinterpret_cast<f32x4*>(tile + row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4)); };
+  constexpr int TILES = Cfg::X * Cfg::Y, FIT = Cfg::LDS / Cfg::NW / 4096, PASS = FIT < TILES ? FIT : TILES;
+  static_assert(TILES % PASS == 0, "passes");
+  unsigned char* tiles = smem + wave * PASS * 4096;
+  auto at = [&](int tile, int row, int chunk) {
+    return reinterpret_cast<f32x4*>(tiles + tile * 4096 + row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4));
+  };
 #pragma unroll
-  for (int y = 0; y < Cfg::Y; ++y) {
-    const int n = n0 + 32 * (Cfg::Y * wn + y) + 8 * (lane & 3);
-    f32x8 b = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (a.bias && n < a.O) b = load8_any((const T*)a.bias + n, a.O - n);
+  for (int p = 0; p < TILES; p += PASS) {
 #pragma unroll
-    for (int x = 0; x < Cfg::X; ++x) {
+    for (int t = 0; t < PASS; ++t)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *at(l32, 4 * (q / 2) + 2 * g + q % 2) = f32x4{acc[x][y][4 * q], acc[x][y][4 * q + 1], acc[x][y][4 * q + 2],
-                                                      acc[x][y][4 * q + 3]};
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = 16 * i + (lane >> 2);
-        const f32x4 lo = *at(row, 2 * (lane & 3)), hi = *at(row, 2 * (lane & 3) + 1);
-        const int64_t m = m0 + 32 * (Cfg::X * wm + x) + row;
-        if (m < a.M && n < a.out_cols) finish8<T>(a, f32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, b, m, n);
+      for (int q = 0; q < 4; ++q) {
+        const f32x16& v = acc[(p + t) % Cfg::X][(p + t) / Cfg::X];
+        *at(t, l32, 4 * (q / 2) + 2 * g + q % 2) = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
       }
+#pragma unroll 2
+    for (int h = 0; h < 2 * PASS; ++h) {
+      const int t = h >> 1, x = (p + t) % Cfg::X, y = (p + t) / Cfg::X;
+      const int row = 16 * (h & 1) + (lane >> 2), n = n0 + 32 * (Cfg::Y * wn + y) + 8 * (lane & 3);
+      const int64_t m = m0 + 32 * (Cfg::X * wm + x) + row;
+      const f32x4 lo = *at(t, row, 2 * (lane & 3)), hi = *at(t, row, 2 * (lane & 3) + 1);
+      f32x8 b = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (a.bias && n < a.O) b = load8_any((const T*)a.bias + n, a.O - n);
+      if (m < a.M && n < a.out_cols) finish8<T>(a, f32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, b, m, n);
     }
   }
 }
@@ -237,20 +258,17 @@ __global__ __launch_bounds__(FW_NT, 2) void linear_few_kernel(const LinArgs a) {
   finish8<T>(a, z, b, m, n);
 }
 
-#ifndef GNN_LIN_FORCE
-#define GNN_LIN_FORCE 0
-#endif
 template <typename T, int PREC>
 int run(const LinArgs& a, hipStream_t st) {
   typedef Tile<T, 2, 2, 1, 1, 128, 4> Small;
   typedef Tile<T, 2, 2, 2, 2, 128, 4> Medium;
   const int64_t cus = compute_units();
   if constexpr (sizeof(T) == 2) {
-    typedef Tile<T, 2, 4, 4, 2, 64, 4> Large;
-    if (GNN_LIN_FORCE == 3 || (GNN_LIN_FORCE == 0 && tiles_of<Large>(a) >= cus)) return launch<T, PREC, Large>(a, st);
+    typedef Tile<T, 2, 4, 4, 2, 128, 2> Large;
+    if (tiles_of<Large>(a) >= cus) return launch<T, PREC, Large>(a, st);
   }
-  if (GNN_LIN_FORCE == 2 || (GNN_LIN_FORCE == 0 && tiles_of<Medium>(a) >= cus)) return launch<T, PREC, Medium>(a, st);
-  if (GNN_LIN_FORCE == 1 || (GNN_LIN_FORCE == 0 && tiles_of<Small>(a) >= cus / 2)) return launch<T, PREC, Small>(a, st);
+  if (tiles_of<Medium>(a) >= cus) return launch<T, PREC, Medium>(a, st);
+  if (tiles_of<Small>(a) >= cus / 2) return launch<T, PREC, Small>(a, st);
   const int64_t few = (a.M + 31) / 32 * ((a.out_cols + 31) / 32);
   hipLaunchKernelGGL((linear_few_kernel<T, PREC>), dim3((uint32_t)few), dim3(FW_NT), 0, st, a);
   return (int)hipGetLastError();
