@@ -534,6 +534,21 @@ int gnn_linear_takes_dx(const gnn_linear_args* args) { return args && args->dx &
 
 int gnn_linear_takes_transposed(const gnn_linear_args* args) { return args && linear_takes_transposed(*args) ? 1 : 0; }
 
+int gnn_pad_rows(const gnn_pad_rows_args* args, void* stream) {
+  if (!args) return set_error(GNN_ERR_ARG, "pad_rows: args is NULL");
+  const gnn_pad_rows_args& a = *args;
+  if (!a.src || !a.dst) return set_error(GNN_ERR_ARG, "pad_rows: src and dst are required");
+  if (!known_dtype(a.dtype)) return set_error(GNN_ERR_ARG, "pad_rows: unknown dtype");
+  const int chunk = a.dtype == GNN_F32 ? 4 : 8;
+  if (a.rows < 1 || a.cols < 1 || a.ld < a.cols || a.ld > ((int64_t)1 << 24) || a.ld % chunk)
+    return set_error(GNN_ERR_ARG, "pad_rows: rows and cols must be positive, ld a multiple of 16 bytes from cols to 2^24");
+  if (!aligned(a.src, 16 / chunk) || !aligned(a.dst, 16))
+    return set_error(GNN_ERR_ARG, "pad_rows: src must be aligned to its elements, dst to 16 bytes");
+  int rc = pad_rows(a, (hipStream_t)stream);
+  if (rc < 0) return rc;
+  return hip_status((hipError_t)rc, "pad_rows");
+}
+
 int64_t gnn_column_sums_parts(int64_t M, int64_t O) { return M < 1 || O < 1 ? 0 : column_sums_parts(M, O); }
 
 int gnn_column_sums(const gnn_column_sums_args* args, void* stream) {

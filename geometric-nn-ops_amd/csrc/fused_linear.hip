@@ -120,9 +120,9 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::WGS * Cfg::NW / 4) void linear_kernel
   // the steps' products (4096 x 4096 -> 1024, bf16: 44 us; all at the stage's start 52). With two buffers it has
   // only until the stage's end to land and goes in the first two steps (4096^3: 142 us; in shares 149). Stages
   // past the end are zeros.
-  constexpr int KS = Cfg::BK / 16, SHARE = Cfg::QPS / KS;
+  constexpr int KS = Cfg::BK / 16, SHARE = Cfg::QPS / KS, FIRST = KS > 2 ? 2 : 1;
   constexpr bool SPREAD = Cfg::STAGES > 2;
-  static_assert(KS % 2 == 0 && SHARE * KS == Cfg::QPS && (SPREAD || KS > 2), "steps");
+  static_assert(KS % 2 == 0 && (!SPREAD || SHARE * KS == Cfg::QPS), "steps");
   V8 xf[2][Cfg::X], wf[2][Cfg::Y];
   auto load_frags = [&](int slot, int kt, int kk) {
     const unsigned char* sx = smem + (kt % Cfg::STAGES) * Cfg::STAGE;
@@ -152,8 +152,8 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::WGS * Cfg::NW / 4) void linear_kernel
       load_frags((kk + 1) & 1, last ? kt + 1 : kt, last ? 0 : kk + 1);
       if (SPREAD)
         issue(last ? next + 1 : next, last ? 0 : (kk + 1) * SHARE, last ? SHARE : (kk + 2) * SHARE);
-      else if (kk < 2)
-        issue(next, kk * Cfg::QPS / 2, (kk + 1) * Cfg::QPS / 2);
+      else if (kk < FIRST)  // before the stage's last step, which waits for it
+        issue(next, kk * Cfg::QPS / FIRST, (kk + 1) * Cfg::QPS / FIRST);
 #pragma unroll
       for (int x = 0; x < Cfg::X; ++x)
 #pragma unroll
@@ -260,17 +260,79 @@ __global__ __launch_bounds__(FW_NT, 2) void linear_few_kernel(const LinArgs a) {
 
 template <typename T, int PREC>
 int run(const LinArgs& a, hipStream_t st) {
-  typedef Tile<T, 2, 2, 1, 1, 128, 4> Small;
-  typedef Tile<T, 2, 2, 2, 2, 128, 4> Medium;
+  // 16-bit types: the larger the tile the less LDS is read a product, as long as every CU has one (4096^3: 136 us in
+  // 256 x 256, 185 in 128 x 128; 4096 x 4096 -> 1024, 64 tiles of 256 x 256: 44 in 128 x 128, 56 in 64 x 64; 2048 x
+  // 1024 -> 1024, 128 tiles of 128 x 128: 11 in 64 x 64, 17 in 128 x 128; 384 x 384 -> 1536, 144 tiles of 64 x 64:
+  // 5.5, in the kernel for few tiles 8.0). fp32 products are bound by the matrix rate: smaller tiles with fewer
+  // stages, several workgroups a CU, one's epilogue beside another's products (40401 x 136 -> 257: 65 us, in one
+  // workgroup of 128 x 128 a CU 90; 2048 x 1024 -> 1024, one tile of 128 x 64 a CU: 45 in 64 x 64, 52 in 128 x 64).
+  constexpr bool F32 = sizeof(T) == 4;
+  typedef Tile<T, 2, 2, 1, 1, 128, F32 ? 3 : 4> Small;
+  typedef Tile<T, 2, 2, 2, F32 ? 1 : 2, 128, F32 ? 2 : 4> Medium;
   const int64_t cus = compute_units();
-  if constexpr (sizeof(T) == 2) {
+  if constexpr (!F32) {
     typedef Tile<T, 2, 4, 4, 2, 128, 2> Large;
     if (tiles_of<Large>(a) >= cus) return launch<T, PREC, Large>(a, st);
   }
-  if (tiles_of<Medium>(a) >= cus) return launch<T, PREC, Medium>(a, st);
+  if (tiles_of<Medium>(a) >= (F32 ? 2 : 1) * cus) return launch<T, PREC, Medium>(a, st);
   if (tiles_of<Small>(a) >= cus / 2) return launch<T, PREC, Small>(a, st);
   const int64_t few = (a.M + 31) / 32 * ((a.out_cols + 31) / 32);
   hipLaunchKernelGGL((linear_few_kernel<T, PREC>), dim3((uint32_t)few), dim3(FW_NT), 0, st, a);
+  return (int)hipGetLastError();
+}
+
+// ---- padded rows ------------------------------------------------------------------------------
+// dst[r][c] = src[r row_stride + c col_stride] for c < cols, 0 up to ld: a thread writes 16 bytes. Sources whose
+// rows are not contiguous but whose columns are (a transposed weight) go through LDS in tiles of 64 x 64, read
+// along the columns. (40401 x 131 fp32: 8.6 us, a fill and a strided copy 13.9; 1024 x 4096 bf16 turned: 5.7, a
+// strided copy 28.4.)
+template <typename E>
+__global__ __launch_bounds__(256) void pad_rows_kernel(const gnn_pad_rows_args a) {
+  constexpr int N = 16 / (int)sizeof(E);
+  typedef E V __attribute__((ext_vector_type(N)));
+  const uint32_t chunks = (uint32_t)(a.ld / N);
+  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t r = (int64_t)(i / chunks);
+  if (r >= a.rows) return;
+  const int64_t c = (int64_t)(i % chunks) * N;
+  const E* src = (const E*)a.src + r * a.row_stride + c * a.col_stride;
+  V v;
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] = c + e < a.cols ? src[e * a.col_stride] : (E)0;
+  reinterpret_cast<V*>(a.dst)[i] = v;
+}
+
+template <typename E>
+__global__ __launch_bounds__(256) void pad_rows_turned_kernel(const gnn_pad_rows_args a) {
+  constexpr int N = 16 / (int)sizeof(E), B = 64;
+  typedef E V __attribute__((ext_vector_type(N)));
+  __shared__ E tile[B][B + 1];  // [column][row]
+  const uint32_t across = (uint32_t)((a.ld + B - 1) / B);
+  const int64_t r0 = (int64_t)(blockIdx.x / across) * B, c0 = (int64_t)(blockIdx.x % across) * B;
+  for (int k = threadIdx.x; k < B * B; k += 256) {
+    const int64_t r = r0 + k % B, c = c0 + k / B;
+    tile[k / B][k % B] = r < a.rows && c < a.cols ? ((const E*)a.src)[r * a.row_stride + c * a.col_stride] : (E)0;
+  }
+  __syncthreads();
+  for (int k = threadIdx.x; k < B * B / N; k += 256) {
+    const int r = k / (B / N), c = k % (B / N) * N;
+    V v;
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = tile[c + e][r];
+    if (r0 + r < a.rows && c0 + c < a.ld) *reinterpret_cast<V*>((E*)a.dst + (r0 + r) * a.ld + c0 + c) = v;
+  }
+}
+
+template <typename E>
+int pad_rows_typed(const gnn_pad_rows_args& a, hipStream_t st) {
+  const bool turned = a.col_stride != 1 && a.row_stride == 1;
+  const int64_t blocks = turned ? (a.rows + 63) / 64 * ((a.ld + 63) / 64)
+                                : (a.rows * (a.ld * (int64_t)sizeof(E) / 16) + 255) / 256;
+  if (blocks >= ((int64_t)1 << 31)) return set_error(GNN_ERR_UNSUPPORTED, "pad_rows: grid too large");
+  if (turned)
+    hipLaunchKernelGGL(pad_rows_turned_kernel<E>, dim3((uint32_t)blocks), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL(pad_rows_kernel<E>, dim3((uint32_t)blocks), dim3(256), 0, st, a);
   return (int)hipGetLastError();
 }
 
@@ -314,6 +376,10 @@ int linear(const gnn_linear_args& g, hipStream_t st) {
     case GNN_F16: return run<f16, PREC_NATIVE>(a, st);
     default: return g.precision == GNN_PREC_BF16X3 ? run<float, PREC_BF16X3>(a, st) : run<float, PREC_IEEE>(a, st);
   }
+}
+
+int pad_rows(const gnn_pad_rows_args& a, hipStream_t st) {
+  return a.dtype == GNN_F32 ? pad_rows_typed<uint32_t>(a, st) : pad_rows_typed<uint16_t>(a, st);
 }
 
 int64_t column_sums_parts(int64_t M, int64_t O) {

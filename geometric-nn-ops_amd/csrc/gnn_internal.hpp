@@ -69,6 +69,7 @@ bool linear_takes_transposed(const gnn_linear_args& a);
 bool linear_takes_dx(const gnn_linear_args& a);
 int64_t column_sums_parts(int64_t M, int64_t O);
 int column_sums(const gnn_column_sums_args& a, hipStream_t stream);
+int pad_rows(const gnn_pad_rows_args& a, hipStream_t stream);
 int relpos(const gnn_relpos_args& a, bool backward, hipStream_t stream);
 int64_t relpos_parts(const gnn_relpos_args& a);
 int layer_norm_fwd(const gnn_layer_norm_fwd_args& a, hipStream_t stream);

@@ -423,6 +423,25 @@ class LinearArgs(ctypes.Structure):
 pack_linear = packer(LinearArgs)
 
 
+class PadRowsArgs(ctypes.Structure):
+    """Mirror of ``gnn_pad_rows_args``."""
+
+    _fields_ = [
+        ("src", ctypes.c_void_p),
+        ("dst", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("cols", ctypes.c_int64),
+        ("ld", ctypes.c_int64),
+        ("row_stride", ctypes.c_int64),
+        ("col_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+pack_pad_rows = packer(PadRowsArgs)
+
+
 class ColumnSumsArgs(ctypes.Structure):
     """Mirror of ``gnn_column_sums_args``."""
 
@@ -569,6 +588,7 @@ _SIGNATURES = {
     "gnn_linear_takes_dx": (ctypes.c_int, [ctypes.POINTER(LinearArgs)]),
     "gnn_linear_takes_transposed": (ctypes.c_int, [ctypes.POINTER(LinearArgs)]),
     "gnn_linear": (ctypes.c_int, [ctypes.POINTER(LinearArgs), ctypes.c_void_p]),
+    "gnn_pad_rows": (ctypes.c_int, [ctypes.POINTER(PadRowsArgs), ctypes.c_void_p]),
     "gnn_column_sums_parts": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64]),
     "gnn_column_sums": (ctypes.c_int, [ctypes.POINTER(ColumnSumsArgs), ctypes.c_void_p]),
     "gnn_last_error": (ctypes.c_char_p, []),

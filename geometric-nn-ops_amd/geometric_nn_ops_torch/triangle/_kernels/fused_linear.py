@@ -8,7 +8,6 @@ written in place at any alignment."""
 import ctypes
 
 import torch
-import torch.nn.functional as F
 
 from ... import _lib
 from .trimul import reduce_parts_hip
@@ -25,14 +24,16 @@ def supports(weight: torch.Tensor) -> bool:
 def _chunked(t: torch.Tensor) -> torch.Tensor:
     """``[R, C]`` rows of 16-byte chunks: C padded with zeros to a multiple of 8."""
     c = t.shape[1]
-    if c % 8:
-        return F.pad(t, (0, 8 - c % 8))
     if t.shape[0] == 1 and t.stride(1) == 1:
         t = t.as_strided((1, c), (c, 1))  # one row: its pitch says nothing
-    if t.stride(1) == 1 and t.stride(0) >= c and t.stride(0) * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0:
+    if c % 8 == 0 and t.stride(1) == 1 and t.stride(0) >= c and t.stride(0) * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0:
         return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    out = torch.empty((t.shape[0], (c + 7) // 8 * 8), device=t.device, dtype=t.dtype)
+    a = _lib.PadRowsArgs()
+    _lib.pack_pad_rows(a, 0, t.data_ptr(), out.data_ptr(), t.shape[0], c, out.shape[1], t.stride(0), t.stride(1),
+                       _lib.DTYPE_CODE[t.dtype], 0)
+    _lib.call("gnn_pad_rows", a, t.device)
+    return out
 
 
 def _unit(t: torch.Tensor) -> torch.Tensor:

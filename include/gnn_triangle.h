@@ -694,6 +694,17 @@ int gnn_linear_takes_transposed(const gnn_linear_args* args);
 int gnn_linear_takes_dx(const gnn_linear_args* args);
 int gnn_linear(const gnn_linear_args* args, void* stream);
 
+/* dst [rows, ld], contiguous and 16-byte aligned: src's cols columns (element (r, c) at r row_stride +
+ * c col_stride) and zeros behind. ld a multiple of 16 bytes' elements, at least cols. */
+typedef struct gnn_pad_rows_args {
+  const void* src;
+  void* dst;
+  int64_t rows, cols, ld, row_stride, col_stride;
+  int32_t dtype;
+  int32_t reserved;
+} gnn_pad_rows_args;
+int gnn_pad_rows(const gnn_pad_rows_args* args, void* stream);
+
 /* Sums over the rows of d [M, O] (pitch ld), as fp32 partial sums [parts][O] to be added with
  * gnn_reduce_parts; parts as gnn_column_sums_parts(M, O) returns it (any from 1 on is right). */
 typedef struct gnn_column_sums_args {

@@ -71,18 +71,6 @@ def test_refusals():
         fused_linear(torch.tensor(1.0), w)
 
 
-def test_chunked_rows():
-    base = torch.arange(4 * 64, dtype=torch.bfloat16).reshape(4, 64)
-    for t, same in ((base, True), (base[:, 8:24], True), (base[:, 4:20], False), (base[:, :13], False),
-                    (base.t()[:8, :2].t(), True), (base[:, ::4], False), (base[:1].expand(3, 64), False), (base[1:2, 16:24], True),
-                    (torch.arange(66, dtype=torch.bfloat16)[2:].view(1, 64), False)):
-        c = _hip._chunked(t)
-        assert torch.equal(c[:, :t.shape[1]], t) and not c[:, t.shape[1]:].any()
-        assert c.shape[1] % 8 == 0 and c.stride(1) == 1 and c.stride(0) % 8 == 0 and c.data_ptr() % 16 == 0
-        assert c.stride(0) >= c.shape[1]
-        assert (c.data_ptr() == t.data_ptr()) == same
-
-
 def test_argument_errors():
     lib = _lib.load()
     assert lib.gnn_linear(None, None) == _lib.GNN_ERR_ARG
@@ -172,3 +160,28 @@ def test_calls_that_take_a_transposed_weight_or_dx():
     a.M, a.dx, a.w_transposed, a.w_ld = 64, None, 1, 512
     assert lib.gnn_linear(ctypes.byref(a), None) == _lib.GNN_ERR_UNSUPPORTED
     assert b"transposed" in lib.gnn_last_error()
+
+
+def test_padding_refuses_what_it_cannot_write():
+    lib = _lib.load()
+    a = _lib.PadRowsArgs()
+
+    def refused(text):
+        assert lib.gnn_pad_rows(ctypes.byref(a), None) == _lib.GNN_ERR_ARG
+        assert text in lib.gnn_last_error()
+
+    assert lib.gnn_pad_rows(None, None) == _lib.GNN_ERR_ARG
+    refused(b"required")
+    a.src, a.dst, a.dtype, a.rows, a.cols, a.row_stride, a.col_stride = 4096, 8192, _lib.GNN_BF16, 3, 13, 13, 1
+    for ld in (0, 8, 13, 20):  # fewer than the columns, or no multiple of 16 bytes
+        a.ld = ld
+        refused(b"multiple of 16 bytes")
+    a.ld, a.rows = 16, 0
+    refused(b"positive")
+    a.rows, a.src = 3, 4097
+    refused(b"aligned")
+    a.src, a.dst = 4098, 8200
+    refused(b"aligned")
+    a.dst, a.dtype = 8192, 77
+    refused(b"dtype")
+    lib.gnn_last_error()

@@ -342,3 +342,33 @@ def test_operator_registration():
     with torch.no_grad():
         f = lambda t: fused_linear(t, w, b, "gelu", r)  # noqa: E731
         assert torch.equal(torch.compile(f, fullgraph=True, backend="aot_eager")(x), f(x))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 24), (5, 7), (65, 63), (64, 130), (1000, 131)])
+def test_rows_of_whole_chunks(rows, cols, dtype):
+    from geometric_nn_ops_torch.triangle._kernels.fused_linear import _chunked
+
+    base = torch.randn(2 * rows + 1, 2 * cols + 3, generator=torch.Generator().manual_seed(7)).to(DEV, dtype)
+    turned = torch.randn(cols, rows, generator=torch.Generator().manual_seed(8)).to(DEV, dtype)
+    views = [base[:rows, :cols].contiguous(), base[1:rows + 1, 1:cols + 1], base[:2 * rows:2, 0:2 * cols:2], turned.t(),
+             base[:1, :cols].expand(rows, cols)]
+    for t in views:
+        got = _chunked(t)
+        pitch = got.stride(0) if rows > 1 else got.shape[1]
+        assert got.shape == (rows, -(-cols // 8) * 8) and got.data_ptr() % 16 == 0 and pitch * got.element_size() % 16 == 0
+        assert torch.equal(got[:, :cols], t) and not got[:, cols:].any()
+
+
+def test_chunked_rows_are_copied_only_where_they_must():
+    base = torch.arange(4 * 64, dtype=torch.bfloat16, device=DEV).reshape(4, 64)
+    from geometric_nn_ops_torch.triangle._kernels.fused_linear import _chunked
+
+    for t, same in ((base, True), (base[:, 8:24], True), (base[:, 4:20], False), (base[:, :13], False),
+                    (base.t()[:8, :2].t(), True), (base[:, ::4], False), (base[:1].expand(3, 64), False), (base[1:2, 16:24], True),
+                    (torch.arange(66, dtype=torch.bfloat16, device=DEV)[2:].view(1, 64), False)):
+        c = _chunked(t)
+        assert torch.equal(c[:, :t.shape[1]], t) and not c[:, t.shape[1]:].any()
+        assert c.shape[1] % 8 == 0 and c.stride(1) == 1 and c.stride(0) % 8 == 0 and c.data_ptr() % 16 == 0
+        assert c.stride(0) >= c.shape[1]
+        assert (c.data_ptr() == t.data_ptr()) == same
