@@ -443,7 +443,19 @@ int gnn_layer_norm_bwd(const gnn_layer_norm_bwd_args* args, void* stream) {
   if (int rc = check_layer_norm(a.rows, a.K, a.dtype, a.param_dtype, a.weight)) return rc;
   if (int rc = check_layer_norm_rows(a.x, a.rows, a.x_inner, a.x_outer_stride, a.x_stride, a.dtype)) return rc;
   if (int rc = check_layer_norm_rows(a.dy, a.rows, a.dy_inner, a.dy_outer_stride, a.dy_stride, a.dtype)) return rc;
+  const int param_bytes = a.param_dtype == GNN_F32 ? 4 : 2;
+  if ((a.dweight || a.dbias) && !a.partial)
+    return set_error(GNN_ERR_ARG, "layer_norm backward: dweight and dbias need partial");
+  if (!aligned(a.dweight, param_bytes) || !aligned(a.dbias, param_bytes))
+    return set_error(GNN_ERR_ARG, "layer_norm backward: dweight and dbias must be aligned to their elements");
   int rc = layer_norm_bwd(a, (hipStream_t)stream);
+  if (rc == 0 && (a.dweight || a.dbias)) {
+    gnn_reduce_args r{};
+    for (int i = 0; i < 2; ++i)
+      if (void* dst = i ? a.dbias : a.dweight)
+        r.seg[r.count++] = {a.partial + i * a.K, dst, a.parts, 2 * a.K, a.K, a.param_dtype, 0};
+    rc = reduce_parts(r, (hipStream_t)stream);
+  }
   if (rc < 0) return rc;
   return hip_status((hipError_t)rc, "layer_norm backward");
 }
@@ -496,7 +508,15 @@ int gnn_relpos_bwd(const gnn_relpos_args* args, void* stream) {
     return set_error(GNN_ERR_ARG, "relative_position_bias backward: positions, dout, partial and parts are required");
   if (!aligned(args->dout, args->dtype == GNN_F32 ? 4 : 2))
     return set_error(GNN_ERR_ARG, "relative_position_bias backward: dout must be aligned to its elements");
+  if (!aligned(args->dtable, args->dtype == GNN_F32 ? 4 : 2))
+    return set_error(GNN_ERR_ARG, "relative_position_bias backward: dtable must be aligned to its elements");
   int rc = relpos(*args, true, (hipStream_t)stream);
+  if (rc == 0 && args->dtable) {
+    const int64_t n = args->buckets * args->H;
+    gnn_reduce_args r{};
+    r.seg[r.count++] = {args->partial, args->dtable, args->parts, n, n, args->dtype, 0};
+    rc = reduce_parts(r, (hipStream_t)stream);
+  }
   if (rc < 0) return rc;
   return hip_status((hipError_t)rc, "relative_position_bias backward");
 }

@@ -324,13 +324,14 @@ Shape shape_for(int64_t K, int32_t dtype) {
   if (n <= 96) return {32, 1, 3, 256};
   if (n <= 128) return {64, 1, 2, 256};
   if (n <= 192) return {64, 1, 3, 256};
-  if (n <= 256) return {64, 4, 1, 1024};
-  if (n <= 512) return {64, 4, 2, 1024};
-  if (n <= 768) return {64, 4, 3, 512};
-  if (n <= 1024) return {64, 8, 2, 1024};
-  if (n <= 1536) return {64, 8, 3, 512};
-  if (n <= 2048) return {64, 16, 2, 1024};
-  if (n <= 3072) return {64, 16, 3, 1024};
+  // several waves a row: 64 lanes x waves x chunks
+  if (n <= 64 * 4) return {64, 4, 1, 1024};
+  if (n <= 64 * 4 * 2) return {64, 4, 2, 1024};
+  if (n <= 64 * 4 * 3) return {64, 4, 3, 512};
+  if (n <= 64 * 8 * 2) return {64, 8, 2, 1024};
+  if (n <= 64 * 8 * 3) return {64, 8, 3, 512};
+  if (n <= 64 * 16 * 2) return {64, 16, 2, 1024};
+  if (n <= 64 * 16 * 3) return {64, 16, 3, 1024};
   return {64, 16, 4, 1024};
 }
 

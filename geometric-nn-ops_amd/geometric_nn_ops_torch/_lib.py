@@ -487,6 +487,7 @@ class RelposArgs(ctypes.Structure):
         ("pos_bytes", ctypes.c_int32),
         ("dtype", ctypes.c_int32),
         ("reserved", ctypes.c_int32),
+        ("dtable", ctypes.c_void_p),
     ]
 
 
@@ -540,6 +541,8 @@ class LayerNormBwdArgs(ctypes.Structure):
         ("dy_stride", ctypes.c_int64),
         ("dtype", ctypes.c_int32),
         ("param_dtype", ctypes.c_int32),
+        ("dweight", ctypes.c_void_p),
+        ("dbias", ctypes.c_void_p),
     ]
 
 

@@ -8,7 +8,6 @@ import torch
 
 from ... import _lib
 from .._reference.relative_position import log_borders, side_buckets
-from .trimul import reduce_parts_hip
 
 MAX_BUCKETS = 4096
 MAX_BORDERS = 256  # logarithmic buckets of a side
@@ -52,7 +51,7 @@ def _args(table_ptr, out_ptr, dout_ptr, strides, weight, query_pos, key_pos, max
         a, 0, table_ptr, query_pos.data_ptr(), key_pos.data_ptr(), out_ptr, dout_ptr, 0, borders, 0,
         query_pos.stride(0), key_pos.stride(0), *strides, query_pos.shape[0], query_pos.shape[1], key_pos.shape[1],
         heads, buckets, max_distance, spacing == "log", bidirectional, channels_last, query_pos.element_size(),
-        _lib.DTYPE_CODE[weight.dtype], 0)
+        _lib.DTYPE_CODE[weight.dtype], 0, 0)
     return a
 
 
@@ -96,7 +95,6 @@ def relative_position_bias_bwd_hip(weight, query_pos, key_pos, dout, max_distanc
               channels_last)
     a.parts = _lib.load().gnn_relpos_parts(ctypes.byref(a))
     part = torch.empty((a.parts, *weight.shape), device=weight.device, dtype=torch.float32)
-    a.partial = part.data_ptr()
+    a.partial, a.dtable = part.data_ptr(), grad.data_ptr()
     _lib.call("gnn_relpos_bwd", a, weight.device)
-    reduce_parts_hip([(part, 0, weight.numel(), grad)], weight.device)
     return grad

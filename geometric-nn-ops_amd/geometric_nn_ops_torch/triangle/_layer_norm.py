@@ -25,19 +25,19 @@ class _LayerNormHip(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = _hip.layer_norm_hip(x, weight, bias, eps, stats=True)
-        ctx.save_for_backward(x, weight, mean, rstd)
+        y, stats = _hip.layer_norm_hip(x, weight, bias, eps, stats=True)
+        ctx.save_for_backward(x, weight, stats)
         ctx.bias_dtype = None if bias is None else bias.dtype
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
+        x, weight, stats = ctx.saved_tensors
         need_x, need_w, need_b, _ = ctx.needs_input_grad
         dw = torch.empty(weight.shape, device=x.device, dtype=weight.dtype) if need_w else None
         db = torch.empty(x.shape[-1:], device=x.device, dtype=ctx.bias_dtype) if need_b else None
-        dx = _hip.layer_norm_bwd_hip(x, weight, mean, rstd, dy, need_dx=need_x, dweight=dw, dbias=db)
+        dx = _hip.layer_norm_bwd_hip(x, weight, stats, dy, need_dx=need_x, dweight=dw, dbias=db)
         return dx, dw, db, None
 
 

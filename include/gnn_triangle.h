@@ -598,8 +598,8 @@ typedef struct gnn_layer_norm_fwd_args {
 int gnn_layer_norm_fwd(const gnn_layer_norm_fwd_args* args, void* stream);
 
 /* Its backward: dx (dense, or NULL) and, where partial is not NULL, fp32 [parts][2][K]: partial sums of
- * the weight's and the bias's gradient, to be added with gnn_reduce_parts. parts is the number of
- * workgroups, gnn_layer_norm_bwd_parts(rows, K, dtype) the best one for the current device. dy is
+ * the weight's and the bias's gradient, which are added in order into dweight and dbias where those are not
+ * NULL (they need partial; gnn_reduce_parts adds them otherwise). parts is the number of workgroups, gnn_layer_norm_bwd_parts(rows, K, dtype) the best one for the current device. dy is
  * addressed as x is. */
 typedef struct gnn_layer_norm_bwd_args {
   const void* x;
@@ -615,6 +615,8 @@ typedef struct gnn_layer_norm_bwd_args {
   int64_t dy_inner, dy_outer_stride, dy_stride;
   int32_t dtype;
   int32_t param_dtype;
+  void* dweight; /* [K] in param_dtype, or NULL */
+  void* dbias;
 } gnn_layer_norm_bwd_args;
 int64_t gnn_layer_norm_bwd_parts(int64_t rows, int64_t K, int32_t dtype);
 int gnn_layer_norm_bwd(const gnn_layer_norm_bwd_args* args, void* stream);
@@ -622,8 +624,8 @@ int gnn_layer_norm_bwd(const gnn_layer_norm_bwd_args* args, void* stream);
 /* Learned bias by buckets of the distance between keys and queries, forward:
  *   out[b, h, i, j] (channels_last: out[b, i, j, h]) = table[bucket(key_pos[b, j] - query_pos[b, i])][h]
  * and backward: dtable[t][h] = sum over the (b, i, j) of bucket t of dout[b, h, i, j], as fp32 partial sums
- * [parts][buckets][H] to be added with gnn_reduce_parts; parts as gnn_relpos_parts returns it (any from 1
- * on is right). With D = max_distance and a = key_pos - query_pos:
+ * [parts][buckets][H], which are added in order into dtable ([buckets][H] in dtype) where that is not NULL
+ * (gnn_reduce_parts adds them otherwise); parts as gnn_relpos_parts returns it (any from 1 on is right). With D = max_distance and a = key_pos - query_pos:
  *   clip, two-sided: clamp(a, -D, D) + D (2 D + 1 buckets); one-sided: clamp(-a, 0, D) (D + 1 buckets);
  *   log: n buckets a side (buckets / 2 where two-sided, those of keys ahead, a > 0, in the second half),
  *     near = n / 2 of them for distances d < near, bucket near + k from the least d on with
@@ -650,6 +652,7 @@ typedef struct gnn_relpos_args {
   int32_t pos_bytes;
   int32_t dtype; /* enum gnn_dtype of table, out and dout */
   int32_t reserved;
+  void* dtable;
 } gnn_relpos_args;
 int gnn_relpos_fwd(const gnn_relpos_args* args, void* stream);
 int64_t gnn_relpos_parts(const gnn_relpos_args* args);
