@@ -185,3 +185,28 @@ def test_padding_refuses_what_it_cannot_write():
     a.dst, a.dtype = 8192, 77
     refused(b"dtype")
     lib.gnn_last_error()
+
+
+def test_the_fitted_normal_distribution():
+    """The polynomials of the 16-bit gelu and its slope, read from the source and evaluated in fp32, against the
+    normal distribution in 64 bits: within the bounds that the source states, and zero or one far out."""
+    text = (pathlib.Path(__file__).resolve().parent.parent / "geometric-nn-ops_amd/csrc/linear_common.hpp").read_text()
+
+    def poly(name, m):
+        c = [float(v.rstrip("f")) for v in text.split(f"float {name}[] = {{")[1].split("}")[0].replace("\n", " ").split(", ")]
+        out = torch.full_like(m, c[-1])
+        for k in reversed(c[:-1]):
+            out = out * m + torch.tensor(k, dtype=torch.float32)
+        return out.double()
+
+    m = torch.linspace(0, 16, 160001)
+    z = m.double()
+    tail, pdf = torch.special.ndtr(-z), torch.exp(-z * z / 2) / (2 * torch.pi) ** 0.5
+    near = torch.exp2(poly("P", m))
+    # 2e-7 of the fit, and a step of the fp32 evaluation's argument (below 2 where the tail counts): 2^-23 of the tail
+    assert (z * (near - tail).abs() <= 2e-7 + z * tail * 2.0 ** -22).all()
+    inner = z <= 5.5
+    assert ((near / tail - 1).abs()[inner] <= 1.6e-4).all()
+    slope = poly("S", m) * torch.exp2(-0.7213475204444817 * z * z)
+    assert ((slope - (tail - z * pdf)).abs() <= 4e-7).all()
+    assert near[-1] < 1e-100 and slope[-1].abs() < 1e-45
