@@ -47,7 +47,7 @@ def _pitch(t: torch.Tensor) -> int:
 
 def _linear(x, w, bias, side, outputs, activation, precision, *, dz=False, pad=False, transposed=False,
             want_dx=False):
-    """One kernel over chunked rows ``x [M, K]`` and ``w [>= outputs, K]`` (``transposed``: ``[K, >= outputs]``);
+    """One kernel over chunked rows ``x [M, K]`` and ``w [>= outputs, K]`` (``transposed``: ``[<= K, >= outputs]``);
     ``[M, outputs]``, with ``pad`` in rows of a multiple of 8 columns, zeros behind. With ``dz`` ``(out, dx)``,
     dx None unless it is wanted and the kernel forms ``dx = out w`` in the same pass."""
     M, K = x.shape
@@ -58,7 +58,8 @@ def _linear(x, w, bias, side, outputs, activation, precision, *, dz=False, pad=F
         a, 0, x.data_ptr(), w.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if side is None else side.data_ptr(),
         out.data_ptr(), M, K, outputs, cols, _pitch(x), _pitch(w), 0 if side is None else _pitch(side), cols, 0, 0,
         ACTIVATION_CODE[activation], dz, transposed, _lib.DTYPE_CODE[x.dtype], _lib.PRECISION_CODE[precision], 0)
-    if transposed and not _lib.load().gnn_linear_takes_transposed(ctypes.byref(a)):
+    # a weight of fewer rows than the padded columns of x has nothing to stand beside their zeros
+    if transposed and (w.shape[0] < K or not _lib.load().gnn_linear_takes_transposed(ctypes.byref(a))):
         w = _chunked(w[:, :outputs].t())
         a.w, a.w_ld, a.w_transposed = w.data_ptr(), _pitch(w), 0
     dx = None

@@ -372,3 +372,26 @@ def test_chunked_rows_are_copied_only_where_they_must():
         assert c.shape[1] % 8 == 0 and c.stride(1) == 1 and c.stride(0) % 8 == 0 and c.data_ptr() % 16 == 0
         assert c.stride(0) >= c.shape[1]
         assert (c.data_ptr() == t.data_ptr()) == same
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("act", [None, "silu"])
+@pytest.mark.parametrize("m,i,o", [(32770, 64, 4), (32768, 72, 13), (300, 64, 4), (40, 200, 13)])
+def test_nothing_around_the_operands_is_read(m, i, o, act, dtype):
+    """Weight, rows, bias and output gradient as parts of tensors that hold NaN everywhere else."""
+    def within(t, columns):
+        buf = torch.full((t.shape[0] + 40, t.shape[1] + (16 if columns else 0)), float("nan"), device=DEV, dtype=dtype)
+        part = buf[16:16 + t.shape[0], 8:8 + t.shape[1]] if columns else buf[16:16 + t.shape[0]]
+        part.copy_(t)
+        return part
+
+    x, w, b, _, dy = _inputs(m, i, o, dtype, residual=False, seed=11)
+    plain = [x.to(DEV), w.to(DEV), b.to(DEV)]
+    parts = [within(x, False), within(w, False), within(b[:, None], False)[:, 0]]
+    results = []
+    for leaves, d in ((plain, dy.to(DEV)), (parts, within(dy, True))):
+        leaves = [t.requires_grad_() for t in leaves]
+        y = fused_linear(*leaves, act)
+        results.append((y, *torch.autograd.grad(y, leaves, d)))
+    for name, a, e in zip(("y", "dx", "dw", "db"), results[1], results[0]):
+        assert torch.equal(a, e), name
