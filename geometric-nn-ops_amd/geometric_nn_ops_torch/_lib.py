@@ -657,7 +657,7 @@ def call(fn_name: str, args, device: torch.device, *extra) -> None:
     idx = device.index
     if idx is None or device.type != "cuda":
         rc = fn(ctypes.byref(args), *extra, stream_handle(device))
-    elif idx == torch.cuda.current_device():
+    elif idx == torch._C._cuda_getDevice():  # a tensor is there: nothing is left to initialise
         # the handle itself: building a torch.cuda.Stream around it takes 1.5 us a launch
         rc = fn(ctypes.byref(args), *extra, torch._C._cuda_getCurrentRawStream(idx))
     else:

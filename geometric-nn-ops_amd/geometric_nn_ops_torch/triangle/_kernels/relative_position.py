@@ -39,62 +39,58 @@ def _pos(t):
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
-def _args(table_ptr, out_ptr, dout_ptr, strides, weight, query_pos, key_pos, max_distance, spacing, bidirectional,
-          channels_last):
-    buckets, heads = weight.shape
-    borders = 0
-    if spacing == "log":
-        n, near = side_buckets(buckets, bidirectional)
-        borders = ctypes.addressof(_borders(n, near, max_distance))
-    a = _lib.RelposArgs()
-    _lib.pack_relpos(
-        a, 0, table_ptr, query_pos.data_ptr(), key_pos.data_ptr(), out_ptr, dout_ptr, 0, borders, 0,
-        query_pos.stride(0), key_pos.stride(0), *strides, query_pos.shape[0], query_pos.shape[1], key_pos.shape[1],
-        heads, buckets, max_distance, spacing == "log", bidirectional, channels_last, query_pos.element_size(),
-        _lib.DTYPE_CODE[weight.dtype], 0, 0)
-    return a
-
-
-def relative_position_bias_hip(weight, query_pos, key_pos, max_distance, spacing, bidirectional, channels_last):
+def relative_position_bias_hip(weight, query_pos, key_pos, max_distance, spacing, bidirectional, channels_last, *,
+                               keep=False):
     """``[B, H, U, V]``, a view with a row pitch rounded up to 8 elements (what the attention kernels read
-    without a copy), or the contiguous ``[B, U, V, H]``."""
+    without a copy), or the contiguous ``[B, U, V, H]``. With ``keep`` ``(out, args, query_pos, key_pos)``: the
+    call's arguments (None for an empty result) and the positions that they point to, for the backward."""
     B, U = query_pos.shape
-    V, H = key_pos.shape[1], weight.shape[1]
+    V, (buckets, H) = key_pos.shape[1], weight.shape
     query_pos, key_pos, weight = _pos(query_pos), _pos(key_pos), weight.contiguous()
+    device, dtype, pitch = weight.device, weight.dtype, (V + 7) // 8 * 8
     if channels_last:
-        buf = out = torch.empty((B, U, V, H), device=weight.device, dtype=weight.dtype)
-        strides = (buf.stride(0), 0, buf.stride(1))
+        out = torch.empty((B, U, V, H), device=device, dtype=dtype)
+        strides = (U * V * H, 0, V * H)
     else:
-        buf = torch.empty((B, H, U, (V + 7) // 8 * 8), device=weight.device, dtype=weight.dtype)
-        out = buf[..., :V]
-        strides = buf.stride()[:3]
-    if out.numel():
-        a = _args(weight.data_ptr(), buf.data_ptr(), 0, strides, weight, query_pos, key_pos, max_distance, spacing,
-                  bidirectional, channels_last)
-        _lib.call("gnn_relpos_fwd", a, weight.device)
-    return out
+        out = torch.empty((B, H, U, pitch), device=device, dtype=dtype)
+        strides = (H * U * pitch, U * pitch, pitch)
+        if pitch != V:
+            out = out[..., :V]
+    a = None
+    if B and U and V and H:
+        log, borders = spacing == "log", 0
+        if log:
+            n, near = side_buckets(buckets, bidirectional)
+            borders = ctypes.addressof(_borders(n, near, max_distance))
+        a = _lib.RelposArgs()
+        _lib.pack_relpos(
+            a, 0, weight.data_ptr(), query_pos.data_ptr(), key_pos.data_ptr(), out.data_ptr(), 0, 0, borders, 0,
+            query_pos.stride(0), key_pos.stride(0), *strides, B, U, V, H, buckets, max_distance, log, bidirectional,
+            channels_last, query_pos.element_size(), _lib.DTYPE_CODE[dtype], 0, 0)
+        _lib.call("gnn_relpos_fwd", a, device)
+    return (out, a, query_pos, key_pos) if keep else out
 
 
-def relative_position_bias_bwd_hip(weight, query_pos, key_pos, dout, max_distance, spacing, bidirectional,
-                                   channels_last):
-    """The table's gradient, like ``weight``."""
-    grad = torch.empty(weight.shape, device=weight.device, dtype=weight.dtype)
-    if not dout.numel():
+def relative_position_bias_bwd_hip(shape, args, dout):
+    """The table's gradient ``[buckets, H]`` in dout's dtype, from the forward's kept arguments."""
+    grad = torch.empty(shape, device=dout.device, dtype=dout.dtype)
+    if args is None:
         return grad.zero_()
-    query_pos, key_pos = _pos(query_pos), _pos(key_pos)
-    if channels_last:
-        H, V = weight.shape[1], key_pos.shape[1]
-        if (H > 1 and dout.stride(3) != 1) or (V > 1 and dout.stride(2) != H):
+    s0, s1, s2, s3 = dout.stride()
+    if args.channels_last:
+        if (args.H > 1 and s3 != 1) or (args.V > 1 and s2 != args.H):
             dout = dout.contiguous()
-        strides = (dout.stride(0), 0, dout.stride(1))
+            s0, s1 = dout.stride()[:2]
+        strides = (s0, 0, s1)
     else:
-        if key_pos.shape[1] > 1 and dout.stride(3) != 1:
+        if args.V > 1 and s3 != 1:
             dout = dout.contiguous()
-        strides = dout.stride()[:3]
-    a = _args(0, 0, dout.data_ptr(), strides, weight, query_pos, key_pos, max_distance, spacing, bidirectional,
-              channels_last)
-    a.parts = _lib.load().gnn_relpos_parts(ctypes.byref(a))
-    part = torch.empty((a.parts, *weight.shape), device=weight.device, dtype=torch.float32)
-    a.partial, a.dtable = part.data_ptr(), grad.data_ptr()
-    _lib.call("gnn_relpos_bwd", a, weight.device)
+            s0, s1, s2 = dout.stride()[:3]
+        strides = (s0, s1, s2)
+    a = _lib.RelposArgs.from_buffer_copy(args)  # a graph that is kept may run its backward again, on any thread
+    a.stride = strides
+    parts = _lib.load().gnn_relpos_parts(ctypes.byref(a))
+    part = torch.empty((parts, *shape), device=dout.device, dtype=torch.float32)
+    a.dout, a.parts, a.partial, a.dtable = dout.data_ptr(), parts, part.data_ptr(), grad.data_ptr()
+    _lib.call("gnn_relpos_bwd", a, dout.device)
     return grad

@@ -26,17 +26,17 @@ class _RelativePositionHip(torch.autograd.Function):
     derivative raises."""
 
     @staticmethod
-    def forward(ctx, weight, query_pos, key_pos, *how):
-        ctx.save_for_backward(weight, query_pos, key_pos)
-        ctx.how = how
-        return _hip.relative_position_bias_hip(weight, query_pos, key_pos, *how)
+    def forward(ctx, weight, query_pos, key_pos, how):
+        out, ctx.args, query_pos, key_pos = _hip.relative_position_bias_hip(weight, query_pos, key_pos, *how, keep=True)
+        ctx.save_for_backward(query_pos, key_pos)
+        ctx.shape = weight.shape
+        return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        weight, query_pos, key_pos = ctx.saved_tensors
-        grad = _hip.relative_position_bias_bwd_hip(weight, query_pos, key_pos, dout, *ctx.how)
-        return (grad, None, None, *(None for _ in ctx.how))
+        _ = ctx.saved_tensors  # what args points to, checked for changes in place
+        return _hip.relative_position_bias_bwd_hip(ctx.shape, ctx.args, dout), None, None, None
 
 
 def _check(weight, query_pos, key_pos, max_distance, spacing, bidirectional) -> None:
@@ -104,7 +104,10 @@ def relative_position_bias(
     if key_pos is None:
         key_pos = query_pos
     _check(weight, query_pos, key_pos, max_distance, spacing, bidirectional)
-    query_pos, key_pos = (t if t.dim() == 2 else t[None] for t in (query_pos, key_pos))
+    if query_pos.dim() == 1:
+        query_pos = query_pos[None]
+    if key_pos.dim() == 1:
+        key_pos = key_pos[None]
     if query_pos.shape[0] != key_pos.shape[0]:
         if 1 not in (query_pos.shape[0], key_pos.shape[0]):
             raise ValueError(f"query_pos and key_pos have batches {query_pos.shape[0]} and {key_pos.shape[0]}")
@@ -116,7 +119,7 @@ def relative_position_bias(
     if not weight.is_cuda or weight.dtype not in _KERNEL_DTYPES or not _hip.supports(weight, query_pos, key_pos, *how[:3]):
         return relative_position_bias_torch(weight, query_pos, key_pos, *how)
     if torch.is_grad_enabled() and weight.requires_grad:
-        return _RelativePositionHip.apply(weight, query_pos, key_pos, *how)
+        return _RelativePositionHip.apply(weight, query_pos, key_pos, how)
     fwd = (_ops.relative_position_bias_fwd_impl if _ops.eager_ok(weight, query_pos, key_pos)
            else _ops.relative_position_bias_fwd)
     return fwd(weight, query_pos, key_pos, *how)

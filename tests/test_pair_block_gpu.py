@@ -139,6 +139,7 @@ def test_block_and_gradients(n, b, dtype):
 
     def near(name, a, e, stages):
         assert a.dtype == dtype and a.shape == e.shape, name
+        a = a.detach()
         off, scale = float((a.double().cpu() - e).norm()), float(e.norm())
         assert off <= max(stages * step * scale, least), f"{name}: off by {off:.3g}, its norm {scale:.3g}"
 
