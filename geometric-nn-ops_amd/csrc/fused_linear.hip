@@ -9,8 +9,12 @@
 // global_load_lds into LDS (STAGES - 1 of them in flight, one barrier a stage) in 16-byte chunks whose order
 // within a row the source addresses permute (chunk_swizzle). The products are formed transposed (W's rows as the
 // rows of the 32x32 MFMA tile, in an order that leaves a lane 8 consecutive outputs of one row of x): these
-// take bias, activation and residual in fp32, round once and leave as one 16-byte store (two in fp32). Workgroups that share rows of x
-// follow each other on one XCD, whose L2 then serves x.
+// take bias, activation and residual in fp32, round once and leave as one 16-byte store (two in fp32).
+// 8192 x 4096 -> 4096, bf16: 252 us without an activation (1090 TFLOP/s), 262 with gelu; the vendor's product alone
+// 190. It is bound by how the DMA and the matrix unit overlap: with the DMA left out the products take 176, with
+// the products left out the DMA 76 of the 142 us of 4096^3, and neither more stages of half the size (149), shares
+// between the products (150 to 158), half of the waves a step behind (146 to 153) nor 4 waves of 128 x 128 (153)
+// brought them closer together.
 #include <algorithm>
 
 #include "linear_common.hpp"

@@ -13,6 +13,8 @@
 // registers until the workgroup leaves one fp32 row of partial sums (added in order by reduce_parts).
 // The forward leaves mean and rstd of each row in fp32 where a backward will follow: 8 bytes a row
 // instead of both sums over again, with their latency, in front of the backward's own.
+// Kernel times, with the ordered sums: 147456 x 128 bf16 forward 14 us (5.4 TB/s), backward 26; 8192 x 5120 bf16 33
+// and 60 (5.1, 4.2 TB/s); 8191 x 5003 fp16, rows at odd addresses, 40 and 70 (4.1, 3.5); 8192 x 3000 fp32 33 and 56.
 // Rows of any alignment and width are read in the same 16-byte accesses (gfx950 takes them at any
 // element's address); the last chunk of a width that is no multiple of 16 bytes goes by elements.
 #include <algorithm>
@@ -236,20 +238,41 @@ __global__ __launch_bounds__(NT) void layer_norm_bwd_kernel(const LnArgs a) {
 #pragma unroll
     for (int e = 0; e < E; ++e) dw[c][e] = db[c][e] = 0.f;
   }
-  int slot = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * Tm::N; r0 < a.rows; r0 += (int64_t)gridDim.x * Tm::N, slot ^= 1) {
-    const bool live = r0 + team < a.rows;
-    const int64_t row = live ? r0 + team : a.rows - 1;
+  struct Row {
+    V x[C], dy[C];
+    float mean, rstd;
+  };
+  auto load = [&](Row& r, int64_t row) {
+    row = min(row, a.rows - 1);
     const T* x = row_at((const T*)a.x, a.xr, row);
     const T* dy = row_at((const T*)a.dy, a.dyr, row);
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    V xv[C], gv[C];
+    r.mean = a.mean[row], r.rstd = a.rstd[row];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int col = (lane + c * Tm::LANES) * E;
-      xv[c] = load_chunk(x + col, K - col);
-      gv[c] = load_chunk(dy + col, K - col);
+      r.x[c] = load_chunk(x + col, K - col);
+      r.dy[c] = load_chunk(dy + col, K - col);
     }
+  };
+  // Workgroups of 8 waves have a CU, and registers, to themselves: their next row is on its way while they are
+  // at this one (8192 x 3000 fp32: 56 us, 61 without, 8191 x 5003 fp16: 70 and 72, with the sums of the parts; the
+  // smaller teams hide it behind other workgroups)
+  constexpr bool AHEAD = NW > 1 && NT <= 512;
+  const int64_t step = (int64_t)gridDim.x * Tm::N;
+  Row now, next;
+  if (AHEAD) load(next, (int64_t)blockIdx.x * Tm::N + team);
+  int slot = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * Tm::N; r0 < a.rows; r0 += step, slot ^= 1) {
+    const bool live = r0 + team < a.rows;
+    const int64_t row = live ? r0 + team : a.rows - 1;
+    if (AHEAD) {
+      now = next;
+      if (r0 + step < a.rows) load(next, r0 + step + team);
+    } else {
+      load(now, row);
+    }
+    const V (&xv)[C] = now.x, (&gv)[C] = now.dy;
+    const float mean = now.mean, rstd = now.rstd;
     float2 s = {0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < C; ++c) {
