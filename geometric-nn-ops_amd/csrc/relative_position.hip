@@ -17,8 +17,9 @@
 // Backward: bound by the one read of dout. The sums are kept in fp32 and in a fixed order: every lane adds
 // to bins of its own in LDS (heads first: [bucket][lane]; heads last: a wave's lanes own its channels,
 // [bucket][channel]), and a wave leaves one row of partial sums, added in order by reduce_parts.
-// 2048^2 x 16 heads, bf16, log, 134 MB: forward 29 us (4.6 TB/s), backward 51 (2.6: a wave has four turns of 8
-// queries x 512 keys, and the latency of each turn's loads; half or twice the waves 68 and 62). 509^2 x 128
+// 2048^2 x 16 heads, bf16, log, 134 MB: forward 29 us (4.6 TB/s), backward 51 (2.6: the blocks of keys
+// across the diagonal, whose lanes look buckets up and add to bins, and each wave's set-up; the next loads issued a
+// turn ahead 55, half or twice the waves 68 and 62). 509^2 x 128
 // channels, clip, 66 MB: 19 (3.5 TB/s) and 38 (1.7: the chain of bins; half or twice the workgroups 58 and 50).
 #include <algorithm>
 
