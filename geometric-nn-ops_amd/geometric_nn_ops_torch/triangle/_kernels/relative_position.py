@@ -59,10 +59,11 @@ def relative_position_bias_hip(weight, query_pos, key_pos, max_distance, spacing
     a = None
     if B and U and V and H:
         log, borders = spacing == "log", 0
+        a = _lib.RelposArgs()
         if log:
             n, near = side_buckets(buckets, bidirectional)
-            borders = ctypes.addressof(_borders(n, near, max_distance))
-        a = _lib.RelposArgs()
+            a.kept = _borders(n, near, max_distance)  # the arguments may outlive the cache's entry
+            borders = ctypes.addressof(a.kept)
         _lib.pack_relpos(
             a, 0, weight.data_ptr(), query_pos.data_ptr(), key_pos.data_ptr(), out.data_ptr(), 0, 0, borders, 0,
             query_pos.stride(0), key_pos.stride(0), *strides, B, U, V, H, buckets, max_distance, log, bidirectional,

@@ -223,3 +223,21 @@ def test_operator_registration():
     with torch.no_grad():
         f = lambda t: relative_position_bias(t, q, k, max_distance=32, spacing="clip")  # noqa: E731
         assert torch.equal(torch.compile(f, fullgraph=True, backend="aot_eager")(w), f(w))
+
+
+def test_the_borders_live_as_long_as_the_graph():
+    import gc
+
+    from geometric_nn_ops_torch.triangle._kernels import relative_position as kernels
+
+    pos = torch.arange(200, device=DEV)
+    grads = []
+    for drop in (False, True):
+        table = torch.randn(32, 4, generator=torch.Generator().manual_seed(2)).to(DEV).requires_grad_()
+        y = relative_position_bias(table, pos, max_distance=100)
+        if drop:
+            kernels._borders.cache_clear()
+            gc.collect()
+            others = [(type(kernels._borders(16, 8, 99)))(*range(1, 8)) for _ in range(2000)]  # noqa: F841
+        grads.append(torch.autograd.grad(y, table, torch.ones_like(y))[0])
+    assert torch.equal(*grads)
