@@ -162,3 +162,25 @@ def test_block_repeats_and_replays_in_a_graph():
         assert torch.equal(a, e), f"replay {replay}"
 
     replays_match(block, same)
+
+
+def test_block_on_another_stream():
+    p, pos, keep = _case(33, 2, torch.bfloat16)
+    p = {k: t.to(DEV).requires_grad_() for k, t in p.items()}
+    pos, mask, smask = pos.to(DEV), keep[:, None, None, None, :].to(DEV), keep.to(DEV, torch.bfloat16)
+
+    def run():
+        outs = _block(p, pos, mask, smask)
+        return [t.detach() for t in outs] + list(torch.autograd.grad(outs, list(p.values()), [torch.ones_like(t) for t in outs]))
+
+    want = run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    busy = torch.randn(2048, 2048, device=DEV)
+    for _ in range(20):  # the default stream is at work meanwhile
+        busy = busy @ busy * 1e-3
+    with torch.cuda.stream(side):
+        got = run()
+    torch.cuda.current_stream().wait_stream(side)
+    for name, a, e in zip(("z", "s", *p), got, want):
+        assert torch.equal(a, e), name
