@@ -264,22 +264,38 @@ __global__ __launch_bounds__(FW_NT, 2) void linear_few_kernel(const LinArgs a) {
 
 template <typename T, int PREC>
 int run(const LinArgs& a, hipStream_t st) {
-  // 16-bit types: the larger the tile the less LDS is read a product, as long as every CU has one (4096^3: 136 us in
-  // 256 x 256, 185 in 128 x 128; 4096 x 4096 -> 1024, 64 tiles of 256 x 256: 44 in 128 x 128, 56 in 64 x 64; 2048 x
-  // 1024 -> 1024, 128 tiles of 128 x 128: 11 in 64 x 64, 17 in 128 x 128; 384 x 384 -> 1536, 144 tiles of 64 x 64:
-  // 5.5, in the kernel for few tiles 8.0). fp32 products are bound by the matrix rate: smaller tiles with fewer
-  // stages, several workgroups a CU, one's epilogue beside another's products (40401 x 136 -> 257: 65 us, in one
+  // The larger the tile the less LDS is read a product, but a CU should have one at least, and the more of them it
+  // holds at once the better one's epilogue hides behind another's products. 16-bit types, us (4096 x 4096 -> 1024
+  // has 256 tiles of 128 x 128, one a CU; 16384 x 4096 -> 512 has two, 6977 x 384 -> 1024 440):
+  //   256 x 256 (4096^3: 136; 185 in 128 x 128) where its rounds of the card, four times as long as those of 128 x 128
+  //     and 1.2 times as fast, end before those of two 128 x 128 tiles a CU (45475 x 512 -> 512: 55 and 50);
+  //   128 x 128, two a CU, where there are more than CUs (6977 x 384 -> 1024: 18, one a CU and four stages 23;
+  //     16384 x 4096 -> 512: 76 and 92), or about one a CU with four stages (4096 x 4096 -> 1024: 44 and 60);
+  //   64 x 64, two or, where there are more, five a CU (2048 x 1024 -> 1024: 11, 17 in 128 x 128; 2048 x 384 -> 1536,
+  //     three a CU: 9.5, two at once 11.4);
+  //   few tiles: below (384 x 384 -> 1536, 144 tiles of 64 x 64: 5.5, in that kernel 8.0).
+  // fp32 products are bound by the matrix rate, and smaller tiles do (40401 x 136 -> 257: 65 us in 128 x 64, in one
   // workgroup of 128 x 128 a CU 90; 2048 x 1024 -> 1024, one tile of 128 x 64 a CU: 45 in 64 x 64, 52 in 128 x 64).
-  constexpr bool F32 = sizeof(T) == 4;
-  typedef Tile<T, 2, 2, 1, 1, 128, F32 ? 3 : 4> Small;
-  typedef Tile<T, 2, 2, 2, F32 ? 1 : 2, 128, F32 ? 2 : 4> Medium;
   const int64_t cus = compute_units();
-  if constexpr (!F32) {
+  if constexpr (sizeof(T) == 4) {
+    typedef Tile<T, 2, 2, 1, 1, 128, 3> Small;
+    typedef Tile<T, 2, 2, 2, 1, 128, 2> Medium;
+    if (tiles_of<Medium>(a) >= 2 * cus) return launch<T, PREC, Medium>(a, st);
+    if (tiles_of<Small>(a) >= cus / 2) return launch<T, PREC, Small>(a, st);
+  } else {
     typedef Tile<T, 2, 4, 4, 2, 128, 2> Large;
-    if (tiles_of<Large>(a) >= cus) return launch<T, PREC, Large>(a, st);
+    typedef Tile<T, 2, 2, 2, 2, 128, 2> Medium;
+    typedef Tile<T, 2, 2, 2, 2, 128, 4> MediumAlone;
+    typedef Tile<T, 2, 2, 1, 1, 128, 2> Small;
+    typedef Tile<T, 2, 2, 1, 1, 128, 4> SmallAlone;
+    const int64_t large = tiles_of<Large>(a), medium = tiles_of<Medium>(a), small = tiles_of<Small>(a);
+    const int64_t large_rounds = (large + cus - 1) / cus, medium_rounds = (medium + 2 * cus - 1) / (2 * cus);
+    if (large >= cus && 10 * 4 * large_rounds <= 12 * 2 * medium_rounds) return launch<T, PREC, Large>(a, st);
+    if (medium > cus) return launch<T, PREC, Medium>(a, st);
+    if (8 * medium >= 7 * cus) return launch<T, PREC, MediumAlone>(a, st);
+    if (small > 2 * cus) return launch<T, PREC, Small>(a, st);
+    if (small >= cus / 2) return launch<T, PREC, SmallAlone>(a, st);
   }
-  if (tiles_of<Medium>(a) >= (F32 ? 2 : 1) * cus) return launch<T, PREC, Medium>(a, st);
-  if (tiles_of<Small>(a) >= cus / 2) return launch<T, PREC, Small>(a, st);
   const int64_t few = (a.M + 31) / 32 * ((a.out_cols + 31) / 32);
   hipLaunchKernelGGL((linear_few_kernel<T, PREC>), dim3((uint32_t)few), dim3(FW_NT), 0, st, a);
   return (int)hipGetLastError();
