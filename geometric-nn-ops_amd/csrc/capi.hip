@@ -349,14 +349,6 @@ int gnn_rows_product(const gnn_rows_product_args* args, void* stream) {
   return hip_status((hipError_t)rc, "rows_product");
 }
 
-int gnn_rows_product_sums(const gnn_rows_product_args* args, float* sums, void* stream) {
-  if (int rc = check_rows_product(args, true)) return rc;
-  if (!sums || !aligned(sums, 4)) return set_error(GNN_ERR_ARG, "rows_product: sums is required, aligned to its elements");
-  int rc = rows_product(*args, sums, (hipStream_t)stream);
-  if (rc < 0) return rc;
-  return hip_status((hipError_t)rc, "rows_product");
-}
-
 int gnn_reduce_parts(const gnn_reduce_args* args, void* stream) {
   if (!args) return set_error(GNN_ERR_ARG, "reduce_parts: args is NULL");
   const gnn_reduce_args& a = *args;
@@ -553,6 +545,45 @@ int gnn_linear(const gnn_linear_args* args, void* stream) {
 int gnn_linear_takes_dx(const gnn_linear_args* args) { return args && args->dx && linear_takes_dx(*args) ? 1 : 0; }
 
 int gnn_linear_takes_transposed(const gnn_linear_args* args) { return args && linear_takes_transposed(*args) ? 1 : 0; }
+
+static gnn_rows_product_args wgrad_product(const gnn_linear_wgrad_args& a) {
+  gnn_rows_product_args r{};
+  r.rows = a.M, r.count = 1, r.dtype = a.dtype;
+  r.p[0] = {a.dz, a.x, a.partial, a.dz_ld, a.x_ld, a.O, a.I};
+  if (a.slices > 0 && a.M > 0) r.slice_rows = ((a.M + a.slices - 1) / a.slices + 31) / 32 * 32;
+  return r;
+}
+
+int64_t gnn_linear_wgrad_slices(const gnn_linear_wgrad_args* args) {
+  if (!args) return 0;
+  gnn_linear_wgrad_args a = *args;
+  a.slices = 0;
+  const gnn_rows_product_args r = wgrad_product(a);
+  return gnn_rows_product_slices(&r);
+}
+
+int gnn_linear_wgrad(const gnn_linear_wgrad_args* args, void* stream) {
+  if (!args) return set_error(GNN_ERR_ARG, "fused_linear gradients: args is NULL");
+  const gnn_linear_wgrad_args& a = *args;
+  if (a.slices < 1 || a.slices >= ((int64_t)1 << 31) || a.outputs < 1 || a.outputs > a.O)
+    return set_error(GNN_ERR_ARG, "fused_linear gradients: slices must be positive, outputs from 1 to O");
+  const gnn_rows_product_args r = wgrad_product(a);
+  if (int rc = check_rows_product(&r, true)) return rc;
+  const int bytes = a.dtype == GNN_F32 ? 4 : 2;
+  if (!a.dw || !aligned(a.dw, bytes) || !aligned(a.db, bytes) || !aligned(a.partial, 4))
+    return set_error(GNN_ERR_ARG, "fused_linear gradients: dw is required, dw, db and partial aligned to their elements");
+  const int64_t used = (a.M + r.slice_rows - 1) / r.slice_rows, each = a.O * a.I;
+  float* sums = a.db ? a.partial + used * each : nullptr;
+  int rc = rows_product(r, sums, (hipStream_t)stream);
+  if (rc == 0) {
+    gnn_reduce_args add{};
+    add.seg[add.count++] = {a.partial, a.dw, used, each, a.outputs * a.I, a.dtype, 0};
+    if (a.db) add.seg[add.count++] = {sums, a.db, used, a.O, a.outputs, a.dtype, 0};
+    rc = reduce_parts(add, (hipStream_t)stream);
+  }
+  if (rc < 0) return rc;
+  return hip_status((hipError_t)rc, "fused_linear gradients");
+}
 
 int gnn_pad_rows(const gnn_pad_rows_args* args, void* stream) {
   if (!args) return set_error(GNN_ERR_ARG, "pad_rows: args is NULL");

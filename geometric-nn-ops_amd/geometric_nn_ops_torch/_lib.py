@@ -423,6 +423,30 @@ class LinearArgs(ctypes.Structure):
 pack_linear = packer(LinearArgs)
 
 
+class LinearWgradArgs(ctypes.Structure):
+    """Mirror of ``gnn_linear_wgrad_args``."""
+
+    _fields_ = [
+        ("dz", ctypes.c_void_p),
+        ("x", ctypes.c_void_p),
+        ("partial", ctypes.c_void_p),
+        ("dw", ctypes.c_void_p),
+        ("db", ctypes.c_void_p),
+        ("M", ctypes.c_int64),
+        ("O", ctypes.c_int64),
+        ("I", ctypes.c_int64),
+        ("outputs", ctypes.c_int64),
+        ("dz_ld", ctypes.c_int64),
+        ("x_ld", ctypes.c_int64),
+        ("slices", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+pack_linear_wgrad = packer(LinearWgradArgs)
+
+
 class PadRowsArgs(ctypes.Structure):
     """Mirror of ``gnn_pad_rows_args``."""
 
@@ -580,7 +604,6 @@ _SIGNATURES = {
     "gnn_relayout_f32": (ctypes.c_int, [ctypes.POINTER(TrimulRelayoutArgs), ctypes.c_void_p]),
     "gnn_rows_product_slices": (ctypes.c_int64, [ctypes.POINTER(RowsProductArgs)]),
     "gnn_rows_product": (ctypes.c_int, [ctypes.POINTER(RowsProductArgs), ctypes.c_void_p]),
-    "gnn_rows_product_sums": (ctypes.c_int, [ctypes.POINTER(RowsProductArgs), ctypes.c_void_p, ctypes.c_void_p]),
     "gnn_reduce_parts": (ctypes.c_int, [ctypes.POINTER(ReduceArgs), ctypes.c_void_p]),
     "gnn_layer_norm_fwd": (ctypes.c_int, [ctypes.POINTER(LayerNormFwdArgs), ctypes.c_void_p]),
     "gnn_layer_norm_bwd_parts": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32]),
@@ -591,6 +614,8 @@ _SIGNATURES = {
     "gnn_linear_takes_dx": (ctypes.c_int, [ctypes.POINTER(LinearArgs)]),
     "gnn_linear_takes_transposed": (ctypes.c_int, [ctypes.POINTER(LinearArgs)]),
     "gnn_linear": (ctypes.c_int, [ctypes.POINTER(LinearArgs), ctypes.c_void_p]),
+    "gnn_linear_wgrad_slices": (ctypes.c_int64, [ctypes.POINTER(LinearWgradArgs)]),
+    "gnn_linear_wgrad": (ctypes.c_int, [ctypes.POINTER(LinearWgradArgs), ctypes.c_void_p]),
     "gnn_pad_rows": (ctypes.c_int, [ctypes.POINTER(PadRowsArgs), ctypes.c_void_p]),
     "gnn_column_sums_parts": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64]),
     "gnn_column_sums": (ctypes.c_int, [ctypes.POINTER(ColumnSumsArgs), ctypes.c_void_p]),

@@ -84,24 +84,20 @@ def fused_linear_hip(x, weight, bias=None, activation=None, residual=None, *, pr
     return _linear(_chunked(x.reshape(M, I)), _chunked(weight), bias, side, O, activation, precision).view(shape)
 
 
-def _weight_grad(dz, x, sums):
-    """fp32 partial sums of ``dz^T x`` and, with ``sums``, of dz's columns, over the same slices of rows."""
-    lib = _lib.load()
-    a = _lib.RowsProductArgs()
-    a.rows, a.count, a.dtype = dz.shape[0], 1, _lib.DTYPE_CODE[dz.dtype]
-    p, (O, I) = a.p[0], (dz.shape[1], x.shape[1])
-    p.d, p.t, p.d_ld, p.t_ld, p.O, p.I = dz.data_ptr(), x.data_ptr(), _pitch(dz), _pitch(x), O, I
-    slices = lib.gnn_rows_product_slices(ctypes.byref(a))
-    # that count depends on the device current here, the launch must not: pin its split
-    a.slice_rows = (-(-a.rows // slices) + 31) // 32 * 32
-    part = torch.empty((slices, O, I), device=dz.device, dtype=torch.float32)
-    p.partial = part.data_ptr()
-    if not sums:
-        _lib.call("gnn_rows_product", a, dz.device)
-        return part, None
-    sum_part = torch.empty((slices, O), device=dz.device, dtype=torch.float32)
-    _lib.call("gnn_rows_product_sums", a, dz.device, sum_part.data_ptr())
-    return part, sum_part
+def _parameter_grads(dz, x, outputs, want_b):
+    """``(dw, db)`` from chunked rows ``dz [M, >= outputs]`` and ``x [M, I]``: ``[outputs, I]`` and, where wanted,
+    ``[outputs]``."""
+    (M, O), I, dt, device = dz.shape, x.shape[1], dz.dtype, dz.device
+    dw = torch.empty((outputs, I), device=device, dtype=dt)
+    db = torch.empty((outputs,), device=device, dtype=dt) if want_b else None
+    a = _lib.LinearWgradArgs()
+    _lib.pack_linear_wgrad(a, 0, dz.data_ptr(), x.data_ptr(), 0, dw.data_ptr(), 0 if db is None else db.data_ptr(), M, O, I,
+                           outputs, _pitch(dz), _pitch(x), 0, _lib.DTYPE_CODE[dt], 0)
+    a.slices = _lib.load().gnn_linear_wgrad_slices(ctypes.byref(a))
+    part = torch.empty((a.slices, O * I + O), device=device, dtype=torch.float32)
+    a.partial = part.data_ptr()
+    _lib.call("gnn_linear_wgrad", a, device)
+    return dw, db
 
 
 def _column_sums(d, outputs):
@@ -137,16 +133,11 @@ def fused_linear_bwd_hip(x, weight, bias, activation, dy, *, precision, need_x=T
         if dx is None:
             dx = _linear(dz, w2, None, None, I, None, precision, transposed=True)
         dx = dx.view(x.shape)
-    segments = []
     if need_w:
-        part, sum_part = _weight_grad(dz, x2, need_b)
-        dw = torch.empty(part.shape[1:], device=x.device, dtype=x.dtype)
-        segments.append((part, 0, dw.numel(), dw))
-    if need_b:
+        dw, db = _parameter_grads(dz, x2, O, need_b)
+        if x2.shape[1] != I:
+            dw = dw[:, :I].contiguous()
+    elif need_b:
         db = torch.empty((O,), device=x.device, dtype=x.dtype)
-        segments.append((sum_part if need_w else _column_sums(dz, O), 0, O, db))
-    if segments:
-        reduce_parts_hip(segments, x.device)
-    if need_w and dw.shape != weight.shape:
-        dw = dw[:O, :I].contiguous()
+        reduce_parts_hip([(_column_sums(dz, O), 0, O, db)], x.device)
     return dx, dw, db

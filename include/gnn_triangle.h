@@ -553,10 +553,6 @@ typedef struct gnn_rows_product_args {
  * _reference/trimul.py:86-97); the reference has no kernel for them. */
 int64_t gnn_rows_product_slices(const gnn_rows_product_args* args);
 int gnn_rows_product(const gnn_rows_product_args* args, void* stream);
-/* The same, and the sums of the first product's d over the rows (a bias's gradient), as fp32 partial sums
- * [slices][O]. */
-int gnn_rows_product_sums(const gnn_rows_product_args* args, float* sums, void* stream);
-
 /* dst[e] = sum over p < parts of src[p * stride + e] (e < n), in a fixed order, for up to
  * GNN_REDUCE_MAX segments in one launch; dst is in the segment's dtype. Adds the partials that
  * gnn_rows_product, gnn_layernorm_rows, gnn_trimul_gate_bwd, gnn_trimul_proj_bwd and
@@ -696,6 +692,25 @@ int gnn_linear_takes_transposed(const gnn_linear_args* args);
  * be NULL then. */
 int gnn_linear_takes_dx(const gnn_linear_args* args);
 int gnn_linear(const gnn_linear_args* args, void* stream);
+
+/* The gradients of a linear layer's parameters from dz [M, O] and x [M, I]: dw[o][i] = sum over the rows of dz x for
+ * o < outputs, db[o] = sum over the rows of dz (db or NULL), in dtype. O, I and the pitches are multiples of 8
+ * (columns of dz past outputs are zeros), dz and x 16-byte aligned, dw is [outputs][I]. partial: fp32 [slices][O][I],
+ * and with db [slices][O] behind; slices as gnn_linear_wgrad_slices returns it (any from 1 on is right). */
+typedef struct gnn_linear_wgrad_args {
+  const void* dz;
+  const void* x;
+  float* partial;
+  void* dw;
+  void* db;
+  int64_t M, O, I, outputs;
+  int64_t dz_ld, x_ld;
+  int64_t slices;
+  int32_t dtype;
+  int32_t reserved;
+} gnn_linear_wgrad_args;
+int64_t gnn_linear_wgrad_slices(const gnn_linear_wgrad_args* args);
+int gnn_linear_wgrad(const gnn_linear_wgrad_args* args, void* stream);
 
 /* dst [rows, ld], contiguous and 16-byte aligned: src's cols columns (element (r, c) at r row_stride +
  * c col_stride) and zeros behind. ld a multiple of 16 bytes' elements, at least cols. */

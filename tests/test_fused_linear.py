@@ -119,7 +119,8 @@ def test_argument_errors():
 
 def test_args_match_the_c_layout(tmp_path):
     root = pathlib.Path(__file__).resolve().parent.parent
-    structs = {"gnn_linear_args": _lib.LinearArgs, "gnn_column_sums_args": _lib.ColumnSumsArgs}
+    structs = {"gnn_linear_args": _lib.LinearArgs, "gnn_column_sums_args": _lib.ColumnSumsArgs,
+               "gnn_linear_wgrad_args": _lib.LinearWgradArgs, "gnn_pad_rows_args": _lib.PadRowsArgs}
     body = "".join(f'printf("%zu\\n", sizeof({s}));' + "".join(
         f'printf("%zu\\n", offsetof({s}, {f[0]}));' for f in c._fields_) for s, c in structs.items())
     src = tmp_path / "layout.c"
@@ -131,16 +132,32 @@ def test_args_match_the_c_layout(tmp_path):
     assert [int(v) for v in out] == want
 
 
-def test_product_with_sums_refuses_missing_sums():
+def test_parameter_gradients_refuse_what_they_cannot_write():
     lib = _lib.load()
-    a = _lib.RowsProductArgs()
-    a.rows, a.count, a.dtype = 64, 1, _lib.GNN_BF16
-    p = a.p[0]
-    p.d, p.t, p.partial, p.d_ld, p.t_ld, p.O, p.I = 4096, 8192, 4096, 32, 16, 32, 16
-    assert lib.gnn_rows_product_sums(None, None, None) == _lib.GNN_ERR_ARG
-    assert lib.gnn_rows_product_sums(ctypes.byref(a), None, None) == _lib.GNN_ERR_ARG
-    assert b"sums" in lib.gnn_last_error()
-    assert lib.gnn_rows_product_sums(ctypes.byref(a), 4098, None) == _lib.GNN_ERR_ARG
+    a = _lib.LinearWgradArgs()
+
+    def refused(text):
+        assert lib.gnn_linear_wgrad(ctypes.byref(a), None) == _lib.GNN_ERR_ARG
+        assert text in lib.gnn_last_error(), lib.gnn_last_error()
+
+    assert lib.gnn_linear_wgrad(None, None) == _lib.GNN_ERR_ARG and lib.gnn_linear_wgrad_slices(None) == 0
+    a.dz, a.x, a.partial, a.dw = 4096, 8192, 4096, 4096
+    a.M, a.O, a.I, a.dz_ld, a.x_ld, a.dtype = 64, 32, 16, 32, 16, _lib.GNN_BF16
+    refused(b"slices")
+    a.slices = 1
+    for outputs in (0, 33):
+        a.outputs = outputs
+        refused(b"outputs")
+    a.outputs, a.dw = 30, None
+    refused(b"dw is required")
+    a.dw, a.db = 4096, 4097
+    refused(b"aligned")
+    a.db, a.partial = None, 4098
+    refused(b"")
+    a.partial, a.x = 4096, 8196
+    refused(b"")
+    a.x, a.O = 8192, 30
+    refused(b"")
 
 
 def test_calls_that_take_a_transposed_weight_or_dx():
