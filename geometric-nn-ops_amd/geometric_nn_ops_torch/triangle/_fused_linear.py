@@ -21,15 +21,18 @@ _KERNEL_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 class _FusedLinearHip(torch.autograd.Function):
-    """HIP forward and backward; the backward forms the activation's input again (nothing but the inputs is
-    kept) with the precision that the forward resolved, and records no graph: a second derivative raises."""
+    """HIP forward and backward; the backward forms the activation's input again from x and the weight (which are
+    kept as the kernels read them: themselves, or their padded copies) with the precision that the forward resolved,
+    and records no graph: a second derivative raises."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, activation, residual):
         ctx.precision = _precision.matmul_precision(fp32_operands=x.dtype == torch.float32)
         ctx.activation = activation
+        ctx.shape = x.shape
+        out, x, weight = _hip.fused_linear_hip(x, weight, bias, activation, residual, precision=ctx.precision, keep=True)
         ctx.save_for_backward(x, weight, bias)
-        return _hip.fused_linear_hip(x, weight, bias, activation, residual, precision=ctx.precision)
+        return out
 
     @staticmethod
     @once_differentiable
@@ -38,8 +41,8 @@ class _FusedLinearHip(torch.autograd.Function):
         need_x, need_w, need_b, _, need_r = ctx.needs_input_grad
         dx = dw = db = None
         if need_x or need_w or need_b:
-            dx, dw, db = _hip.fused_linear_bwd_hip(x, weight, bias, ctx.activation, dy, precision=ctx.precision,
-                                                   need_x=need_x, need_w=need_w, need_b=need_b)
+            dx, dw, db = _hip.fused_linear_bwd_hip(ctx.shape, x, weight, bias, ctx.activation, dy,
+                                                   precision=ctx.precision, need_x=need_x, need_w=need_w, need_b=need_b)
         return dx, dw, db, None, dy if need_r else None
 
 

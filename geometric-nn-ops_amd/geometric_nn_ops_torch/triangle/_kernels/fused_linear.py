@@ -72,16 +72,20 @@ def _linear(x, w, bias, side, outputs, activation, precision, *, dz=False, pad=F
     return (out, dx) if dz else out
 
 
-def fused_linear_hip(x, weight, bias=None, activation=None, residual=None, *, precision):
-    """``act(x weight^T + bias) + residual``, fresh and contiguous."""
+def fused_linear_hip(x, weight, bias=None, activation=None, residual=None, *, precision, keep=False):
+    """``act(x weight^T + bias) + residual``, fresh and contiguous; with ``keep`` ``(out, rows of x, weight)``, as
+    the kernels read them, for the backward."""
     O, I = weight.shape
     shape = (*x.shape[:-1], O)
     M = x.numel() // I
     if not M:
-        return torch.empty(shape, device=x.device, dtype=x.dtype)
+        out = torch.empty(shape, device=x.device, dtype=x.dtype)
+        return (out, x.reshape(0, I), weight) if keep else out
     side = None if residual is None else _unit(residual.reshape(M, O))
     bias = None if bias is None else bias.contiguous()
-    return _linear(_chunked(x.reshape(M, I)), _chunked(weight), bias, side, O, activation, precision).view(shape)
+    x, weight = _chunked(x.reshape(M, I)), _chunked(weight)
+    out = _linear(x, weight, bias, side, O, activation, precision).view(shape)
+    return (out, x, weight) if keep else out
 
 
 def _parameter_grads(dz, x, outputs, want_b):
@@ -111,18 +115,16 @@ def _column_sums(d, outputs):
     return part
 
 
-def fused_linear_bwd_hip(x, weight, bias, activation, dy, *, precision, need_x=True, need_w=True, need_b=True):
-    """``(dx, dweight, dbias)``, None where not needed. The activation's input is formed again from x and the
-    weight (in fp32); its gradient dz is rounded to x's dtype once, as the operand of the products."""
-    O, I = weight.shape
-    M = x.numel() // I
+def fused_linear_bwd_hip(shape, x2, w2, bias, activation, dy, *, precision, need_x=True, need_w=True, need_b=True):
+    """``(dx, dweight, dbias)``, None where not needed, for x of ``shape`` from what the forward kept. The
+    activation's input is formed again from x and the weight (in fp32); its gradient dz is rounded to x's dtype
+    once, as the operand of the products."""
+    M, O, I = x2.shape[0], w2.shape[0], shape[-1]
     if not M:
-        grads = (x, weight, weight[:, 0])
-        return tuple(torch.zeros(t.shape, device=x.device, dtype=x.dtype) if need else None
-                     for t, need in zip(grads, (need_x, need_w, need_b)))
+        grads = (shape, (O, I), (O,))
+        return tuple(torch.zeros(s, device=x2.device, dtype=x2.dtype) if need else None
+                     for s, need in zip(grads, (need_x, need_w, need_b)))
     dx = dw = db = None
-    x2 = _chunked(x.reshape(M, I))
-    w2 = _chunked(weight)
     dz = _unit(dy.reshape(M, O))
     if activation is not None:
         b = None if bias is None else bias.contiguous()
@@ -132,12 +134,12 @@ def fused_linear_bwd_hip(x, weight, bias, activation, dy, *, precision, need_x=T
     if need_x:
         if dx is None:
             dx = _linear(dz, w2, None, None, I, None, precision, transposed=True)
-        dx = dx.view(x.shape)
+        dx = dx.view(shape)
     if need_w:
         dw, db = _parameter_grads(dz, x2, O, need_b)
         if x2.shape[1] != I:
             dw = dw[:, :I].contiguous()
     elif need_b:
-        db = torch.empty((O,), device=x.device, dtype=x.dtype)
-        reduce_parts_hip([(_column_sums(dz, O), 0, O, db)], x.device)
+        db = torch.empty((O,), device=x2.device, dtype=x2.dtype)
+        reduce_parts_hip([(_column_sums(dz, O), 0, O, db)], x2.device)
     return dx, dw, db

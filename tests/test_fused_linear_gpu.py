@@ -395,3 +395,18 @@ def test_nothing_around_the_operands_is_read(m, i, o, act, dtype):
         results.append((y, *torch.autograd.grad(y, leaves, d)))
     for name, a, e in zip(("y", "dx", "dw", "db"), results[1], results[0]):
         assert torch.equal(a, e), name
+
+
+def test_operands_changed_in_place_before_the_backward():
+    """Refused where the graph keeps the operand itself; a padded copy keeps the forward's values."""
+    for i in (64, 61):
+        x, w, b, _, dy = (None if t is None else t.to(DEV) for t in _inputs(50, i, 40, torch.bfloat16, residual=False))
+        w.requires_grad_()
+        want = torch.autograd.grad(fused_linear(x, w, b, "silu"), w, dy)[0]
+        y = fused_linear(x, w, b, "silu")
+        x.zero_()
+        if i % 8 == 0:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                torch.autograd.grad(y, w, dy)
+        else:
+            assert torch.equal(torch.autograd.grad(y, w, dy)[0], want)
