@@ -93,5 +93,7 @@ def fused_linear(
         return fused_linear_torch(x, weight, bias, activation, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         return _FusedLinearHip.apply(x, weight, bias, activation, residual)
-    fwd = _ops.fused_linear_fwd_impl if _ops.eager_ok(x, weight, bias, residual) else _ops.fused_linear_fwd
-    return fwd(x, weight, bias, activation, residual)
+    if _ops.eager_ok(x, weight, bias, residual):
+        precision = _precision.matmul_precision(fp32_operands=x.dtype == torch.float32)
+        return _hip.fused_linear_hip(x, weight, bias, activation, residual, precision=precision)
+    return _ops.fused_linear_fwd(x, weight, bias, activation, residual)

@@ -21,13 +21,17 @@ def supports(weight: torch.Tensor) -> bool:
     return 1 <= weight.shape[0] <= MAX_WIDTH and 1 <= weight.shape[1] <= MAX_WIDTH
 
 
+def _pitch(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]  # one row's stride says nothing
+
+
 def _chunked(t: torch.Tensor) -> torch.Tensor:
     """``[R, C]`` rows of 16-byte chunks: C padded with zeros to a multiple of 8."""
     c = t.shape[1]
-    if t.shape[0] == 1 and t.stride(1) == 1:
-        t = t.as_strided((1, c), (c, 1))  # one row: its pitch says nothing
-    if c % 8 == 0 and t.stride(1) == 1 and t.stride(0) >= c and t.stride(0) * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0:
-        return t
+    if c % 8 == 0 and t.stride(1) == 1 and t.data_ptr() % 16 == 0:
+        pitch = _pitch(t)
+        if pitch >= c and pitch * t.element_size() % 16 == 0:
+            return t
     out = torch.empty((t.shape[0], (c + 7) // 8 * 8), device=t.device, dtype=t.dtype)
     a = _lib.PadRowsArgs()
     _lib.pack_pad_rows(a, 0, t.data_ptr(), out.data_ptr(), t.shape[0], c, out.shape[1], t.stride(0), t.stride(1),
@@ -39,10 +43,6 @@ def _chunked(t: torch.Tensor) -> torch.Tensor:
 def _unit(t: torch.Tensor) -> torch.Tensor:
     """``[R, C]`` with unit stride in a row, at any pitch and alignment."""
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
-
-
-def _pitch(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _linear(x, w, bias, side, outputs, activation, precision, *, dz=False, pad=False, transposed=False,
@@ -83,8 +83,10 @@ def fused_linear_hip(x, weight, bias=None, activation=None, residual=None, *, pr
         return (out, x.reshape(0, I), weight) if keep else out
     side = None if residual is None else _unit(residual.reshape(M, O))
     bias = None if bias is None else bias.contiguous()
-    x, weight = _chunked(x.reshape(M, I)), _chunked(weight)
-    out = _linear(x, weight, bias, side, O, activation, precision).view(shape)
+    x, weight = _chunked(x if x.dim() == 2 else x.reshape(M, I)), _chunked(weight)
+    out = _linear(x, weight, bias, side, O, activation, precision)
+    if len(shape) != 2:
+        out = out.view(shape)
     return (out, x, weight) if keep else out
 
 

@@ -83,5 +83,6 @@ def layer_norm(
         return layer_norm_torch(x, weight, bias, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return _LayerNormHip.apply(x, weight, bias, eps)
-    fwd = _ops.layer_norm_fwd_impl if _ops.eager_ok(x, weight, bias) else _ops.layer_norm_fwd
-    return fwd(x, weight, bias, eps)
+    if _ops.eager_ok(x, weight, bias):
+        return _hip.layer_norm_hip(x, weight, bias, eps)
+    return _ops.layer_norm_fwd(x, weight, bias, eps)

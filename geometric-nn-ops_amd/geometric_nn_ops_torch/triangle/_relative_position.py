@@ -120,6 +120,6 @@ def relative_position_bias(
         return relative_position_bias_torch(weight, query_pos, key_pos, *how)
     if torch.is_grad_enabled() and weight.requires_grad:
         return _RelativePositionHip.apply(weight, query_pos, key_pos, how)
-    fwd = (_ops.relative_position_bias_fwd_impl if _ops.eager_ok(weight, query_pos, key_pos)
-           else _ops.relative_position_bias_fwd)
-    return fwd(weight, query_pos, key_pos, *how)
+    if _ops.eager_ok(weight, query_pos, key_pos):
+        return _hip.relative_position_bias_hip(weight, query_pos, key_pos, *how)
+    return _ops.relative_position_bias_fwd(weight, query_pos, key_pos, *how)
