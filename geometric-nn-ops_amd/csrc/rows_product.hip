@@ -40,12 +40,12 @@ constexpr int RP_WGS = 2;
 // 16.1; 4096 rows stay at 128 with 22.6 us, at 64 24.3)
 constexpr int RP_MIN_ROWS = 256, RP_MIN_ROWS_F32 = 64, RP_FULL_ROWS_F32 = 128;
 
-template <typename T>
+template <typename T, int BLK>
 struct RowsProduct {
   static constexpr int STAGES = 4;
   static constexpr int RS = sizeof(T) == 2 ? 32 : 16;           // rows per stage
-  static constexpr int ROWB = RP_BLK * (int)sizeof(T);          // bytes per LDS row
-  static constexpr int OP_BYTES = RS * ROWB;                    // one operand's stage: 8 KB
+  static constexpr int ROWB = BLK * (int)sizeof(T);             // bytes per LDS row
+  static constexpr int OP_BYTES = RS * ROWB;                    // one operand's stage: 8 KB (BLK 64: 4)
   static constexpr int STAGE_BYTES = 2 * OP_BYTES;
   static constexpr int RPI = 1024 / ROWB;                       // rows per DMA instruction: 4 or 2
   static constexpr int Q = OP_BYTES / 1024 / 4;                 // DMA instructions per wave and operand: 2
@@ -101,10 +101,13 @@ struct RowsProductGrid {
 // SUMS: the first product's column sums of d beside it, sums[slice][O]: on the matrix unit as one more product,
 // with ones, of the fragments that the first 128 columns of t already hold in registers (fp32: added up there),
 // in the waves of their first half. A pass of its own over d took 23 us of 151 MB.
-template <typename T, bool SUMS>
-__global__ __launch_bounds__(RP_NT, RP_WGS) void rows_product_kernel(const gnn_rows_product_args a, const RowsProductGrid G,
-                                                                    float* sums) {
-  typedef RowsProduct<T> Cfg;
+// BLK: the output block's edge, 128 or, in fp32, 64 where a good part of the 128s would lie outside of C.
+template <typename T, bool SUMS, int BLK>
+__global__ __launch_bounds__(RP_NT, BLK == 64 ? 4 : RP_WGS) void rows_product_kernel(const gnn_rows_product_args a,
+                                                                                    const RowsProductGrid G, float* sums) {
+  typedef RowsProduct<T, BLK> Cfg;
+  constexpr int X = BLK / 64;  // 32 x 32 tiles of a wave, either way
+  static_assert(BLK == 128 || (BLK == 64 && sizeof(T) == 4), "16-bit stages are read two blocks at a time");
   __shared__ __align__(16) unsigned char smem[Cfg::LDS];
   const uint32_t w = xcd_remap(blockIdx.x, gridDim.x);
   int blk = (int)(w % (uint32_t)G.total), pi = 0;
@@ -112,8 +115,8 @@ __global__ __launch_bounds__(RP_NT, RP_WGS) void rows_product_kernel(const gnn_r
   while (blk >= G.nb[pi]) blk -= G.nb[pi++];
   const gnn_rows_product_item& P = a.p[pi];
   const int O = (int)P.O, I = (int)P.I;
-  const int nbi = (I + RP_BLK - 1) / RP_BLK;
-  const int o0 = blk / nbi * RP_BLK, i0 = blk % nbi * RP_BLK;
+  const int nbi = (I + BLK - 1) / BLK;
+  const int o0 = blk / nbi * BLK, i0 = blk % nbi * BLK;
   const int64_t m0 = slice * G.rps, m1 = min(m0 + G.rps, a.rows);
   const int nkt = (int)((m1 - m0 + Cfg::RS - 1) / Cfg::RS);
 
@@ -143,21 +146,23 @@ __global__ __launch_bounds__(RP_NT, RP_WGS) void rows_product_kernel(const gnn_r
   // fp32: two sums, of the even and the odd row pairs, added at the end: slices of 128 rows are 1.47e-7
   // off, in one sum 2.04e-7 (the vendor's products and sums over 64 slices lay between: weight gradients
   // at N = 64, c_z = c_hidden = 128 4.0e-7, here 3.9e-7, with one sum 4.3e-7)
-  f32x16 acc[2][2], odd[2][2];
+  f32x16 acc[X][X], odd[X][X];
 #pragma unroll
-  for (int x = 0; x < 2; ++x)
+  for (int x = 0; x < X; ++x)
 #pragma unroll
-    for (int y = 0; y < 2; ++y)
+    for (int y = 0; y < X; ++y)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[x][y][r] = odd[x][y][r] = 0.f;
 
   const bool summing = SUMS && pi == 0 && i0 == 0 && wn == 0;  // uniform in a wave
-  f32x16 sum16[2];
-  float sum32[2] = {0.f, 0.f};
+  f32x16 sum16[X];
+  float sum32[X];
 #pragma unroll
-  for (int x = 0; x < 2; ++x)
+  for (int x = 0; x < X; ++x) {
+    sum32[x] = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) sum16[x][r] = 0.f;
+  }
 
 #pragma unroll
   for (int st = 0; st < Cfg::STAGES - 1; ++st)
@@ -221,26 +226,26 @@ __global__ __launch_bounds__(RP_NT, RP_WGS) void rows_product_kernel(const gnn_r
         return *reinterpret_cast<const float*>(s + off + 2 * kk * Cfg::ROWB + ((b ^ g) << 7));
       };
       constexpr int KS = Cfg::RS / 2;
-      float xf[KS][2], yf[KS][2];
+      float xf[KS][X], yf[KS][X];
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          xf[kk][x] = col(sx, 2 * wm + x, kk);
-          yf[kk][x] = col(sy, 2 * wn + x, kk);
+        for (int x = 0; x < X; ++x) {
+          xf[kk][x] = col(sx, X * wm + x, kk);
+          yf[kk][x] = col(sy, X * wn + x, kk);
         }
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk)
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+        for (int x = 0; x < X; ++x)
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
+          for (int y = 0; y < X; ++y) {
             f32x16& s = kk % 2 ? odd[x][y] : acc[x][y];
             s = __builtin_amdgcn_mfma_f32_32x32x2f32(xf[kk][x], yf[kk][y], s, 0, 0, 0);
           }
       if (summing) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {  // a stage's rows in a tree of their own
+        for (int x = 0; x < X; ++x) {  // a stage's rows in a tree of their own
           float s = 0.f;
 #pragma unroll
           for (int kk = 0; kk < KS; ++kk) s += xf[kk][x];
@@ -253,8 +258,8 @@ __global__ __launch_bounds__(RP_NT, RP_WGS) void rows_product_kernel(const gnn_r
   if (summing) {
     float* out = sums + slice * O;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int o = o0 + 64 * wm + 32 * x;
+    for (int x = 0; x < X; ++x) {
+      const int o = o0 + 32 * (X * wm + x);
       if constexpr (sizeof(T) == 4) {  // rows of one parity a lane half, column l32
         const float s = pair_sum(sum32[x]);
         if (g == 0 && o + l32 < O) out[o + l32] = s;
@@ -268,26 +273,30 @@ __global__ __launch_bounds__(RP_NT, RP_WGS) void rows_product_kernel(const gnn_r
     }
   }
 
-  // acc[x][y][r] = C[o0 + 64 wm + 32 x + 8 (r / 4) + 4 g + r % 4][i0 + 64 wn + 32 y + l32]
+  // acc[x][y][r] = C[o0 + 32 (X wm + x) + 8 (r / 4) + 4 g + r % 4][i0 + 32 (X wn + y) + l32]
   float* out = P.partial + slice * (int64_t)O * I;
 #pragma unroll
-  for (int x = 0; x < 2; ++x)
+  for (int x = 0; x < X; ++x)
 #pragma unroll
-    for (int y = 0; y < 2; ++y) {
-      const int i = i0 + 64 * wn + 32 * y + l32;
+    for (int y = 0; y < X; ++y) {
+      const int i = i0 + 32 * (X * wn + y) + l32;
       if constexpr (sizeof(T) == 4) acc[x][y] += odd[x][y];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int o = o0 + 64 * wm + 32 * x + 8 * (r / 4) + 4 * g + (r % 4);
+        const int o = o0 + 32 * (X * wm + x) + 8 * (r / 4) + 4 * g + (r % 4);
         if (o < O && i < I) out[(int64_t)o * I + i] = acc[x][y][r];
       }
     }
 }
 
-RowsProductGrid rows_product_grid(const gnn_rows_product_args& a) {
+int64_t output_blocks(const gnn_rows_product_item& p, int blk) {
+  return ((p.O + blk - 1) / blk) * ((p.I + blk - 1) / blk);
+}
+
+RowsProductGrid rows_product_grid(const gnn_rows_product_args& a, int blk = RP_BLK) {
   RowsProductGrid G{};
   for (int i = 0; i < a.count; ++i) {
-    G.nb[i] = (int)(((a.p[i].O + RP_BLK - 1) / RP_BLK) * ((a.p[i].I + RP_BLK - 1) / RP_BLK));
+    G.nb[i] = (int)output_blocks(a.p[i], blk);
     G.total += G.nb[i];
   }
   if (a.slice_rows > 0) {
@@ -373,14 +382,26 @@ int64_t rows_product_slices(const gnn_rows_product_args& a) {
 
 template <bool SUMS>
 static int rows_product(const gnn_rows_product_args& a, float* sums, hipStream_t st) {
-  const RowsProductGrid G = rows_product_grid(a);
+  // a linear layer's own gradients: fp32 products in blocks of 64 x 64 (several workgroups a CU) where these cover
+  // less than 3/4 of the area (40401 rows, 264 x 136: 75 us with the ordered sum, in blocks of 128 86; 20000 rows,
+  // 72 x 40: 15 and 21; 512 x 128, the same area either way: 74, in blocks of 128 67)
+  const bool small = SUMS && a.dtype == GNN_F32 &&
+                     64 * 64 * 4 * output_blocks(a.p[0], 64) < 128 * 128 * 3 * output_blocks(a.p[0], 128);
+  const RowsProductGrid G = rows_product_grid(a, small ? 64 : RP_BLK);
   const int64_t nblk = (a.rows + G.rps - 1) / G.rps * G.total;
   if (nblk >= ((int64_t)1 << 31)) return set_error(GNN_ERR_UNSUPPORTED, "rows_product: grid too large");
   const dim3 grid((uint32_t)nblk), blk(RP_NT);
   switch (a.dtype) {
-    case GNN_BF16: hipLaunchKernelGGL((rows_product_kernel<bf16, SUMS>), grid, blk, 0, st, a, G, sums); break;
-    case GNN_F16: hipLaunchKernelGGL((rows_product_kernel<f16, SUMS>), grid, blk, 0, st, a, G, sums); break;
-    default: hipLaunchKernelGGL((rows_product_kernel<float, SUMS>), grid, blk, 0, st, a, G, sums); break;
+    case GNN_BF16: hipLaunchKernelGGL((rows_product_kernel<bf16, SUMS, RP_BLK>), grid, blk, 0, st, a, G, sums); break;
+    case GNN_F16: hipLaunchKernelGGL((rows_product_kernel<f16, SUMS, RP_BLK>), grid, blk, 0, st, a, G, sums); break;
+    default:
+      if constexpr (SUMS)
+        if (small) {
+          hipLaunchKernelGGL((rows_product_kernel<float, true, 64>), grid, blk, 0, st, a, G, sums);
+          break;
+        }
+      hipLaunchKernelGGL((rows_product_kernel<float, SUMS, RP_BLK>), grid, blk, 0, st, a, G, sums);
+      break;
   }
   return (int)hipGetLastError();
 }
