@@ -226,24 +226,31 @@ __global__ __launch_bounds__(FW_NT, 2) void linear_few_kernel(const LinArgs a) {
   const uint32_t ntn = (uint32_t)(a.out_cols + 31) / 32;
   const int n0 = (int)(blockIdx.x % ntn) * 32, m0 = (int)(blockIdx.x / ntn) * 32;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, g = lane >> 5;
-  // rows past the end repeat the last one; chunks past the contraction are zeros
+  // rows past the end repeat the last one
   const T* x = (const T*)a.x + min((int64_t)(m0 + l32), a.M - 1) * a.x_ld + 8 * g;
   const T* w = (const T*)a.w + (int64_t)min(n0 + tile_output(l32), a.O - 1) * a.w_ld + 8 * g;
-  const int steps = (a.I + 15) / 16, each = (steps + FW_NW - 1) / FW_NW;
-  const int k0 = wave * each, k1 = min(steps, k0 + each);
+  const int steps = (a.I + 15) / 16, whole = a.I / 16, each = (steps + FW_NW - 1) / FW_NW;
+  const int k0 = wave * each, k1 = min(whole, k0 + each);
   f32x16 acc;
 #pragma unroll
   for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+  // No load in a branch: a batch's last steps may be read again, and are not multiplied
   for (int k = k0; k < k1; k += FW_AHEAD) {
     V8 xf[FW_AHEAD], wf[FW_AHEAD];
 #pragma unroll
     for (int u = 0; u < FW_AHEAD; ++u) {
-      const bool in = k + u < k1 && 16 * (k + u) + 8 * g < a.I;
-      xf[u] = in ? load8_global(x + 16 * (k + u)) : zero8<T>();
-      wf[u] = in ? load8_global(w + 16 * (k + u)) : zero8<T>();
+      const int at = 16 * min(k + u, k1 - 1);
+      xf[u] = load8_global(x + at);
+      wf[u] = load8_global(w + at);
     }
 #pragma unroll
-    for (int u = 0; u < FW_AHEAD; ++u) Mma<T, PREC>::step(acc, wf[u], xf[u]);
+    for (int u = 0; u < FW_AHEAD; ++u)
+      if (k + u < k1) Mma<T, PREC>::step(acc, wf[u], xf[u]);
+  }
+  if (whole < steps && whole >= k0 && whole < k0 + each) {  // half a step: its other lanes hold zeros
+    V8 xf = zero8<T>(), wf = zero8<T>();
+    if (g == 0) xf = load8_global(x + 16 * whole), wf = load8_global(w + 16 * whole);
+    Mma<T, PREC>::step(acc, wf, xf);
   }
 #pragma unroll
   for (int q = 0; q < 4; ++q)
