@@ -32,9 +32,15 @@ def _chunked(t: torch.Tensor) -> torch.Tensor:
         pitch = _pitch(t)
         if pitch >= c and pitch * t.element_size() % 16 == 0:
             return t
-    out = torch.empty((t.shape[0], (c + 7) // 8 * 8), device=t.device, dtype=t.dtype)
+    return _padded(t, t.shape[0], c, t.stride(0), t.stride(1))
+
+
+def _padded(t, rows, cols, row_stride, col_stride):
+    """t's elements at these strides as ``[rows, cols padded with zeros to a multiple of 8]``."""
+    pitch = (cols + 7) // 8 * 8
+    out = torch.empty((rows, pitch), device=t.device, dtype=t.dtype)
     a = _lib.PadRowsArgs()
-    _lib.pack_pad_rows(a, 0, t.data_ptr(), out.data_ptr(), t.shape[0], c, out.shape[1], t.stride(0), t.stride(1),
+    _lib.pack_pad_rows(a, 0, t.data_ptr(), out.data_ptr(), rows, cols, pitch, row_stride, col_stride,
                        _lib.DTYPE_CODE[t.dtype], 0)
     _lib.call("gnn_pad_rows", a, t.device)
     return out
@@ -60,14 +66,16 @@ def _linear(x, w, bias, side, outputs, activation, precision, *, dz=False, pad=F
         ACTIVATION_CODE[activation], dz, transposed, _lib.DTYPE_CODE[x.dtype], _lib.PRECISION_CODE[precision], 0)
     # a weight of fewer rows than the padded columns of x has nothing to stand beside their zeros
     if transposed and (w.shape[0] < K or not _lib.load().gnn_linear_takes_transposed(ctypes.byref(a))):
-        w = _chunked(w[:, :outputs].t())
-        a.w, a.w_ld, a.w_transposed = w.data_ptr(), _pitch(w), 0
+        w = _padded(w, outputs, w.shape[0], 1, _pitch(w))
+        a.w, a.w_ld, a.w_transposed = w.data_ptr(), w.shape[1], 0
     dx = None
     if want_dx:
-        dx = torch.empty((M, K), device=x.device, dtype=x.dtype)
-        a.dx, a.dx_ld = dx.data_ptr(), K
-        if not _lib.load().gnn_linear_takes_dx(ctypes.byref(a)):
-            dx, a.dx = None, None
+        a.dx, a.dx_ld = a.out, K  # as aligned as what is allocated where the kernel takes it
+        if _lib.load().gnn_linear_takes_dx(ctypes.byref(a)):
+            dx = torch.empty((M, K), device=x.device, dtype=x.dtype)
+            a.dx = dx.data_ptr()
+        else:
+            a.dx = None
     _lib.call("gnn_linear", a, x.device)
     return (out, dx) if dz else out
 
@@ -136,7 +144,8 @@ def fused_linear_bwd_hip(shape, x2, w2, bias, activation, dy, *, precision, need
     if need_x:
         if dx is None:
             dx = _linear(dz, w2, None, None, I, None, precision, transposed=True)
-        dx = dx.view(shape)
+        if len(shape) != 2:
+            dx = dx.view(shape)
     if need_w:
         dw, db = _parameter_grads(dz, x2, O, need_b)
         if x2.shape[1] != I:
