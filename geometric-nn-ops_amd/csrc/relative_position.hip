@@ -367,8 +367,10 @@ __global__ __launch_bounds__(256) void relpos_last_bwd_kernel(const RpArgs a, in
   load_borders(a, border);
   for (int t = 0; t < 2 * count; ++t) bins[t * 64 + lane] = 0.f;
   __syncthreads();
-  const int c = c0 + 2 * lane;
-  const bool has0 = c < a.H, has1 = c + 1 < a.H;
+  // Two channels are there to be read for every lane: the last of an odd number comes with the one before it, and
+  // lanes past the last channel read along (their bins are not)
+  const int c = c0 + 2 * lane, read = min(c, a.H - 2);
+  const bool second = c == a.H - 1;
   const uint32_t groups = (uint32_t)(a.V + 63) / 64, items = (uint32_t)(a.B * a.U) * groups;
   const uint32_t w0 = min(items, (uint32_t)(part * waves + wave) * (uint32_t)a.rows), w1 = min(items, w0 + (uint32_t)a.rows);
   float2* const mybins = (float2*)bins + lane;
@@ -380,19 +382,14 @@ __global__ __launch_bounds__(256) void relpos_last_bwd_kernel(const RpArgs a, in
     const int b = (int)(r / (uint32_t)a.U), i = (int)(r - (uint32_t)b * (uint32_t)a.U);
     const P* kp = (const P*)a.kpos + b * a.k_bstride;
     const P q = ((const P*)a.qpos)[b * a.q_bstride + i];
-    const T* src = (const T*)a.dout + b * a.sb + i * a.si + c;
+    const T* src = (const T*)a.dout + b * a.sb + i * a.si + read;
     const int mine = bucket_of(a.bk, border, ahead_of(kp[min(j0 + lane, a.V - 1)], q, a.bk.far)) - first;
     const int n = min(64, a.V - j0);
     for (int p0 = 0; p0 < n; p0 += RP_BATCH) {
       V2 x[RP_BATCH];
 #pragma unroll
       for (int p = 0; p < RP_BATCH; ++p) {
-        const T* at = src + (int64_t)(j0 + min(p0 + p, n - 1)) * a.H;
-        x[p] = V2{(T)0.f, (T)0.f};
-        if (has1)
-          x[p] = *(const __attribute__((address_space(1))) V2U*)at;
-        else if (has0)
-          x[p][0] = at[0];
+        x[p] = *(const __attribute__((address_space(1))) V2U*)(src + (int64_t)(j0 + min(p0 + p, n - 1)) * a.H);
       }
 #pragma unroll
       for (int p = 0; p < RP_BATCH; ++p) {
@@ -403,7 +400,7 @@ __global__ __launch_bounds__(256) void relpos_last_bwd_kernel(const RpArgs a, in
           if ((unsigned)t < (unsigned)count) sum = mybins[t * 64];
           cur = t;
         }
-        sum.x += (float)x[p][0];
+        sum.x += (float)(second ? x[p][1] : x[p][0]);
         sum.y += (float)x[p][1];
       }
     }
@@ -415,6 +412,76 @@ __global__ __launch_bounds__(256) void relpos_last_bwd_kernel(const RpArgs a, in
     if (ch >= a.H) continue;
     float s = 0.f;
     for (int k = 0; k < waves; ++k) s += ((const float*)smem)[k * count * 128 + e];
+    a.partial[((int64_t)part * a.buckets + first + t) * a.H + ch] = s;
+  }
+}
+
+// The same for 2 to 64 channels, where one pixel would leave most lanes idle: `lanes` (a power of two, two
+// channels each) take a pixel and a wave 64 / lanes neighbouring ones at once, each group of lanes in bins of its
+// own. The buckets of RP_PIXELS pixels pass through LDS. (2048^2 x 16
+// channels, bf16: 50 us, a pixel a wave 470.)
+constexpr int RP_PIXELS = 256;
+template <typename T, typename P>
+__global__ __launch_bounds__(256) void relpos_last_narrow_bwd_kernel(const RpArgs a, int first, int count, int lanes) {
+  typedef T V2 __attribute__((ext_vector_type(2)));
+  typedef V2 V2U __attribute__((aligned(sizeof(T))));
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ int border[GNN_RELPOS_MAX_BORDERS + 2];
+  __shared__ uint16_t buckets[4][RP_PIXELS];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int at_once = 64 / lanes, sub = lane / lanes, c = 2 * (lane % lanes);
+  float* bins = (float*)smem + wave * count * 128;
+  load_borders(a, border);
+  for (int t = 0; t < 2 * count; ++t) bins[t * 64 + lane] = 0.f;
+  __syncthreads();
+  const int read = min(c, a.H - 2);  // as above
+  const bool second = c == a.H - 1;
+  const uint32_t groups = (uint32_t)(a.V + RP_PIXELS - 1) / RP_PIXELS, items = (uint32_t)(a.B * a.U) * groups;
+  const uint32_t part = blockIdx.x;
+  const uint32_t w0 = min(items, (part * waves + wave) * (uint32_t)a.rows), w1 = min(items, w0 + (uint32_t)a.rows);
+  float2* const mybins = (float2*)bins + lane;
+  int cur = -1;
+  float2 sum = {0.f, 0.f};
+  for (uint32_t w = w0; w < w1; ++w) {
+    const uint32_t r = w / groups;
+    const int j0 = (int)(w - r * groups) * RP_PIXELS;
+    const int b = (int)(r / (uint32_t)a.U), i = (int)(r - (uint32_t)b * (uint32_t)a.U);
+    const P* kp = (const P*)a.kpos + b * a.k_bstride;
+    const P q = ((const P*)a.qpos)[b * a.q_bstride + i];
+    const T* src = (const T*)a.dout + b * a.sb + i * a.si + (int64_t)j0 * a.H + read;
+    const int n = min(RP_PIXELS, a.V - j0);
+#pragma unroll
+    for (int k = 0; k < RP_PIXELS / 64; ++k) {  // a wave's LDS accesses stay in order
+      const int p = 64 * k + lane;
+      const int t = bucket_of(a.bk, border, ahead_of(kp[min(j0 + p, a.V - 1)], q, a.bk.far));
+      buckets[wave][p] = p < n ? (uint16_t)t : (uint16_t)0xffff;  // in no pass's range
+    }
+    for (int p0 = 0; p0 < n; p0 += RP_BATCH * at_once) {
+      V2 x[RP_BATCH];
+#pragma unroll
+      for (int k = 0; k < RP_BATCH; ++k)
+        x[k] = *(const __attribute__((address_space(1))) V2U*)(src + min(p0 + k * at_once + sub, n - 1) * a.H);
+#pragma unroll
+      for (int k = 0; k < RP_BATCH; ++k) {
+        if (p0 + k * at_once >= n) break;  // uniform
+        const int t = (int)buckets[wave][p0 + k * at_once + sub] - first;
+        if (t != cur) {
+          if ((unsigned)cur < (unsigned)count) mybins[cur * 64] = sum;
+          if ((unsigned)t < (unsigned)count) sum = mybins[t * 64];
+          cur = t;
+        }
+        sum.x += (float)(second ? x[k][1] : x[k][0]);
+        sum.y += (float)x[k][1];
+      }
+    }
+  }
+  if ((unsigned)cur < (unsigned)count) mybins[cur * 64] = sum;
+  __syncthreads();
+  for (int e = threadIdx.x; e < count * a.H; e += blockDim.x) {
+    const int t = e / a.H, ch = e - t * a.H;
+    float s = 0.f;
+    for (int k = 0; k < waves; ++k)
+      for (int g = 0; g < at_once; ++g) s += ((const float*)smem)[(k * count + t) * 128 + g * 2 * lanes + ch];
     a.partial[((int64_t)part * a.buckets + first + t) * a.H + ch] = s;
   }
 }
@@ -486,7 +553,11 @@ Bins bins_of(const gnn_relpos_args& g) {
   return b;
 }
 int64_t across(const gnn_relpos_args& g) { return g.channels_last ? (g.H + 127) / 128 : g.H; }
-int64_t bwd_items(const gnn_relpos_args& g) { return g.B * g.U * (g.channels_last ? (g.V + 63) / 64 : 1); }
+bool narrow(const gnn_relpos_args& g) { return g.channels_last && g.H <= 64; }
+int64_t bwd_items(const gnn_relpos_args& g) {
+  const int64_t pixels = narrow(g) ? RP_PIXELS : 64;
+  return g.B * g.U * (g.channels_last ? (g.V + pixels - 1) / pixels : 1);
+}
 
 template <typename T, typename P>
 int backward(const gnn_relpos_args& g, hipStream_t st) {
@@ -500,10 +571,16 @@ int backward(const gnn_relpos_args& g, hipStream_t st) {
     const int n = std::min(bins.count, a.buckets - first);
     const size_t lds = (size_t)bins.waves * n * (bins.bytes / bins.count) +
                        (!g.channels_last && a.bk.far <= RP_LUT_FAR ? 2 * (2 * a.bk.far + 2) : 0);
-    if (lds > 64 * 1024)
-      (void)hipFuncSetAttribute((const void*)relpos_last_bwd_kernel<T, P>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)lds);
-    if (g.channels_last)
+    if (lds > 64 * 1024) {
+      const void* fn = narrow(g) ? (const void*)relpos_last_narrow_bwd_kernel<T, P> : (const void*)relpos_last_bwd_kernel<T, P>;
+      (void)hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    }
+    if (narrow(g)) {
+      int lanes = 1;
+      while (2 * lanes < a.H) lanes *= 2;
+      hipLaunchKernelGGL((relpos_last_narrow_bwd_kernel<T, P>), dim3((uint32_t)grid), dim3(64 * bins.waves), lds, st, a, first,
+                         n, lanes);
+    } else if (g.channels_last)
       hipLaunchKernelGGL((relpos_last_bwd_kernel<T, P>), dim3((uint32_t)grid), dim3(64 * bins.waves), lds, st, a, first, n);
     else
       hipLaunchKernelGGL((relpos_bwd_kernel<T, P>), dim3((uint32_t)grid), dim3(64), lds, st, a, first, n);
@@ -522,7 +599,14 @@ int by_dtype(const gnn_relpos_args& g, bool bwd, hipStream_t st) {
 
 }  // namespace
 
-int relpos(const gnn_relpos_args& g, bool bwd, hipStream_t st) {
+// One channel last is one head first
+static gnn_relpos_args one_layout(gnn_relpos_args g) {
+  if (g.H == 1) g.channels_last = 0;
+  return g;
+}
+
+int relpos(const gnn_relpos_args& args, bool bwd, hipStream_t st) {
+  const gnn_relpos_args g = one_layout(args);
   const int64_t most = (int64_t)1 << 31;
   if (g.B * g.U >= most || (g.channels_last && g.B * g.U * ((g.V * g.H + 63) / 64 + 1) >= most))
     return set_error(GNN_ERR_UNSUPPORTED, "relative_position_bias: more than 2^31 rows or pieces of rows");
@@ -532,7 +616,8 @@ int relpos(const gnn_relpos_args& g, bool bwd, hipStream_t st) {
 }
 
 // Rows of partial sums: as many workgroups as the card holds by their bins, not more than there is work
-int64_t relpos_parts(const gnn_relpos_args& g) {
+int64_t relpos_parts(const gnn_relpos_args& args) {
+  const gnn_relpos_args g = one_layout(args);
   if (g.buckets > RP_MAX_BUCKETS) return 0;
   const Bins b = bins_of(g);
   const int64_t per_cu = std::max<int64_t>(1, std::min<int64_t>(16 / b.waves, (150 << 10) / (b.bytes * b.waves)));

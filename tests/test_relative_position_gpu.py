@@ -241,3 +241,27 @@ def test_the_borders_live_as_long_as_the_graph():
             others = [(type(kernels._borders(16, 8, 99)))(*range(1, 8)) for _ in range(2000)]  # noqa: F841
         grads.append(torch.autograd.grad(y, table, torch.ones_like(y))[0])
     assert torch.equal(*grads)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("h", [1, 2, 3, 5, 8, 16, 31, 33, 64, 65, 129, 200])
+def test_channels_last_of_every_width(h, dtype):
+    """The gradient of narrow tables, whose channels leave room for several pixels in a wave, and of odd ones;
+    the output gradient lies between NaN."""
+    u, v, far = 7, 301, 5
+    g = torch.Generator().manual_seed(h)
+    w = torch.randn(2 * far + 1, h, generator=g).to(dtype)
+    q = torch.randint(-9, 300, (2, u), generator=g)
+    k = torch.randint(-9, 300, (2, v), generator=g)
+    dout = torch.randn(2, u, v, h, generator=g).to(dtype)
+    at = (k[:, None, :] - q[:, :, None]).clamp(-far, far) + far
+    want = torch.zeros(2 * far + 1, h, dtype=torch.float64).index_add_(0, at.reshape(-1), dout.double().reshape(-1, h))
+    size = torch.zeros(2 * far + 1, h, dtype=torch.float64).index_add_(0, at.reshape(-1), dout.double().abs().reshape(-1, h))
+    table = w.to(DEV).requires_grad_()
+    y = relative_position_bias(table, q.to(DEV), k.to(DEV), max_distance=far, spacing="clip", channels_last=True)
+    assert torch.equal(y.detach().cpu(), w[at])
+    buf = torch.full((dout.numel() + 512,), float("nan"), device=DEV, dtype=dtype)
+    inner = buf[256:256 + dout.numel()].view(dout.shape)
+    inner.copy_(dout)
+    grad = torch.autograd.grad(y, table, inner)[0]
+    assert_within(f"gradient of {h} channels", grad, want, 100 * U * size)
