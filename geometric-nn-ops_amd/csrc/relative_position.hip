@@ -20,7 +20,7 @@
 // 2048^2 x 16 heads, bf16, log, 134 MB: forward 29 us (4.6 TB/s), backward 51 (2.6: the blocks of keys
 // across the diagonal, whose lanes look buckets up and add to bins, and each wave's set-up; the next loads issued a
 // turn ahead 55, half or twice the waves 68 and 62). 509^2 x 128
-// channels, clip, 66 MB: 19 (3.5 TB/s) and 38 (1.7: the chain of bins; half or twice the workgroups 58 and 50).
+// channels, clip, 66 MB: 19 (3.5 TB/s) and 32 (2.1: the chain of bins; half or twice the workgroups 47 and 45).
 #include <algorithm>
 
 #include "gnn_common.hpp"
