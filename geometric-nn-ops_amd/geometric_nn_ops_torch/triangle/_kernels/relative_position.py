@@ -43,7 +43,7 @@ def relative_position_bias_hip(weight, query_pos, key_pos, max_distance, spacing
                                keep=False):
     """``[B, H, U, V]``, a view with a row pitch rounded up to 8 elements (what the attention kernels read
     without a copy), or the contiguous ``[B, U, V, H]``. With ``keep`` ``(out, args, query_pos, key_pos)``: the
-    call's arguments (None for an empty result) and the positions that they point to, for the backward."""
+    call's arguments (None for an empty result) and its positions, for the backward."""
     B, U = query_pos.shape
     V, (buckets, H) = key_pos.shape[1], weight.shape
     query_pos, key_pos, weight = _pos(query_pos), _pos(key_pos), weight.contiguous()
@@ -72,8 +72,9 @@ def relative_position_bias_hip(weight, query_pos, key_pos, max_distance, spacing
     return (out, a, query_pos, key_pos) if keep else out
 
 
-def relative_position_bias_bwd_hip(shape, args, dout):
-    """The table's gradient ``[buckets, H]`` in dout's dtype, from the forward's kept arguments."""
+def relative_position_bias_bwd_hip(shape, args, query_pos, key_pos, dout):
+    """The table's gradient ``[buckets, H]`` in dout's dtype, from the forward's kept shape and buckets and its
+    positions, wherever they lie now."""
     grad = torch.empty(shape, device=dout.device, dtype=dout.dtype)
     if args is None:
         return grad.zero_()
@@ -90,6 +91,10 @@ def relative_position_bias_bwd_hip(shape, args, dout):
         strides = (s0, s1, s2)
     a = _lib.RelposArgs.from_buffer_copy(args)  # a graph that is kept may run its backward again, on any thread
     a.stride = strides
+    query_pos, key_pos = _pos(query_pos), _pos(key_pos)
+    a.query_pos, a.query_stride, a.key_pos, a.key_stride = (
+        query_pos.data_ptr(), query_pos.stride(0), key_pos.data_ptr(), key_pos.stride(0))
+    a.table = a.out = None  # the forward's
     parts = _lib.load().gnn_relpos_parts(ctypes.byref(a))
     part = torch.empty((parts, *shape), device=dout.device, dtype=torch.float32)
     a.dout, a.parts, a.partial, a.dtable = dout.data_ptr(), parts, part.data_ptr(), grad.data_ptr()

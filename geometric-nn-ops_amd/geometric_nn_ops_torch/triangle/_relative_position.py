@@ -35,8 +35,9 @@ class _RelativePositionHip(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        _ = ctx.saved_tensors  # what args points to, checked for changes in place
-        return _hip.relative_position_bias_bwd_hip(ctx.shape, ctx.args, dout), None, None, None
+        # what saved-tensor hooks and checkpoints hand back may lie elsewhere than what the forward read
+        query_pos, key_pos = ctx.saved_tensors
+        return _hip.relative_position_bias_bwd_hip(ctx.shape, ctx.args, query_pos, key_pos, dout), None, None, None
 
 
 def _check(weight, query_pos, key_pos, max_distance, spacing, bidirectional) -> None:

@@ -1,0 +1,52 @@
+"""Gradients under saved-tensor hooks and activation checkpoints: the same bits as without them."""
+
+import pytest
+import torch
+from torch.autograd.graph import save_on_cpu, saved_tensors_hooks
+from torch.utils.checkpoint import checkpoint
+
+from geometric_nn_ops_torch.triangle import relative_position_bias
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _under(kind, block, *leaves):
+    """The block's output with what it saves kept as ``kind`` says, and nothing else holding it."""
+    if kind == "checkpoint":
+        return checkpoint(block, *leaves, use_reentrant=False)
+    if kind == "cpu":
+        with save_on_cpu():
+            return block(*leaves)
+    with saved_tensors_hooks(torch.clone, lambda t: t):
+        return block(*leaves)
+
+
+def _same_gradients(block, leaves, dout):
+    """The gradients without hooks, and bit for bit the same ones under each kind of them, with the memory that
+    the forward left free taken by other values before the backward."""
+    plain = torch.autograd.grad(block(*leaves), leaves, dout)
+    for kind in ("clone", "cpu", "checkpoint"):
+        out = _under(kind, block, *leaves)
+        taken = [torch.full((1 << k,), -999, device=DEV, dtype=torch.int64) for k in range(4, 18) for _ in range(4)]
+        got = torch.autograd.grad(out, leaves, dout)
+        del taken
+        for a, e in zip(got, plain):
+            assert torch.equal(a, e), kind
+
+
+@pytest.mark.parametrize("last", [False, True], ids=["heads_first", "heads_last"])
+@pytest.mark.parametrize("mixed", [False, True], ids=["one_type", "mixed_types"])
+def test_relative_position_bias(last, mixed):
+    """Positions made inside the block, those of mixed types converted there once more."""
+    u, v, h = 70, 131, 6
+    table = torch.randn(32, h, generator=torch.Generator().manual_seed(1)).to(DEV).requires_grad_()
+    dout = torch.randn((2, u, v, h) if last else (2, h, u, v), generator=torch.Generator().manual_seed(2)).to(DEV)
+    base = torch.arange(2 * v, device=DEV).view(2, v) * 3
+
+    def block(t):
+        k = base + 5
+        q = k[:, -u:] - 40
+        return relative_position_bias(t, q.int() if mixed else q, k, max_distance=128, channels_last=last)
+
+    _same_gradients(block, [table], dout)
