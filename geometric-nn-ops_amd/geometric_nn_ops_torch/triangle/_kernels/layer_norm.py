@@ -53,6 +53,7 @@ def layer_norm_bwd_hip(x, weight, stats, dy, *, need_dx=True, dweight=None, dbia
     gr, _, ginner, gouter, gstride = as_rows(dy)
     dt = _lib.DTYPE_CODE[x.dtype]
     w = None if weight is None else weight.contiguous()
+    stats = stats.contiguous()  # two rows, one behind the other, in whatever pitch saved-tensor hooks return them
     part = None
     parts = _lib.load().gnn_layer_norm_bwd_parts(rows, K, dt)
     if dweight is not None or dbias is not None:

@@ -10,7 +10,7 @@ from torch.autograd.graph import saved_tensors_hooks
 from torch.utils.checkpoint import checkpoint
 
 from geometric_nn_ops_torch import _lib
-from geometric_nn_ops_torch.triangle import _relative_position
+from geometric_nn_ops_torch.triangle import _layer_norm, _relative_position
 
 
 @pytest.fixture
@@ -22,7 +22,8 @@ def recorded(monkeypatch):
         calls.append((name, type(args).from_buffer_copy(args)))
 
     monkeypatch.setattr(_lib, "call", call)
-    monkeypatch.setattr(_lib, "load", lambda: types.SimpleNamespace(gnn_relpos_parts=lambda a: 1))
+    monkeypatch.setattr(_lib, "load", lambda: types.SimpleNamespace(
+        gnn_relpos_parts=lambda a: 1, gnn_layer_norm_bwd_parts=lambda *a: 1))
     return calls
 
 
@@ -78,3 +79,29 @@ def test_relative_position_in_a_checkpoint_reads_the_recomputed_positions(record
     first, again, bwd = (a for _, a in recorded)
     assert first.query_pos != again.query_pos and len(taken) == 64
     assert (bwd.query_pos, bwd.key_pos) == (again.query_pos, again.key_pos)
+
+
+def test_layer_norm_reads_the_unpacked_statistics(monkeypatch):
+    """Each row's mean and 1 / standard deviation, whatever pitch they come back in."""
+    rows, found = 6, []
+
+    def floats(address):
+        return [ctypes.c_float.from_address(address + 4 * r).value for r in range(rows)]
+
+    def call(name, args, device):
+        if name == "gnn_layer_norm_fwd":
+            for at, base in ((args.mean, 10.0), (args.rstd, 20.0)):
+                for r in range(rows):
+                    ctypes.c_float.from_address(at + 4 * r).value = base + r
+        else:
+            found.append(floats(args.mean) + floats(args.rstd))
+
+    monkeypatch.setattr(_lib, "call", call)
+    monkeypatch.setattr(_lib, "load", lambda: types.SimpleNamespace(gnn_layer_norm_bwd_parts=lambda *a: 1))
+    x = torch.randn(rows, 16, requires_grad=True)
+    for pack in (torch.clone, lambda t: torch.nn.functional.pad(t, (0, 5))[..., :t.shape[-1]],
+                 lambda t: t.t().contiguous().t() if t.dim() == 2 else t):
+        with saved_tensors_hooks(pack, lambda t: t):
+            y = _layer_norm._LayerNormHip.apply(x, None, None, 1e-5)
+        y.backward(torch.ones_like(y))
+        assert found.pop() == [10.0 + r for r in range(rows)] + [20.0 + r for r in range(rows)]

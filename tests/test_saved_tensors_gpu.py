@@ -5,7 +5,7 @@ import torch
 from torch.autograd.graph import save_on_cpu, saved_tensors_hooks
 from torch.utils.checkpoint import checkpoint
 
-from geometric_nn_ops_torch.triangle import relative_position_bias
+from geometric_nn_ops_torch.triangle import layer_norm, relative_position_bias
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -50,3 +50,11 @@ def test_relative_position_bias(last, mixed):
         return relative_position_bias(t, q.int() if mixed else q, k, max_distance=128, channels_last=last)
 
     _same_gradients(block, [table], dout)
+
+
+def test_layer_norm():
+    g = torch.Generator().manual_seed(3)
+    x, dy = (torch.randn(301, 96, generator=g).bfloat16().to(DEV) for _ in range(2))
+    weight, bias = (torch.randn(96, generator=g).to(DEV) for _ in range(2))
+    leaves = [t.requires_grad_() for t in (x, weight, bias)]
+    _same_gradients(lambda x, w, b: layer_norm(x * 1.5, w, b), leaves, dy)
