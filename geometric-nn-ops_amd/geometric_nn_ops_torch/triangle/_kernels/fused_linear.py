@@ -134,6 +134,7 @@ def fused_linear_bwd_hip(shape, x2, w2, bias, activation, dy, *, precision, need
         grads = (shape, (O, I), (O,))
         return tuple(torch.zeros(s, device=x2.device, dtype=x2.dtype) if need else None
                      for s, need in zip(grads, (need_x, need_w, need_b)))
+    x2, w2 = _chunked(x2), _chunked(w2)  # as kept, but where saved-tensor hooks return them in another layout
     dx = dw = db = None
     dz = _unit(dy.reshape(M, O))
     if activation is not None:

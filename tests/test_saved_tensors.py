@@ -10,7 +10,7 @@ from torch.autograd.graph import saved_tensors_hooks
 from torch.utils.checkpoint import checkpoint
 
 from geometric_nn_ops_torch import _lib
-from geometric_nn_ops_torch.triangle import _layer_norm, _relative_position
+from geometric_nn_ops_torch.triangle import _fused_linear, _layer_norm, _relative_position
 
 
 @pytest.fixture
@@ -105,3 +105,46 @@ def test_layer_norm_reads_the_unpacked_statistics(monkeypatch):
             y = _layer_norm._LayerNormHip.apply(x, None, None, 1e-5)
         y.backward(torch.ones_like(y))
         assert found.pop() == [10.0 + r for r in range(rows)] + [20.0 + r for r in range(rows)]
+
+
+def test_fused_linear_reads_unpacked_operands_in_whole_chunks(monkeypatch):
+    """The kernels take x and the weight in aligned 16-byte chunks, wherever the two come back."""
+    m, i, o = 6, 16, 8
+    x, w = torch.randn(m, i, requires_grad=True), torch.randn(o, i, requires_grad=True)
+    found = []
+
+    def rows(address, ld, n, k):
+        assert address % 16 == 0 and ld % 4 == 0 and ld >= k
+        return torch.tensor([[ctypes.c_float.from_address(address + 4 * (r * ld + j)).value for j in range(k)]
+                             for r in range(n)])
+
+    def call(name, args, device):
+        if name == "gnn_linear" and args.dz:
+            found.append((rows(args.x, args.x_ld, m, i), rows(args.w, args.w_ld, o, i)))
+        elif name == "gnn_linear_wgrad":
+            found.append(rows(args.x, args.x_ld, m, i))
+        elif name == "gnn_pad_rows":  # copies element by element
+            for r in range(args.rows):
+                for c in range(args.ld):
+                    at = args.src + 4 * (r * args.row_stride + c * args.col_stride)
+                    ctypes.c_float.from_address(args.dst + 4 * (r * args.ld + c)).value = (
+                        ctypes.c_float.from_address(at).value if c < args.cols else 0.0)
+
+    monkeypatch.setattr(_lib, "call", call)
+    monkeypatch.setattr(_lib, "load", lambda: types.SimpleNamespace(
+        gnn_linear_takes_transposed=lambda a: 0, gnn_linear_takes_dx=lambda a: 0, gnn_linear_wgrad_slices=lambda a: 1))
+
+    def shifted(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype)[1:]
+        return flat.copy_(t.reshape(-1)).view(t.shape)
+
+    def spread(t):
+        return torch.stack([t, -t], -1)[..., 0]
+
+    for pack in (torch.clone, shifted, spread, lambda t: t.t().contiguous().t()):
+        with saved_tensors_hooks(pack, lambda t: t):
+            y = _fused_linear._FusedLinearHip.apply(x, w, None, "silu", None)
+        torch.autograd.grad(y, (x, w), torch.ones_like(y))
+        (in_dz, weight), in_dw = found
+        found.clear()
+        assert torch.equal(in_dz, x) and torch.equal(weight, w) and torch.equal(in_dw, x)

@@ -5,7 +5,7 @@ import torch
 from torch.autograd.graph import save_on_cpu, saved_tensors_hooks
 from torch.utils.checkpoint import checkpoint
 
-from geometric_nn_ops_torch.triangle import layer_norm, relative_position_bias
+from geometric_nn_ops_torch.triangle import fused_linear, layer_norm, relative_position_bias
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -58,3 +58,30 @@ def test_layer_norm():
     weight, bias = (torch.randn(96, generator=g).to(DEV) for _ in range(2))
     leaves = [t.requires_grad_() for t in (x, weight, bias)]
     _same_gradients(lambda x, w, b: layer_norm(x * 1.5, w, b), leaves, dy)
+
+
+@pytest.mark.parametrize("m,i,o", [(45, 40, 24), (300, 61, 13), (32800, 64, 72)])
+def test_fused_linear(m, i, o):
+    g = torch.Generator().manual_seed(4)
+    x, r, dy = (torch.randn(m, k, generator=g).bfloat16().to(DEV) for k in (i, o, o))
+    w, b = (torch.randn(*s, generator=g).mul(i ** -0.5).bfloat16().to(DEV) for s in ((o, i), (o,)))
+    leaves = [t.requires_grad_() for t in (x, w, b, r)]
+    _same_gradients(lambda x, w, b, r: fused_linear(x * 1.5, w, b, "silu", r), leaves, dy)
+
+
+def test_fused_linear_from_unaligned_operands():
+    """Hooks that keep what they are given in one flat buffer return it at any address."""
+    m, i, o = 45, 40, 24
+    g = torch.Generator().manual_seed(5)
+    x, dy = (torch.randn(m, k, generator=g).bfloat16().to(DEV) for k in (i, o))
+    w = torch.randn(o, i, generator=g).mul(i ** -0.5).bfloat16().to(DEV)
+    leaves = [t.requires_grad_() for t in (x, w)]
+    plain = torch.autograd.grad(fused_linear(x, w, None, "gelu"), leaves, dy)
+
+    def shifted(t):
+        return torch.empty(t.numel() + 1, device=DEV, dtype=t.dtype)[1:].copy_(t.reshape(-1)).view(t.shape)
+
+    with saved_tensors_hooks(shifted, lambda t: t):
+        y = fused_linear(x, w, None, "gelu")
+    for a, e in zip(torch.autograd.grad(y, leaves, dy), plain):
+        assert torch.equal(a, e)
