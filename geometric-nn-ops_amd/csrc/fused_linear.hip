@@ -247,9 +247,16 @@ __global__ __launch_bounds__(FW_NT, 2) void linear_few_kernel(const LinArgs a) {
     for (int u = 0; u < FW_AHEAD; ++u)
       if (k + u < k1) Mma<T, PREC>::step(acc, wf[u], xf[u]);
   }
-  if (whole < steps && whole >= k0 && whole < k0 + each) {  // half a step: its other lanes hold zeros
+  if (whole < steps && whole >= k0 && whole < k0 + each) {  // part of a step: what lies past the row's end is zero
     V8 xf = zero8<T>(), wf = zero8<T>();
-    if (g == 0) xf = load8_global(x + 16 * whole), wf = load8_global(w + 16 * whole);
+    const int left = a.I - 16 * whole - 8 * g;  // of this lane's 8 elements
+    if (left >= 8) {
+      xf = load8_global(x + 16 * whole), wf = load8_global(w + 16 * whole);
+    } else if (sizeof(T) == 4 && left > 0) {  // fp32 rows of 16-byte chunks may end after 4
+      const auto xh = load4(x + 16 * whole), wh = load4(w + 16 * whole);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) xf[e] = xh[e], wf[e] = wh[e];
+    }
     Mma<T, PREC>::step(acc, wf, xf);
   }
 #pragma unroll

@@ -410,3 +410,37 @@ def test_operands_changed_in_place_before_the_backward():
                 torch.autograd.grad(y, w, dy)
         else:
             assert torch.equal(torch.autograd.grad(y, w, dy)[0], want)
+
+
+@pytest.mark.parametrize("i", [4, 8, 12, 16, 20, 28, 132, 260, 500])
+@pytest.mark.parametrize("m,o", [(1, 1), (5, 40), (33, 24), (700, 200)])
+@pytest.mark.parametrize("mode", ["ieee", "bf16x3"])
+def test_full_precision_rows_of_whole_chunks(m, o, i, mode):
+    """The C entry takes fp32 rows of any number of 16-byte chunks; NaN follows each row, and the last one."""
+    from geometric_nn_ops_torch import _lib
+
+    x, w, b, r, _ = _inputs(m, i, o, torch.float32, seed=i)
+    bufs = []
+    for t in (x, w):
+        buf = torch.full((t.shape[0] + 2, i + 4), float("nan"), device=DEV)
+        buf[:t.shape[0], :i] = t.to(DEV)
+        bufs.append(buf)
+    out, bd, rd = torch.empty(m, o, device=DEV), b.to(DEV), r.to(DEV)
+    a = _lib.LinearArgs()
+    a.x, a.w, a.bias, a.side, a.out = bufs[0].data_ptr(), bufs[1].data_ptr(), bd.data_ptr(), rd.data_ptr(), out.data_ptr()
+    a.M, a.I, a.O, a.out_cols, a.x_ld, a.w_ld, a.side_ld, a.out_ld = m, i, o, o, i + 4, i + 4, o, o
+    a.dtype, a.precision, a.activation = _lib.GNN_F32, _lib.PRECISION_CODE[mode], _lib_act("silu")
+    _lib.call("gnn_linear", a, out.device)
+    want, slack = _exact(x, w, b, r, "silu")[0]
+    if mode == "bf16x3":
+        # x in [2^e, 2^(e+1)) is hi + lo + rest: |x - hi| <= 2^(e-8), half a bf16 step, so that lo has an exponent of
+        # e - 9 at most (or is exact) and |rest| <= 2^(e-17). A product loses both rests and lo lo:
+        # (2^-17 + 2^-17 + 2^-16) |x w| = 2^-15 |x w|. One short sum can be off by all of that (the slope is below 1.2).
+        slack = slack + 1.2 * 2.0 ** -15 * (x.double().abs() @ w.double().abs().t())
+    assert_within(f"{m}x{i}->{o}", out, want, slack)
+
+
+def _lib_act(name):
+    from geometric_nn_ops_torch.triangle._kernels.fused_linear import ACTIVATION_CODE
+
+    return ACTIVATION_CODE[name]
