@@ -340,7 +340,7 @@ __global__ __launch_bounds__(RP_NT) void relpos_last_fwd_kernel(const RpArgs a) 
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         v[e] = a.heads ? table[t * a.H + c] : gtable[(int64_t)t * a.H + c];
-        if (++c == a.H && x + e + 1 < len) {
+        if (x + e + 1 < len && ++c == a.H) {  // past the row's end the last element again, which is not stored
           c = 0;
           t = bucket_of(a.bk, border, ahead_of(kp[++j], q, a.bk.far));
         }

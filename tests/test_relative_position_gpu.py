@@ -265,3 +265,25 @@ def test_channels_last_of_every_width(h, dtype):
     inner.copy_(dout)
     grad = torch.autograd.grad(y, table, inner)[0]
     assert_within(f"gradient of {h} channels", grad, want, 100 * U * size)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("buckets,h,v", [(64, 500, 3), (256, 100, 61), (256, 101, 7), (255, 257, 5), (128, 193, 1)])
+def test_channels_last_tables_outside_lds(buckets, h, v, dtype):
+    """Tables above 48 KB whose heads fill no whole chunks, in rows that end inside one: the last pixel lies in the
+    last bucket, so that nothing of the table follows it, and NaN lies around the table."""
+    far = buckets - 1
+    g = torch.Generator().manual_seed(h)
+    w = torch.randn(buckets, h, generator=g).to(dtype)
+    q = torch.arange(5)[None] + far + 400
+    k = torch.randint(0, far, (1, v), generator=g) + 400
+    k[0, -1] = 0
+    rows = buckets_torch(q, k, buckets, far, "clip", False)
+    assert (rows[..., -1] == buckets - 1).all() and w.numel() * w.element_size() > 48 << 10
+    buf = torch.full((w.numel() + 128,), float("nan"), device=DEV, dtype=dtype)
+    table = buf[64:64 + w.numel()].view(w.shape)
+    table.copy_(w)
+    how = dict(max_distance=far, spacing="clip", bidirectional=False, channels_last=True)
+    with torch.no_grad():
+        out = relative_position_bias(table, q.to(DEV), k.to(DEV), **how)
+    assert torch.equal(out.cpu(), w[rows])
