@@ -572,7 +572,9 @@ int backward(const gnn_relpos_args& g, hipStream_t st) {
     const size_t lds = (size_t)bins.waves * n * (bins.bytes / bins.count) +
                        (!g.channels_last && a.bk.far <= RP_LUT_FAR ? 2 * (2 * a.bk.far + 2) : 0);
     if (lds > 64 * 1024) {
-      const void* fn = narrow(g) ? (const void*)relpos_last_narrow_bwd_kernel<T, P> : (const void*)relpos_last_bwd_kernel<T, P>;
+      const void* fn = narrow(g)          ? (const void*)relpos_last_narrow_bwd_kernel<T, P>
+                       : g.channels_last ? (const void*)relpos_last_bwd_kernel<T, P>
+                                         : (const void*)relpos_bwd_kernel<T, P>;
       (void)hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     }
     if (narrow(g)) {

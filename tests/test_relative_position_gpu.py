@@ -287,3 +287,12 @@ def test_channels_last_tables_outside_lds(buckets, h, v, dtype):
     with torch.no_grad():
         out = relative_position_bias(table, q.to(DEV), k.to(DEV), **how)
     assert torch.equal(out.cpu(), w[rows])
+
+
+@pytest.mark.parametrize("case", [(255, 127, "clip", True), (256, 255, "clip", False), (511, 255, "clip", True),
+                                  (256, 1000, "log", True), (255, 900, "log", False), (512, 1023, "log", False)],
+                         ids=["255", "256", "511", "log256", "log255", "log512"])
+def test_tables_whose_bins_and_differences_pass_64_kb(case):
+    """Heads first: the bins of 255 or 256 buckets a pass and the table of differences beside them."""
+    for i, dtype in enumerate(DTYPES):
+        _check(1, 70, 300, 3, case, dtype, ("run", "gaps", "any")[i], seed=200 + i, pos_dtype=(torch.int32, torch.int64)[i % 2])
