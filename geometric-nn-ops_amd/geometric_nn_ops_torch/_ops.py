@@ -18,9 +18,10 @@ torch.compile, FakeTensor or any dispatch mode the callers go through the operat
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 __all__ = ["triangle_attention_fwd", "trimul_fwd", "attention_pair_bias_fwd", "layer_norm_fwd",
-           "relative_position_bias_fwd", "fused_linear_fwd", "eager_ok"]
+           "relative_position_bias_fwd", "fused_linear_fwd", "eager_ok", "carries_tangent"]
 
 
 _PLAIN_TYPES = (torch.Tensor, torch.nn.Parameter)  # Parameter disables __torch_function__
@@ -34,6 +35,13 @@ def eager_ok(*tensors) -> bool:
     if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0:
         return False
     return all(t is None or type(t) in _PLAIN_TYPES for t in tensors)
+
+
+def carries_tangent(*tensors) -> bool:
+    """True where forward-mode differentiation goes through one of the tensors (or None): neither the
+    operators nor their implementations have a tangent's formula, and would drop it without a word."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def triangle_attention_fwd_impl(

@@ -4,8 +4,9 @@ transitions and the projections around a pairformer's updates need it.
 The reference has no such entry point; its linear layers are ``F.linear`` and separate elementwise ops
 (geometric_nn_ops_torch/triangle/_reference/trimul.py:86-97, _reference/attention_pair_bias.py:86-89).
 Dispatch: bf16, fp16 and fp32 tensors on a HIP device run the gfx950 kernels, forward (through the
-``gnn_amd::fused_linear_fwd`` operator where no backward can follow) and backward; CPU tensors, fp64 and
-widths above 2^20 take the differentiable torch path. Without the HIP library a GPU call raises.
+``gnn_amd::fused_linear_fwd`` operator where no backward can follow) and backward; CPU tensors, fp64,
+widths above 2^20 and forward-mode differentiation take the differentiable torch path. Without the HIP
+library a GPU call raises.
 """
 
 import torch
@@ -89,7 +90,8 @@ def fused_linear(
         repeated calls give the same bits.
     """
     _check(x, weight, bias, activation, residual)
-    if not x.is_cuda or x.dtype not in _KERNEL_DTYPES or not _hip.supports(weight):
+    if (not x.is_cuda or x.dtype not in _KERNEL_DTYPES or not _hip.supports(weight)
+            or _ops.carries_tangent(x, weight, bias, residual)):
         return fused_linear_torch(x, weight, bias, activation, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         return _FusedLinearHip.apply(x, weight, bias, activation, residual)

@@ -3,8 +3,9 @@
 The reference has no such entry point; its LayerNorms are ``F.layer_norm`` inside the ops
 (geometric_nn_ops_torch/triangle/_reference/trimul.py:85, 94). Dispatch: bf16, fp16 and fp32 tensors on
 a HIP device with rows of up to 16384 elements run the gfx950 kernels, forward (through the
-``gnn_amd::layer_norm_fwd`` operator where no backward can follow) and backward; CPU tensors, fp64 and
-wider rows take the differentiable torch path. Without the HIP library a GPU call raises.
+``gnn_amd::layer_norm_fwd`` operator where no backward can follow) and backward; CPU tensors, fp64, wider
+rows and forward-mode differentiation take the differentiable torch path. Without the HIP library a GPU
+call raises.
 """
 
 import torch
@@ -79,7 +80,8 @@ def layer_norm(
         same bits.
     """
     _check(x, weight, bias)
-    if not x.is_cuda or x.dtype not in _KERNEL_DTYPES or not _hip.supports(x):
+    if (not x.is_cuda or x.dtype not in _KERNEL_DTYPES or not _hip.supports(x)
+            or _ops.carries_tangent(x, weight, bias)):
         return layer_norm_torch(x, weight, bias, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return _LayerNormHip.apply(x, weight, bias, eps)

@@ -5,7 +5,8 @@ The reference has no such entry point; its callers build the bias that they hand
 or ``attention_pair_bias``, and the pair stream, with stock torch. Dispatch: bf16, fp16 and fp32 tables on a
 HIP device run the gfx950 kernels, forward (through the ``gnn_amd::relative_position_bias_fwd`` operator
 where no backward can follow) and backward; CPU tensors, fp64, tables of more than 4096 buckets or 256
-logarithmic ones a side take the differentiable torch path. Without the HIP library a GPU call raises.
+logarithmic ones a side, and forward-mode differentiation take the differentiable torch path. Without the
+HIP library a GPU call raises.
 """
 
 import torch
@@ -117,7 +118,8 @@ def relative_position_bias(
     if query_pos.dtype != key_pos.dtype:
         query_pos, key_pos = query_pos.to(torch.int64), key_pos.to(torch.int64)
     how = (max_distance, spacing, bool(bidirectional), bool(channels_last))
-    if not weight.is_cuda or weight.dtype not in _KERNEL_DTYPES or not _hip.supports(weight, query_pos, key_pos, *how[:3]):
+    if (not weight.is_cuda or weight.dtype not in _KERNEL_DTYPES or not _hip.supports(weight, query_pos, key_pos, *how[:3])
+            or _ops.carries_tangent(weight)):
         return relative_position_bias_torch(weight, query_pos, key_pos, *how)
     if torch.is_grad_enabled() and weight.requires_grad:
         return _RelativePositionHip.apply(weight, query_pos, key_pos, how)
