@@ -81,8 +81,10 @@ __device__ __forceinline__ float slope(float z) {
     return s * (1.0f + z * (1.0f - s));
   }
   if constexpr (ACT == GNN_ACT_SIGMOID) {
-    const float s = sigmoid<F32>(z);
-    return s * (1.0f - s);
+    // e / (1 + e)^2 with e = exp(-|z|), which is even: s (1 - s) has no digits left where s rounds to 1
+    const float e = F32 ? expf(-fabsf(z)) : fast_exp2(-1.4426950408889634f * fabsf(z));
+    const float r = F32 ? 1.0f / (1.0f + e) : __builtin_amdgcn_rcpf(1.0f + e);
+    return e * r * r;
   }
   return 1.f;
 }

@@ -444,3 +444,25 @@ def _lib_act(name):
     from geometric_nn_ops_torch.triangle._kernels.fused_linear import ACTIVATION_CODE
 
     return ACTIVATION_CODE[name]
+
+
+def _slopes(act, dtype, m, top):
+    """``(got, exact)`` slopes at m x 8 points within ``top``: dx of a layer whose weight is the identity and whose output
+    gradient is 1, where z is x and dx is dz, to the last bit."""
+    x = torch.linspace(-top, top, 8 * m, dtype=torch.float64).to(dtype).view(m, 8).to(DEV).requires_grad_()
+    w = torch.eye(8, dtype=dtype, device=DEV)
+    (dx,) = torch.autograd.grad(fused_linear(x, w, None, act), x, torch.ones(m, 8, dtype=dtype, device=DEV))
+    return x.detach().double(), dx
+
+
+@pytest.mark.parametrize("m", [700, 33000])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_sigmoid_slope_far_out(dtype, m):
+    """e / (1 + e)^2, e = exp(-|z|), keeps its digits where the sigmoid rounds to 1. The exponential's argument is off
+    by 2 U |z| where it is scaled to base 2 first (its result by 2 U), the sum, the reciprocal and three products by
+    2 U each at most; both roundings of the result (dz, dx) are of the same value."""
+    with precision("ieee"):
+        z, got = _slopes("sigmoid", dtype, m, 60.0)
+    e = torch.exp(-z.abs())
+    want = e / (1 + e) ** 2
+    assert_within("slope", got, want, (2 * z.abs() + 16) * U * want)
