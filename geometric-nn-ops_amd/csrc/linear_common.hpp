@@ -27,8 +27,11 @@ __device__ __forceinline__ int chunk_swizzle(int r) {
 // ---- activations ------------------------------------------------------------------------
 // 16-bit results: exp2 and rcp of the hardware (1 ulp each) and polynomials fitted to the normal distribution (in
 // 64 bits, weighted least squares iterated to an even error). With m = |z|, Phi(-m) = 2^P(m), off by at most 2e-7 / m
-// and by 1.5e-4 of itself to m = 5.5; the slope's part Phi(-m) - m phi(m) = exp(-m^2 / 2) S(m), off by at most 4e-7.
-// Both are far below half a step of fp16 (2.4e-4) and vanish beyond m = 16. The vector unit's time, which the
+// and by 1.5e-4 of itself to m = 7 (1.5 % at 8, half at 10, where gelu is -5e-15 and -8e-23 and only bf16 holds it);
+// the slope's part Phi(-m) - m phi(m) = exp(-m^2 / 2) S(m), off by at most 4e-7 and from m = 2 to 4 by 3.2e-4 of
+// itself. Beyond, S alone would be 15 % off at 5.5 and a cubic of its own takes over, 2.5e-4 off to the end of bf16's
+// range (the slopes and both gradients of 147456 x 128 -> 512, bf16: 164 us, with S alone 158). Half a step of fp16
+// is 2.4e-4 to 4.9e-4 of a value, of bf16 eight times that. Both vanish beyond m = 16. The vector unit's time, which the
 // products and the stores hide only in part, is what the wide layers with an activation pay: 147456 x 128 -> 512
 // in bf16 takes 40 us without one, 54 with silu, 77 with gelu (90 with Phi by one exponential and one reciprocal,
 // Abramowitz and Stegun 7.1.26; the slopes with both gradients 121 and 129). fp32: the library's functions and
@@ -60,7 +63,8 @@ __device__ __forceinline__ float gelu_slope(float z) {
   float s = S[9];
 #pragma unroll
   for (int k = 8; k >= 0; --k) s = fmaf(s, m, S[k]);
-  s *= fast_exp2(-0.7213475204444817f * m * m);
+  const float far = fmaf(fmaf(fmaf(-0.000113982198f, m, 0.00370404311f), m, -0.442016602f), m, 0.214368284f);
+  s = (m > 4.f ? far : s) * fast_exp2(-0.7213475204444817f * m * m);
   return z < 0.f ? s : 1.0f - s;
 }
 

@@ -466,3 +466,20 @@ def test_sigmoid_slope_far_out(dtype, m):
     e = torch.exp(-z.abs())
     want = e / (1 + e) ** 2
     assert_within("slope", got, want, (2 * z.abs() + 16) * U * want)
+
+
+@pytest.mark.parametrize("m", [700, 33000])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_gelu_slope_far_out(dtype, m):
+    """Phi(z) + z phi(z) to where it leaves bf16's range. 16-bit types: the fit is off by 4e-7 (it passes zero near
+    z = -0.75), and from |z| = 2 on by less than 3.2e-4 of the value; fp32 and the exponential's argument, z^2 / 2,
+    add (z^2 + 16) 4 U of both terms."""
+    with precision("ieee"):
+        z, got = _slopes("gelu", dtype, m, 13.0)
+    # not torch.special.ndtr, which is (1 + erf) / 2 and has no digits left beyond z = -8
+    cdf, pdf = torch.special.erfc(-z * 0.5 ** 0.5) / 2, torch.exp(-z * z / 2) / (2 * torch.pi) ** 0.5
+    want = cdf + z * pdf
+    slack = (z * z + 16) * 4 * U * (cdf + z.abs() * pdf)
+    if dtype != torch.float32:
+        slack = slack + 4e-7 * (z.abs() < 2) + 3.2e-4 * want.abs() * (z < -2) + 4e-7 * (z >= 2)
+    assert_within("slope", got, want, slack)
