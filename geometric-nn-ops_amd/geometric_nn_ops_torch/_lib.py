@@ -674,20 +674,20 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def call(fn_name: str, args, device: torch.device, *extra) -> None:
-    """``fn_name(&args, *extra, stream)`` on ``device``'s current stream, with ``device`` current for
+def call(fn_name: str, args, device: torch.device) -> None:
+    """``fn_name(&args, stream)`` on ``device``'s current stream, with ``device`` current for
     the call (the current device is switched only when it differs: the guard costs host time
     on every launch), raising on a non-zero status."""
     fn = getattr(_lib or load(), fn_name)
     idx = device.index
     if idx is None or device.type != "cuda":
-        rc = fn(ctypes.byref(args), *extra, stream_handle(device))
+        rc = fn(ctypes.byref(args), stream_handle(device))
     elif idx == torch._C._cuda_getDevice():  # a tensor is there: nothing is left to initialise
         # the handle itself: building a torch.cuda.Stream around it takes 1.5 us a launch
-        rc = fn(ctypes.byref(args), *extra, torch._C._cuda_getCurrentRawStream(idx))
+        rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(idx))
     else:
         with torch.cuda.device(idx):
-            rc = fn(ctypes.byref(args), *extra, torch._C._cuda_getCurrentRawStream(idx))
+            rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(idx))
     if rc != GNN_OK:
         check(rc, fn_name)
 
