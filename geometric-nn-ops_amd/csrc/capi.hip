@@ -516,7 +516,7 @@ int gnn_relpos_bwd(const gnn_relpos_args* args, void* stream) {
 int gnn_linear(const gnn_linear_args* args, void* stream) {
   if (!args) return set_error(GNN_ERR_ARG, "fused_linear: args is NULL");
   const gnn_linear_args& a = *args;
-  if (!a.x || !a.w || (!a.out && !a.dx) || (a.dz && !a.side))
+  if (!a.x || !a.w || !a.out || (a.dz && !a.side))
     return set_error(GNN_ERR_ARG, "fused_linear: x, w, out and, for dz, the output gradient are required");
   if (!known_dtype(a.dtype)) return set_error(GNN_ERR_ARG, "fused_linear: unknown dtype");
   if (a.precision != GNN_PREC_IEEE && a.precision != GNN_PREC_BF16X3)
@@ -529,7 +529,8 @@ int gnn_linear(const gnn_linear_args* args, void* stream) {
   const int64_t e = a.dtype == GNN_F32 ? 4 : 2;
   if (!aligned(a.x, 16) || !aligned(a.w, 16) || (a.I * e) % 16 || (a.x_ld * e) % 16 || (a.w_ld * e) % 16)
     return set_error(GNN_ERR_ARG, "fused_linear: rows of x and w must be 16-byte aligned and multiples of 16 bytes");
-  if (a.x_ld < 0 || a.w_ld < (a.w_transposed ? a.O : a.I) || (a.side && a.side_ld < 0) || a.out_ld < a.out_cols)
+  if (a.x_ld < 0 || a.w_ld < (a.w_transposed ? a.O : a.I) || (a.side && a.side_ld < 0) || a.out_ld < a.out_cols ||
+      (a.dx && a.dx_ld < a.I))
     return set_error(GNN_ERR_ARG, "fused_linear: row pitches must cover their rows");
   if (!aligned(a.bias, e) || !aligned(a.side, e) || !aligned(a.out, e))
     return set_error(GNN_ERR_ARG, "fused_linear: tensors must be aligned to their elements");

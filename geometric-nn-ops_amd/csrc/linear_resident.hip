@@ -346,7 +346,7 @@ __global__ __launch_bounds__(NT, NT / 256) void linear_rows_bwd_kernel(const Lin
     load_rows(x, grp);
     turn_rows();
     const auto srs = rows_rsrc<T>(a.side, grp * 32, a.M, a.side_ld, a.O);
-    const auto ors = rows_rsrc<T>(a.out, grp * 32, a.out ? a.M : 0, a.out_ld, a.O);
+    const auto ors = rows_rsrc<T>(a.out, grp * 32, a.M, a.out_ld, a.O);
     const auto drs = rows_rsrc<T>(a.dx, grp * 32, a.M, a.dx_ld, a.I);
     f32x16 dx[KB];
 #pragma unroll

@@ -688,8 +688,7 @@ typedef struct gnn_linear_args {
 /* Whether this call could read w transposed, [I] rows of O (w_ld apart, O a multiple of 8): the input gradient's
  * product takes the weight as it is then. gnn_linear refuses w_transposed where this is 0. */
 int gnn_linear_takes_transposed(const gnn_linear_args* args);
-/* Whether this call, with dx and dx_ld set, could write dx too; gnn_linear refuses dx where this is 0. out may
- * be NULL then. */
+/* Whether this call, with dx and dx_ld set, could write dx too; gnn_linear refuses dx where this is 0. */
 int gnn_linear_takes_dx(const gnn_linear_args* args);
 int gnn_linear(const gnn_linear_args* args, void* stream);
 

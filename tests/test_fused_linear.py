@@ -227,3 +227,17 @@ def test_the_fitted_normal_distribution():
     slope = poly("S", m) * torch.exp2(-0.7213475204444817 * z * z)
     assert ((slope - (tail - z * pdf)).abs() <= 4e-7).all()
     assert near[-1] < 1e-100 and slope[-1].abs() < 1e-45
+
+
+def test_dx_comes_with_dz_in_rows_that_hold_it():
+    lib = _lib.load()
+    a = _lib.LinearArgs()
+    a.x = a.w = a.out = a.side = a.dx = 4096
+    a.M, a.I, a.O, a.out_cols, a.x_ld, a.w_ld, a.side_ld, a.out_ld = 1 << 16, 128, 512, 512, 128, 128, 512, 512
+    a.dtype, a.dz, a.activation, a.dx_ld = _lib.GNN_BF16, 1, 1, 128
+    a.out = None
+    assert lib.gnn_linear(ctypes.byref(a), None) == _lib.GNN_ERR_ARG and b"required" in lib.gnn_last_error()
+    a.out = 4096
+    for pitch in (120, 0, -128):
+        a.dx_ld = pitch
+        assert lib.gnn_linear(ctypes.byref(a), None) == _lib.GNN_ERR_ARG and b"pitches" in lib.gnn_last_error(), pitch
