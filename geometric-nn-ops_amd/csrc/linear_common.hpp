@@ -34,8 +34,8 @@ __device__ __forceinline__ int chunk_swizzle(int r) {
 // is 2.4e-4 to 4.9e-4 of a value, of bf16 eight times that. Both vanish beyond m = 16. The vector unit's time, which the
 // products and the stores hide only in part, is what the wide layers with an activation pay: 147456 x 128 -> 512
 // in bf16 takes 40 us without one, 54 with silu, 77 with gelu (90 with Phi by one exponential and one reciprocal,
-// Abramowitz and Stegun 7.1.26; the slopes with both gradients 121 and 129). fp32: the library's functions and
-// full divisions.
+// Abramowitz and Stegun 7.1.26; dz and dx in one pass 122, with silu 101). fp32: the library's functions and full
+// divisions.
 template <bool F32>
 __device__ __forceinline__ float sigmoid(float z) {
   if constexpr (F32) return 1.0f / (1.0f + expf(-z));

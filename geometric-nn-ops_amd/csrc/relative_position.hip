@@ -19,8 +19,11 @@
 // [bucket][channel]), and a wave leaves one row of partial sums, added in order by reduce_parts.
 // 2048^2 x 16 heads, bf16, log, 134 MB: forward 29 us (4.6 TB/s), backward 51 (2.6: the blocks of keys
 // across the diagonal, whose lanes look buckets up and add to bins, and each wave's set-up; the next loads issued a
-// turn ahead 55, half or twice the waves 68 and 62). 509^2 x 128
-// channels, clip, 66 MB: 19 (3.5 TB/s) and 32 (2.1: the chain of bins; half or twice the workgroups 47 and 45).
+// turn ahead 55, half or twice the waves 68 and 62); positions in random order, where every group straddles, 322.
+// 509^2 x 128 channels, clip, 66 MB: 20 (3.3 TB/s, start and end of a short launch: 1018^2 takes 56, 4.7 TB/s) and 32
+// (2.1: the chain of bins; half or twice the workgroups 47 and 45).
+// More than 256 buckets (heads last 128) take a pass over dout for each 256 (128): 1024^2 x 16, 129, 257, 513 and 2049
+// buckets 53, 101, 191 and 705 us (heads last 61, 120, 253 and 964).
 #include <algorithm>
 
 #include "gnn_common.hpp"

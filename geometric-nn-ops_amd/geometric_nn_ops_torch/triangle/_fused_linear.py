@@ -83,7 +83,9 @@ def fused_linear(
         residual: ``[..., O]`` or ``None``, added after the activation.
 
     All in one dtype. Products and epilogue run in fp32 and the result rounds once; fp32 products follow
-    ``torch.backends.cuda.matmul.fp32_precision`` (the weight's gradient is full precision).
+    ``torch.backends.cuda.matmul.fp32_precision`` (the weight's gradient is full precision). In the backward the
+    gradient at the activation's input is rounded to x's dtype once, as the operand of x's, the weight's and the
+    bias's gradients, as stock torch's linear layers in that dtype have it.
 
     Returns:
         A fresh contiguous ``[..., O]`` tensor of x's dtype. Differentiable in x, weight, bias and residual;

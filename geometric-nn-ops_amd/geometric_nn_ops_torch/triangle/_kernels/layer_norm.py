@@ -62,7 +62,7 @@ def layer_norm_bwd_hip(x, weight, stats, dy, *, need_dx=True, dweight=None, dbia
     _lib.pack_layer_norm_bwd(
         a, 0, xr.data_ptr(), gr.data_ptr(), 0 if w is None else w.data_ptr(), stats.data_ptr(),
         stats.data_ptr() + 4 * rows, 0 if dx is None else dx.data_ptr(),
-        0 if part is None else part.data_ptr(), parts, rows, K, inner, outer, stride, ginner, gouter, gstride, dt, _param_code(x, w, dbias), 0 if dweight is None else dweight.data_ptr(),
-        0 if dbias is None else dbias.data_ptr())
+        0 if part is None else part.data_ptr(), parts, rows, K, inner, outer, stride, ginner, gouter, gstride, dt,
+        _param_code(x, w, dbias), 0 if dweight is None else dweight.data_ptr(), 0 if dbias is None else dbias.data_ptr())
     _lib.call("gnn_layer_norm_bwd", a, x.device)
     return dx

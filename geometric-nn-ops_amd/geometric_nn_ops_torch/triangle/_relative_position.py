@@ -101,7 +101,9 @@ def relative_position_bias(
     Returns:
         The bias in ``weight``'s dtype; B is 1 for positions without a batch. ``[B, heads, U, V]`` is a view
         whose row pitch is V rounded up to 8, which ``triangle_attention`` and ``attention_pair_bias`` read
-        without a copy. Differentiable in ``weight``; the gradient is summed in fp32 in a fixed order.
+        without a copy. Differentiable in ``weight``; the gradient is summed in fp32 in a fixed order. It reads the
+        output gradient once for every 256 buckets (128 with ``channels_last``), and without ``channels_last`` it
+        is fastest where positions ascend or descend: neighbouring keys then share buckets.
     """
     if key_pos is None:
         key_pos = query_pos

@@ -553,6 +553,7 @@ typedef struct gnn_rows_product_args {
  * _reference/trimul.py:86-97); the reference has no kernel for them. */
 int64_t gnn_rows_product_slices(const gnn_rows_product_args* args);
 int gnn_rows_product(const gnn_rows_product_args* args, void* stream);
+
 /* dst[e] = sum over p < parts of src[p * stride + e] (e < n), in a fixed order, for up to
  * GNN_REDUCE_MAX segments in one launch; dst is in the segment's dtype. Adds the partials that
  * gnn_rows_product, gnn_layernorm_rows, gnn_trimul_gate_bwd, gnn_trimul_proj_bwd and
@@ -595,8 +596,8 @@ int gnn_layer_norm_fwd(const gnn_layer_norm_fwd_args* args, void* stream);
 
 /* Its backward: dx (dense, or NULL) and, where partial is not NULL, fp32 [parts][2][K]: partial sums of
  * the weight's and the bias's gradient, which are added in order into dweight and dbias where those are not
- * NULL (they need partial; gnn_reduce_parts adds them otherwise). parts is the number of workgroups, gnn_layer_norm_bwd_parts(rows, K, dtype) the best one for the current device. dy is
- * addressed as x is. */
+ * NULL (they need partial; gnn_reduce_parts adds them otherwise). parts is the number of workgroups,
+ * gnn_layer_norm_bwd_parts(rows, K, dtype) the best one for the current device. dy is addressed as x is. */
 typedef struct gnn_layer_norm_bwd_args {
   const void* x;
   const void* dy;
@@ -621,7 +622,8 @@ int gnn_layer_norm_bwd(const gnn_layer_norm_bwd_args* args, void* stream);
  *   out[b, h, i, j] (channels_last: out[b, i, j, h]) = table[bucket(key_pos[b, j] - query_pos[b, i])][h]
  * and backward: dtable[t][h] = sum over the (b, i, j) of bucket t of dout[b, h, i, j], as fp32 partial sums
  * [parts][buckets][H], which are added in order into dtable ([buckets][H] in dtype) where that is not NULL
- * (gnn_reduce_parts adds them otherwise); parts as gnn_relpos_parts returns it (any from 1 on is right). With D = max_distance and a = key_pos - query_pos:
+ * (gnn_reduce_parts adds them otherwise); parts as gnn_relpos_parts returns it (any from 1 on is right). dout is
+ * read once for every 256 buckets (channels_last: 128). With D = max_distance and a = key_pos - query_pos:
  *   clip, two-sided: clamp(a, -D, D) + D (2 D + 1 buckets); one-sided: clamp(-a, 0, D) (D + 1 buckets);
  *   log: n buckets a side (buckets / 2 where two-sided, those of keys ahead, a > 0, in the second half),
  *     near = n / 2 of them for distances d < near, bucket near + k from the least d on with
