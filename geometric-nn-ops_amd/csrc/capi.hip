@@ -617,6 +617,69 @@ int gnn_column_sums(const gnn_column_sums_args* args, void* stream) {
   return hip_status((hipError_t)rc, "column_sums");
 }
 
+static int check_qk_rotary(const gnn_qk_rotary_args* args, bool bwd) {
+  if (!args) return set_error(GNN_ERR_ARG, "qk_norm_rotary: args is NULL");
+  const gnn_qk_rotary_args& a = *args;
+  if (!known_dtype(a.dtype)) return set_error(GNN_ERR_ARG, "qk_norm_rotary: unknown dtype");
+  if (a.param_dtype != a.dtype && a.param_dtype != GNN_F32)
+    return set_error(GNN_ERR_ARG, "qk_norm_rotary: weights must be in the rows' dtype or fp32");
+  if (a.pos_bytes != 4 && a.pos_bytes != 8)
+    return set_error(GNN_ERR_ARG, "qk_norm_rotary: positions must have 4 or 8 bytes");
+  if (a.D < 8 || a.D > 256 || a.D % 8 || a.R < 0 || a.R > a.D || a.R % 8)
+    return set_error(GNN_ERR_ARG, "qk_norm_rotary: D must be a multiple of 8 up to 256, R a multiple of 8 up to D");
+  if (a.R && (a.pos[0] || a.pos[1]) && !a.frequencies)
+    return set_error(GNN_ERR_ARG, "qk_norm_rotary: a rotation needs its frequencies");
+  if (a.B < 0) return set_error(GNN_ERR_ARG, "qk_norm_rotary: B must not be negative");
+  const size_t e = a.dtype == GNN_F32 ? 4 : 2, we = a.param_dtype == GNN_F32 ? 4 : 2;
+  for (int k = 0; k < 2; ++k) {
+    if (a.N[k] < 0 || a.H[k] < 0 || a.H[k] > (1 << 20))
+      return set_error(GNN_ERR_ARG, "qk_norm_rotary: N must not be negative, H in 0 .. 2^20");
+    if (!a.norm && (a.weight[k] || a.dweight[k])) return set_error(GNN_ERR_ARG, "qk_norm_rotary: weights go with norms");
+    if (!aligned(a.x[k], e) || !aligned(a.dy[k], e) || !aligned(a.out[k], e) || !aligned(a.weight[k], we) ||
+        !aligned(a.dweight[k], we) || !aligned(a.pos[k], a.pos_bytes))
+      return set_error(GNN_ERR_ARG, "qk_norm_rotary: tensors must be aligned to their elements");
+    if (!a.B || !a.N[k] || !a.H[k]) continue;
+    if (!a.x[k] || (bwd ? !a.dy[k] : !a.out[k]))
+      return set_error(GNN_ERR_ARG, "qk_norm_rotary: x and out, or in the backward x and dy, are required");
+    if (bwd && (a.parts[k] < 1 || a.parts[k] >= ((int64_t)1 << 30)))
+      return set_error(GNN_ERR_ARG, "qk_norm_rotary: parts must be positive and fit a grid");
+    if (bwd && a.dweight[k] && !a.partial) return set_error(GNN_ERR_ARG, "qk_norm_rotary: dweight needs partial");
+  }
+  return GNN_OK;
+}
+
+int gnn_qk_rotary_fwd(const gnn_qk_rotary_args* args, void* stream) {
+  if (int rc = check_qk_rotary(args, false)) return rc;
+  int rc = qk_rotary(*args, false, (hipStream_t)stream);
+  if (rc < 0) return rc;
+  return hip_status((hipError_t)rc, "qk_norm_rotary");
+}
+
+int64_t gnn_qk_rotary_parts(const gnn_qk_rotary_args* args, int32_t side) {
+  if (!args || side < 0 || side > 1 || args->D < 8 || args->D > 256 || args->B < 0 || args->N[side] < 0 ||
+      args->H[side] < 1)
+    return 0;
+  return qk_rotary_parts(*args, side);
+}
+
+int gnn_qk_rotary_bwd(const gnn_qk_rotary_args* args, void* stream) {
+  if (int rc = check_qk_rotary(args, true)) return rc;
+  const gnn_qk_rotary_args& a = *args;
+  int rc = qk_rotary(a, true, (hipStream_t)stream);
+  if (rc == 0) {
+    gnn_reduce_args r{};
+    const float* partial = a.partial;
+    for (int k = 0; k < 2; ++k)
+      if (a.dweight[k] && a.B && a.N[k] && a.H[k]) {
+        r.seg[r.count++] = {partial, a.dweight[k], a.parts[k], a.D, a.D, a.param_dtype, 0};
+        partial += a.parts[k] * a.D;
+      }
+    if (r.count) rc = reduce_parts(r, (hipStream_t)stream);
+  }
+  if (rc < 0) return rc;
+  return hip_status((hipError_t)rc, "qk_norm_rotary backward");
+}
+
 const char* gnn_last_error(void) { return g_last_error.c_str(); }
 
 const char* gnn_version(void) { return "0.1.0 gfx950"; }

@@ -22,8 +22,11 @@ GNN_OK, GNN_ERR_ARG, GNN_ERR_UNSUPPORTED, GNN_ERR_WORKSPACE = 0, -1, -2, -3
 DTYPE_CODE = {torch.float32: GNN_F32, torch.bfloat16: GNN_BF16, torch.float16: GNN_F16}
 PRECISION_CODE = {"ieee": GNN_PREC_IEEE, "bf16x3": GNN_PREC_BF16X3}
 
+Ptrx2 = ctypes.c_void_p * 2
+I64x2 = ctypes.c_int64 * 2
 I64x3 = ctypes.c_int64 * 3
 I64x4 = ctypes.c_int64 * 4
+I64x6 = ctypes.c_int64 * 6
 
 
 _FORMATS = {ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_float: "f", ctypes.c_size_t: "N"}
@@ -573,6 +576,39 @@ class LayerNormBwdArgs(ctypes.Structure):
 pack_layer_norm_bwd = packer(LayerNormBwdArgs)
 
 
+class QkRotaryArgs(ctypes.Structure):
+    """Mirror of ``gnn_qk_rotary_args``: pairs are queries, keys; strides ``[side][batch, token, head]``."""
+
+    _fields_ = [
+        ("x", Ptrx2),
+        ("dy", Ptrx2),
+        ("weight", Ptrx2),
+        ("pos", Ptrx2),
+        ("out", Ptrx2),
+        ("dweight", Ptrx2),
+        ("frequencies", ctypes.c_void_p),
+        ("partial", ctypes.c_void_p),
+        ("B", ctypes.c_int64),
+        ("N", I64x2),
+        ("H", I64x2),
+        ("D", ctypes.c_int64),
+        ("R", ctypes.c_int64),
+        ("x_stride", I64x6),
+        ("dy_stride", I64x6),
+        ("pos_stride", I64x2),
+        ("parts", I64x2),
+        ("eps", ctypes.c_float),
+        ("norm", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("pos_bytes", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("param_dtype", ctypes.c_int32),
+    ]
+
+
+pack_qk_rotary = packer(QkRotaryArgs)
+
+
 RELAYOUT_PLANES_TO_PIXELS, RELAYOUT_PIXELS_TO_BLOCKED, RELAYOUT_PIXELS_TO_PLANES = 0, 1, 2
 
 _SIGNATURES = {
@@ -619,6 +655,9 @@ _SIGNATURES = {
     "gnn_pad_rows": (ctypes.c_int, [ctypes.POINTER(PadRowsArgs), ctypes.c_void_p]),
     "gnn_column_sums_parts": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64]),
     "gnn_column_sums": (ctypes.c_int, [ctypes.POINTER(ColumnSumsArgs), ctypes.c_void_p]),
+    "gnn_qk_rotary_fwd": (ctypes.c_int, [ctypes.POINTER(QkRotaryArgs), ctypes.c_void_p]),
+    "gnn_qk_rotary_parts": (ctypes.c_int64, [ctypes.POINTER(QkRotaryArgs), ctypes.c_int32]),
+    "gnn_qk_rotary_bwd": (ctypes.c_int, [ctypes.POINTER(QkRotaryArgs), ctypes.c_void_p]),
     "gnn_last_error": (ctypes.c_char_p, []),
     "gnn_version": (ctypes.c_char_p, []),
 }

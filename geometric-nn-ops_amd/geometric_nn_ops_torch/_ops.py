@@ -21,7 +21,7 @@ import torch
 from torch.autograd import forward_ad
 
 __all__ = ["triangle_attention_fwd", "trimul_fwd", "attention_pair_bias_fwd", "layer_norm_fwd",
-           "relative_position_bias_fwd", "fused_linear_fwd", "eager_ok", "carries_tangent"]
+           "relative_position_bias_fwd", "fused_linear_fwd", "qk_norm_rotary_fwd", "eager_ok", "carries_tangent"]
 
 
 _PLAIN_TYPES = (torch.Tensor, torch.nn.Parameter)  # Parameter disables __torch_function__
@@ -226,3 +226,29 @@ fused_linear_fwd = torch.library.custom_op("gnn_amd::fused_linear_fwd", fused_li
 @fused_linear_fwd.register_fake
 def _fused_linear_fwd_fake(x, weight, bias, activation, residual):
     return x.new_empty((*x.shape[:-1], weight.shape[0]))
+
+
+def qk_norm_rotary_fwd_impl(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    q_pos: Optional[torch.Tensor],
+    k_pos: Optional[torch.Tensor],
+    q_weight: Optional[torch.Tensor],
+    k_weight: Optional[torch.Tensor],
+    eps: Optional[float],
+    frequencies: list[float],
+    interleaved: bool,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``q [B, U, H, D]``, ``k [B, V, Hk, D]``, positions ``[B or 1, U]`` / ``[B or 1, V]``; returns fresh contiguous
+    tensors of q's and k's shapes."""
+    from .triangle._kernels.qk_norm_rotary import qk_norm_rotary_hip
+
+    return qk_norm_rotary_hip(q, k, q_pos, k_pos, q_weight, k_weight, eps, tuple(frequencies), interleaved)
+
+
+qk_norm_rotary_fwd = torch.library.custom_op("gnn_amd::qk_norm_rotary_fwd", qk_norm_rotary_fwd_impl, mutates_args=())
+
+
+@qk_norm_rotary_fwd.register_fake
+def _qk_norm_rotary_fwd_fake(q, k, q_pos, k_pos, q_weight, k_weight, eps, frequencies, interleaved):
+    return q.new_empty(q.shape), k.new_empty(k.shape)

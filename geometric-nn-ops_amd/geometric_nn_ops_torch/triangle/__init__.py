@@ -3,6 +3,7 @@
 from ._attention_pair_bias import attention_pair_bias
 from ._fused_linear import fused_linear
 from ._layer_norm import layer_norm
+from ._qk_norm_rotary import qk_norm_rotary
 from ._relative_position import relative_position_bias
 from ._triattn import triangle_attention
 from ._trimul import triangle_multiplicative_update
@@ -11,6 +12,7 @@ __all__ = [
     "attention_pair_bias",
     "fused_linear",
     "layer_norm",
+    "qk_norm_rotary",
     "relative_position_bias",
     "triangle_attention",
     "triangle_multiplicative_update",

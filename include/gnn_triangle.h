@@ -736,6 +736,41 @@ typedef struct gnn_column_sums_args {
 int64_t gnn_column_sums_parts(int64_t M, int64_t O);
 int gnn_column_sums(const gnn_column_sums_args* args, void* stream);
 
+/* Norms of queries and keys for each head (x / sqrt(mean(x^2) + eps) w over the D elements) and the rotation by
+ * positions behind them, side 0 the queries [B, N[0], H[0], D] and side 1 the keys [B, N[1], H[1], D]: pair j of the
+ * first R elements (elements j and j + R / 2; interleaved: 2 j and 2 j + 1) turns by pos frequencies[j]. x and dy:
+ * strides of batch, token and head, unit stride over D, any alignment of their elements; out dense. A side without
+ * tokens or heads is left out. weight: [D] in param_dtype (the rows' dtype or GNN_F32), or NULL; pos: int32 or int64
+ * (pos_bytes), [N] pos_stride apart a batch, or NULL (no rotation of that side); frequencies: R / 2 doubles on the
+ * host, read during the call. D: a multiple of 8 up to 256, R: a multiple of 8 up to D (0: none). norm 0: no norms.
+ * Backward: out is dx (or NULL), and for each side with dweight the weight's gradient ([D] in param_dtype) is summed
+ * over parts[side] workgroups (as gnn_qk_rotary_parts returns it; any from 1 on is right) through partial, fp32 rows
+ * of D, parts[0] (where dweight[0]) and then parts[1]. The reference has no such op. */
+typedef struct gnn_qk_rotary_args {
+  const void* x[2];
+  const void* dy[2];
+  const void* weight[2];
+  const void* pos[2];
+  void* out[2];
+  void* dweight[2];
+  const double* frequencies;
+  float* partial;
+  int64_t B;
+  int64_t N[2], H[2];
+  int64_t D, R;
+  int64_t x_stride[2][3];
+  int64_t dy_stride[2][3];
+  int64_t pos_stride[2];
+  int64_t parts[2];
+  float eps;
+  int32_t norm, interleaved, pos_bytes;
+  int32_t dtype;       /* enum gnn_dtype of x, dy and out */
+  int32_t param_dtype; /* enum gnn_dtype of weight and dweight */
+} gnn_qk_rotary_args;
+int gnn_qk_rotary_fwd(const gnn_qk_rotary_args* args, void* stream);
+int64_t gnn_qk_rotary_parts(const gnn_qk_rotary_args* args, int32_t side);
+int gnn_qk_rotary_bwd(const gnn_qk_rotary_args* args, void* stream);
+
 /* Message for the last failing call on this thread ("" if none). */
 const char* gnn_last_error(void);
 
