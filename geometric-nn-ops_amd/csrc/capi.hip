@@ -617,6 +617,91 @@ int gnn_column_sums(const gnn_column_sums_args* args, void* stream) {
   return hip_status((hipError_t)rc, "column_sums");
 }
 
+int gnn_gated_linear(const gnn_gated_linear_args* args, void* stream) {
+  if (!args) return set_error(GNN_ERR_ARG, "gated_linear: args is NULL");
+  const gnn_gated_linear_args& a = *args;
+  if (!a.x || !a.wg || !a.wu || !a.out) return set_error(GNN_ERR_ARG, "gated_linear: x, wg, wu and out are required");
+  if (!known_dtype(a.dtype)) return set_error(GNN_ERR_ARG, "gated_linear: unknown dtype");
+  if (a.precision != GNN_PREC_IEEE && a.precision != GNN_PREC_BF16X3)
+    return set_error(GNN_ERR_ARG, "gated_linear: unknown precision");
+  if (a.activation < GNN_ACT_NONE || a.activation > GNN_ACT_SIGMOID)
+    return set_error(GNN_ERR_ARG, "gated_linear: unknown activation");
+  const int64_t most = (int64_t)1 << 29;
+  if (a.M < 1 || a.I < 1 || a.O < 1 || a.I > most || a.O > most || a.out_cols != (a.O + 7) / 8 * 8)
+    return set_error(GNN_ERR_ARG, "gated_linear: M, I and O must be positive, I and O at most 2^29, out_cols O rounded up to 8");
+  const int64_t e = a.dtype == GNN_F32 ? 4 : 2;
+  if (!aligned(a.x, 16) || !aligned(a.wg, 16) || !aligned(a.wu, 16) || (a.I * e) % 16 || (a.x_ld * e) % 16 ||
+      (a.wg_ld * e) % 16 || (a.wu_ld * e) % 16)
+    return set_error(GNN_ERR_ARG, "gated_linear: rows of x, wg and wu must be 16-byte aligned and multiples of 16 bytes");
+  if (a.x_ld < 0 || a.wg_ld < a.I || a.wu_ld < a.I || (a.dy && a.dy_ld < 0) || a.out_ld < (a.dy ? 2 * a.out_cols : a.O))
+    return set_error(GNN_ERR_ARG, "gated_linear: row pitches must cover their rows");
+  if (!aligned(a.bg, e) || !aligned(a.bu, e) || !aligned(a.dy, e) || !aligned(a.out, e))
+    return set_error(GNN_ERR_ARG, "gated_linear: tensors must be aligned to their elements");
+  int rc = gated_linear(a, (hipStream_t)stream);
+  if (rc < 0) return rc;
+  return hip_status((hipError_t)rc, "gated_linear");
+}
+
+int gnn_gated_turn(const gnn_gated_turn_args* args, void* stream) {
+  if (!args) return set_error(GNN_ERR_ARG, "gated_turn: args is NULL");
+  const gnn_gated_turn_args& a = *args;
+  if (!a.wg || !a.wu || !a.dst) return set_error(GNN_ERR_ARG, "gated_turn: wg, wu and dst are required");
+  if (!known_dtype(a.dtype)) return set_error(GNN_ERR_ARG, "gated_turn: unknown dtype");
+  const int64_t most = (int64_t)1 << 29;
+  if (a.I < 1 || a.O < 1 || a.I > most || a.O > most || a.out_cols < a.O || a.out_cols > most || a.out_cols % 8)
+    return set_error(GNN_ERR_ARG, "gated_turn: I and O must be positive, out_cols a multiple of 8 from O on");
+  const size_t e = a.dtype == GNN_F32 ? 4 : 2;
+  if (a.wg_ld < a.I || a.wu_ld < a.I) return set_error(GNN_ERR_ARG, "gated_turn: row pitches must cover their rows");
+  if (!aligned(a.wg, e) || !aligned(a.wu, e) || !aligned(a.dst, 16))
+    return set_error(GNN_ERR_ARG, "gated_turn: weights must be aligned to their elements, dst to 16 bytes");
+  int rc = gated_turn(a, (hipStream_t)stream);
+  if (rc < 0) return rc;
+  return hip_status((hipError_t)rc, "gated_turn");
+}
+
+static gnn_rows_product_args gated_wgrad_product(const gnn_gated_linear_wgrad_args& a) {
+  gnn_rows_product_args r{};
+  r.rows = a.M, r.count = 1, r.dtype = a.dtype;
+  r.p[0] = {a.dz, a.x, a.partial, a.dz_ld, a.x_ld, 2 * a.O, a.I};
+  if (a.slices > 0 && a.M > 0) r.slice_rows = ((a.M + a.slices - 1) / a.slices + 31) / 32 * 32;
+  return r;
+}
+
+int64_t gnn_gated_linear_wgrad_slices(const gnn_gated_linear_wgrad_args* args) {
+  if (!args) return 0;
+  gnn_gated_linear_wgrad_args a = *args;
+  a.slices = 0;
+  const gnn_rows_product_args r = gated_wgrad_product(a);
+  return gnn_rows_product_slices(&r);
+}
+
+int gnn_gated_linear_wgrad(const gnn_gated_linear_wgrad_args* args, void* stream) {
+  if (!args) return set_error(GNN_ERR_ARG, "gated_linear gradients: args is NULL");
+  const gnn_gated_linear_wgrad_args& a = *args;
+  if (a.slices < 1 || a.slices >= ((int64_t)1 << 31) || a.O < 8 || a.O % 8 || a.outputs < 1 || a.outputs > a.O)
+    return set_error(GNN_ERR_ARG, "gated_linear gradients: slices must be positive, O a multiple of 8, outputs from 1 to O");
+  const gnn_rows_product_args r = gated_wgrad_product(a);
+  if (int rc = check_rows_product(&r, true)) return rc;
+  const int bytes = a.dtype == GNN_F32 ? 4 : 2;
+  void* dst[4] = {a.dwg, a.dwu, a.dbg, a.dbu};
+  for (void* p : dst)
+    if (!aligned(p, bytes)) return set_error(GNN_ERR_ARG, "gated_linear gradients: outputs must be aligned to their elements");
+  if (!a.dwg && !a.dwu && !a.dbg && !a.dbu) return set_error(GNN_ERR_ARG, "gated_linear gradients: an output is required");
+  const int64_t used = (a.M + r.slice_rows - 1) / r.slice_rows, each = 2 * a.O * a.I;
+  float* sums = a.dbg || a.dbu ? a.partial + used * each : nullptr;
+  int rc = rows_product(r, sums, (hipStream_t)stream);
+  if (rc == 0) {
+    gnn_reduce_args add{};
+    for (int k = 0; k < 2; ++k) {
+      if (dst[k]) add.seg[add.count++] = {a.partial + k * a.O * a.I, dst[k], used, each, a.outputs * a.I, a.dtype, 0};
+      if (dst[2 + k]) add.seg[add.count++] = {sums + k * a.O, dst[2 + k], used, 2 * a.O, a.outputs, a.dtype, 0};
+    }
+    rc = reduce_parts(add, (hipStream_t)stream);
+  }
+  if (rc < 0) return rc;
+  return hip_status((hipError_t)rc, "gated_linear gradients");
+}
+
 static int check_qk_rotary(const gnn_qk_rotary_args* args, bool bwd) {
   if (!args) return set_error(GNN_ERR_ARG, "qk_norm_rotary: args is NULL");
   const gnn_qk_rotary_args& a = *args;

@@ -75,6 +75,8 @@ int64_t relpos_parts(const gnn_relpos_args& a);
 int layer_norm_fwd(const gnn_layer_norm_fwd_args& a, hipStream_t stream);
 int64_t layer_norm_bwd_parts(int64_t rows, int64_t K, int32_t dtype);
 int layer_norm_bwd(const gnn_layer_norm_bwd_args& a, hipStream_t stream);
+int gated_linear(const gnn_gated_linear_args& a, hipStream_t stream);
+int gated_turn(const gnn_gated_turn_args& a, hipStream_t stream);
 int64_t qk_rotary_parts(const gnn_qk_rotary_args& a, int side);
 int qk_rotary(const gnn_qk_rotary_args& a, bool backward, hipStream_t stream);
 

@@ -576,6 +576,82 @@ class LayerNormBwdArgs(ctypes.Structure):
 pack_layer_norm_bwd = packer(LayerNormBwdArgs)
 
 
+class GatedLinearArgs(ctypes.Structure):
+    """Mirror of ``gnn_gated_linear_args``."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("wg", ctypes.c_void_p),
+        ("wu", ctypes.c_void_p),
+        ("bg", ctypes.c_void_p),
+        ("bu", ctypes.c_void_p),
+        ("dy", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("M", ctypes.c_int64),
+        ("I", ctypes.c_int64),
+        ("O", ctypes.c_int64),
+        ("out_cols", ctypes.c_int64),
+        ("x_ld", ctypes.c_int64),
+        ("wg_ld", ctypes.c_int64),
+        ("wu_ld", ctypes.c_int64),
+        ("dy_ld", ctypes.c_int64),
+        ("out_ld", ctypes.c_int64),
+        ("activation", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("precision", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+pack_gated_linear = packer(GatedLinearArgs)
+
+
+class GatedTurnArgs(ctypes.Structure):
+    """Mirror of ``gnn_gated_turn_args``."""
+
+    _fields_ = [
+        ("wg", ctypes.c_void_p),
+        ("wu", ctypes.c_void_p),
+        ("dst", ctypes.c_void_p),
+        ("I", ctypes.c_int64),
+        ("O", ctypes.c_int64),
+        ("out_cols", ctypes.c_int64),
+        ("wg_ld", ctypes.c_int64),
+        ("wu_ld", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+pack_gated_turn = packer(GatedTurnArgs)
+
+
+class GatedLinearWgradArgs(ctypes.Structure):
+    """Mirror of ``gnn_gated_linear_wgrad_args``."""
+
+    _fields_ = [
+        ("dz", ctypes.c_void_p),
+        ("x", ctypes.c_void_p),
+        ("partial", ctypes.c_void_p),
+        ("dwg", ctypes.c_void_p),
+        ("dwu", ctypes.c_void_p),
+        ("dbg", ctypes.c_void_p),
+        ("dbu", ctypes.c_void_p),
+        ("M", ctypes.c_int64),
+        ("O", ctypes.c_int64),
+        ("I", ctypes.c_int64),
+        ("outputs", ctypes.c_int64),
+        ("dz_ld", ctypes.c_int64),
+        ("x_ld", ctypes.c_int64),
+        ("slices", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+pack_gated_linear_wgrad = packer(GatedLinearWgradArgs)
+
+
 class QkRotaryArgs(ctypes.Structure):
     """Mirror of ``gnn_qk_rotary_args``: pairs are queries, keys; strides ``[side][batch, token, head]``."""
 
@@ -655,6 +731,10 @@ _SIGNATURES = {
     "gnn_pad_rows": (ctypes.c_int, [ctypes.POINTER(PadRowsArgs), ctypes.c_void_p]),
     "gnn_column_sums_parts": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64]),
     "gnn_column_sums": (ctypes.c_int, [ctypes.POINTER(ColumnSumsArgs), ctypes.c_void_p]),
+    "gnn_gated_linear": (ctypes.c_int, [ctypes.POINTER(GatedLinearArgs), ctypes.c_void_p]),
+    "gnn_gated_turn": (ctypes.c_int, [ctypes.POINTER(GatedTurnArgs), ctypes.c_void_p]),
+    "gnn_gated_linear_wgrad_slices": (ctypes.c_int64, [ctypes.POINTER(GatedLinearWgradArgs)]),
+    "gnn_gated_linear_wgrad": (ctypes.c_int, [ctypes.POINTER(GatedLinearWgradArgs), ctypes.c_void_p]),
     "gnn_qk_rotary_fwd": (ctypes.c_int, [ctypes.POINTER(QkRotaryArgs), ctypes.c_void_p]),
     "gnn_qk_rotary_parts": (ctypes.c_int64, [ctypes.POINTER(QkRotaryArgs), ctypes.c_int32]),
     "gnn_qk_rotary_bwd": (ctypes.c_int, [ctypes.POINTER(QkRotaryArgs), ctypes.c_void_p]),

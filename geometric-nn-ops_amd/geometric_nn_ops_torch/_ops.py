@@ -21,7 +21,8 @@ import torch
 from torch.autograd import forward_ad
 
 __all__ = ["triangle_attention_fwd", "trimul_fwd", "attention_pair_bias_fwd", "layer_norm_fwd",
-           "relative_position_bias_fwd", "fused_linear_fwd", "qk_norm_rotary_fwd", "eager_ok", "carries_tangent"]
+           "relative_position_bias_fwd", "fused_linear_fwd", "gated_linear_fwd", "qk_norm_rotary_fwd", "eager_ok",
+           "carries_tangent"]
 
 
 _PLAIN_TYPES = (torch.Tensor, torch.nn.Parameter)  # Parameter disables __torch_function__
@@ -226,6 +227,30 @@ fused_linear_fwd = torch.library.custom_op("gnn_amd::fused_linear_fwd", fused_li
 @fused_linear_fwd.register_fake
 def _fused_linear_fwd_fake(x, weight, bias, activation, residual):
     return x.new_empty((*x.shape[:-1], weight.shape[0]))
+
+
+def gated_linear_fwd_impl(
+    x: torch.Tensor,
+    gate_weight: torch.Tensor,
+    up_weight: torch.Tensor,
+    gate_bias: Optional[torch.Tensor],
+    up_bias: Optional[torch.Tensor],
+    activation: Optional[str],
+) -> torch.Tensor:
+    """``x [..., I]``, weights ``[O, I]``; returns a fresh contiguous ``[..., O]`` tensor of x's dtype."""
+    from . import _precision
+    from .triangle._kernels.gated_linear import gated_linear_hip
+
+    precision = _precision.matmul_precision(fp32_operands=x.dtype == torch.float32)
+    return gated_linear_hip(x, gate_weight, up_weight, gate_bias, up_bias, activation, precision=precision)
+
+
+gated_linear_fwd = torch.library.custom_op("gnn_amd::gated_linear_fwd", gated_linear_fwd_impl, mutates_args=())
+
+
+@gated_linear_fwd.register_fake
+def _gated_linear_fwd_fake(x, gate_weight, up_weight, gate_bias, up_bias, activation):
+    return x.new_empty((*x.shape[:-1], gate_weight.shape[0]))
 
 
 def qk_norm_rotary_fwd_impl(

@@ -2,6 +2,7 @@
 
 from ._attention_pair_bias import attention_pair_bias
 from ._fused_linear import fused_linear
+from ._gated_linear import gated_linear
 from ._layer_norm import layer_norm
 from ._qk_norm_rotary import qk_norm_rotary
 from ._relative_position import relative_position_bias
@@ -11,6 +12,7 @@ from ._trimul import triangle_multiplicative_update
 __all__ = [
     "attention_pair_bias",
     "fused_linear",
+    "gated_linear",
     "layer_norm",
     "qk_norm_rotary",
     "relative_position_bias",

@@ -736,6 +736,63 @@ typedef struct gnn_column_sums_args {
 int64_t gnn_column_sums_parts(int64_t M, int64_t O);
 int gnn_column_sums(const gnn_column_sums_args* args, void* stream);
 
+/* A gated layer, out = act(x wg^T + bg) (x wu^T + bu), or with dy the gradients at its two products' sums, side by
+ * side: out[m][n] = dy zu act'(zg) and out[m][out_cols + n] = dy act(zg), zeros for n from O to out_cols. x: rows of I
+ * elements, x_ld apart; wg, wu: [O] rows of I; all 16-byte aligned with I and the pitches multiples of 16 bytes (pad
+ * with zeros). bg, bu: [O] or NULL. dy: rows of O, any alignment of their elements; out: rows of O (any alignment),
+ * with dy of 2 out_cols, out_cols = O rounded up to 8. All in dtype; products and epilogue in fp32, one rounding.
+ * precision: fp32 products (GNN_PREC_IEEE or GNN_PREC_BF16X3). The reference has no such op. */
+typedef struct gnn_gated_linear_args {
+  const void* x;
+  const void* wg;
+  const void* wu;
+  const void* bg;
+  const void* bu;
+  const void* dy;
+  void* out;
+  int64_t M, I, O, out_cols;
+  int64_t x_ld, wg_ld, wu_ld, dy_ld, out_ld;
+  int32_t activation; /* enum gnn_activation */
+  int32_t dtype;
+  int32_t precision;
+  int32_t reserved;
+} gnn_gated_linear_args;
+int gnn_gated_linear(const gnn_gated_linear_args* args, void* stream);
+
+/* dst [I] rows of 2 out_cols, 16-byte aligned: both weights [O] rows of I turned and side by side, zeros from column O
+ * to out_cols (a multiple of 8) of each: the weight of the input gradient's product. */
+typedef struct gnn_gated_turn_args {
+  const void* wg;
+  const void* wu;
+  void* dst;
+  int64_t I, O, out_cols;
+  int64_t wg_ld, wu_ld;
+  int32_t dtype;
+  int32_t reserved;
+} gnn_gated_turn_args;
+int gnn_gated_turn(const gnn_gated_turn_args* args, void* stream);
+
+/* The gradients of a gated layer's parameters from dz [M] rows of 2 O (dz_ld apart) and x [M, I]: dwg, dwu [outputs][I]
+ * and dbg, dbu [outputs], each or NULL, in dtype. O (both halves' width), I and the pitches are multiples of 8, dz
+ * and x 16-byte aligned. partial: fp32 [slices][2 O][I], and behind it [slices][2 O]; slices as
+ * gnn_gated_linear_wgrad_slices returns it (any from 1 on is right). */
+typedef struct gnn_gated_linear_wgrad_args {
+  const void* dz;
+  const void* x;
+  float* partial;
+  void* dwg;
+  void* dwu;
+  void* dbg;
+  void* dbu;
+  int64_t M, O, I, outputs;
+  int64_t dz_ld, x_ld;
+  int64_t slices;
+  int32_t dtype;
+  int32_t reserved;
+} gnn_gated_linear_wgrad_args;
+int64_t gnn_gated_linear_wgrad_slices(const gnn_gated_linear_wgrad_args* args);
+int gnn_gated_linear_wgrad(const gnn_gated_linear_wgrad_args* args, void* stream);
+
 /* Norms of queries and keys for each head (x / sqrt(mean(x^2) + eps) w over the D elements) and the rotation by
  * positions behind them, side 0 the queries [B, N[0], H[0], D] and side 1 the keys [B, N[1], H[1], D]: pair j of the
  * first R elements (elements j and j + R / 2; interleaved: 2 j and 2 j + 1) turns by pos frequencies[j]. x and dy:
