@@ -765,6 +765,63 @@ int gnn_qk_rotary_bwd(const gnn_qk_rotary_args* args, void* stream) {
   return hip_status((hipError_t)rc, "qk_norm_rotary backward");
 }
 
+extern "C++" {
+// Shapes and types that the attention's two directions share
+template <typename Args>
+static int check_cross_attn(const Args* args) {
+  if (!args) return set_error(GNN_ERR_ARG, "cross_attention: args is NULL");
+  const Args& a = *args;
+  if (!known_dtype(a.dtype)) return set_error(GNN_ERR_ARG, "cross_attention: unknown dtype");
+  if (a.precision != GNN_PREC_IEEE && a.precision != GNN_PREC_BF16X3)
+    return set_error(GNN_ERR_ARG, "cross_attention: unknown precision");
+  if (a.D < 8 || a.D > 128 || a.D % 8)
+    return set_error(GNN_ERR_UNSUPPORTED, "cross_attention: the head dim must be a multiple of 8 up to 128");
+  const int64_t most = (int64_t)1 << 30;
+  if (a.B < 1 || a.U < 1 || a.V < 1 || a.H < 1 || a.Hk < 1 || a.B > most || a.U > most || a.V > most || a.H > most ||
+      a.H % a.Hk || a.U * (a.H / a.Hk) > most)
+    return set_error(GNN_ERR_ARG, "cross_attention: B, U, V, H and Hk must be positive, U H / Hk and V at most 2^30, H a multiple of Hk");
+  if (!(a.scale > 0.f) || a.scale > 3e38f) return set_error(GNN_ERR_ARG, "cross_attention: scale must be positive");
+  if (!a.q || !a.k || !a.v) return set_error(GNN_ERR_ARG, "cross_attention: q, k and v are required");
+  const size_t e = a.dtype == GNN_F32 ? 4 : 2;
+  if (!aligned(a.q, e) || !aligned(a.k, e) || !aligned(a.v, e) || !aligned(a.bias, e) || !aligned(a.stats, 4))
+    return set_error(GNN_ERR_ARG, "cross_attention: tensors must be aligned to their elements");
+  return GNN_OK;
+}
+}  // extern "C++"
+
+size_t gnn_cross_attn_workspace_bytes(const gnn_cross_attn_args* args) {
+  return check_cross_attn(args) ? 0 : cross_attn_workspace_bytes(*args);
+}
+
+int gnn_cross_attn_fwd(const gnn_cross_attn_args* args, void* stream) {
+  if (int rc = check_cross_attn(args)) return rc;
+  if (!args->o || !aligned(args->o, 16) || !aligned(args->workspace, 16))
+    return set_error(GNN_ERR_ARG, "cross_attention: o is required, o and the workspace 16-byte aligned");
+  int rc = cross_attn_fwd(*args, (hipStream_t)stream);
+  if (rc < 0) return rc;
+  return hip_status((hipError_t)rc, "cross_attention");
+}
+
+size_t gnn_cross_attn_bwd_workspace_bytes(const gnn_cross_attn_bwd_args* args) {
+  return check_cross_attn(args) ? 0 : cross_attn_bwd_workspace_bytes(*args);
+}
+
+int gnn_cross_attn_bwd(const gnn_cross_attn_bwd_args* args, void* stream) {
+  if (int rc = check_cross_attn(args)) return rc;
+  const gnn_cross_attn_bwd_args& a = *args;
+  if (!a.o || !a.dout || !a.stats || !a.dq || !a.dk != !a.dv || (a.dbias && !a.bias))
+    return set_error(GNN_ERR_ARG, "cross_attention backward: o, dout, stats and dq are required, dk and dv go together, dbias with bias");
+  if (a.shared_bias && a.bias_stride[0] != 0)
+    return set_error(GNN_ERR_ARG, "cross_attention backward: a shared bias has batch stride 0");
+  const size_t e = a.dtype == GNN_F32 ? 4 : 2;
+  if (!aligned(a.o, e) || !aligned(a.dout, e) || !aligned(a.dbias, e) || !aligned(a.dq, 16) || !aligned(a.dk, 16) ||
+      !aligned(a.dv, 16) || !aligned(a.workspace, 16))
+    return set_error(GNN_ERR_ARG, "cross_attention backward: o, dout and dbias must be aligned to their elements, dq, dk, dv and the workspace to 16 bytes");
+  int rc = cross_attn_bwd(a, (hipStream_t)stream);
+  if (rc < 0) return rc;
+  return hip_status((hipError_t)rc, "cross_attention backward");
+}
+
 const char* gnn_last_error(void) { return g_last_error.c_str(); }
 
 const char* gnn_version(void) { return "0.1.0 gfx950"; }

@@ -1,0 +1,551 @@
+// Backward of attention over the states of another sequence (cross_fwd.hip). With x the logits, m and l the reference
+// maximum and the log2 of the sum that the forward leaves of each row, and P = 2^((x - m) log2(e) - l) (as one number,
+// m + l would lose l beside the lowest values of a type):
+//   dV_j = sum_r P_rj dO_r,   dP_rj = dO_r . v_j,   Delta_r = dO_r . O_r,   dS_rj = P_rj (dP_rj - Delta_r),
+//   dQ_r = scale sum_j dS_rj k_j,   dK_j = scale sum_r dS_rj q_r,   dbias = dS (summed over a batch that shares it).
+// Rows r are the queries of all heads that share a key head, so that dK and dV of a shared head are one sum.
+//
+// Every sum has one owner and one order; S and dP are formed in each of the kernels that need them:
+//   cross_dq    the forward's layout (a lane holds a row and 16 keys): the dS^T accumulator is the operand of
+//               dQ^T += K^T dS^T as it stands, K being read turned from LDS. It runs first, forms Delta from dO and O
+//               and leaves it in fp32; it also writes dbias where every sequence has its own.
+//   cross_dkdv  keys on the lanes, a wave 32 of them; tiles of 64 rows of Q and dO in LDS, read plain for S and dP and
+//               turned for dV^T += dO^T P and dK^T += Q^T dS.
+//   cross_dbias a bias for all sequences: a tile of 128 rows x 64 keys of one head group walks over the batch.
+// Where one of the first two leaves CUs idle its loop is split over workgroups, whose fp32 sums are added in order.
+// P and dS are rounded to the operands' type for the products behind them. fp16: P is held 2^10 times as large for dV,
+// or a row spread over 10^5 keys would fall below fp16's normal range.
+#include <algorithm>
+
+#include "cross_common.hpp"
+
+namespace gnn {
+
+namespace {
+
+using namespace cross;
+
+constexpr int NT = 256;
+constexpr int KT = 64;   // keys a tile (dq), rows a tile (dk, dv)
+
+struct BwdArgs {
+  Shape s;
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* o;
+  const void* dout;
+  const void* bias;
+  const uint8_t* mask;
+  const float* stats;  // [B][H][U][2]
+  float* delta;      // [B][H][U]
+  void* dq;
+  void* dk;
+  void* dv;
+  void* dbias;       // [B or 1][H][U][V]
+  float* part_q;     // [q_splits][B][U][H][D], or NULL
+  float* part_k;     // [k_splits][2][B][V][Hk][D], or NULL
+  int64_t qs[3], ks[3], vs[3], os[3], ds[3], bs[3], ms[2];
+  float scale, logit_scale;  // the caller's; without a bias times log2(e)
+  int q_splits, q_tiles;  // tiles of keys a split
+  int k_splits, k_tiles;  // tiles of rows a split
+};
+
+template <typename T> constexpr float p_shift() { return 0.f; }
+template <> constexpr float p_shift<f16>() { return 10.f; }
+template <typename T> constexpr float p_unit() { return 1.f; }  // 2^-p_shift
+template <> constexpr float p_unit<f16>() { return 0x1p-10f; }
+
+// Fragments of one row of a lane, zeros past D
+template <typename T, int DP>
+__device__ __forceinline__ void load_row(typename TypeOps<T>::V8 (&f)[DP / 16], const T* p, int D, int g) {
+#pragma unroll
+  for (int kk = 0; kk < DP / 16; ++kk) {
+    const int d = 16 * kk + 8 * g;
+    f[kk] = load8_at(p + (d < D ? d : 0));
+    if (d >= D) f[kk] = zero8<T>();
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ f32x4 bias4(const T* row, int key, int V) {
+  return key < V ? load4_at(row + key, V - key) : f32x4{0.f, 0.f, 0.f, 0.f};
+}
+
+// 2^((score scale + bias - m) log2(e) - l); without a bias scale and m are in log2 units
+template <bool BIAS>
+__device__ __forceinline__ float probability(float score, float scale, float bias, float m, float l) {
+  if constexpr (BIAS) return fast_exp2(__builtin_fmaf(__builtin_fmaf(score, scale, bias) - m, LOG2E, -l));
+  return fast_exp2(__builtin_fmaf(score, scale, -(m + l)));
+}
+
+// dS^T = P (dP - Delta) of one half tile of 32 keys for the lane's row.
+// `word`: the kept keys of the half tile.
+template <typename T, int PREC, int DP, bool BIAS>
+__device__ __forceinline__ void half_tile(f32x16& dp, const unsigned char* ks, const unsigned char* vs, int at,
+                                          const typename TypeOps<T>::V8 (&qf)[DP / 16],
+                                          const typename TypeOps<T>::V8 (&df)[DP / 16], const T* bias_row, int key0, int V,
+                                          float scale, float m, float l, float delta, uint32_t word) {
+  typedef RowTile<T, DP> Tile;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+  f32x16 sc;
+  clear(sc), clear(dp);
+#pragma unroll
+  for (int kk = 0; kk < DP / 16; ++kk) {
+    Mma<T, PREC>::step(sc, Tile::row8(ks, at + l32, kk, g), qf[kk]);
+    Mma<T, PREC>::step(dp, Tile::row8(vs, at + l32, kk, g), df[kk]);
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    f32x4 add = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (BIAS) add = bias4(bias_row, key0 + 8 * q + 4 * g, V);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = 4 * q + e;
+      const float p = probability<BIAS>(sc[i], scale, add[e], m, l);
+      dp[i] = p * (dp[i] - delta);
+    }
+  }
+  if (word != ~0u) {  // uniform
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dp[i] = word >> acc_row(i, g) & 1 ? dp[i] : 0.f;
+  }
+}
+
+// -------------------------------------------------------------------------------------- dQ
+template <typename T, int PREC, int DP, bool BIAS>
+__global__ __launch_bounds__(NT, sizeof(T) == 4 ? 1 : 2) void cross_dq_kernel(const BwdArgs a) {
+  typedef RowTile<T, DP> Tile;
+  typedef typename TypeOps<T>::V8 V8;
+  constexpr int TILE = KT * Tile::PITCH, NBUF = sizeof(T) == 2 ? 2 : 1;
+  __shared__ __align__(16) unsigned char smem[NBUF * 2 * TILE];
+  __shared__ int found[2];
+  const Shape& s = a.s;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
+  const uint32_t nrb = (uint32_t)(s.rows + 127) / 128;
+  uint32_t w = xcd_remap(blockIdx.x, gridDim.x);
+  const int rb = w % nrb;
+  w /= nrb;
+  const int split = w % a.q_splits;
+  w /= a.q_splits;
+  const int hk = w % s.Hk, b = w / s.Hk;
+  const int row = rb * 128 + wave * 32 + l32;
+  const bool row_ok = row < s.rows;
+  const int safe = min(row, s.rows - 1), u = safe / s.G, h = hk * s.G + safe % s.G;
+  const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
+  const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
+  const T* bias_row = BIAS ? (const T*)a.bias + b * a.bs[0] + h * a.bs[1] + u * a.bs[2] : nullptr;
+  const uint8_t* mask = a.mask ? a.mask + b * a.ms[0] : nullptr;
+  const int64_t stat = ((int64_t)b * s.H + h) * s.U + u;
+
+  V8 qf[DP / 16], df[DP / 16];
+  load_row<T, DP>(qf, (const T*)a.q + b * a.qs[0] + u * a.qs[1] + h * a.qs[2], s.D, g);
+  load_row<T, DP>(df, (const T*)a.dout + b * a.ds[0] + u * a.ds[1] + h * a.ds[2], s.D, g);
+  const float m = a.stats[2 * stat], l = a.stats[2 * stat + 1];
+  float delta = 0.f;
+  {
+    const T* op = (const T*)a.o + b * a.os[0] + u * a.os[1] + h * a.os[2];
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+      const int d = 16 * kk + 8 * g;
+      const f32x8 x = TypeOps<T>::to_f32(load8_at(op + (d < s.D ? d : 0))) * TypeOps<T>::to_f32(df[kk]);
+      delta += d < s.D ? ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])) : 0.f;
+    }
+    delta = pair_sum(delta);
+    if (row_ok && g == 0 && split == 0) a.delta[stat] = delta;
+  }
+  // own bias: every tile is visited, so that what no row keeps gets its zeros
+  T* dbias = BIAS && a.dbias ? (T*)a.dbias + stat * s.V : nullptr;
+  int key_end = min(s.V, (split + 1) * a.q_tiles * KT), key0 = split * a.q_tiles * KT;
+  if (mask && !a.dbias) live_range<NT>(mask, a.ms[1], key0, key_end, found);
+  const int t_end = key0 < key_end ? (key_end + KT - 1) / KT : 0;
+
+  f32x16 dq[DP / 32];
+#pragma unroll
+  for (int cc = 0; cc < DP / 32; ++cc) clear(dq[cc]);
+  Staged<T, DP, KT, NT> kreg, vreg;
+  auto seek = [&](int t, uint64_t& word) {
+    for (; t < t_end; ++t) {
+      word = live_keys(mask, a.ms[1], t * KT, s.V);
+      if (word || a.dbias) break;
+    }
+    return t;
+  };
+  auto load = [&](int t) {
+    kreg.load(kp, s.D, [&](int r) { return (int64_t)min(t * KT + r, s.V - 1) * a.ks[1]; });
+    vreg.load(vp, s.D, [&](int r) { return (int64_t)min(t * KT + r, s.V - 1) * a.vs[1]; });
+  };
+  auto put = [&](int buf, uint64_t word) {  // what masked keys hold, NaN too, meets only zeros
+    unsigned char* st = smem + buf * 2 * TILE;
+    kreg.store(st, s.D, [&](int r) { return (word >> r & 1) != 0; });
+    vreg.store(st + TILE, s.D, [&](int r) { return (word >> r & 1) != 0; });
+  };
+  uint64_t live = 0, next_live = 0;
+  int t = seek(key0 / KT, live);
+  if (t < t_end) {
+    load(t);
+    put(0, live);
+  }
+  __syncthreads();
+  for (int buf = 0; t < t_end; buf ^= NBUF - 1) {
+    const int next = seek(t + 1, next_live);
+    if (next < t_end) load(next);
+    const unsigned char* ks = smem + buf * 2 * TILE;
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      f32x16 ds;
+      half_tile<T, PREC, DP, BIAS>(ds, ks, ks + TILE, 32 * sub, qf, df, bias_row, t * KT + 32 * sub, s.V, a.logit_scale, m, l,
+                                   delta, (uint32_t)(live >> (32 * sub)));
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        const V8 f = acc_frag<T>(ds, kk);
+#pragma unroll
+        for (int cc = 0; cc < DP / 32; ++cc) Mma<T, PREC>::step(dq[cc], Tile::turned8(ks, 32 * sub, kk, cc, lane), f);
+      }
+      if constexpr (BIAS) {
+        if (dbias && row_ok)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int key = t * KT + 32 * sub + 8 * q + 4 * g;
+            if (key < s.V) store4_at(dbias + key, f32x4{ds[4 * q], ds[4 * q + 1], ds[4 * q + 2], ds[4 * q + 3]}, s.V - key);
+          }
+      }
+    }
+    if constexpr (NBUF == 1) __syncthreads();
+    if (next < t_end) put(NBUF == 1 ? 0 : buf ^ 1, next_live);
+    __syncthreads();
+    t = next, live = next_live;
+  }
+  if (!row_ok) return;
+  const int64_t head = ((int64_t)b * s.U + u) * s.H + h, each = (int64_t)s.B * s.U * s.H * s.D;
+#pragma unroll
+  for (int cc = 0; cc < DP / 32; ++cc)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int d = 32 * cc + 8 * q + 4 * g;
+      if (d >= s.D) continue;
+      const f32x4 x = f32x4{dq[cc][4 * q], dq[cc][4 * q + 1], dq[cc][4 * q + 2], dq[cc][4 * q + 3]} * a.scale;
+      if (a.part_q)
+        *reinterpret_cast<f32x4*>(a.part_q + split * each + head * s.D + d) = x;
+      else
+        store4((T*)a.dq + head * s.D + d, TypeOps<T>::from_f32(x));
+    }
+}
+
+// ---------------------------------------------------------------------------------- dK, dV
+template <typename T, int PREC, int DP, bool BIAS>
+__global__ __launch_bounds__(NT, DP > 64 || sizeof(T) == 4 ? 1 : 2) void cross_dkdv_kernel(const BwdArgs a) {
+  typedef RowTile<T, DP> Tile;
+  typedef typename TypeOps<T>::V8 V8;
+  constexpr int TILE = KT * Tile::PITCH, NBUF = sizeof(T) == 2 ? 2 : 1;
+  __shared__ __align__(16) unsigned char smem[NBUF * 2 * TILE];
+  __shared__ float ms[NBUF][KT], ls[NBUF][KT], deltas[NBUF][KT];
+  __shared__ int64_t bias_at[BIAS ? NBUF : 1][BIAS ? KT : 1];
+  const Shape& s = a.s;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
+  const uint32_t nkb = (uint32_t)(s.V + 127) / 128;
+  uint32_t w = xcd_remap(blockIdx.x, gridDim.x);
+  const int kb = w % nkb;
+  w /= nkb;
+  const int split = w % a.k_splits;
+  w /= a.k_splits;
+  const int hk = w % s.Hk, b = w / s.Hk;
+  const int key = kb * 128 + wave * 32 + l32, safe = min(key, s.V - 1);
+  const bool kept = key < s.V && (!a.mask || a.mask[b * a.ms[0] + (int64_t)safe * a.ms[1]] != 0);
+  const bool all_kept = __all(kept), any_kept = __syncthreads_or(kept);
+  const T* qp = (const T*)a.q + b * a.qs[0];
+  const T* dop = (const T*)a.dout + b * a.ds[0];
+
+  // what masked keys hold meets only zeros
+  V8 kf[DP / 16], vf[DP / 16];
+  load_row<T, DP>(kf, (const T*)a.k + b * a.ks[0] + (int64_t)safe * a.ks[1] + hk * a.ks[2], s.D, g);
+  load_row<T, DP>(vf, (const T*)a.v + b * a.vs[0] + (int64_t)safe * a.vs[1] + hk * a.vs[2], s.D, g);
+  if (!kept)
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) kf[kk] = vf[kk] = zero8<T>();
+  const T* bias_key = BIAS ? (const T*)a.bias + b * a.bs[0] + safe : nullptr;
+
+  f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int cc = 0; cc < DP / 32; ++cc) clear(dk[cc]), clear(dv[cc]);
+  const int tiles = (s.rows + KT - 1) / KT;
+  const int t0 = split * a.k_tiles, t_end = any_kept ? min(tiles, t0 + a.k_tiles) : t0;
+  Staged<T, DP, KT, NT> qreg, dreg;
+  float next_m = 0.f, next_l = 0.f, next_delta = 0.f;
+  int64_t next_bias = 0;
+  auto load = [&](int t) {
+    auto place = [&](int r, int& u, int& h) {
+      const int row = min(t * KT + r, s.rows - 1);
+      u = row / s.G, h = hk * s.G + row % s.G;
+    };
+    qreg.load(qp, s.D, [&](int r) {
+      int u, h;
+      place(r, u, h);
+      return u * a.qs[1] + h * a.qs[2];
+    });
+    dreg.load(dop, s.D, [&](int r) {
+      int u, h;
+      place(r, u, h);
+      return u * a.ds[1] + h * a.ds[2];
+    });
+    if (threadIdx.x < KT) {
+      int u, h;
+      place(threadIdx.x, u, h);
+      const int64_t stat = ((int64_t)b * s.H + h) * s.U + u;
+      next_m = a.stats[2 * stat], next_l = a.stats[2 * stat + 1];
+      if (t * KT + (int)threadIdx.x >= s.rows) next_m = INFINITY;  // P = 2^-inf, and zeros of Q and dO
+      next_delta = a.delta[stat];
+      if constexpr (BIAS) next_bias = h * a.bs[1] + u * a.bs[2];
+    }
+  };
+  auto put = [&](int t, int buf) {
+    unsigned char* st = smem + buf * 2 * TILE;
+    qreg.store(st, s.D, [&](int r) { return t * KT + r < s.rows; });
+    dreg.store(st + TILE, s.D, [&](int r) { return t * KT + r < s.rows; });
+    if (threadIdx.x < KT) {
+      ms[buf][threadIdx.x] = next_m;
+      ls[buf][threadIdx.x] = next_l - p_shift<T>();
+      deltas[buf][threadIdx.x] = next_delta * p_unit<T>();
+      if constexpr (BIAS) bias_at[buf][threadIdx.x] = next_bias;
+    }
+  };
+  if (t0 < t_end) {
+    load(t0);
+    put(t0, 0);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int t = t0; t < t_end; ++t, buf ^= NBUF - 1) {
+    if (t + 1 < t_end) load(t + 1);
+    const unsigned char* qs = smem + buf * 2 * TILE;
+    const unsigned char* ds = qs + TILE;
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      const int r0 = 32 * sub;
+      f32x16 p, dp;
+      clear(p), clear(dp);
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        Mma<T, PREC>::step(p, Tile::row8(qs, r0 + l32, kk, g), kf[kk]);
+        Mma<T, PREC>::step(dp, Tile::row8(ds, r0 + l32, kk, g), vf[kk]);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 m4 = *reinterpret_cast<const f32x4*>(&ms[buf][r0 + 8 * q + 4 * g]);
+        const f32x4 l4 = *reinterpret_cast<const f32x4*>(&ls[buf][r0 + 8 * q + 4 * g]);
+        const f32x4 d4 = *reinterpret_cast<const f32x4*>(&deltas[buf][r0 + 8 * q + 4 * g]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = 4 * q + e;
+          float add = 0.f;
+          if constexpr (BIAS) add = TypeOps<T>::to_f32(bias_key[bias_at[buf][r0 + 8 * q + 4 * g + e]]);
+          p[i] = probability<BIAS>(p[i], a.logit_scale, add, m4[e], l4[e]);
+          dp[i] = __builtin_fmaf(dp[i], p_unit<T>(), -d4[e]);
+        }
+      }
+      if (!all_kept)  // uniform
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[i] = kept ? p[i] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dp[i] *= p[i];
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        const V8 pf = acc_frag<T>(p, kk), sf = acc_frag<T>(dp, kk);
+#pragma unroll
+        for (int cc = 0; cc < DP / 32; ++cc) {
+          Mma<T, PREC>::step(dv[cc], Tile::turned8(ds, r0, kk, cc, lane), pf);
+          Mma<T, PREC>::step(dk[cc], Tile::turned8(qs, r0, kk, cc, lane), sf);
+        }
+      }
+    }
+    if constexpr (NBUF == 1) __syncthreads();
+    if (t + 1 < t_end) put(t + 1, NBUF == 1 ? 0 : buf ^ 1);
+    __syncthreads();
+  }
+  if (key >= s.V) return;
+  const int64_t at = (((int64_t)b * s.V + key) * s.Hk + hk) * s.D, each = (int64_t)s.B * s.V * s.Hk * s.D;
+#pragma unroll
+  for (int cc = 0; cc < DP / 32; ++cc)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int d = 32 * cc + 8 * q + 4 * g;
+      if (d >= s.D) continue;
+      const f32x4 x = f32x4{dk[cc][4 * q], dk[cc][4 * q + 1], dk[cc][4 * q + 2], dk[cc][4 * q + 3]} * a.scale;
+      const f32x4 y = f32x4{dv[cc][4 * q], dv[cc][4 * q + 1], dv[cc][4 * q + 2], dv[cc][4 * q + 3]} * p_unit<T>();
+      if (a.part_k) {
+        *reinterpret_cast<f32x4*>(a.part_k + 2 * split * each + at + d) = x;
+        *reinterpret_cast<f32x4*>(a.part_k + (2 * split + 1) * each + at + d) = y;
+      } else {
+        store4((T*)a.dk + at + d, TypeOps<T>::from_f32(x));
+        store4((T*)a.dv + at + d, TypeOps<T>::from_f32(y));
+      }
+    }
+}
+
+// ------------------------------------------------------------------- dbias of a shared bias
+template <typename T, int PREC, int DP>
+__global__ __launch_bounds__(NT, sizeof(T) == 4 ? 1 : 2) void cross_dbias_kernel(const BwdArgs a) {
+  typedef RowTile<T, DP> Tile;
+  typedef typename TypeOps<T>::V8 V8;
+  constexpr int TILE = KT * Tile::PITCH;
+  __shared__ __align__(16) unsigned char smem[2 * TILE];
+  const Shape& s = a.s;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
+  const uint32_t nrb = (uint32_t)(s.rows + 127) / 128, nkb = (uint32_t)(s.V + KT - 1) / KT;
+  uint32_t w = xcd_remap(blockIdx.x, gridDim.x);
+  const int rb = w % nrb;
+  w /= nrb;
+  const int kb = w % nkb, hk = w / nkb;
+  const int row = rb * 128 + wave * 32 + l32;
+  const int safe = min(row, s.rows - 1), u = safe / s.G, h = hk * s.G + safe % s.G;
+  const T* bias_row = (const T*)a.bias + h * a.bs[1] + u * a.bs[2];
+  f32x16 sum[2];
+  clear(sum[0]), clear(sum[1]);
+  for (int b = 0; b < s.B; ++b) {
+    const uint64_t live = live_keys(a.mask ? a.mask + b * a.ms[0] : nullptr, a.ms[1], kb * KT, s.V);
+    if (!live) continue;  // the same for the whole workgroup
+    const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
+    const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
+    Staged<T, DP, KT, NT> kreg, vreg;
+    kreg.load(kp, s.D, [&](int r) { return (int64_t)min(kb * KT + r, s.V - 1) * a.ks[1]; });
+    vreg.load(vp, s.D, [&](int r) { return (int64_t)min(kb * KT + r, s.V - 1) * a.vs[1]; });
+    V8 qf[DP / 16], df[DP / 16];
+    load_row<T, DP>(qf, (const T*)a.q + b * a.qs[0] + u * a.qs[1] + h * a.qs[2], s.D, g);
+    load_row<T, DP>(df, (const T*)a.dout + b * a.ds[0] + u * a.ds[1] + h * a.ds[2], s.D, g);
+    const int64_t stat = ((int64_t)b * s.H + h) * s.U + u;
+    const float m = a.stats[2 * stat], l = a.stats[2 * stat + 1], delta = a.delta[stat];
+    __syncthreads();  // the sequence before is done with
+    kreg.store(smem, s.D, [&](int r) { return (live >> r & 1) != 0; });
+    vreg.store(smem + TILE, s.D, [&](int r) { return (live >> r & 1) != 0; });
+    __syncthreads();
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      f32x16 ds;
+      half_tile<T, PREC, DP, true>(ds, smem, smem + TILE, 32 * sub, qf, df, bias_row, kb * KT + 32 * sub, s.V, a.logit_scale,
+                                   m, l, delta, (uint32_t)(live >> (32 * sub)));
+      sum[sub] += ds;
+    }
+  }
+  if (row >= s.rows) return;
+  T* out = (T*)a.dbias + ((int64_t)h * s.U + u) * s.V;
+#pragma unroll
+  for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int key = kb * KT + 32 * sub + 8 * q + 4 * g;
+      const f32x16& x = sum[sub];
+      if (key < s.V) store4_at(out + key, f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]}, s.V - key);
+    }
+}
+
+struct Plan {
+  int64_t q_blocks, q_splits, q_tiles, k_blocks, k_splits, k_tiles;
+};
+void split(int64_t base, int64_t tiles, int64_t& splits, int64_t& each) {
+  // a workgroup a CU where the tiles allow it, of 8 at least
+  const int64_t want = std::max<int64_t>(1, (int64_t)compute_units() / base), most = std::max<int64_t>(1, tiles / 8);
+  each = (tiles + std::min(want, most) - 1) / std::min(want, most);
+  splits = (tiles + each - 1) / each;
+}
+Plan plan(const gnn_cross_attn_bwd_args& g) {
+  Plan p{};
+  const int64_t rows = g.U * (g.H / g.Hk), heads = g.B * g.Hk;
+  split((rows + 127) / 128 * heads, (g.V + KT - 1) / KT, p.q_splits, p.q_tiles);
+  split((g.V + 127) / 128 * heads, (rows + KT - 1) / KT, p.k_splits, p.k_tiles);
+  p.q_blocks = (rows + 127) / 128 * heads * p.q_splits;
+  p.k_blocks = (g.V + 127) / 128 * heads * p.k_splits;
+  return p;
+}
+
+template <typename T, int PREC, int DP, bool BIAS>
+int launch(const BwdArgs& a, const Plan& p, bool shared_bias, hipStream_t st) {
+  BwdArgs q = a;
+  if (shared_bias) q.dbias = nullptr;
+  hipLaunchKernelGGL((cross_dq_kernel<T, PREC, DP, BIAS>), dim3((uint32_t)p.q_blocks), dim3(NT), 0, st, q);
+  if (int rc = (int)hipGetLastError()) return rc;
+  if (a.dk) {
+    hipLaunchKernelGGL((cross_dkdv_kernel<T, PREC, DP, BIAS>), dim3((uint32_t)p.k_blocks), dim3(NT), 0, st, a);
+    if (int rc = (int)hipGetLastError()) return rc;
+  }
+  if constexpr (BIAS)
+    if (shared_bias && a.dbias) {
+      const int64_t blocks = (int64_t)((a.s.rows + 127) / 128) * ((a.s.V + KT - 1) / KT) * a.s.Hk;
+      if (blocks >= ((int64_t)1 << 31)) return set_error(GNN_ERR_UNSUPPORTED, "cross_attention: grid too large");
+      hipLaunchKernelGGL((cross_dbias_kernel<T, PREC, DP>), dim3((uint32_t)blocks), dim3(NT), 0, st, a);
+    }
+  return (int)hipGetLastError();
+}
+
+template <typename T, int PREC, int DP>
+int launch(const BwdArgs& a, const Plan& p, bool shared_bias, hipStream_t st) {
+  return a.bias ? launch<T, PREC, DP, true>(a, p, shared_bias, st) : launch<T, PREC, DP, false>(a, p, shared_bias, st);
+}
+
+template <typename T, int PREC>
+int run(const BwdArgs& a, const Plan& p, bool shared_bias, hipStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (a.s.D <= 32) return launch<T, PREC, 32>(a, p, shared_bias, st);
+    if (a.s.D > 64 && a.s.D <= 96) return launch<T, PREC, 96>(a, p, shared_bias, st);
+  }
+  if (a.s.D <= 64) return launch<T, PREC, 64>(a, p, shared_bias, st);
+  return launch<T, PREC, 128>(a, p, shared_bias, st);
+}
+
+// fp32 sums of the splits: dQ's, and behind them dK's and dV's
+void partial_sums(const gnn_cross_attn_bwd_args& g, const Plan& p, int64_t& q, int64_t& k) {
+  q = p.q_splits > 1 ? p.q_splits * g.B * g.U * g.H * g.D : 0;
+  k = p.k_splits > 1 && g.dk ? 2 * p.k_splits * g.B * g.V * g.Hk * g.D : 0;
+}
+
+}  // namespace
+
+size_t cross_attn_bwd_workspace_bytes(const gnn_cross_attn_bwd_args& g) {
+  int64_t q, k;
+  partial_sums(g, plan(g), q, k);
+  return ((size_t)g.B * g.U * g.H + 3) / 4 * 16 + (size_t)(q + k) * sizeof(float);
+}
+
+int cross_attn_bwd(const gnn_cross_attn_bwd_args& g, hipStream_t st) {
+  const Plan p = plan(g);
+  if (p.q_blocks >= ((int64_t)1 << 31) || p.k_blocks >= ((int64_t)1 << 31) || g.B * g.U * g.H >= ((int64_t)1 << 31))
+    return set_error(GNN_ERR_UNSUPPORTED, "cross_attention: grid too large");
+  if (!g.workspace || g.workspace_bytes < cross_attn_bwd_workspace_bytes(g))
+    return set_error(GNN_ERR_WORKSPACE, "cross_attention: workspace missing or too small");
+  BwdArgs a{};
+  a.s = {(int)g.B, (int)g.U, (int)g.V, (int)g.H, (int)g.Hk, (int)(g.H / g.Hk), (int)g.D, (int)(g.U * (g.H / g.Hk))};
+  a.q = g.q, a.k = g.k, a.v = g.v, a.o = g.o, a.dout = g.dout, a.bias = g.bias, a.mask = g.mask, a.stats = g.stats;
+  a.dq = g.dq, a.dk = g.dk, a.dv = g.dv, a.dbias = g.dbias;
+  for (int i = 0; i < 3; ++i) {
+    a.qs[i] = g.q_stride[i], a.ks[i] = g.k_stride[i], a.vs[i] = g.v_stride[i];
+    a.os[i] = g.o_stride[i], a.ds[i] = g.do_stride[i], a.bs[i] = g.bias_stride[i];
+  }
+  for (int i = 0; i < 2; ++i) a.ms[i] = g.mask_stride[i];
+  a.scale = g.scale, a.logit_scale = g.bias ? g.scale : g.scale * LOG2E;
+  a.q_splits = (int)p.q_splits, a.q_tiles = (int)p.q_tiles, a.k_splits = (int)p.k_splits, a.k_tiles = (int)p.k_tiles;
+  int64_t nq, nk;
+  partial_sums(g, p, nq, nk);
+  a.delta = (float*)g.workspace;
+  float* parts = a.delta + (g.B * g.U * g.H + 3) / 4 * 4;
+  if (nq) a.part_q = parts;
+  if (nk) a.part_k = parts + nq;
+  const bool shared_bias = g.bias && g.shared_bias && g.B > 1;
+  int rc;
+  switch (g.dtype) {
+    case GNN_BF16: rc = run<bf16, PREC_NATIVE>(a, p, shared_bias, st); break;
+    case GNN_F16: rc = run<f16, PREC_NATIVE>(a, p, shared_bias, st); break;
+    default:
+      rc = g.precision == GNN_PREC_BF16X3 ? run<float, PREC_BF16X3>(a, p, shared_bias, st)
+                                          : run<float, PREC_IEEE>(a, p, shared_bias, st);
+  }
+  if (rc || (!nq && !nk)) return rc;
+  gnn_reduce_args r{};
+  if (nq) r.seg[r.count++] = {a.part_q, g.dq, p.q_splits, nq / p.q_splits, nq / p.q_splits, g.dtype, 0};
+  if (nk) {
+    const int64_t each = nk / p.k_splits / 2;
+    r.seg[r.count++] = {a.part_k, g.dk, p.k_splits, 2 * each, each, g.dtype, 0};
+    r.seg[r.count++] = {a.part_k + each, g.dv, p.k_splits, 2 * each, each, g.dtype, 0};
+  }
+  return reduce_parts(r, st);
+}
+
+}  // namespace gnn

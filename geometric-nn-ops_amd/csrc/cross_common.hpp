@@ -1,0 +1,188 @@
+// What the kernels of attention over states of another length share: the shapes, a tile of rows in LDS and its
+// fragments, and the keys that a mask leaves.
+//
+// The queries of the heads that share a key head are the rows of one product: row r of the U G rows of (batch, key
+// head) is query r / G of head hk G + r % G, so that K and V are read once for all of them.
+#pragma once
+
+#include "gnn_common.hpp"
+#include "gnn_internal.hpp"
+
+namespace gnn {
+namespace cross {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Shape {
+  int B, U, V, H, Hk, G, D;
+  int rows;  // U G
+};
+
+// 8 elements at any element's address
+template <typename T>
+__device__ __forceinline__ typename TypeOps<T>::V8 load8_at(const T* p) {
+  typedef typename TypeOps<T>::V8 V8;
+  typedef V8 VU __attribute__((aligned(sizeof(T))));
+  return *(const __attribute__((address_space(1))) VU*)p;
+}
+// 16 bytes at any element's address
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <typename T>
+__device__ __forceinline__ u32x4 load16_at(const T* p) {
+  typedef u32x4 VU __attribute__((aligned(2)));
+  return *(const __attribute__((address_space(1))) VU*)p;
+}
+// 4 elements at any element's address, the first `left` of them
+template <typename T>
+__device__ __forceinline__ f32x4 load4_at(const T* p, int left) {
+  typedef typename TypeOps<T>::V4 V4;
+  typedef V4 VU __attribute__((aligned(sizeof(T))));
+  if (left >= 4) {
+    const V4 v = *(const __attribute__((address_space(1))) VU*)p;
+    return TypeOps<T>::to_f32(v);
+  }
+  f32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = e < left ? TypeOps<T>::to_f32(p[e]) : 0.f;
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store4_at(T* p, const f32x4& v, int left) {
+  typedef typename TypeOps<T>::V4 V4;
+  typedef V4 VU __attribute__((aligned(sizeof(T))));
+  const V4 o = TypeOps<T>::from_f32(v);
+  if (left >= 4) {
+    *(__attribute__((address_space(1))) VU*)p = o;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < left) p[e] = o[e];
+}
+
+// Rows of DP elements in LDS, their 16-byte chunks in chunk_swizzle's order: fragments of 32 rows (8 consecutive
+// elements a lane) and turned ones (8 rows of one column a lane) are both read without bank conflicts.
+template <typename T, int DP>
+struct RowTile {
+  static constexpr int BYTES = DP * (int)sizeof(T);
+  static constexpr int PITCH = BYTES <= 64 ? 64 : BYTES <= 128 ? 128 : BYTES <= 256 ? 256 : 512;
+  static constexpr int CPR = BYTES / 16;            // chunks a row
+  static constexpr int EPC = 16 / (int)sizeof(T);   // elements a chunk
+  typedef typename TypeOps<T>::V8 V8;
+  typedef typename TypeOps<T>::V4 V4;
+  static __device__ __forceinline__ int at(int row, int chunk) {
+    return row * PITCH + ((chunk ^ chunk_swizzle<(PITCH < 256 ? PITCH : 256)>(row)) << 4);
+  }
+  // elements 16 kk + 8 g .. + 7 of a row
+  static __device__ __forceinline__ V8 row8(const unsigned char* tile, int row, int kk, int g) {
+    if constexpr (sizeof(T) == 2) {
+      return *reinterpret_cast<const V8*>(tile + at(row, 2 * kk + g));
+    } else {
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(tile + at(row, 4 * kk + 2 * g));
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(tile + at(row, 4 * kk + 2 * g + 1));
+      return V8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    }
+  }
+  // column 32 cc + lane % 32 of the rows row0 + 16 kk + 8 (e / 4) + 4 g + e % 4: the order in which a 32x32
+  // accumulator holds its rows. 16-bit: ds_read_b64_tr_b16 hands the 16 lanes of a group a block of 4 rows x 16
+  // columns turned.
+  static __device__ __forceinline__ V8 turned8(const unsigned char* tile, int row0, int kk, int cc, int lane) {
+    const int g = lane >> 5;
+    V8 f;
+    if constexpr (sizeof(T) == 2) {
+      typedef short v4i16 __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
+      const int r16 = lane & 15, col = 32 * cc + 16 * ((lane >> 4) & 1) + 4 * (r16 & 3);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const unsigned char* p = tile + at(row0 + 16 * kk + 8 * h + 4 * g + (r16 >> 2), col >> 3) + 2 * (col & 7);
+        const V4 x = __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                (lds_v4i16*)(__attribute__((address_space(3))) const unsigned char*)p));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[4 * h + e] = x[e];
+      }
+    } else {
+      const int col = 32 * cc + (lane & 31);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        f[e] = *reinterpret_cast<const float*>(tile + at(row0 + 16 * kk + 8 * (e >> 2) + 4 * g + (e & 3), col >> 2) +
+                                               4 * (col & 3));
+    }
+    return f;
+  }
+};
+
+// ROWS rows of a tensor on their way to LDS through registers: chunk i of a thread is row(i), elements col(i) ..
+template <typename T, int DP, int ROWS, int NT>
+struct Staged {
+  typedef RowTile<T, DP> Tile;
+  static constexpr int N = ROWS * Tile::CPR / NT;
+  static_assert(N * NT == ROWS * Tile::CPR, "chunks a thread");
+  u32x4 reg[N];
+  static __device__ __forceinline__ int row(int i) { return ((int)threadIdx.x + i * NT) / Tile::CPR; }
+  static __device__ __forceinline__ int chunk(int i) { return ((int)threadIdx.x + i * NT) % Tile::CPR; }
+  // row r from base + offset(r): always a readable row; columns past D read column 0
+  template <typename Offset>
+  __device__ __forceinline__ void load(const T* base, int D, Offset offset) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = chunk(i) * Tile::EPC;
+      reg[i] = load16_at(base + offset(row(i)) + (c < D ? c : 0));
+    }
+  }
+  // rows for which `keep` is false, and columns past D, are zeros
+  template <typename Keep>
+  __device__ __forceinline__ void store(unsigned char* tile, int D, Keep keep) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const bool ok = chunk(i) * Tile::EPC < D && keep(row(i));
+      *reinterpret_cast<u32x4*>(tile + Tile::at(row(i), chunk(i))) = ok ? reg[i] : u32x4{0u, 0u, 0u, 0u};
+    }
+  }
+};
+
+// Bit j of the result: key `key0 + j` is below V and kept. The same for the whole wave.
+__device__ __forceinline__ uint64_t live_keys(const uint8_t* mask, int64_t stride, int key0, int V) {
+  const int key = key0 + (int)(threadIdx.x & 63);
+  bool live = key < V;
+  if (mask) live = live && mask[(int64_t)min(key, V - 1) * stride] != 0;
+  return __ballot(live);
+}
+
+// The first and one past the last kept key of [k0, k1), found by all threads of a workgroup; first >= end where there
+// is none. `found`: two ints of LDS. Padded sequences end early, and a tile of theirs that is not visited costs nothing.
+template <int NT>
+__device__ __forceinline__ void live_range(const uint8_t* mask, int64_t stride, int& k0, int& k1, int* found) {
+  if (threadIdx.x == 0) found[0] = k1, found[1] = k0;
+  __syncthreads();
+  constexpr int AT_ONCE = 8;
+  int first = k1, last = k0;
+  for (int base = k0 + (int)threadIdx.x; base < k1; base += NT * AT_ONCE) {
+    uint8_t m[AT_ONCE];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) m[i] = mask[(int64_t)min(base + i * NT, k1 - 1) * stride];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i)
+      if (m[i] && base + i * NT < k1) first = min(first, base + i * NT), last = max(last, base + i * NT + 1);
+  }
+  if (first < last) atomicMin(&found[0], first), atomicMax(&found[1], last);
+  __syncthreads();
+  k0 = found[0], k1 = found[1];
+}
+
+// Fragment kk of an accumulator: its 8 elements 8 kk .. as T
+template <typename T>
+__device__ __forceinline__ typename TypeOps<T>::V8 acc_frag(const f32x16& a, int kk) {
+  const f32x8 x = {a[8 * kk + 0], a[8 * kk + 1], a[8 * kk + 2], a[8 * kk + 3],
+                   a[8 * kk + 4], a[8 * kk + 5], a[8 * kk + 6], a[8 * kk + 7]};
+  return TypeOps<T>::from_f32(x);
+}
+__device__ __forceinline__ void clear(f32x16& a) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) a[i] = 0.f;
+}
+// row of element i of an accumulator in lane group g
+__device__ __forceinline__ int acc_row(int i, int g) { return 8 * (i / 4) + 4 * g + i % 4; }
+
+}  // namespace cross
+}  // namespace gnn

@@ -177,6 +177,17 @@ __device__ __forceinline__ uint32_t lds_addr(const unsigned char* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)p;
 }
 
+// 16-byte chunk c of row r lies at chunk c ^ chunk_swizzle(r) of its row. LDS serves 16 lanes' chunks, 256
+// bytes, at once: the swizzle spreads 16 consecutive rows' chunk c over all of them, whatever a row's bytes
+// (8 rows over 128 bytes, r % 8, left two-fold conflicts), and also 4-chunk blocks of 8 rows, which the
+// transposed reads take.
+template <int ROWB>
+__device__ __forceinline__ int chunk_swizzle(int r) {
+  if constexpr (ROWB == 64) return (r >> 2) & 3;
+  if constexpr (ROWB == 128) return (r & 2) << 1 | ((r >> 2) & 3);
+  return (r & 3) << 2 | ((r >> 2) & 3);
+}
+
 // ---- 32x32 tile, one K=16 step ----------------------------------------------------------
 // acc[row, col] += sum_k A[row, k] * B[k, col] over the 16 k of this step, with both
 // operands given as fragments (see the file comment).

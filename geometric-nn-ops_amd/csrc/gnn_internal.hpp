@@ -77,6 +77,10 @@ int64_t layer_norm_bwd_parts(int64_t rows, int64_t K, int32_t dtype);
 int layer_norm_bwd(const gnn_layer_norm_bwd_args& a, hipStream_t stream);
 int gated_linear(const gnn_gated_linear_args& a, hipStream_t stream);
 int gated_turn(const gnn_gated_turn_args& a, hipStream_t stream);
+size_t cross_attn_workspace_bytes(const gnn_cross_attn_args& a);
+int cross_attn_fwd(const gnn_cross_attn_args& a, hipStream_t stream);
+size_t cross_attn_bwd_workspace_bytes(const gnn_cross_attn_bwd_args& a);
+int cross_attn_bwd(const gnn_cross_attn_bwd_args& a, hipStream_t stream);
 int64_t qk_rotary_parts(const gnn_qk_rotary_args& a, int side);
 int qk_rotary(const gnn_qk_rotary_args& a, bool backward, hipStream_t stream);
 

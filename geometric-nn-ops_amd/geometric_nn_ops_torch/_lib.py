@@ -685,6 +685,81 @@ class QkRotaryArgs(ctypes.Structure):
 pack_qk_rotary = packer(QkRotaryArgs)
 
 
+class CrossAttnArgs(ctypes.Structure):
+    """Mirror of ``gnn_cross_attn_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("mask", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("stats", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("B", ctypes.c_int64),
+        ("U", ctypes.c_int64),
+        ("V", ctypes.c_int64),
+        ("H", ctypes.c_int64),
+        ("Hk", ctypes.c_int64),
+        ("D", ctypes.c_int64),
+        ("q_stride", I64x3),
+        ("k_stride", I64x3),
+        ("v_stride", I64x3),
+        ("bias_stride", I64x3),
+        ("mask_stride", I64x2),
+        ("scale", ctypes.c_float),
+        ("dtype", ctypes.c_int32),
+        ("precision", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+pack_cross_attn = packer(CrossAttnArgs)
+
+
+class CrossAttnBwdArgs(ctypes.Structure):
+    """Mirror of ``gnn_cross_attn_bwd_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("dout", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("mask", ctypes.c_void_p),
+        ("stats", ctypes.c_void_p),
+        ("dq", ctypes.c_void_p),
+        ("dk", ctypes.c_void_p),
+        ("dv", ctypes.c_void_p),
+        ("dbias", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("B", ctypes.c_int64),
+        ("U", ctypes.c_int64),
+        ("V", ctypes.c_int64),
+        ("H", ctypes.c_int64),
+        ("Hk", ctypes.c_int64),
+        ("D", ctypes.c_int64),
+        ("q_stride", I64x3),
+        ("k_stride", I64x3),
+        ("v_stride", I64x3),
+        ("o_stride", I64x3),
+        ("do_stride", I64x3),
+        ("bias_stride", I64x3),
+        ("mask_stride", I64x2),
+        ("scale", ctypes.c_float),
+        ("dtype", ctypes.c_int32),
+        ("precision", ctypes.c_int32),
+        ("shared_bias", ctypes.c_int32),
+    ]
+
+
+pack_cross_attn_bwd = packer(CrossAttnBwdArgs)
+
+
 RELAYOUT_PLANES_TO_PIXELS, RELAYOUT_PIXELS_TO_BLOCKED, RELAYOUT_PIXELS_TO_PLANES = 0, 1, 2
 
 _SIGNATURES = {
@@ -738,6 +813,10 @@ _SIGNATURES = {
     "gnn_qk_rotary_fwd": (ctypes.c_int, [ctypes.POINTER(QkRotaryArgs), ctypes.c_void_p]),
     "gnn_qk_rotary_parts": (ctypes.c_int64, [ctypes.POINTER(QkRotaryArgs), ctypes.c_int32]),
     "gnn_qk_rotary_bwd": (ctypes.c_int, [ctypes.POINTER(QkRotaryArgs), ctypes.c_void_p]),
+    "gnn_cross_attn_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(CrossAttnArgs)]),
+    "gnn_cross_attn_fwd": (ctypes.c_int, [ctypes.POINTER(CrossAttnArgs), ctypes.c_void_p]),
+    "gnn_cross_attn_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(CrossAttnBwdArgs)]),
+    "gnn_cross_attn_bwd": (ctypes.c_int, [ctypes.POINTER(CrossAttnBwdArgs), ctypes.c_void_p]),
     "gnn_last_error": (ctypes.c_char_p, []),
     "gnn_version": (ctypes.c_char_p, []),
 }

@@ -21,8 +21,8 @@ import torch
 from torch.autograd import forward_ad
 
 __all__ = ["triangle_attention_fwd", "trimul_fwd", "attention_pair_bias_fwd", "layer_norm_fwd",
-           "relative_position_bias_fwd", "fused_linear_fwd", "gated_linear_fwd", "qk_norm_rotary_fwd", "eager_ok",
-           "carries_tangent"]
+           "relative_position_bias_fwd", "fused_linear_fwd", "gated_linear_fwd", "cross_attention_fwd",
+           "qk_norm_rotary_fwd", "eager_ok", "carries_tangent"]
 
 
 _PLAIN_TYPES = (torch.Tensor, torch.nn.Parameter)  # Parameter disables __torch_function__
@@ -251,6 +251,31 @@ gated_linear_fwd = torch.library.custom_op("gnn_amd::gated_linear_fwd", gated_li
 @gated_linear_fwd.register_fake
 def _gated_linear_fwd_fake(x, gate_weight, up_weight, gate_bias, up_bias, activation):
     return x.new_empty((*x.shape[:-1], gate_weight.shape[0]))
+
+
+def cross_attention_fwd_impl(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    bias: Optional[torch.Tensor],
+    mask: Optional[torch.Tensor],
+    scale: float,
+) -> torch.Tensor:
+    """``q [B, U, H, D]``, ``k``, ``v [B, V, Hk, D]``, bias ``[B or 1, H, U, V]``, bool mask ``[B, V]``; returns a fresh
+    contiguous tensor of q's shape and dtype."""
+    from . import _precision
+    from .triangle._kernels.cross_attention import cross_attention_hip
+
+    precision = _precision.matmul_precision(fp32_operands=q.dtype == torch.float32)
+    return cross_attention_hip(q, k, v, bias, mask, scale, precision=precision)
+
+
+cross_attention_fwd = torch.library.custom_op("gnn_amd::cross_attention_fwd", cross_attention_fwd_impl, mutates_args=())
+
+
+@cross_attention_fwd.register_fake
+def _cross_attention_fwd_fake(q, k, v, bias, mask, scale):
+    return q.new_empty(q.shape)
 
 
 def qk_norm_rotary_fwd_impl(

@@ -1,6 +1,7 @@
 """Triangle (protein-folding) ops (reference geometric_nn_ops_torch/triangle/__init__.py:6-14)."""
 
 from ._attention_pair_bias import attention_pair_bias
+from ._cross_attention import cross_attention
 from ._fused_linear import fused_linear
 from ._gated_linear import gated_linear
 from ._layer_norm import layer_norm
@@ -11,6 +12,7 @@ from ._trimul import triangle_multiplicative_update
 
 __all__ = [
     "attention_pair_bias",
+    "cross_attention",
     "fused_linear",
     "gated_linear",
     "layer_norm",

@@ -828,6 +828,73 @@ int gnn_qk_rotary_fwd(const gnn_qk_rotary_args* args, void* stream);
 int64_t gnn_qk_rotary_parts(const gnn_qk_rotary_args* args, int32_t side);
 int gnn_qk_rotary_bwd(const gnn_qk_rotary_args* args, void* stream);
 
+/* Attention of queries over the states of another sequence:
+ *   o[b,u,h,:] = sum_j softmax_j(scale q[b,u,h,:].k[b,j,h/G,:] + bias[b,h,u,j]) v[b,j,h/G,:] over the kept keys j,
+ * zero where none is kept. q: [B,U,H,D], k and v: [B,V,Hk,D] with H = G Hk, strides of batch, token and head, unit
+ * stride over D (a multiple of 8 up to 128), any alignment of their elements; o: dense [B,U,H,D], 16-byte aligned.
+ * bias: strides of batch (0 where one goes with every sequence), head and query, unit stride over the keys, or NULL;
+ * mask: bytes [B,V] with strides, nonzero = keep, or NULL: what masked keys hold, in bias, k or v, has no effect.
+ * scale is positive. stats: fp32 [B,H,U,2], written where not NULL, what the backward needs of each row's sum (a
+ * reference maximum, +inf where no key is kept, and the log2 of the sum). workspace: gnn_cross_attn_workspace_bytes(args) bytes, 16-byte aligned (NULL when 0), used during the call.
+ * The reference's attention has one length and as many key heads as query heads (triangle/_triattn.py:23-106). */
+typedef struct gnn_cross_attn_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* bias;
+  const uint8_t* mask;
+  void* o;
+  float* stats;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t B, U, V, H, Hk, D;
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t bias_stride[3];
+  int64_t mask_stride[2];
+  float scale;
+  int32_t dtype;     /* enum gnn_dtype of q, k, v, bias and o */
+  int32_t precision; /* fp32 products: GNN_PREC_IEEE or GNN_PREC_BF16X3 */
+  int32_t reserved;
+} gnn_cross_attn_args;
+size_t gnn_cross_attn_workspace_bytes(const gnn_cross_attn_args* args);
+int gnn_cross_attn_fwd(const gnn_cross_attn_args* args, void* stream);
+
+/* Its backward from the forward's inputs, output o and stats and the output gradient dout (o and dout: strides as q's).
+ * dq, dk, dv: dense like q, k and v, 16-byte aligned; dk and dv both or neither. dbias: dense [B,H,U,V] (any alignment
+ * of its elements), with shared_bias (bias_stride[0] is 0 then) [1,H,U,V] summed over the batch; or NULL. */
+typedef struct gnn_cross_attn_bwd_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* o;
+  const void* dout;
+  const void* bias;
+  const uint8_t* mask;
+  const float* stats;
+  void* dq;
+  void* dk;
+  void* dv;
+  void* dbias;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t B, U, V, H, Hk, D;
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t o_stride[3];
+  int64_t do_stride[3];
+  int64_t bias_stride[3];
+  int64_t mask_stride[2];
+  float scale;
+  int32_t dtype;
+  int32_t precision;
+  int32_t shared_bias;
+} gnn_cross_attn_bwd_args;
+size_t gnn_cross_attn_bwd_workspace_bytes(const gnn_cross_attn_bwd_args* args);
+int gnn_cross_attn_bwd(const gnn_cross_attn_bwd_args* args, void* stream);
+
 /* Message for the last failing call on this thread ("" if none). */
 const char* gnn_last_error(void);
 
