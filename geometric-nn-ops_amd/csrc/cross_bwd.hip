@@ -172,11 +172,16 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 ? 1 : 2) void cross_dq_kernel(co
     return t;
   };
   auto load = [&](int t) {
-    kreg.load(kp, s.D, [&](int r) { return (int64_t)min(t * KT + r, s.V - 1) * a.ks[1]; });
-    vreg.load(vp, s.D, [&](int r) { return (int64_t)min(t * KT + r, s.V - 1) * a.vs[1]; });
+    kreg.load_rows(kp, a.ks[1], t * KT, s.V, s.D);
+    vreg.load_rows(vp, a.vs[1], t * KT, s.V, s.D);
   };
   auto put = [&](int buf, uint64_t word) {  // what masked keys hold, NaN too, meets only zeros
     unsigned char* st = smem + buf * 2 * TILE;
+    if (s.D == DP && word == ~0ull) {  // uniform
+      kreg.store(st);
+      vreg.store(st + TILE);
+      return;
+    }
     kreg.store(st, s.D, [&](int r) { return (word >> r & 1) != 0; });
     vreg.store(st + TILE, s.D, [&](int r) { return (word >> r & 1) != 0; });
   };
@@ -407,8 +412,8 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 ? 1 : 2) void cross_dbias_kernel
     const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
     const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
     Staged<T, DP, KT, NT> kreg, vreg;
-    kreg.load(kp, s.D, [&](int r) { return (int64_t)min(kb * KT + r, s.V - 1) * a.ks[1]; });
-    vreg.load(vp, s.D, [&](int r) { return (int64_t)min(kb * KT + r, s.V - 1) * a.vs[1]; });
+    kreg.load_rows(kp, a.ks[1], kb * KT, s.V, s.D);
+    vreg.load_rows(vp, a.vs[1], kb * KT, s.V, s.D);
     V8 qf[DP / 16], df[DP / 16];
     load_row<T, DP>(qf, (const T*)a.q + b * a.qs[0] + u * a.qs[1] + h * a.qs[2], s.D, g);
     load_row<T, DP>(df, (const T*)a.dout + b * a.ds[0] + u * a.ds[1] + h * a.ds[2], s.D, g);

@@ -112,16 +112,32 @@ struct RowTile {
   }
 };
 
-// ROWS rows of a tensor on their way to LDS through registers: chunk i of a thread is row(i), elements col(i) ..
+// ROWS rows of a tensor on their way to LDS through registers: chunk i of a thread is row(i), elements col(i) .. A
+// thread's first row and column are the same for every tile, its other rows whole steps further on: where all ROWS rows
+// exist the addresses are a uniform base each and one 32-bit offset (the host keeps 64 rows below 2^31 bytes).
 template <typename T, int DP, int ROWS, int NT>
 struct Staged {
   typedef RowTile<T, DP> Tile;
   static constexpr int N = ROWS * Tile::CPR / NT;
+  static constexpr bool EVEN = NT % Tile::CPR == 0;  // every chunk of a thread is in the same column
+  static constexpr int STEP = NT / Tile::CPR;        // rows from one chunk to the next, where EVEN
   static_assert(N * NT == ROWS * Tile::CPR, "chunks a thread");
   u32x4 reg[N];
-  static __device__ __forceinline__ int row(int i) { return ((int)threadIdx.x + i * NT) / Tile::CPR; }
-  static __device__ __forceinline__ int chunk(int i) { return ((int)threadIdx.x + i * NT) % Tile::CPR; }
-  // row r from base + offset(r): always a readable row; columns past D read column 0
+  static __device__ __forceinline__ int row(int i) { return EVEN ? (int)threadIdx.x / Tile::CPR + i * STEP : ((int)threadIdx.x + i * NT) / Tile::CPR; }
+  static __device__ __forceinline__ int chunk(int i) { return EVEN ? (int)threadIdx.x % Tile::CPR : ((int)threadIdx.x + i * NT) % Tile::CPR; }
+  // rows first .. first + ROWS - 1 of `end` rows, those past the last one its copies; columns past D read column 0
+  __device__ __forceinline__ void load_rows(const T* base, int64_t stride, int first, int end, int D) {
+    if (EVEN && first + ROWS <= end) {  // uniform
+      const int c = chunk(0) * Tile::EPC;
+      const uint32_t lane = (uint32_t)((int)threadIdx.x / Tile::CPR * (int)stride + (c < D ? c : 0)) * (uint32_t)sizeof(T);
+      const T* tile = base + first * stride;
+#pragma unroll
+      for (int i = 0; i < N; ++i) reg[i] = load16_at((const T*)((const char*)(tile + i * STEP * stride) + lane));
+      return;
+    }
+    load(base, D, [&](int r) { return (int64_t)min(first + r, end - 1) * stride; });
+  }
+  // row r from base + offset(r): always a readable row
   template <typename Offset>
   __device__ __forceinline__ void load(const T* base, int D, Offset offset) {
 #pragma unroll
@@ -130,23 +146,28 @@ struct Staged {
       reg[i] = load16_at(base + offset(row(i)) + (c < D ? c : 0));
     }
   }
+  // whole rows of D = DP elements
+  __device__ __forceinline__ void store(unsigned char* tile) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) *reinterpret_cast<u32x4*>(tile + Tile::at(row(i), chunk(i))) = reg[i];
+  }
   // rows for which `keep` is false, and columns past D, are zeros
   template <typename Keep>
   __device__ __forceinline__ void store(unsigned char* tile, int D, Keep keep) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const bool ok = chunk(i) * Tile::EPC < D && keep(row(i));
-      *reinterpret_cast<u32x4*>(tile + Tile::at(row(i), chunk(i))) = ok ? reg[i] : u32x4{0u, 0u, 0u, 0u};
+      const uint32_t ok = chunk(i) * Tile::EPC < D && keep(row(i)) ? ~0u : 0u;
+      *reinterpret_cast<u32x4*>(tile + Tile::at(row(i), chunk(i))) = reg[i] & u32x4{ok, ok, ok, ok};
     }
   }
 };
 
 // Bit j of the result: key `key0 + j` is below V and kept. The same for the whole wave.
 __device__ __forceinline__ uint64_t live_keys(const uint8_t* mask, int64_t stride, int key0, int V) {
-  const int key = key0 + (int)(threadIdx.x & 63);
-  bool live = key < V;
-  if (mask) live = live && mask[(int64_t)min(key, V - 1) * stride] != 0;
-  return __ballot(live);
+  const int left = V - key0;
+  uint64_t live = left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
+  if (mask && live) live &= __ballot(mask[(int64_t)min(key0 + (int)(threadIdx.x & 63), V - 1) * stride] != 0);
+  return live;
 }
 
 // The first and one past the last kept key of [k0, k1), found by all threads of a workgroup; first >= end where there
@@ -180,6 +201,11 @@ __device__ __forceinline__ typename TypeOps<T>::V8 acc_frag(const f32x16& a, int
 __device__ __forceinline__ void clear(f32x16& a) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) a[i] = 0.f;
+}
+// maximum and sum over the lane pair (l, l ^ 32) without a trip through LDS
+__device__ __forceinline__ float pair_top(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 // row of element i of an accumulator in lane group g
 __device__ __forceinline__ int acc_row(int i, int g) { return 8 * (i / 4) + 4 * g + i % 4; }

@@ -119,11 +119,19 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void cross
     return t;
   };
   auto load = [&](int t) {
-    kreg.load(kp, s.D, [&](int r) { return (int64_t)min(t * C::KT + r, s.V - 1) * a.ks[1]; });
-    vreg.load(vp, s.D, [&](int r) { return (int64_t)min(t * C::KT + r, s.V - 1) * a.vs[1]; });
+    kreg.load_rows(kp, a.ks[1], t * C::KT, s.V, s.D);
+    vreg.load_rows(vp, a.vs[1], t * C::KT, s.V, s.D);
   };
   auto put = [&](int buf, const uint64_t (&words)[(C::KT + 63) / 64]) {
     unsigned char* st = smem + buf * 2 * C::TILE;
+    bool whole = s.D == DP;
+#pragma unroll
+    for (int i = 0; i < (C::KT + 63) / 64; ++i) whole = whole && words[i] == ~0ull;
+    if (whole) {  // uniform
+      kreg.store(st);
+      vreg.store(st + C::TILE);
+      return;
+    }
     kreg.store(st, s.D, [](int) { return true; });
     vreg.store(st + C::TILE, s.D, [&](int r) { return (words[r / 64] >> (r & 63) & 1) != 0; });
   };
@@ -141,6 +149,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void cross
     const unsigned char* vs = ks + C::TILE;
     const int r0 = WK == 1 ? 0 : 32 * wave;  // this wave's keys of the tile
     f32x16 sc[C::SUBS];
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int sub = 0; sub < C::SUBS; ++sub) {
       clear(sc[sub]);
@@ -148,6 +157,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void cross
       for (int kk = 0; kk < DP / 16; ++kk)
         Mma<T, PREC>::step(sc[sub], Tile::row8(ks, r0 + 32 * sub + l32, kk, g), qf[kk]);
     }
+    __builtin_amdgcn_s_setprio(0);
     if constexpr (BIAS) {
 #pragma unroll
       for (int sub = 0; sub < C::SUBS; ++sub)
@@ -173,7 +183,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void cross
     for (int sub = 0; sub < C::SUBS; ++sub)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[sub][i]);
-    top = pair_max(top) * (BIAS ? 1.f : a.scale);
+    top = pair_top(top) * (BIAS ? 1.f : a.scale);
     if (__any(top > m + RISE / unit<BIAS>())) {
       const float mn = fmaxf(m, top);
       const float alpha = fast_exp2(mn == -INFINITY ? 0.f : (m - mn) * unit<BIAS>());
