@@ -128,7 +128,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 ? 1 : 2) void cross_dq_kernel(co
   w /= nrb;
   const int split = w % a.q_splits;
   w /= a.q_splits;
-  const int hk = w % s.Hk, b = w / s.Hk;
+  const int b = w % s.B, hk = w / s.B;
   const int row = rb * 128 + wave * 32 + l32;
   const bool row_ok = row < s.rows;
   const int safe = min(row, s.rows - 1), u = safe / s.G, h = hk * s.G + safe % s.G;
@@ -254,7 +254,7 @@ __global__ __launch_bounds__(NT, DP > 64 || sizeof(T) == 4 ? 1 : 2) void cross_d
   w /= nkb;
   const int split = w % a.k_splits;
   w /= a.k_splits;
-  const int hk = w % s.Hk, b = w / s.Hk;
+  const int b = w % s.B, hk = w / s.B;
   const int key = kb * 128 + wave * 32 + l32, safe = min(key, s.V - 1);
   const bool kept = key < s.V && (!a.mask || a.mask[b * a.ms[0] + (int64_t)safe * a.ms[1]] != 0);
   const bool all_kept = __all(kept), any_kept = __syncthreads_or(kept);

@@ -60,18 +60,31 @@ __device__ __forceinline__ void store4_at(T* p, const f32x4& v, int left) {
     if (e < left) p[e] = o[e];
 }
 
-// Rows of DP elements in LDS, their 16-byte chunks in chunk_swizzle's order: fragments of 32 rows (8 consecutive
-// elements a lane) and turned ones (8 rows of one column a lane) are both read without bank conflicts.
-template <typename T, int DP>
+// Rows of DP elements in LDS, laid out so that the reads hit no bank twice: fragments of 32 rows (8 consecutive elements
+// a lane), turned ones (8 rows of one column a lane), or both. LDS serves 16 lanes' 16 bytes, and 32 lanes' 8, at once.
+//   BY_ROWS     a pitch of an odd number of 16-byte chunks: 16 rows' chunk c lie on different banks;
+//   BY_COLUMNS  a pitch of 64 (or 192) bytes modulo 256: 4 rows' 64 bytes do; fp32: 4 rows further on is 128 bytes on;
+//   BOTH        a pitch of a power of two with the chunks in chunk_swizzle's order, which costs exclusive-ors for addresses
+//               that are one register and constants in the other two.
+enum Layout { BOTH, BY_ROWS, BY_COLUMNS };
+
+template <typename T, int DP, Layout LAYOUT = BOTH>
 struct RowTile {
   static constexpr int BYTES = DP * (int)sizeof(T);
-  static constexpr int PITCH = BYTES <= 64 ? 64 : BYTES <= 128 ? 128 : BYTES <= 256 ? 256 : 512;
+  static constexpr int PITCH = LAYOUT == BY_ROWS                       ? BYTES + 16
+                               : LAYOUT == BY_COLUMNS && sizeof(T) == 4 ? BYTES + 32
+                               : LAYOUT == BY_COLUMNS                   ? (BYTES % 128 == 64 ? BYTES : BYTES + 64)
+                               : BYTES <= 64                            ? 64
+                               : BYTES <= 128                           ? 128
+                               : BYTES <= 256                           ? 256
+                                                                        : 512;
   static constexpr int CPR = BYTES / 16;            // chunks a row
   static constexpr int EPC = 16 / (int)sizeof(T);   // elements a chunk
   typedef typename TypeOps<T>::V8 V8;
   typedef typename TypeOps<T>::V4 V4;
   static __device__ __forceinline__ int at(int row, int chunk) {
-    return row * PITCH + ((chunk ^ chunk_swizzle<(PITCH < 256 ? PITCH : 256)>(row)) << 4);
+    if constexpr (LAYOUT == BOTH) return row * PITCH + ((chunk ^ chunk_swizzle<(PITCH < 256 ? PITCH : 256)>(row)) << 4);
+    return row * PITCH + (chunk << 4);
   }
   // elements 16 kk + 8 g .. + 7 of a row
   static __device__ __forceinline__ V8 row8(const unsigned char* tile, int row, int kk, int g) {
@@ -123,12 +136,18 @@ struct Staged {
   static constexpr int STEP = NT / Tile::CPR;        // rows from one chunk to the next, where EVEN
   static_assert(N * NT == ROWS * Tile::CPR, "chunks a thread");
   u32x4 reg[N];
-  static __device__ __forceinline__ int row(int i) { return EVEN ? (int)threadIdx.x / Tile::CPR + i * STEP : ((int)threadIdx.x + i * NT) / Tile::CPR; }
-  static __device__ __forceinline__ int chunk(int i) { return EVEN ? (int)threadIdx.x % Tile::CPR : ((int)threadIdx.x + i * NT) % Tile::CPR; }
+  static __device__ __forceinline__ int row(int i, int tid) { return EVEN ? tid / Tile::CPR + i * STEP : (tid + i * NT) / Tile::CPR; }
+  static __device__ __forceinline__ int chunk(int i, int tid) { return EVEN ? tid % Tile::CPR : (tid + i * NT) % Tile::CPR; }
+  // the thread's index where it is rarely needed: opaque, so that what follows from it is not kept in registers
+  static __device__ __forceinline__ int rare_tid() {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    return tid;
+  }
   // rows first .. first + ROWS - 1 of `end` rows, those past the last one its copies; columns past D read column 0
   __device__ __forceinline__ void load_rows(const T* base, int64_t stride, int first, int end, int D) {
     if (EVEN && first + ROWS <= end) {  // uniform
-      const int c = chunk(0) * Tile::EPC;
+      const int c = chunk(0, threadIdx.x) * Tile::EPC;
       const uint32_t lane = (uint32_t)((int)threadIdx.x / Tile::CPR * (int)stride + (c < D ? c : 0)) * (uint32_t)sizeof(T);
       const T* tile = base + first * stride;
 #pragma unroll
@@ -140,24 +159,28 @@ struct Staged {
   // row r from base + offset(r): always a readable row
   template <typename Offset>
   __device__ __forceinline__ void load(const T* base, int D, Offset offset) {
+    const int tid = rare_tid();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = chunk(i) * Tile::EPC;
-      reg[i] = load16_at(base + offset(row(i)) + (c < D ? c : 0));
+      const int c = chunk(i, tid) * Tile::EPC;
+      reg[i] = load16_at(base + offset(row(i, tid)) + (c < D ? c : 0));
     }
   }
-  // whole rows of D = DP elements
+  // whole rows of D = DP elements, into a tile of any layout
+  template <typename To = Tile>
   __device__ __forceinline__ void store(unsigned char* tile) const {
 #pragma unroll
-    for (int i = 0; i < N; ++i) *reinterpret_cast<u32x4*>(tile + Tile::at(row(i), chunk(i))) = reg[i];
+    for (int i = 0; i < N; ++i)
+      *reinterpret_cast<u32x4*>(tile + To::at(row(i, threadIdx.x), chunk(i, threadIdx.x))) = reg[i];
   }
   // rows for which `keep` is false, and columns past D, are zeros
-  template <typename Keep>
+  template <typename To = Tile, typename Keep>
   __device__ __forceinline__ void store(unsigned char* tile, int D, Keep keep) const {
+    const int tid = rare_tid();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const uint32_t ok = chunk(i) * Tile::EPC < D && keep(row(i)) ? ~0u : 0u;
-      *reinterpret_cast<u32x4*>(tile + Tile::at(row(i), chunk(i))) = reg[i] & u32x4{ok, ok, ok, ok};
+      const uint32_t ok = chunk(i, tid) * Tile::EPC < D && keep(row(i, tid)) ? ~0u : 0u;
+      *reinterpret_cast<u32x4*>(tile + To::at(row(i, tid), chunk(i, tid))) = reg[i] & u32x4{ok, ok, ok, ok};
     }
   }
 };

@@ -20,6 +20,7 @@
 //   maxima, sums and outputs meet in LDS at the end.
 // Where these leave CUs idle the keys are split over workgroups, whose fp32 outputs a second kernel joins.
 #include <algorithm>
+#include <type_traits>
 
 #include "cross_common.hpp"
 
@@ -50,70 +51,85 @@ struct FwdArgs {
   int splits, tiles_per_split;
 };
 
-// WK waves share rows and divide keys (1 or 4)
-template <typename T, int DP, int WK>
+// WK waves share rows and divide keys (1 or 4); a wave has QW times 32 rows
+template <typename T, int DP, int WK, int QW>
 struct Cfg {
   static constexpr int SUBS = WK == 1 ? 2 : 1;    // half tiles of 32 keys a wave
   static constexpr int KT = 32 * SUBS * WK;       // keys a tile
-  static constexpr int ROWS = 128 / WK;           // rows a workgroup
+  static constexpr int WORDS = (KT + 63) / 64;
+  static constexpr int ROWS = 128 / WK * QW;      // rows a workgroup
   static constexpr int NBUF = sizeof(T) == 2 && WK == 1 ? 2 : 1;
-  static constexpr int TILE = KT * RowTile<T, DP>::PITCH;
+  typedef RowTile<T, DP, BY_ROWS> KTile;
+  typedef RowTile<T, DP, BY_COLUMNS> VTile;
+  static constexpr int KBYTES = KT * KTile::PITCH, TILE = KBYTES + KT * VTile::PITCH;
   static constexpr int MERGE = WK == 1 ? 0 : 4 * 64 * (16 * (DP / 32) + 4) * 4;  // of the waves' results
-  static constexpr int LDS = NBUF * 2 * TILE > MERGE ? NBUF * 2 * TILE : MERGE;
+  static constexpr int LDS = NBUF * TILE > MERGE ? NBUF * TILE : MERGE;
+  static constexpr int WGS = (sizeof(T) == 4 && DP == 128) || (QW == 2 && DP > 64) ? 1 : 2;  // workgroups a CU
 };
 
-template <typename T, int PREC, int DP, int WK, bool BIAS>
-__global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void cross_fwd_kernel(const FwdArgs a) {
-  typedef Cfg<T, DP, WK> C;
-  typedef RowTile<T, DP> Tile;
+template <typename T, int PREC, int DP, int WK, int QW, bool BIAS>
+__global__ __launch_bounds__(NT, (Cfg<T, DP, WK, QW>::WGS)) void cross_fwd_kernel(const FwdArgs a) {
+  typedef Cfg<T, DP, WK, QW> C;
+  typedef typename C::KTile KTile;
+  typedef typename C::VTile VTile;
   typedef typename TypeOps<T>::V8 V8;
   __shared__ __align__(16) unsigned char smem[C::LDS];
   __shared__ int found[2];
   const Shape& s = a.s;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
 
-  // blocks of rows fastest: those of one key head share its K and V in an XCD's L2
+  // blocks of rows fastest: those of one key head share its K and V in an XCD's L2; then the sequences, whose lengths
+  // differ, so that every XCD has some of each
   const uint32_t nrb = (uint32_t)(s.rows + C::ROWS - 1) / C::ROWS;
   uint32_t w = xcd_remap(blockIdx.x, gridDim.x);
   const int rb = w % nrb;
   w /= nrb;
   const int split = w % a.splits;
   w /= a.splits;
-  const int hk = w % s.Hk, b = w / s.Hk;
+  const int b = w % s.B, hk = w / s.B;
 
-  const int row = rb * C::ROWS + (WK == 1 ? wave * 32 : 0) + l32;
-  const bool row_ok = row < s.rows;
-  const int safe = min(row, s.rows - 1), u = safe / s.G, h = hk * s.G + safe % s.G;
-  const T* qp = (const T*)a.q + b * a.qs[0] + u * a.qs[1] + h * a.qs[2];
+  int u[QW], h[QW];
+  const int row0 = rb * C::ROWS + (WK == 1 ? wave * 32 * QW : 0) + l32;
+#pragma unroll
+  for (int i = 0; i < QW; ++i) {
+    const int row = min(row0 + 32 * i, s.rows - 1);
+    u[i] = row / s.G, h[i] = hk * s.G + row % s.G;
+  }
   const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
   const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
-  const T* bp = BIAS ? (const T*)a.bias + b * a.bs[0] + h * a.bs[1] + u * a.bs[2] : nullptr;
   const uint8_t* mask = a.mask ? a.mask + b * a.ms[0] : nullptr;
 
   int key_end = min(s.V, (split + 1) * a.tiles_per_split * C::KT), key0 = split * a.tiles_per_split * C::KT;
   if (mask) live_range<NT>(mask, a.ms[1], key0, key_end, found);
   const int t_end = key0 < key_end ? (key_end + C::KT - 1) / C::KT : 0;
 
-  V8 qf[DP / 16];
+  V8 qf[QW][DP / 16];
+  f32x16 o[QW][DP / 32];
+  float m[QW], sum[QW];
+  const T* bp[QW];
 #pragma unroll
-  for (int kk = 0; kk < DP / 16; ++kk) {
-    const int d = 16 * kk + 8 * g;
-    qf[kk] = load8_at(qp + (d < s.D ? d : 0));
-    if (d >= s.D) qf[kk] = zero8<T>();
+  for (int i = 0; i < QW; ++i) {
+    const T* qp = (const T*)a.q + b * a.qs[0] + u[i] * a.qs[1] + h[i] * a.qs[2];
+    bp[i] = BIAS ? (const T*)a.bias + b * a.bs[0] + h[i] * a.bs[1] + u[i] * a.bs[2] : nullptr;
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+      const int d = 16 * kk + 8 * g;
+      qf[i][kk] = load8_at(qp + (d < s.D ? d : 0));
+      if (d >= s.D) qf[i][kk] = zero8<T>();
+    }
+#pragma unroll
+    for (int cc = 0; cc < DP / 32; ++cc) clear(o[i][cc]);
+    m[i] = -INFINITY, sum[i] = 0.f;
   }
-  f32x16 o[DP / 32];
-#pragma unroll
-  for (int cc = 0; cc < DP / 32; ++cc) clear(o[cc]);
-  float m = -INFINITY, sum = 0.f;
 
   Staged<T, DP, C::KT, NT> kreg, vreg;
-  uint64_t live[(C::KT + 63) / 64], next_live[(C::KT + 63) / 64];
+  uint64_t live[C::WORDS], next_live[C::WORDS];
   // the words of the next tile from t on that keeps a key; t_end where there is none
-  auto seek = [&](int t, uint64_t (&words)[(C::KT + 63) / 64]) {
+  auto seek = [&](int t, uint64_t (&words)[C::WORDS]) {
     for (; t < t_end; ++t) {
       uint64_t any = 0;
 #pragma unroll
-      for (int i = 0; i < (C::KT + 63) / 64; ++i) any |= words[i] = live_keys(mask, a.ms[1], t * C::KT + 64 * i, s.V);
+      for (int i = 0; i < C::WORDS; ++i) any |= words[i] = live_keys(mask, a.ms[1], t * C::KT + 64 * i, s.V);
       if (any) break;
     }
     return t;
@@ -122,18 +138,18 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void cross
     kreg.load_rows(kp, a.ks[1], t * C::KT, s.V, s.D);
     vreg.load_rows(vp, a.vs[1], t * C::KT, s.V, s.D);
   };
-  auto put = [&](int buf, const uint64_t (&words)[(C::KT + 63) / 64]) {
-    unsigned char* st = smem + buf * 2 * C::TILE;
+  auto put = [&](int buf, const uint64_t (&words)[C::WORDS]) {
+    unsigned char* st = smem + buf * C::TILE;
     bool whole = s.D == DP;
 #pragma unroll
-    for (int i = 0; i < (C::KT + 63) / 64; ++i) whole = whole && words[i] == ~0ull;
+    for (int i = 0; i < C::WORDS; ++i) whole = whole && words[i] == ~0ull;
     if (whole) {  // uniform
-      kreg.store(st);
-      vreg.store(st + C::TILE);
+      kreg.template store<KTile>(st);
+      vreg.template store<VTile>(st + C::KBYTES);
       return;
     }
-    kreg.store(st, s.D, [](int) { return true; });
-    vreg.store(st + C::TILE, s.D, [&](int r) { return (words[r / 64] >> (r & 63) & 1) != 0; });
+    kreg.template store<KTile>(st, s.D, [](int) { return true; });
+    vreg.template store<VTile>(st + C::KBYTES, s.D, [&](int r) { return (words[r / 64] >> (r & 63) & 1) != 0; });
   };
 
   int t = seek(key0 / C::KT, live);
@@ -145,29 +161,35 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void cross
   for (int buf = 0; t < t_end; buf ^= C::NBUF - 1) {
     const int next = seek(t + 1, next_live);
     if (next < t_end) load(next);
-    const unsigned char* ks = smem + buf * 2 * C::TILE;
-    const unsigned char* vs = ks + C::TILE;
+    const unsigned char* ks = smem + buf * C::TILE;
+    const unsigned char* vs = ks + C::KBYTES;
     const int r0 = WK == 1 ? 0 : 32 * wave;  // this wave's keys of the tile
-    f32x16 sc[C::SUBS];
+    f32x16 sc[C::SUBS][QW];
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int sub = 0; sub < C::SUBS; ++sub) {
-      clear(sc[sub]);
 #pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk)
-        Mma<T, PREC>::step(sc[sub], Tile::row8(ks, r0 + 32 * sub + l32, kk, g), qf[kk]);
+      for (int i = 0; i < QW; ++i) clear(sc[sub][i]);
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        const V8 kf = KTile::row8(ks, r0 + 32 * sub + l32, kk, g);
+#pragma unroll
+        for (int i = 0; i < QW; ++i) Mma<T, PREC>::step(sc[sub][i], kf, qf[i][kk]);
+      }
     }
     __builtin_amdgcn_s_setprio(0);
     if constexpr (BIAS) {
 #pragma unroll
       for (int sub = 0; sub < C::SUBS; ++sub)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int key = t * C::KT + r0 + 32 * sub + 8 * q + 4 * g;
-          const f32x4 bv = key < s.V ? load4_at(bp + key, s.V - key) : f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < QW; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[sub][4 * q + e] = __builtin_fmaf(sc[sub][4 * q + e], a.scale, bv[e]);
-        }
+          for (int q = 0; q < 4; ++q) {
+            const int key = t * C::KT + r0 + 32 * sub + 8 * q + 4 * g;
+            const f32x4 bv = key < s.V ? load4_at(bp[i] + key, s.V - key) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[sub][i][4 * q + e] = __builtin_fmaf(sc[sub][i][4 * q + e], a.scale, bv[e]);
+          }
     }
 #pragma unroll
     for (int sub = 0; sub < C::SUBS; ++sub) {
@@ -175,53 +197,75 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void cross
       const uint32_t word = (uint32_t)(live[at / 64] >> (at & 63));
       if (word != ~0u) {  // uniform
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sc[sub][i] = word >> acc_row(i, g) & 1 ? sc[sub][i] : -INFINITY;
+        for (int i = 0; i < QW; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sc[sub][i][e] = word >> acc_row(e, g) & 1 ? sc[sub][i][e] : -INFINITY;
       }
     }
-    float top = sc[0][0];
+    float top[QW];
+    bool rises = false;
 #pragma unroll
-    for (int sub = 0; sub < C::SUBS; ++sub)
+    for (int i = 0; i < QW; ++i) {
+      top[i] = sc[0][i][0];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[sub][i]);
-    top = pair_top(top) * (BIAS ? 1.f : a.scale);
-    if (__any(top > m + RISE / unit<BIAS>())) {
-      const float mn = fmaxf(m, top);
-      const float alpha = fast_exp2(mn == -INFINITY ? 0.f : (m - mn) * unit<BIAS>());
-      m = mn;
-      sum *= alpha;
+      for (int sub = 0; sub < C::SUBS; ++sub)
 #pragma unroll
-      for (int cc = 0; cc < DP / 32; ++cc)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[cc][i] *= alpha;
+        for (int e = 0; e < 16; ++e) top[i] = fmaxf(top[i], sc[sub][i][e]);
+      top[i] = pair_top(top[i]) * (BIAS ? 1.f : a.scale);
+      rises = rises || top[i] > m[i] + RISE / unit<BIAS>();
     }
-    const float base = m == -INFINITY ? 0.f : m;
+    if (__any(rises)) {
 #pragma unroll
-    for (int sub = 0; sub < C::SUBS; ++sub) {
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        sc[sub][i] = fast_exp2(BIAS ? (sc[sub][i] - base) * LOG2E : __builtin_fmaf(sc[sub][i], a.scale, -base));
-        part[i % 4] += sc[sub][i];
-      }
-      sum += (part[0] + part[1]) + (part[2] + part[3]);
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        const V8 p = acc_frag<T>(sc[sub], kk);
+      for (int i = 0; i < QW; ++i) {
+        const float mn = fmaxf(m[i], top[i]);
+        const float alpha = fast_exp2(mn == -INFINITY ? 0.f : (m[i] - mn) * unit<BIAS>());
+        m[i] = mn;
+        sum[i] *= alpha;
 #pragma unroll
         for (int cc = 0; cc < DP / 32; ++cc)
-          Mma<T, PREC>::step(o[cc], Tile::turned8(vs, r0 + 32 * sub, kk, cc, lane), p);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[i][cc][e] *= alpha;
       }
+    }
+#pragma unroll
+    for (int sub = 0; sub < C::SUBS; ++sub) {
+      V8 p[QW][2];
+#pragma unroll
+      for (int i = 0; i < QW; ++i) {
+        const float base = m[i] == -INFINITY ? 0.f : m[i];
+        f32x16& x = sc[sub][i];
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          x[e] = fast_exp2(BIAS ? (x[e] - base) * LOG2E : __builtin_fmaf(x[e], a.scale, -base));
+          part[e % 4] += x[e];
+        }
+        sum[i] += (part[0] + part[1]) + (part[2] + part[3]);
+        p[i][0] = acc_frag<T>(x, 0), p[i][1] = acc_frag<T>(x, 1);
+      }
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int cc = 0; cc < DP / 32; ++cc) {
+          const V8 vf = VTile::turned8(vs, r0 + 32 * sub, kk, cc, lane);
+#pragma unroll
+          for (int i = 0; i < QW; ++i) Mma<T, PREC>::step(o[i][cc], vf, p[i][kk]);
+        }
+      __builtin_amdgcn_s_setprio(0);
     }
     if constexpr (C::NBUF == 1) __syncthreads();
     if (next < t_end) put(C::NBUF == 1 ? 0 : buf ^ 1, next_live);
     __syncthreads();
     t = next;
 #pragma unroll
-    for (int i = 0; i < (C::KT + 63) / 64; ++i) live[i] = next_live[i];
+    for (int i = 0; i < C::WORDS; ++i) live[i] = next_live[i];
   }
-  sum = pair_sum(sum);
+#pragma unroll
+  for (int i = 0; i < QW; ++i) sum[i] = pair_sum(sum[i]);
 
   if constexpr (WK > 1) {  // the waves' results, in wave order
+    static_assert(QW == 1, "shared rows");
     constexpr int LD = 16 * (DP / 32) + 4;  // floats a lane: 4 more keep the lanes on different banks
     float* mine = (float*)smem + (wave * 64 + lane) * LD;
 #pragma unroll
@@ -229,8 +273,8 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void cross
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         *reinterpret_cast<f32x4*>(mine + 16 * cc + 4 * q) =
-            f32x4{o[cc][4 * q], o[cc][4 * q + 1], o[cc][4 * q + 2], o[cc][4 * q + 3]};
-    mine[LD - 4] = m, mine[LD - 3] = sum;
+            f32x4{o[0][cc][4 * q], o[0][cc][4 * q + 1], o[0][cc][4 * q + 2], o[0][cc][4 * q + 3]};
+    mine[LD - 4] = m[0], mine[LD - 3] = sum[0];
     __syncthreads();
     if (wave >= DP / 32) return;
     // wave cc joins the columns 32 cc ..
@@ -248,34 +292,38 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void cross
 #pragma unroll
       for (int i = 0; i < 16; ++i) joined[i] += f * from[16 * wave + i];
     }
-    m = top, sum = total;
-    o[0] = joined;
-  }
-  if (!row_ok) return;
-  const int64_t head = ((int64_t)b * s.U + u) * s.H + h, stat = ((int64_t)b * s.H + h) * s.U + u;
-  const bool first = g == 0 && (WK == 1 || wave == 0);
-  const float inv = a.splits > 1 ? 1.f : sum > 0.f ? 1.0f / sum : sum == 0.f ? 0.f : sum;  // NaN stays
-  if (a.splits > 1) {
-    if (first) {
-      float* ml = a.part_ml + (split * (int64_t)s.B * s.H * s.U + stat) * 2;
-      ml[0] = m, ml[1] = sum;
-    }
-  } else if (first && a.stats) {
-    a.stats[2 * stat] = sum == 0.f ? INFINITY : m, a.stats[2 * stat + 1] = sum == 0.f ? 0.f : log2f(sum);
+    m[0] = top, sum[0] = total;
+    o[0][0] = joined;
   }
   const int64_t each = (int64_t)s.B * s.U * s.H * s.D;
 #pragma unroll
-  for (int k = 0; k < (WK == 1 ? DP / 32 : 1); ++k) {
-    const int cc = WK == 1 ? k : wave;
+  for (int i = 0; i < QW; ++i) {
+    if (row0 + 32 * i >= s.rows) break;
+    const int64_t head = ((int64_t)b * s.U + u[i]) * s.H + h[i], stat = ((int64_t)b * s.H + h[i]) * s.U + u[i];
+    const bool first = g == 0 && (WK == 1 || wave == 0);
+    const float inv = a.splits > 1 ? 1.f : sum[i] > 0.f ? 1.0f / sum[i] : sum[i] == 0.f ? 0.f : sum[i];  // NaN stays
+    if (a.splits > 1) {
+      if (first) {
+        float* ml = a.part_ml + (split * (int64_t)s.B * s.H * s.U + stat) * 2;
+        ml[0] = m[i], ml[1] = sum[i];
+      }
+    } else if (first && a.stats) {
+      a.stats[2 * stat] = sum[i] == 0.f ? INFINITY : m[i], a.stats[2 * stat + 1] = sum[i] == 0.f ? 0.f : log2f(sum[i]);
+    }
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int d = 32 * cc + 8 * q + 4 * g;
-      if (d >= s.D) continue;
-      const f32x4 x = f32x4{o[k][4 * q], o[k][4 * q + 1], o[k][4 * q + 2], o[k][4 * q + 3]} * inv;
-      if (a.splits > 1)
-        *reinterpret_cast<f32x4*>(a.part_o + split * each + head * s.D + d) = x;
-      else
-        store4((T*)a.o + head * s.D + d, TypeOps<T>::from_f32(x));
+    for (int k = 0; k < (WK == 1 ? DP / 32 : 1); ++k) {
+      const int cc = WK == 1 ? k : wave;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int d = 32 * cc + 8 * q + 4 * g;
+        if (d >= s.D) continue;
+        const f32x16& v = o[i][k];
+        const f32x4 x = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]} * inv;
+        if (a.splits > 1)
+          *reinterpret_cast<f32x4*>(a.part_o + split * each + head * s.D + d) = x;
+        else
+          store4((T*)a.o + head * s.D + d, TypeOps<T>::from_f32(x));
+      }
     }
   }
 }
@@ -307,14 +355,16 @@ __global__ __launch_bounds__(NT) void cross_join_kernel(const FwdArgs a) {
 }
 
 struct Plan {
-  bool few;  // up to 32 rows
+  bool few;   // up to 32 rows
+  bool wide;  // 64 rows a wave
   int64_t blocks, splits, tiles_per_split;
 };
 Plan plan(const gnn_cross_attn_args& g) {
   Plan p{};
   const int64_t rows = g.U * (g.H / g.Hk);
   p.few = rows <= 32;
-  const int64_t base = (p.few ? 1 : (rows + 127) / 128) * g.B * g.Hk, kt = p.few ? 128 : 64, tiles = (g.V + kt - 1) / kt;
+  p.wide = g.dtype != GNN_F32 && g.D <= 64 && (rows + 255) / 256 * g.B * g.Hk >= 2 * (int64_t)compute_units();
+  const int64_t per = p.wide ? 256 : 128, base = (p.few ? 1 : (rows + per - 1) / per) * g.B * g.Hk, kt = p.few ? 128 : 64, tiles = (g.V + kt - 1) / kt;
   // two workgroups a CU where the keys allow it, of 4 tiles at least
   const int64_t want = std::max<int64_t>(1, 2 * (int64_t)compute_units() / base);
   const int64_t most = std::max<int64_t>(1, tiles / 4);
@@ -327,17 +377,23 @@ Plan plan(const gnn_cross_attn_args& g) {
 template <typename T, int PREC, int DP>
 int launch(const FwdArgs& a, const Plan& p, hipStream_t st) {
   const dim3 grid((uint32_t)p.blocks), blk(NT);
-  if (p.few) {
-    if (a.bias)
-      hipLaunchKernelGGL((cross_fwd_kernel<T, PREC, DP, 4, true>), grid, blk, 0, st, a);
-    else
-      hipLaunchKernelGGL((cross_fwd_kernel<T, PREC, DP, 4, false>), grid, blk, 0, st, a);
-  } else {
-    if (a.bias)
-      hipLaunchKernelGGL((cross_fwd_kernel<T, PREC, DP, 1, true>), grid, blk, 0, st, a);
-    else
-      hipLaunchKernelGGL((cross_fwd_kernel<T, PREC, DP, 1, false>), grid, blk, 0, st, a);
-  }
+  auto go = [&](auto bias) {
+    constexpr bool BIAS = decltype(bias)::value;
+    if (p.few) {
+      hipLaunchKernelGGL((cross_fwd_kernel<T, PREC, DP, 4, 1, BIAS>), grid, blk, 0, st, a);
+      return;
+    }
+    if constexpr (sizeof(T) == 2 && DP <= 64)
+      if (p.wide) {
+        hipLaunchKernelGGL((cross_fwd_kernel<T, PREC, DP, 1, 2, BIAS>), grid, blk, 0, st, a);
+        return;
+      }
+    hipLaunchKernelGGL((cross_fwd_kernel<T, PREC, DP, 1, 1, BIAS>), grid, blk, 0, st, a);
+  };
+  if (a.bias)
+    go(std::true_type{});
+  else
+    go(std::false_type{});
   int rc = (int)hipGetLastError();
   if (rc == 0 && a.splits > 1) {
     const int64_t threads = (int64_t)a.s.B * a.s.U * a.s.H * (a.s.D / 4);
