@@ -5,17 +5,21 @@
 //   dQ_r = scale sum_j dS_rj k_j,   dK_j = scale sum_r dS_rj q_r,   dbias = dS (summed over a batch that shares it).
 // Rows r are the queries of all heads that share a key head, so that dK and dV of a shared head are one sum.
 //
-// Every sum has one owner and one order; S and dP are formed in each of the kernels that need them:
-//   cross_dq    the forward's layout (a lane holds a row and 16 keys): the dS^T accumulator is the operand of
-//               dQ^T += K^T dS^T as it stands, K being read turned from LDS. It runs first, forms Delta from dO and O
-//               and leaves it in fp32; it also writes dbias where every sequence has its own.
-//   cross_dkdv  keys on the lanes, a wave 32 of them; tiles of 64 rows of Q and dO in LDS, read plain for S and dP and
+// Every sum has one owner and one order; S and dP are formed by each of the three that need them:
+//   dq_block    the forward's layout (a lane holds a row and 16 keys): the dS^T accumulator is the operand of
+//               dQ^T += K^T dS^T as it stands, K being read turned from LDS; it also writes dbias where every sequence
+//               has its own.
+//   dkdv_block  keys on the lanes, a wave 32 of them; tiles of 64 rows of Q and dO in LDS, read plain for S and dP and
 //               turned for dV^T += dO^T P and dK^T += Q^T dS.
-//   cross_dbias a bias for all sequences: a tile of 128 rows x 64 keys of one head group walks over the batch.
-// Where one of the first two leaves CUs idle its loop is split over workgroups, whose fp32 sums are added in order.
+//   dbias_block a bias for all sequences: a tile of 128 rows x 64 keys of one head group walks over the batch.
+// Delta comes from a kernel of its own, so that the three are workgroups of one launch (dk and dv, the longest, first)
+// whose ends fill each other's: 16 heads, 4 x 2048 x 1400, 64 columns. With more columns dk and dv take all of a CU's
+// registers and go alone. Where one of the first two leaves CUs idle its loop is split over workgroups, whose fp32 sums
+// are added in order.
 // P and dS are rounded to the operands' type for the products behind them. fp16: P is held 2^10 times as large for dV,
 // or a row spread over 10^5 keys would fall below fp16's normal range.
 #include <algorithm>
+#include <type_traits>
 
 #include "cross_common.hpp"
 
@@ -49,6 +53,8 @@ struct BwdArgs {
   float scale, logit_scale;  // the caller's; without a bias times log2(e)
   int q_splits, q_tiles;  // tiles of keys a split
   int k_splits, k_tiles;  // tiles of rows a split
+  uint32_t q_blocks, k_blocks, b_blocks;
+  bool shared_bias;
 };
 
 template <typename T> constexpr float p_shift() { return 0.f; }
@@ -112,18 +118,48 @@ __device__ __forceinline__ void half_tile(f32x16& dp, const unsigned char* ks, c
   }
 }
 
+// ------------------------------------------------------------------------------------ Delta
+// 2^LOG lanes of 8 elements a row
+template <typename T, int LOG>
+__global__ __launch_bounds__(NT) void cross_delta_kernel(const BwdArgs a) {
+  const Shape& s = a.s;
+  const int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x, heads = (int64_t)s.B * s.U * s.H;
+  const int64_t head = min(i >> LOG, heads - 1);
+  const int d = (int)(i & ((1 << LOG) - 1)) * 8, h = (int)(head % s.H);
+  const int64_t bu = head / s.H, b = bu / s.U, u = bu - b * s.U;
+  float sum = 0.f;
+  if (d < s.D) {
+    const f32x8 x = TypeOps<T>::to_f32(load8_at((const T*)a.o + b * a.os[0] + u * a.os[1] + h * a.os[2] + d)) *
+                    TypeOps<T>::to_f32(load8_at((const T*)a.dout + b * a.ds[0] + u * a.ds[1] + h * a.ds[2] + d));
+    sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+  }
+#pragma unroll
+  for (int k = 1; k < (1 << LOG); k *= 2) sum += __shfl_xor(sum, k);
+  if (d == 0 && i >> LOG < heads) a.delta[(b * s.H + h) * s.U + u] = sum;
+}
+
+// LDS of a workgroup
+template <typename T, int DP>
+struct Lds {
+  static constexpr int NBUF = sizeof(T) == 2 ? 2 : 1;
+  static constexpr int TILE = KT * RowTile<T, DP>::PITCH;
+  __align__(16) unsigned char tile[NBUF * 2 * TILE];
+  __align__(16) float m[NBUF][KT], l[NBUF][KT], delta[NBUF][KT];
+  int64_t bias_at[NBUF][KT];
+  int found[2];
+};
+
 // -------------------------------------------------------------------------------------- dQ
 template <typename T, int PREC, int DP, bool BIAS>
-__global__ __launch_bounds__(NT, sizeof(T) == 4 ? 1 : 2) void cross_dq_kernel(const BwdArgs a) {
+__device__ __forceinline__ void dq_block(const BwdArgs& a, Lds<T, DP>& lds, uint32_t block) {
   typedef RowTile<T, DP> Tile;
   typedef typename TypeOps<T>::V8 V8;
-  constexpr int TILE = KT * Tile::PITCH, NBUF = sizeof(T) == 2 ? 2 : 1;
-  __shared__ __align__(16) unsigned char smem[NBUF * 2 * TILE];
-  __shared__ int found[2];
+  constexpr int TILE = Lds<T, DP>::TILE, NBUF = Lds<T, DP>::NBUF;
+  unsigned char* smem = lds.tile;
   const Shape& s = a.s;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
   const uint32_t nrb = (uint32_t)(s.rows + 127) / 128;
-  uint32_t w = xcd_remap(blockIdx.x, gridDim.x);
+  uint32_t w = xcd_remap(block, a.q_blocks);
   const int rb = w % nrb;
   w /= nrb;
   const int split = w % a.q_splits;
@@ -141,23 +177,11 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 ? 1 : 2) void cross_dq_kernel(co
   V8 qf[DP / 16], df[DP / 16];
   load_row<T, DP>(qf, (const T*)a.q + b * a.qs[0] + u * a.qs[1] + h * a.qs[2], s.D, g);
   load_row<T, DP>(df, (const T*)a.dout + b * a.ds[0] + u * a.ds[1] + h * a.ds[2], s.D, g);
-  const float m = a.stats[2 * stat], l = a.stats[2 * stat + 1];
-  float delta = 0.f;
-  {
-    const T* op = (const T*)a.o + b * a.os[0] + u * a.os[1] + h * a.os[2];
-#pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) {
-      const int d = 16 * kk + 8 * g;
-      const f32x8 x = TypeOps<T>::to_f32(load8_at(op + (d < s.D ? d : 0))) * TypeOps<T>::to_f32(df[kk]);
-      delta += d < s.D ? ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])) : 0.f;
-    }
-    delta = pair_sum(delta);
-    if (row_ok && g == 0 && split == 0) a.delta[stat] = delta;
-  }
+  const float m = a.stats[2 * stat], l = a.stats[2 * stat + 1], delta = a.delta[stat];
   // own bias: every tile is visited, so that what no row keeps gets its zeros
-  T* dbias = BIAS && a.dbias ? (T*)a.dbias + stat * s.V : nullptr;
+  T* dbias = BIAS && a.dbias && !a.shared_bias ? (T*)a.dbias + stat * s.V : nullptr;
   int key_end = min(s.V, (split + 1) * a.q_tiles * KT), key0 = split * a.q_tiles * KT;
-  if (mask && !a.dbias) live_range<NT>(mask, a.ms[1], key0, key_end, found);
+  if (mask && !dbias) live_range<NT>(mask, a.ms[1], key0, key_end, lds.found);
   const int t_end = key0 < key_end ? (key_end + KT - 1) / KT : 0;
 
   f32x16 dq[DP / 32];
@@ -167,7 +191,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 ? 1 : 2) void cross_dq_kernel(co
   auto seek = [&](int t, uint64_t& word) {
     for (; t < t_end; ++t) {
       word = live_keys(mask, a.ms[1], t * KT, s.V);
-      if (word || a.dbias) break;
+      if (word || dbias) break;
     }
     return t;
   };
@@ -239,17 +263,15 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 ? 1 : 2) void cross_dq_kernel(co
 
 // ---------------------------------------------------------------------------------- dK, dV
 template <typename T, int PREC, int DP, bool BIAS>
-__global__ __launch_bounds__(NT, DP > 64 || sizeof(T) == 4 ? 1 : 2) void cross_dkdv_kernel(const BwdArgs a) {
+__device__ __forceinline__ void dkdv_block(const BwdArgs& a, Lds<T, DP>& lds, uint32_t block) {
   typedef RowTile<T, DP> Tile;
   typedef typename TypeOps<T>::V8 V8;
-  constexpr int TILE = KT * Tile::PITCH, NBUF = sizeof(T) == 2 ? 2 : 1;
-  __shared__ __align__(16) unsigned char smem[NBUF * 2 * TILE];
-  __shared__ float ms[NBUF][KT], ls[NBUF][KT], deltas[NBUF][KT];
-  __shared__ int64_t bias_at[BIAS ? NBUF : 1][BIAS ? KT : 1];
+  constexpr int TILE = Lds<T, DP>::TILE, NBUF = Lds<T, DP>::NBUF;
+  unsigned char* smem = lds.tile;
   const Shape& s = a.s;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
   const uint32_t nkb = (uint32_t)(s.V + 127) / 128;
-  uint32_t w = xcd_remap(blockIdx.x, gridDim.x);
+  uint32_t w = xcd_remap(block, a.k_blocks);
   const int kb = w % nkb;
   w /= nkb;
   const int split = w % a.k_splits;
@@ -258,8 +280,8 @@ __global__ __launch_bounds__(NT, DP > 64 || sizeof(T) == 4 ? 1 : 2) void cross_d
   const int key = kb * 128 + wave * 32 + l32, safe = min(key, s.V - 1);
   const bool kept = key < s.V && (!a.mask || a.mask[b * a.ms[0] + (int64_t)safe * a.ms[1]] != 0);
   const bool all_kept = __all(kept), any_kept = __syncthreads_or(kept);
-  const T* qp = (const T*)a.q + b * a.qs[0];
-  const T* dop = (const T*)a.dout + b * a.ds[0];
+  const T* qp = (const T*)a.q + b * a.qs[0] + hk * s.G * a.qs[2];
+  const T* dop = (const T*)a.dout + b * a.ds[0] + hk * s.G * a.ds[2];
 
   // what masked keys hold meets only zeros
   V8 kf[DP / 16], vf[DP / 16];
@@ -279,23 +301,10 @@ __global__ __launch_bounds__(NT, DP > 64 || sizeof(T) == 4 ? 1 : 2) void cross_d
   float next_m = 0.f, next_l = 0.f, next_delta = 0.f;
   int64_t next_bias = 0;
   auto load = [&](int t) {
-    auto place = [&](int r, int& u, int& h) {
-      const int row = min(t * KT + r, s.rows - 1);
-      u = row / s.G, h = hk * s.G + row % s.G;
-    };
-    qreg.load(qp, s.D, [&](int r) {
-      int u, h;
-      place(r, u, h);
-      return u * a.qs[1] + h * a.qs[2];
-    });
-    dreg.load(dop, s.D, [&](int r) {
-      int u, h;
-      place(r, u, h);
-      return u * a.ds[1] + h * a.ds[2];
-    });
+    qreg.load_heads(qp, a.qs[1], a.qs[2], s.G, t * KT, s.rows, s.D);
+    dreg.load_heads(dop, a.ds[1], a.ds[2], s.G, t * KT, s.rows, s.D);
     if (threadIdx.x < KT) {
-      int u, h;
-      place(threadIdx.x, u, h);
+      const int row = min(t * KT + (int)threadIdx.x, s.rows - 1), u = row / s.G, h = hk * s.G + row % s.G;
       const int64_t stat = ((int64_t)b * s.H + h) * s.U + u;
       next_m = a.stats[2 * stat], next_l = a.stats[2 * stat + 1];
       if (t * KT + (int)threadIdx.x >= s.rows) next_m = INFINITY;  // P = 2^-inf, and zeros of Q and dO
@@ -305,13 +314,18 @@ __global__ __launch_bounds__(NT, DP > 64 || sizeof(T) == 4 ? 1 : 2) void cross_d
   };
   auto put = [&](int t, int buf) {
     unsigned char* st = smem + buf * 2 * TILE;
-    qreg.store(st, s.D, [&](int r) { return t * KT + r < s.rows; });
-    dreg.store(st + TILE, s.D, [&](int r) { return t * KT + r < s.rows; });
+    if (s.D == DP && (t + 1) * KT <= s.rows) {  // uniform
+      qreg.store(st);
+      dreg.store(st + TILE);
+    } else {
+      qreg.store(st, s.D, [&](int r) { return t * KT + r < s.rows; });
+      dreg.store(st + TILE, s.D, [&](int r) { return t * KT + r < s.rows; });
+    }
     if (threadIdx.x < KT) {
-      ms[buf][threadIdx.x] = next_m;
-      ls[buf][threadIdx.x] = next_l - p_shift<T>();
-      deltas[buf][threadIdx.x] = next_delta * p_unit<T>();
-      if constexpr (BIAS) bias_at[buf][threadIdx.x] = next_bias;
+      lds.m[buf][threadIdx.x] = next_m;
+      lds.l[buf][threadIdx.x] = next_l - p_shift<T>();
+      lds.delta[buf][threadIdx.x] = next_delta * p_unit<T>();
+      if constexpr (BIAS) lds.bias_at[buf][threadIdx.x] = next_bias;
     }
   };
   if (t0 < t_end) {
@@ -336,14 +350,14 @@ __global__ __launch_bounds__(NT, DP > 64 || sizeof(T) == 4 ? 1 : 2) void cross_d
       }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const f32x4 m4 = *reinterpret_cast<const f32x4*>(&ms[buf][r0 + 8 * q + 4 * g]);
-        const f32x4 l4 = *reinterpret_cast<const f32x4*>(&ls[buf][r0 + 8 * q + 4 * g]);
-        const f32x4 d4 = *reinterpret_cast<const f32x4*>(&deltas[buf][r0 + 8 * q + 4 * g]);
+        const f32x4 m4 = *reinterpret_cast<const f32x4*>(&lds.m[buf][r0 + 8 * q + 4 * g]);
+        const f32x4 l4 = *reinterpret_cast<const f32x4*>(&lds.l[buf][r0 + 8 * q + 4 * g]);
+        const f32x4 d4 = *reinterpret_cast<const f32x4*>(&lds.delta[buf][r0 + 8 * q + 4 * g]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int i = 4 * q + e;
           float add = 0.f;
-          if constexpr (BIAS) add = TypeOps<T>::to_f32(bias_key[bias_at[buf][r0 + 8 * q + 4 * g + e]]);
+          if constexpr (BIAS) add = TypeOps<T>::to_f32(bias_key[lds.bias_at[buf][r0 + 8 * q + 4 * g + e]]);
           p[i] = probability<BIAS>(p[i], a.logit_scale, add, m4[e], l4[e]);
           dp[i] = __builtin_fmaf(dp[i], p_unit<T>(), -d4[e]);
         }
@@ -389,15 +403,15 @@ __global__ __launch_bounds__(NT, DP > 64 || sizeof(T) == 4 ? 1 : 2) void cross_d
 
 // ------------------------------------------------------------------- dbias of a shared bias
 template <typename T, int PREC, int DP>
-__global__ __launch_bounds__(NT, sizeof(T) == 4 ? 1 : 2) void cross_dbias_kernel(const BwdArgs a) {
+__device__ __forceinline__ void dbias_block(const BwdArgs& a, Lds<T, DP>& lds, uint32_t block) {
   typedef RowTile<T, DP> Tile;
   typedef typename TypeOps<T>::V8 V8;
-  constexpr int TILE = KT * Tile::PITCH;
-  __shared__ __align__(16) unsigned char smem[2 * TILE];
+  constexpr int TILE = Lds<T, DP>::TILE;
+  unsigned char* smem = lds.tile;
   const Shape& s = a.s;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
   const uint32_t nrb = (uint32_t)(s.rows + 127) / 128, nkb = (uint32_t)(s.V + KT - 1) / KT;
-  uint32_t w = xcd_remap(blockIdx.x, gridDim.x);
+  uint32_t w = xcd_remap(block, a.b_blocks);
   const int rb = w % nrb;
   w /= nrb;
   const int kb = w % nkb, hk = w / nkb;
@@ -443,6 +457,21 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 ? 1 : 2) void cross_dbias_kernel
     }
 }
 
+// The workgroups of DKDV, then those of dQ, then those of a shared dbias
+template <typename T, int PREC, int DP, bool BIAS, bool DKDV, bool DQ>
+__global__ __launch_bounds__(NT, sizeof(T) == 4 || (DKDV && DP > 64) ? 1 : 2) void cross_bwd_kernel(const BwdArgs a) {
+  __shared__ Lds<T, DP> lds;
+  uint32_t block = blockIdx.x;
+  if constexpr (DKDV) {
+    if (!DQ || block < a.k_blocks) return dkdv_block<T, PREC, DP, BIAS>(a, lds, block);
+    block -= a.k_blocks;
+  }
+  if constexpr (DQ) {
+    if (!BIAS || block < a.q_blocks) return dq_block<T, PREC, DP, BIAS>(a, lds, block);
+    if constexpr (BIAS) dbias_block<T, PREC, DP>(a, lds, block - a.q_blocks);
+  }
+}
+
 struct Plan {
   int64_t q_blocks, q_splits, q_tiles, k_blocks, k_splits, k_tiles;
 };
@@ -462,38 +491,40 @@ Plan plan(const gnn_cross_attn_bwd_args& g) {
   return p;
 }
 
-template <typename T, int PREC, int DP, bool BIAS>
-int launch(const BwdArgs& a, const Plan& p, bool shared_bias, hipStream_t st) {
-  BwdArgs q = a;
-  if (shared_bias) q.dbias = nullptr;
-  hipLaunchKernelGGL((cross_dq_kernel<T, PREC, DP, BIAS>), dim3((uint32_t)p.q_blocks), dim3(NT), 0, st, q);
-  if (int rc = (int)hipGetLastError()) return rc;
-  if (a.dk) {
-    hipLaunchKernelGGL((cross_dkdv_kernel<T, PREC, DP, BIAS>), dim3((uint32_t)p.k_blocks), dim3(NT), 0, st, a);
-    if (int rc = (int)hipGetLastError()) return rc;
-  }
-  if constexpr (BIAS)
-    if (shared_bias && a.dbias) {
-      const int64_t blocks = (int64_t)((a.s.rows + 127) / 128) * ((a.s.V + KT - 1) / KT) * a.s.Hk;
-      if (blocks >= ((int64_t)1 << 31)) return set_error(GNN_ERR_UNSUPPORTED, "cross_attention: grid too large");
-      hipLaunchKernelGGL((cross_dbias_kernel<T, PREC, DP>), dim3((uint32_t)blocks), dim3(NT), 0, st, a);
-    }
+template <typename T, int LOG>
+int delta(const BwdArgs& a, hipStream_t st) {
+  const int64_t blocks = (((int64_t)a.s.B * a.s.U * a.s.H << LOG) + NT - 1) / NT;
+  hipLaunchKernelGGL((cross_delta_kernel<T, LOG>), dim3((uint32_t)blocks), dim3(NT), 0, st, a);
   return (int)hipGetLastError();
 }
 
-template <typename T, int PREC, int DP>
-int launch(const BwdArgs& a, const Plan& p, bool shared_bias, hipStream_t st) {
-  return a.bias ? launch<T, PREC, DP, true>(a, p, shared_bias, st) : launch<T, PREC, DP, false>(a, p, shared_bias, st);
+template <typename T, int PREC, int DP, bool BIAS>
+int launch(const BwdArgs& a, hipStream_t st) {
+  constexpr int LOG = DP <= 32 ? 2 : DP <= 64 ? 3 : 4;
+  if (int rc = delta<T, LOG>(a, st)) return rc;
+  const uint32_t rest = a.q_blocks + a.b_blocks;
+  if constexpr (DP <= 64 || sizeof(T) == 4) {
+    hipLaunchKernelGGL((cross_bwd_kernel<T, PREC, DP, BIAS, true, true>), dim3(a.k_blocks + rest), dim3(NT), 0, st, a);
+  } else {
+    if (a.k_blocks)
+      hipLaunchKernelGGL((cross_bwd_kernel<T, PREC, DP, BIAS, true, false>), dim3(a.k_blocks), dim3(NT), 0, st, a);
+    hipLaunchKernelGGL((cross_bwd_kernel<T, PREC, DP, BIAS, false, true>), dim3(rest), dim3(NT), 0, st, a);
+  }
+  return (int)hipGetLastError();
 }
 
 template <typename T, int PREC>
-int run(const BwdArgs& a, const Plan& p, bool shared_bias, hipStream_t st) {
+int run(const BwdArgs& a, hipStream_t st) {
+  auto go = [&](auto dp) {
+    constexpr int DP = decltype(dp)::value;
+    return a.bias ? launch<T, PREC, DP, true>(a, st) : launch<T, PREC, DP, false>(a, st);
+  };
   if constexpr (sizeof(T) == 2) {
-    if (a.s.D <= 32) return launch<T, PREC, 32>(a, p, shared_bias, st);
-    if (a.s.D > 64 && a.s.D <= 96) return launch<T, PREC, 96>(a, p, shared_bias, st);
+    if (a.s.D <= 32) return go(std::integral_constant<int, 32>{});
+    if (a.s.D > 64 && a.s.D <= 96) return go(std::integral_constant<int, 96>{});
   }
-  if (a.s.D <= 64) return launch<T, PREC, 64>(a, p, shared_bias, st);
-  return launch<T, PREC, 128>(a, p, shared_bias, st);
+  if (a.s.D <= 64) return go(std::integral_constant<int, 64>{});
+  return go(std::integral_constant<int, 128>{});
 }
 
 // fp32 sums of the splits: dQ's, and behind them dK's and dV's
@@ -512,7 +543,10 @@ size_t cross_attn_bwd_workspace_bytes(const gnn_cross_attn_bwd_args& g) {
 
 int cross_attn_bwd(const gnn_cross_attn_bwd_args& g, hipStream_t st) {
   const Plan p = plan(g);
-  if (p.q_blocks >= ((int64_t)1 << 31) || p.k_blocks >= ((int64_t)1 << 31) || g.B * g.U * g.H >= ((int64_t)1 << 31))
+  const bool shared_bias = g.bias && g.shared_bias && g.B > 1;
+  const int64_t rows = g.U * (g.H / g.Hk);
+  const int64_t b_blocks = shared_bias && g.dbias ? (rows + 127) / 128 * ((g.V + KT - 1) / KT) * g.Hk : 0;
+  if (p.q_blocks + p.k_blocks + b_blocks >= ((int64_t)1 << 31) || g.B * g.U * g.H >= ((int64_t)1 << 31))
     return set_error(GNN_ERR_UNSUPPORTED, "cross_attention: grid too large");
   if (!g.workspace || g.workspace_bytes < cross_attn_bwd_workspace_bytes(g))
     return set_error(GNN_ERR_WORKSPACE, "cross_attention: workspace missing or too small");
@@ -533,14 +567,13 @@ int cross_attn_bwd(const gnn_cross_attn_bwd_args& g, hipStream_t st) {
   float* parts = a.delta + (g.B * g.U * g.H + 3) / 4 * 4;
   if (nq) a.part_q = parts;
   if (nk) a.part_k = parts + nq;
-  const bool shared_bias = g.bias && g.shared_bias && g.B > 1;
+  a.q_blocks = (uint32_t)p.q_blocks, a.k_blocks = g.dk ? (uint32_t)p.k_blocks : 0, a.b_blocks = (uint32_t)b_blocks;
+  a.shared_bias = shared_bias;
   int rc;
   switch (g.dtype) {
-    case GNN_BF16: rc = run<bf16, PREC_NATIVE>(a, p, shared_bias, st); break;
-    case GNN_F16: rc = run<f16, PREC_NATIVE>(a, p, shared_bias, st); break;
-    default:
-      rc = g.precision == GNN_PREC_BF16X3 ? run<float, PREC_BF16X3>(a, p, shared_bias, st)
-                                          : run<float, PREC_IEEE>(a, p, shared_bias, st);
+    case GNN_BF16: rc = run<bf16, PREC_NATIVE>(a, st); break;
+    case GNN_F16: rc = run<f16, PREC_NATIVE>(a, st); break;
+    default: rc = g.precision == GNN_PREC_BF16X3 ? run<float, PREC_BF16X3>(a, st) : run<float, PREC_IEEE>(a, st);
   }
   if (rc || (!nq && !nk)) return rc;
   gnn_reduce_args r{};

@@ -156,6 +156,22 @@ struct Staged {
     }
     load(base, D, [&](int r) { return (int64_t)min(first + r, end - 1) * stride; });
   }
+  // rows first .. of the `end` rows of G heads that share a key head: row r is token r / G, head r % G, `token` and `head`
+  // elements apart; those past the last one its copies
+  __device__ __forceinline__ void load_heads(const T* base, int64_t token, int64_t head, int G, int first, int end, int D) {
+    if (EVEN && first + ROWS <= end && STEP % G == 0) {  // uniform; first is a multiple of ROWS, and so of STEP
+      const int c = chunk(0, threadIdx.x) * Tile::EPC, r = row(0, threadIdx.x);
+      const uint32_t lane = (uint32_t)(r / G * (int)token + r % G * (int)head + (c < D ? c : 0)) * (uint32_t)sizeof(T);
+      const T* tile = base + first / G * token;
+#pragma unroll
+      for (int i = 0; i < N; ++i) reg[i] = load16_at((const T*)((const char*)(tile + i * (STEP / G) * token) + lane));
+      return;
+    }
+    load(base, D, [&](int r) {
+      const int at = min(first + r, end - 1);
+      return at / G * token + at % G * head;
+    });
+  }
   // row r from base + offset(r): always a readable row
   template <typename Offset>
   __device__ __forceinline__ void load(const T* base, int D, Offset offset) {
