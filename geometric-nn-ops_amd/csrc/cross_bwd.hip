@@ -73,11 +73,6 @@ __device__ __forceinline__ void load_row(typename TypeOps<T>::V8 (&f)[DP / 16], 
   }
 }
 
-template <typename T>
-__device__ __forceinline__ f32x4 bias4(const T* row, int key, int V) {
-  return key < V ? load4_at(row + key, V - key) : f32x4{0.f, 0.f, 0.f, 0.f};
-}
-
 // 2^((score scale + bias - m) log2(e) - l); without a bias scale and m are in log2 units
 template <bool BIAS>
 __device__ __forceinline__ float probability(float score, float scale, float bias, float m, float l) {
@@ -94,6 +89,8 @@ __device__ __forceinline__ void half_tile(f32x16& dp, const unsigned char* ks, c
                                           float scale, float m, float l, float delta, uint32_t word) {
   typedef RowTile<T, DP> Tile;
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+  HalfBias<T> bias;
+  if constexpr (BIAS) bias.load(bias_row, key0, V, g);
   f32x16 sc;
   clear(sc), clear(dp);
 #pragma unroll
@@ -104,7 +101,7 @@ __device__ __forceinline__ void half_tile(f32x16& dp, const unsigned char* ks, c
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     f32x4 add = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (BIAS) add = bias4(bias_row, key0 + 8 * q + 4 * g, V);
+    if constexpr (BIAS) add = bias.at(q);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int i = 4 * q + e;
@@ -475,19 +472,27 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 || (DKDV && DP > 64) ? 1 : 2) vo
 struct Plan {
   int64_t q_blocks, q_splits, q_tiles, k_blocks, k_splits, k_tiles;
 };
-void split(int64_t base, int64_t tiles, int64_t& splits, int64_t& each) {
-  // a workgroup a CU where the tiles allow it, of 8 at least
-  const int64_t want = std::max<int64_t>(1, (int64_t)compute_units() / base), most = std::max<int64_t>(1, tiles / 8);
-  each = (tiles + std::min(want, most) - 1) / std::min(want, most);
-  splits = (tiles + each - 1) / each;
-}
+// One workgroup of 4 waves a CU in fp32 and for the products of more than 64 columns, two otherwise. Where those of dQ
+// and of dK, dV are fewer than that, each is split so that every workgroup has about an equal part of all tiles: a tile
+// of dK and dV costs four products, one of dQ three.
 Plan plan(const gnn_cross_attn_bwd_args& g) {
   Plan p{};
-  const int64_t rows = g.U * (g.H / g.Hk), heads = g.B * g.Hk;
-  split((rows + 127) / 128 * heads, (g.V + KT - 1) / KT, p.q_splits, p.q_tiles);
-  split((g.V + 127) / 128 * heads, (rows + KT - 1) / KT, p.k_splits, p.k_tiles);
-  p.q_blocks = (rows + 127) / 128 * heads * p.q_splits;
-  p.k_blocks = (g.V + 127) / 128 * heads * p.k_splits;
+  const int64_t rows = g.U * (g.H / g.Hk), heads = g.B * g.Hk, cus = compute_units();
+  const int64_t places = g.dtype == GNN_F32 || g.D > 64 ? cus : 2 * cus;
+  const int64_t qb = (rows + 127) / 128 * heads, kb = g.dk ? (g.V + 127) / 128 * heads : 0;
+  const int64_t qt = (g.V + KT - 1) / KT, kt = (rows + KT - 1) / KT;
+  auto divide = [](int64_t tiles, int64_t most, int64_t& splits, int64_t& each) {
+    splits = (tiles + most - 1) / most, each = (tiles + splits - 1) / splits;
+  };
+  int64_t part = qb + kb < places ? (3 * qb * qt + 4 * kb * kt + places - 1) / places : 4 * std::max(qt, kt);
+  const int64_t least = g.dtype == GNN_F32 ? 2 : 4;  // tiles a workgroup, beside its start and its sums
+  for (;; part += part / 16 + 1) {  // until rounding up leaves no second round
+    divide(qt, std::max(least, (part + 2) / 3), p.q_splits, p.q_tiles);
+    divide(kt, std::max(least, (part + 3) / 4), p.k_splits, p.k_tiles);
+    if (qb * p.q_splits + kb * p.k_splits <= places || (p.q_splits == 1 && p.k_splits == 1)) break;
+  }
+  p.q_blocks = qb * p.q_splits;
+  p.k_blocks = kb * p.k_splits;
   return p;
 }
 
@@ -567,7 +572,7 @@ int cross_attn_bwd(const gnn_cross_attn_bwd_args& g, hipStream_t st) {
   float* parts = a.delta + (g.B * g.U * g.H + 3) / 4 * 4;
   if (nq) a.part_q = parts;
   if (nk) a.part_k = parts + nq;
-  a.q_blocks = (uint32_t)p.q_blocks, a.k_blocks = g.dk ? (uint32_t)p.k_blocks : 0, a.b_blocks = (uint32_t)b_blocks;
+  a.q_blocks = (uint32_t)p.q_blocks, a.k_blocks = (uint32_t)p.k_blocks, a.b_blocks = (uint32_t)b_blocks;
   a.shared_bias = shared_bias;
   int rc;
   switch (g.dtype) {

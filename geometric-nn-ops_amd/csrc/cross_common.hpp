@@ -60,6 +60,28 @@ __device__ __forceinline__ void store4_at(T* p, const f32x4& v, int left) {
     if (e < left) p[e] = o[e];
 }
 
+// A row's biases of the keys that a lane holds of a half tile, 8 q + 4 g + (0 .. 3) from `key0` on, on their way while
+// the products run: where the half tile is whole, no load is in a branch. Keys past V: zeros.
+template <typename T>
+struct HalfBias {
+  typedef typename TypeOps<T>::V4 V4;
+  V4 f[4];
+  __device__ __forceinline__ void load(const T* row, int key0, int V, int g) {
+    typedef V4 VU __attribute__((aligned(sizeof(T))));
+    if (key0 + 32 <= V) {  // uniform
+#pragma unroll
+      for (int q = 0; q < 4; ++q) f[q] = *(const __attribute__((address_space(1))) VU*)(row + key0 + 8 * q + 4 * g);
+      return;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int key = key0 + 8 * q + 4 * g;
+      f[q] = TypeOps<T>::from_f32(key < V ? load4_at(row + key, V - key) : f32x4{0.f, 0.f, 0.f, 0.f});
+    }
+  }
+  __device__ __forceinline__ f32x4 at(int q) const { return TypeOps<T>::to_f32(f[q]); }
+};
+
 // Rows of DP elements in LDS, laid out so that the reads hit no bank twice: fragments of 32 rows (8 consecutive elements
 // a lane), turned ones (8 rows of one column a lane), or both. LDS serves 16 lanes' 16 bytes, and 32 lanes' 8, at once.
 //   BY_ROWS     a pitch of an odd number of 16-byte chunks: 16 rows' chunk c lie on different banks;

@@ -164,6 +164,12 @@ __global__ __launch_bounds__(NT, (Cfg<T, DP, WK, QW>::WGS)) void cross_fwd_kerne
     const unsigned char* ks = smem + buf * C::TILE;
     const unsigned char* vs = ks + C::KBYTES;
     const int r0 = WK == 1 ? 0 : 32 * wave;  // this wave's keys of the tile
+    HalfBias<T> bias[BIAS ? C::SUBS : 1][BIAS ? QW : 1];
+    if constexpr (BIAS)
+#pragma unroll
+      for (int sub = 0; sub < C::SUBS; ++sub)
+#pragma unroll
+        for (int i = 0; i < QW; ++i) bias[sub][i].load(bp[i], t * C::KT + r0 + 32 * sub, s.V, g);
     f32x16 sc[C::SUBS][QW];
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -185,8 +191,7 @@ __global__ __launch_bounds__(NT, (Cfg<T, DP, WK, QW>::WGS)) void cross_fwd_kerne
         for (int i = 0; i < QW; ++i)
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const int key = t * C::KT + r0 + 32 * sub + 8 * q + 4 * g;
-            const f32x4 bv = key < s.V ? load4_at(bp[i] + key, s.V - key) : f32x4{0.f, 0.f, 0.f, 0.f};
+            const f32x4 bv = bias[sub][i].at(q);
 #pragma unroll
             for (int e = 0; e < 4; ++e) sc[sub][i][4 * q + e] = __builtin_fmaf(sc[sub][i][4 * q + e], a.scale, bv[e]);
           }
@@ -365,9 +370,9 @@ Plan plan(const gnn_cross_attn_args& g) {
   p.few = rows <= 32;
   p.wide = g.dtype != GNN_F32 && g.D <= 64 && (rows + 255) / 256 * g.B * g.Hk >= 2 * (int64_t)compute_units();
   const int64_t per = p.wide ? 256 : 128, base = (p.few ? 1 : (rows + per - 1) / per) * g.B * g.Hk, kt = p.few ? 128 : 64, tiles = (g.V + kt - 1) / kt;
-  // two workgroups a CU where the keys allow it, of 4 tiles at least
+  // two workgroups a CU where the keys allow it, of 4 tiles at least (2 in fp32, whose products take longer)
   const int64_t want = std::max<int64_t>(1, 2 * (int64_t)compute_units() / base);
-  const int64_t most = std::max<int64_t>(1, tiles / 4);
+  const int64_t most = std::max<int64_t>(1, tiles / (g.dtype == GNN_F32 ? 2 : 4));
   p.tiles_per_split = (tiles + std::min(want, most) - 1) / std::min(want, most);
   p.splits = (tiles + p.tiles_per_split - 1) / p.tiles_per_split;
   p.blocks = base * p.splits;
