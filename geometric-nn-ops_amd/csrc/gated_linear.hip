@@ -11,6 +11,7 @@
 // gradients are one product too.
 #include <algorithm>
 
+#include "linear_rows.hpp"
 #include "linear_tiles.hpp"
 
 namespace gnn {
@@ -242,9 +243,193 @@ __global__ __launch_bounds__(GF_NT, 2) void gated_few_kernel(const GatedArgs a) 
   finish8<T>(a, z[0], z[1], m, o);
 }
 
+// ---- many rows ------------------------------------------------------------------------------
+// The gated layer of a pair transition, which HBM bounds (128 -> 512 over 384^2 rows, bf16: 189 MB against 39 GFLOP): as
+// in linear_resident.hip a workgroup of 8 waves keeps weights in LDS and every wave walks over 32 rows at a time
+// without a barrier. Both weights rarely fit: a workgroup holds `cols` outputs of both, tile y of the gate's 32 rows
+// beside tile y of the other's, and the workgroups that share rows lie on one XCD, whose L2 they read them from.
+constexpr int GR_NT = 512;
+
+template <typename T, int KS, int ACT, bool BWD>
+__global__ __launch_bounds__(GR_NT, GR_NT / 256) void gated_rows_kernel(const GatedArgs a, int cols, int parts) {
+  typedef typename TypeOps<T>::V8 V8;
+  extern __shared__ __align__(16) unsigned char smem[];
+  constexpr int ROWB = 32 * KS, NW = GR_NT / 64;
+  const int part = blockIdx.x / 8 % parts, n0 = part * cols, held = min(cols, a.O - n0);
+  const int64_t worker = (int64_t)(blockIdx.x / 8 / parts) * 8 + blockIdx.x % 8, workers = gridDim.x / parts;
+  const int nb = (held + 63) / 64 * 2;  // tiles of 32 outputs, by twos
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
+  unsigned char* const weight = smem + NW * TURN;
+  float* const bias = (float*)(weight + 2 * 32 * nb * ROWB);
+  // LDS row r: output n0 + 32 (r / 64) + tile_output(r % 32) of matrix r / 32 % 2, zeros past I and O
+  for (int e0 = wave * 64; e0 < 64 * nb * 2 * KS; e0 += GR_NT) {  // 1 KB an instruction
+    const uint32_t e = e0 + lane, r = e / (2 * KS), c = (e % (2 * KS)) ^ chunk_swizzle<(ROWB < 256 ? ROWB : 256)>(r);
+    const int n = n0 + 32 * (r / 64) + tile_output(r & 31);
+    const T* row = r & 32 ? (const T*)a.wu + (int64_t)n * a.wu_ld : (const T*)a.wg + (int64_t)n * a.wg_ld;
+    __builtin_amdgcn_global_load_lds(n < a.O && 8 * (int)c < a.I ? (const void*)(row + 8 * c) : (const void*)zero_chunk,
+                                     (lds_void_t*)(weight + 16 * e0), 16, 0, 0);
+  }
+  for (int r = threadIdx.x; r < 64 * nb; r += GR_NT) {
+    const int n = n0 + 32 * (r / 64) + (r & 31);
+    const T* b = (const T*)(r & 32 ? a.bu : a.bg);
+    bias[r] = b && n < a.O ? (float)b[n] : 0.f;
+  }
+  wait_vm_lgkm0<0>();
+  __syncthreads();
+
+  const Turn turn(smem + wave * TURN, lane);
+  const MemOrder xm(a.x_ld, a.I, lane), dm(a.dy_ld, held, lane), om(a.out_ld, held, lane);
+  const int64_t groups = (a.M + 31) / 32, step = workers * NW;
+  auto load_rows = [&](u32x4_t (&x)[KS / 2][2], int64_t grp) {
+    const auto r = rows_rsrc<T>(a.x, grp * 32, a.M, a.x_ld, a.I);
+#pragma unroll
+    for (int p = 0; p < KS / 2; ++p) xm.load(x[p], r, 32 * p);
+  };
+  const unsigned char* wrow[KS];
+#pragma unroll
+  for (int kk = 0; kk < KS; ++kk)
+    wrow[kk] = weight + l32 * ROWB + (((2 * kk + g) ^ chunk_swizzle<(ROWB < 256 ? ROWB : 256)>(l32)) << 4);
+  // rows of 16 steps take 64 registers: theirs are not loaded ahead
+  constexpr bool AHEAD = KS <= (BWD ? 4 : 8);
+  u32x4_t next[KS / 2][2], x[KS / 2][2];
+  auto turn_rows = [&]() {
+#pragma unroll
+    for (int p = 0; p < KS / 2; ++p) {
+      Turn::put(turn.to_mem, next[p]);
+      Turn::get(turn.to_rows, x[p]);
+    }
+  };
+  // Both sums of tile y; they run beside the epilogue of the tile before, of the last rows' last one at their end
+  struct Sums {
+    f32x16 gate, up;
+  };
+  auto tile = [&](int y) {
+    Sums s = {bias_tile(bias + 64 * y, g), bias_tile(bias + 64 * y + 32, g)};
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) {
+      const unsigned char* w = wrow[kk] + y * 64 * ROWB;
+      const V8 xf = __builtin_bit_cast(V8, x[kk / 2][kk % 2]);
+      Mma<T, PREC_NATIVE>::step(s.gate, *reinterpret_cast<const V8*>(w), xf);
+      Mma<T, PREC_NATIVE>::step(s.up, *reinterpret_cast<const V8*>(w + 32 * ROWB), xf);
+    }
+    return s;
+  };
+  // 32 x 32 outputs in memory order: y, or dzg and dzu
+  auto finish = [&](const Sums& s, const u32x4_t (&dy)[2], u32x4_t (&o)[BWD ? 2 : 1][2]) {
+    u32x4_t d[2];
+    if constexpr (BWD) {
+      Turn::put(turn.to_mem, dy);
+      Turn::get(turn.to_rows, d);
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f32x8 zg = outputs8(s.gate, t), zu = outputs8(s.up, t);
+      if constexpr (BWD) {
+        gradients<false, ACT>(zg, zu, to8<T>(d[t]));
+        o[BWD][t] = __builtin_bit_cast(u32x4_t, TypeOps<T>::from_f32(zu));
+      } else {
+        activate_all<false, ACT>(zg);
+        zg *= zu;
+      }
+      o[0][t] = __builtin_bit_cast(u32x4_t, TypeOps<T>::from_f32(zg));
+    }
+#pragma unroll
+    for (int k = 0; k < (BWD ? 2 : 1); ++k) {
+      Turn::put(turn.to_rows, o[k]);
+      Turn::get(turn.to_mem, o[k]);
+    }
+  };
+  int64_t grp = worker * NW + wave;
+  load_rows(next, grp);
+  turn_rows();
+  if (AHEAD) load_rows(next, grp + step);
+  Sums now = tile(0);
+  for (; grp < groups; grp += step) {
+    const auto drs = rows_rsrc<T>((const T*)a.dy + (BWD ? n0 : 0), grp * 32, BWD ? a.M : 0, a.dy_ld, held);
+    const auto grs = rows_rsrc<T>((const T*)a.out + n0, grp * 32, a.M, a.out_ld, held);
+    const auto urs = rows_rsrc<T>((const T*)a.out + (BWD ? a.out_cols + n0 : 0), grp * 32, BWD ? a.M : 0, a.out_ld, held);
+    u32x4_t dy[2][2];
+    auto load_dy = [&](int y) {
+      dm.load(dy[0], drs, 32 * y);
+      dm.load(dy[1], drs, 32 * (y + 1));
+    };
+    if (BWD) load_dy(0);
+    // tiles by twos, whose 128-byte lines are stored at once
+    for (int y = 0; y < nb; y += 2) {
+      u32x4_t o[2][BWD ? 2 : 1][2];
+      Sums ahead = tile(y + 1);
+      finish(now, dy[0], o[0]);
+      now = ahead;
+      if (y + 2 < nb) {
+        ahead = tile(y + 2);
+      } else {
+        if (!AHEAD) load_rows(next, grp + step);
+        turn_rows();
+        if (AHEAD) load_rows(next, grp + 2 * step);
+        ahead = tile(0);
+      }
+      finish(now, dy[1], o[1]);
+      now = ahead;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        om.store(o[k][0], grs, 32 * (y + k));
+        if (BWD) om.store(o[k][BWD], urs, 32 * (y + k));
+      }
+      if (BWD) load_dy(y + 2);
+    }
+  }
+}
+
+// Outputs of both weights that LDS holds beside the waves' turning tiles, and what they take; 0 where this is no form
+// for the call
+struct RowsForm {
+  int ks, cols, parts;
+  size_t lds;
+};
+RowsForm rows_form(const GatedArgs& a, int bytes) {
+  auto rows16 = [](const void* p, int64_t ld) { return ((uintptr_t)p % 16) == 0 && ld % 8 == 0 && ld < (1 << 24); };
+  if (bytes != 2 || a.M < RS_MIN_ROWS || a.I > 256 || a.O % 8 || a.x_ld >= (1 << 24) || !rows16(a.out, a.out_ld) ||
+      (a.dy && !rows16(a.dy, a.dy_ld)))
+    return {};
+  RowsForm f{};
+  f.ks = a.I <= 64 ? 4 : a.I <= 128 ? 8 : 16;
+  const int each = 2 * (32 * f.ks + 4), most = RS_LDS / each / 64 * 64;
+  f.parts = (a.O + most - 1) / most;
+  f.cols = ((a.O + f.parts - 1) / f.parts + 63) / 64 * 64;
+  f.parts = (a.O + f.cols - 1) / f.cols;
+  f.lds = (size_t)f.cols * each + GR_NT / 64 * TURN;
+  return f;
+}
+
+template <typename T, int KS, bool BWD>
+int launch_rows(const GatedArgs& a, const RowsForm& f, hipStream_t st) {
+  int rc = 0;
+  with_activation(a.act, [&](auto act) {
+    auto fn = gated_rows_kernel<T, KS, decltype(act)::value, BWD>;
+    if (f.lds > 64 * 1024)
+      (void)hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)f.lds);
+    // whole eights of workgroups for each part, so that a part's workgroups and those of the others meet on every XCD
+    const int64_t groups = (a.M + 31) / 32, places = persistent_grid((const void*)fn, GR_NT, f.lds);
+    const int64_t eights = std::max<int64_t>(1, std::min(places / 8 / f.parts, (groups + 63) / 64));
+    hipLaunchKernelGGL(fn, dim3((uint32_t)(8 * eights * f.parts)), dim3(GR_NT), f.lds, st, a, f.cols, f.parts);
+    rc = (int)hipGetLastError();
+  });
+  return rc;
+}
+template <typename T>
+int launch_rows(const GatedArgs& a, const RowsForm& f, hipStream_t st) {
+  if (f.ks == 4) return a.dy ? launch_rows<T, 4, true>(a, f, st) : launch_rows<T, 4, false>(a, f, st);
+  if (f.ks == 8) return a.dy ? launch_rows<T, 8, true>(a, f, st) : launch_rows<T, 8, false>(a, f, st);
+  return a.dy ? launch_rows<T, 16, true>(a, f, st) : launch_rows<T, 16, false>(a, f, st);
+}
+
 template <typename T, int PREC>
 int run(const GatedArgs& a, hipStream_t st) {
   const int64_t cus = compute_units();
+  if constexpr (sizeof(T) == 2) {
+    const RowsForm f = rows_form(a, sizeof(T));
+    if (f.parts && f.parts <= 4) return launch_rows<T>(a, f, st);
+  }
   if constexpr (sizeof(T) == 4) {
     typedef Tile<T, 2, 2, 1, 2, 128, 2> Medium;
     if (tiles_of<Medium>(a) >= cus / 2) return launch<T, PREC, Medium>(a, st);
@@ -273,9 +458,16 @@ __global__ __launch_bounds__(256) void gated_turn_kernel(const gnn_gated_turn_ar
   const int64_t ld = blockIdx.y ? a.wu_ld : a.wg_ld;
   const uint32_t across = (uint32_t)((a.out_cols + B - 1) / B);
   const int64_t i0 = (int64_t)(blockIdx.x / across) * B, o0 = (int64_t)(blockIdx.x % across) * B;
-  for (int k = threadIdx.x; k < B * B; k += 256) {
-    const int64_t o = o0 + k / B, i = i0 + k % B;
-    tile[k / B][k % B] = o < a.O && i < a.I ? src[o * ld + i] : (E)0;
+  E v[B * B / 256];  // no load in a branch: past the end the last row or column, and then zero
+#pragma unroll
+  for (int k = 0; k < B * B / 256; ++k) {
+    const int64_t o = o0 + threadIdx.x / B + k * (256 / B), i = i0 + threadIdx.x % B;
+    v[k] = src[min(o, a.O - 1) * ld + min(i, a.I - 1)];
+  }
+#pragma unroll
+  for (int k = 0; k < B * B / 256; ++k) {
+    const int o = threadIdx.x / B + k * (256 / B);
+    tile[o][threadIdx.x % B] = o0 + o < a.O ? v[k] : (E)0;
   }
   __syncthreads();
   E* dst = (E*)a.dst + blockIdx.y * a.out_cols;
