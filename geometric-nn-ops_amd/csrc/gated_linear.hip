@@ -431,8 +431,8 @@ int run(const GatedArgs& a, hipStream_t st) {
     if (f.parts && f.parts <= 4) return launch_rows<T>(a, f, st);
   }
   if constexpr (sizeof(T) == 4) {
-    typedef Tile<T, 2, 2, 1, 2, 128, 2> Medium;
-    if (tiles_of<Medium>(a) >= cus / 2) return launch<T, PREC, Medium>(a, st);
+    typedef Tile<T, 2, 2, 1, 2, 128, 2> Small;
+    if (tiles_of<Small>(a) >= cus / 2) return launch<T, PREC, Small>(a, st);
   } else {
     typedef Tile<T, 2, 4, 4, 2, 128, 2> Large;
     typedef Tile<T, 2, 2, 2, 2, 128, 2> Medium;

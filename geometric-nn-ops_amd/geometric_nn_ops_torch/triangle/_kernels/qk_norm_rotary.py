@@ -31,67 +31,86 @@ def _rows(t):
 
 
 def _pos(t):
-    """Address and batch stride of positions with unit stride along the tokens."""
-    if t is None:
-        return None, 0
+    """Positions with unit stride along the tokens, and their batch stride."""
     if t.stride(1) != 1 and t.shape[1] != 1:
         t = t.contiguous()
     return t, t.stride(0) if t.shape[0] > 1 else 0
 
 
-def _call(fn, q, k, dys, pos, weights, outs, dweights, parts, partial, eps, frequencies, interleaved):
+def _args(q, k, q_pos, k_pos, q_weight, k_weight, eps, frequencies, interleaved, outs, dys=(None, None)):
+    """The call's arguments and what they point to, from rows of unit stride."""
     B, U, H, D = q.shape
     V, Hk = k.shape[1:3]
-    (q_pos, q_ps), (k_pos, k_ps) = _pos(pos[0]), _pos(pos[1])
-    weights = [None if w is None else w.contiguous() for w in weights]
-    w = next((t for t in weights if t is not None), q)
-    p = q_pos if q_pos is not None else k_pos
+    qp = kp = qs = ks = 0
+    pos_bytes = 4
+    if q_pos is not None:
+        q_pos, qs = _pos(q_pos)
+        qp, pos_bytes = q_pos.data_ptr(), q_pos.element_size()
+    if k_pos is not None:
+        k_pos, ks = _pos(k_pos)
+        kp, pos_bytes = k_pos.data_ptr(), k_pos.element_size()
+    qw = kw = 0
+    dtype = param = _lib.DTYPE_CODE[q.dtype]
+    if q_weight is not None:
+        q_weight = q_weight.contiguous()
+        qw, param = q_weight.data_ptr(), _lib.DTYPE_CODE[q_weight.dtype]
+    if k_weight is not None:
+        k_weight = k_weight.contiguous()
+        kw, param = k_weight.data_ptr(), _lib.DTYPE_CODE[k_weight.dtype]
     host = _host(frequencies)
-    none = (0, 0, 0)
+    dq, dk = dys
     a = _lib.QkRotaryArgs()
     _lib.pack_qk_rotary(
-        a, 0, q.data_ptr(), k.data_ptr(), *(0 if t is None else t.data_ptr() for t in (*dys, *weights, q_pos, k_pos,
-                                                                                       *outs, *dweights)),
-        ctypes.addressof(host), 0 if partial is None else partial.data_ptr(), B, U, V, H, Hk, D, 2 * len(frequencies),
-        *q.stride()[:3], *k.stride()[:3], *(none if dys[0] is None else dys[0].stride()[:3]),
-        *(none if dys[1] is None else dys[1].stride()[:3]), q_ps, k_ps, *parts, 0.0 if eps is None else eps,
-        eps is not None, interleaved, 4 if p is None else p.element_size(), _lib.DTYPE_CODE[q.dtype],
-        _lib.DTYPE_CODE[w.dtype])
-    if fn is None:
-        lib = _lib.load()
-        return [lib.gnn_qk_rotary_parts(ctypes.byref(a), side) for side in (0, 1)]
-    _lib.call(fn, a, q.device)
-    return None
+        a, 0, q.data_ptr(), k.data_ptr(), 0 if dq is None else dq.data_ptr(), 0 if dk is None else dk.data_ptr(), qw, kw, qp,
+        kp, 0 if outs[0] is None else outs[0].data_ptr(), 0 if outs[1] is None else outs[1].data_ptr(), 0, 0,
+        ctypes.addressof(host), 0, B, U, V, H, Hk, D, 2 * len(frequencies), *q.stride()[:3], *k.stride()[:3],
+        *((0, 0, 0) if dq is None else dq.stride()[:3]), *((0, 0, 0) if dk is None else dk.stride()[:3]), qs, ks, 1, 1,
+        0.0 if eps is None else eps, eps is not None, interleaved, pos_bytes, dtype, param)
+    return a, (q_pos, k_pos, q_weight, k_weight, host)
 
 
 def qk_norm_rotary_hip(q, k, q_pos, k_pos, q_weight, k_weight, eps, frequencies, interleaved):
     """``(q', k')``, fresh and contiguous."""
-    outs = [torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k)]
+    outs = (torch.empty(q.shape, device=q.device, dtype=q.dtype), torch.empty(k.shape, device=k.device, dtype=k.dtype))
     if q.numel() or k.numel():
-        _call("gnn_qk_rotary_fwd", _rows(q), _rows(k), (None, None), (q_pos, k_pos), (q_weight, k_weight), outs,
-              (None, None), (0, 0), None, eps, frequencies, interleaved)
-    return tuple(outs)
+        q, k = _rows(q), _rows(k)
+        a, kept = _args(q, k, q_pos, k_pos, q_weight, k_weight, eps, frequencies, interleaved, outs)
+        _lib.call("gnn_qk_rotary_fwd", a, q.device)
+    return outs
 
 
 def qk_norm_rotary_bwd_hip(q, k, dq, dk, q_pos, k_pos, q_weight, k_weight, eps, frequencies, interleaved, need):
     """``(dq, dk, dq_weight, dk_weight)``, None where ``need`` says so, from the output gradients (None: zeros)."""
-    xs, dys = [q, k], [dq, dk]
-    found = [torch.empty(t.shape, device=t.device, dtype=t.dtype) if n else None for t, n in zip(xs, need[:2])]
-    dws = [torch.empty(w.shape, device=w.device, dtype=w.dtype) if n else None
-           for w, n in zip((q_weight, k_weight), need[2:])]
-    for i in range(2):
-        if dys[i] is None or not xs[i].numel():
-            for t in (found[i], dws[i]):
-                if t is not None:
-                    t.zero_()
-            xs[i], dys[i] = xs[i][:, :0], None  # nothing of this side in the call
-    runs = [xs[i].numel() > 0 and (found[i] is not None or dws[i] is not None) for i in range(2)]
-    if any(runs):
-        xs, dys = [_rows(t) for t in xs], [None if t is None else _rows(t) for t in dys]
-        args = (*xs, dys, (q_pos, k_pos), (q_weight, k_weight), [t if r else None for t, r in zip(found, runs)],
-                [t if r else None for t, r in zip(dws, runs)])
-        parts = _call(None, *args, (1, 1), None, eps, frequencies, interleaved)
-        rows = sum(n for n, t, r in zip(parts, dws, runs) if r and t is not None)
-        partial = torch.empty((rows, q.shape[-1]), device=q.device, dtype=torch.float32) if rows else None
-        _call("gnn_qk_rotary_bwd", *args, [max(1, n) for n in parts], partial, eps, frequencies, interleaved)
-    return (*found, *dws)
+    device, D = q.device, q.shape[3]
+    gq = torch.empty(q.shape, device=device, dtype=q.dtype) if need[0] else None
+    gk = torch.empty(k.shape, device=device, dtype=k.dtype) if need[1] else None
+    gqw = torch.empty((D,), device=device, dtype=q_weight.dtype) if need[2] else None
+    gkw = torch.empty((D,), device=device, dtype=k_weight.dtype) if need[3] else None
+    if dq is None or not q.numel():  # nothing of this side in the call
+        for t in (gq, gqw):
+            if t is not None:
+                t.zero_()
+        q, dq = q[:, :0], None
+    if dk is None or not k.numel():
+        for t in (gk, gkw):
+            if t is not None:
+                t.zero_()
+        k, dk = k[:, :0], None
+    if not ((dq is not None and (need[0] or need[2])) or (dk is not None and (need[1] or need[3]))):
+        return gq, gk, gqw, gkw
+    q, k = _rows(q), _rows(k)
+    dq, dk = None if dq is None else _rows(dq), None if dk is None else _rows(dk)
+    a, kept = _args(q, k, q_pos, k_pos, q_weight, k_weight, eps, frequencies, interleaved, (gq, gk), (dq, dk))
+    lib, ref, rows = _lib.load(), ctypes.byref(a), 0
+    for side, (t, dy) in enumerate(((gqw, dq), (gkw, dk))):
+        if dy is None:
+            continue
+        a.parts[side] = parts = lib.gnn_qk_rotary_parts(ref, side)
+        if t is not None:
+            a.dweight[side] = t.data_ptr()
+            rows += parts
+    if rows:
+        partial = torch.empty((rows, D), device=device, dtype=torch.float32)
+        a.partial = partial.data_ptr()
+    _lib.call("gnn_qk_rotary_bwd", a, device)
+    return gq, gk, gqw, gkw
