@@ -8,7 +8,8 @@
 // whole pairs, so that the rotation needs no exchange, and behind the turned part the two halves of 2 E plain ones
 // (angle 0). A team takes some heads of one token: a lane's E angles are the same for all of them and are made
 // once. The product pos f is formed in 64 bits and reduced to a fraction of a turn there: at position 10^6 fp32
-// would be 0.06 off.
+// would be 0.06 off. The hardware's sine and cosine take turns and are off by 2^-23 at most over half a turn to both
+// sides (measured at 2^20 places), with less than a tenth of the library's instructions.
 // Workgroups are the queries' or the keys'; in the backward they stay and walk over their tokens, and each leaves
 // one fp32 row of its weight's gradient, added in order afterwards.
 #include <algorithm>
@@ -142,9 +143,8 @@ __global__ __launch_bounds__(QR_NT) void qk_norm_rotary_kernel(const RotaryArgs 
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const double t = p * a.turns[E * at + e];
-        float sn, cs;
-        sincospif(2.f * (float)(t - rint(t)), &sn, &cs);
-        sinv[e] = sn, cosv[e] = cs;
+        const float turn = (float)(t - rint(t));
+        sinv[e] = __builtin_amdgcn_sinf(turn), cosv[e] = __builtin_amdgcn_cosf(turn);
       }
     }
     const T* x = (const T*)s.x + b * s.xs[0] + n * s.xs[1];
@@ -223,9 +223,10 @@ __global__ __launch_bounds__(QR_NT) void qk_norm_rotary_kernel(const RotaryArgs 
   }
 }
 
-// Heads a unit: as many as leave 8 workgroups a CU busy, so that the angles of a token are made seldom
+// Heads a unit: as many as leave 2 workgroups a CU, so that the angles of a token are made seldom (3 x 1021
+// tokens, 25 heads of 80, fp16: 13 us, with 8 workgroups a CU 18; 2 x 4096 of 32 heads of 128, bf16: 25 and 29)
 void divide(Side& s, int64_t B, int teams) {
-  const int64_t want = (int64_t)compute_units() * 8 * teams, rows = B * s.N * s.H;
+  const int64_t want = (int64_t)compute_units() * 2 * teams, rows = B * s.N * s.H;
   s.heads = (int)std::min<int64_t>(s.H, std::max<int64_t>(1, rows / want));
   s.groups = (s.H + s.heads - 1) / s.heads;
   s.units = B * s.N * s.groups;
