@@ -57,10 +57,8 @@ struct BwdArgs {
   bool shared_bias;
 };
 
-template <typename T> constexpr float p_shift() { return 0.f; }
-template <> constexpr float p_shift<f16>() { return 10.f; }
-template <typename T> constexpr float p_unit() { return 1.f; }  // 2^-p_shift
-template <> constexpr float p_unit<f16>() { return 0x1p-10f; }
+template <typename T> constexpr float p_scale() { return 1.f; }  // of P in dV
+template <> constexpr float p_scale<f16>() { return 0x1p10f; }
 
 // Fragments of one row of a lane, zeros past D
 template <typename T, int DP>
@@ -73,11 +71,17 @@ __device__ __forceinline__ void load_row(typename TypeOps<T>::V8 (&f)[DP / 16], 
   }
 }
 
-// 2^((score scale + bias - m) log2(e) - l); without a bias scale and m are in log2 units
+// A row's part of the exponent: with a bias m and l of 2^((score scale + bias - m) log2(e) - l), without one, where scale
+// and m are in log2 units, their sum.
 template <bool BIAS>
 __device__ __forceinline__ float probability(float score, float scale, float bias, float m, float l) {
   if constexpr (BIAS) return fast_exp2(__builtin_fmaf(__builtin_fmaf(score, scale, bias) - m, LOG2E, -l));
-  return fast_exp2(__builtin_fmaf(score, scale, -(m + l)));
+  return fast_exp2(__builtin_fmaf(score, scale, -m));
+}
+template <bool BIAS>
+__device__ __forceinline__ void row_stats(const float* stats, float& m, float& l) {
+  m = stats[0], l = stats[1];
+  if constexpr (!BIAS) m += l;
 }
 
 // dS^T = P (dP - Delta) of one half tile of 32 keys for the lane's row.
@@ -86,13 +90,14 @@ template <typename T, int PREC, int DP, bool BIAS>
 __device__ __forceinline__ void half_tile(f32x16& dp, const unsigned char* ks, const unsigned char* vs, int at,
                                           const typename TypeOps<T>::V8 (&qf)[DP / 16],
                                           const typename TypeOps<T>::V8 (&df)[DP / 16], const T* bias_row, int key0, int V,
-                                          float scale, float m, float l, float delta, uint32_t word) {
+                                          float scale, float m, float l, const f32x16& minus_delta, uint32_t word) {
   typedef RowTile<T, DP> Tile;
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   HalfBias<T> bias;
-  if constexpr (BIAS) bias.load(bias_row, key0, V, g);
+  if constexpr (BIAS) bias.template load<false>(bias_row, key0, V, g);
   f32x16 sc;
-  clear(sc), clear(dp);
+  clear(sc);
+  dp = minus_delta;
 #pragma unroll
   for (int kk = 0; kk < DP / 16; ++kk) {
     Mma<T, PREC>::step(sc, Tile::row8(ks, at + l32, kk, g), qf[kk]);
@@ -105,8 +110,7 @@ __device__ __forceinline__ void half_tile(f32x16& dp, const unsigned char* ks, c
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int i = 4 * q + e;
-      const float p = probability<BIAS>(sc[i], scale, add[e], m, l);
-      dp[i] = p * (dp[i] - delta);
+      dp[i] *= probability<BIAS>(sc[i], scale, add[e], m, l);
     }
   }
   if (word != ~0u) {  // uniform
@@ -141,7 +145,7 @@ struct Lds {
   static constexpr int NBUF = sizeof(T) == 2 ? 2 : 1;
   static constexpr int TILE = KT * RowTile<T, DP>::PITCH;
   __align__(16) unsigned char tile[NBUF * 2 * TILE];
-  __align__(16) float m[NBUF][KT], l[NBUF][KT], delta[NBUF][KT];
+  __align__(16) float m[NBUF][KT], l[NBUF][KT], minus_delta[NBUF][KT];
   int64_t bias_at[NBUF][KT];
   int found[2];
 };
@@ -174,7 +178,10 @@ __device__ __forceinline__ void dq_block(const BwdArgs& a, Lds<T, DP>& lds, uint
   V8 qf[DP / 16], df[DP / 16];
   load_row<T, DP>(qf, (const T*)a.q + b * a.qs[0] + u * a.qs[1] + h * a.qs[2], s.D, g);
   load_row<T, DP>(df, (const T*)a.dout + b * a.ds[0] + u * a.ds[1] + h * a.ds[2], s.D, g);
-  const float m = a.stats[2 * stat], l = a.stats[2 * stat + 1], delta = a.delta[stat];
+  float m, l;
+  row_stats<BIAS>(a.stats + 2 * stat, m, l);
+  f32x16 minus_delta;  // what the sums of dP start from
+  fill(minus_delta, -a.delta[stat]);
   // own bias: every tile is visited, so that what no row keeps gets its zeros
   T* dbias = BIAS && a.dbias && !a.shared_bias ? (T*)a.dbias + stat * s.V : nullptr;
   int key_end = min(s.V, (split + 1) * a.q_tiles * KT), key0 = split * a.q_tiles * KT;
@@ -221,7 +228,7 @@ __device__ __forceinline__ void dq_block(const BwdArgs& a, Lds<T, DP>& lds, uint
     for (int sub = 0; sub < 2; ++sub) {
       f32x16 ds;
       half_tile<T, PREC, DP, BIAS>(ds, ks, ks + TILE, 32 * sub, qf, df, bias_row, t * KT + 32 * sub, s.V, a.logit_scale, m, l,
-                                   delta, (uint32_t)(live >> (32 * sub)));
+                                   minus_delta, (uint32_t)(live >> (32 * sub)));
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         const V8 f = acc_frag<T>(ds, kk);
@@ -303,7 +310,7 @@ __device__ __forceinline__ void dkdv_block(const BwdArgs& a, Lds<T, DP>& lds, ui
     if (threadIdx.x < KT) {
       const int row = min(t * KT + (int)threadIdx.x, s.rows - 1), u = row / s.G, h = hk * s.G + row % s.G;
       const int64_t stat = ((int64_t)b * s.H + h) * s.U + u;
-      next_m = a.stats[2 * stat], next_l = a.stats[2 * stat + 1];
+      row_stats<BIAS>(a.stats + 2 * stat, next_m, next_l);
       if (t * KT + (int)threadIdx.x >= s.rows) next_m = INFINITY;  // P = 2^-inf, and zeros of Q and dO
       next_delta = a.delta[stat];
       if constexpr (BIAS) next_bias = h * a.bs[1] + u * a.bs[2];
@@ -320,8 +327,8 @@ __device__ __forceinline__ void dkdv_block(const BwdArgs& a, Lds<T, DP>& lds, ui
     }
     if (threadIdx.x < KT) {
       lds.m[buf][threadIdx.x] = next_m;
-      lds.l[buf][threadIdx.x] = next_l - p_shift<T>();
-      lds.delta[buf][threadIdx.x] = next_delta * p_unit<T>();
+      if constexpr (BIAS) lds.l[buf][threadIdx.x] = next_l;
+      lds.minus_delta[buf][threadIdx.x] = -next_delta;
       if constexpr (BIAS) lds.bias_at[buf][threadIdx.x] = next_bias;
     }
   };
@@ -338,8 +345,14 @@ __device__ __forceinline__ void dkdv_block(const BwdArgs& a, Lds<T, DP>& lds, ui
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
       const int r0 = 32 * sub;
-      f32x16 p, dp;
-      clear(p), clear(dp);
+      f32x16 p, dp;  // the sums of dP start from -Delta
+      clear(p);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 d4 = *reinterpret_cast<const f32x4*>(&lds.minus_delta[buf][r0 + 8 * q + 4 * g]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[4 * q + e] = d4[e];
+      }
 #pragma unroll
       for (int kk = 0; kk < DP / 16; ++kk) {
         Mma<T, PREC>::step(p, Tile::row8(qs, r0 + l32, kk, g), kf[kk]);
@@ -348,15 +361,14 @@ __device__ __forceinline__ void dkdv_block(const BwdArgs& a, Lds<T, DP>& lds, ui
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const f32x4 m4 = *reinterpret_cast<const f32x4*>(&lds.m[buf][r0 + 8 * q + 4 * g]);
-        const f32x4 l4 = *reinterpret_cast<const f32x4*>(&lds.l[buf][r0 + 8 * q + 4 * g]);
-        const f32x4 d4 = *reinterpret_cast<const f32x4*>(&lds.delta[buf][r0 + 8 * q + 4 * g]);
+        f32x4 l4 = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (BIAS) l4 = *reinterpret_cast<const f32x4*>(&lds.l[buf][r0 + 8 * q + 4 * g]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int i = 4 * q + e;
           float add = 0.f;
           if constexpr (BIAS) add = TypeOps<T>::to_f32(bias_key[lds.bias_at[buf][r0 + 8 * q + 4 * g + e]]);
           p[i] = probability<BIAS>(p[i], a.logit_scale, add, m4[e], l4[e]);
-          dp[i] = __builtin_fmaf(dp[i], p_unit<T>(), -d4[e]);
         }
       }
       if (!all_kept)  // uniform
@@ -364,6 +376,9 @@ __device__ __forceinline__ void dkdv_block(const BwdArgs& a, Lds<T, DP>& lds, ui
         for (int i = 0; i < 16; ++i) p[i] = kept ? p[i] : 0.f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) dp[i] *= p[i];
+      if constexpr (p_scale<T>() != 1.f)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[i] *= p_scale<T>();
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         const V8 pf = acc_frag<T>(p, kk), sf = acc_frag<T>(dp, kk);
@@ -387,7 +402,7 @@ __device__ __forceinline__ void dkdv_block(const BwdArgs& a, Lds<T, DP>& lds, ui
       const int d = 32 * cc + 8 * q + 4 * g;
       if (d >= s.D) continue;
       const f32x4 x = f32x4{dk[cc][4 * q], dk[cc][4 * q + 1], dk[cc][4 * q + 2], dk[cc][4 * q + 3]} * a.scale;
-      const f32x4 y = f32x4{dv[cc][4 * q], dv[cc][4 * q + 1], dv[cc][4 * q + 2], dv[cc][4 * q + 3]} * p_unit<T>();
+      const f32x4 y = f32x4{dv[cc][4 * q], dv[cc][4 * q + 1], dv[cc][4 * q + 2], dv[cc][4 * q + 3]} * (1.f / p_scale<T>());
       if (a.part_k) {
         *reinterpret_cast<f32x4*>(a.part_k + 2 * split * each + at + d) = x;
         *reinterpret_cast<f32x4*>(a.part_k + (2 * split + 1) * each + at + d) = y;
@@ -429,7 +444,10 @@ __device__ __forceinline__ void dbias_block(const BwdArgs& a, Lds<T, DP>& lds, u
     load_row<T, DP>(qf, (const T*)a.q + b * a.qs[0] + u * a.qs[1] + h * a.qs[2], s.D, g);
     load_row<T, DP>(df, (const T*)a.dout + b * a.ds[0] + u * a.ds[1] + h * a.ds[2], s.D, g);
     const int64_t stat = ((int64_t)b * s.H + h) * s.U + u;
-    const float m = a.stats[2 * stat], l = a.stats[2 * stat + 1], delta = a.delta[stat];
+    float m, l;
+    row_stats<true>(a.stats + 2 * stat, m, l);
+    f32x16 minus_delta;
+    fill(minus_delta, -a.delta[stat]);
     __syncthreads();  // the sequence before is done with
     kreg.store(smem, s.D, [&](int r) { return (live >> r & 1) != 0; });
     vreg.store(smem + TILE, s.D, [&](int r) { return (live >> r & 1) != 0; });
@@ -438,7 +456,7 @@ __device__ __forceinline__ void dbias_block(const BwdArgs& a, Lds<T, DP>& lds, u
     for (int sub = 0; sub < 2; ++sub) {
       f32x16 ds;
       half_tile<T, PREC, DP, true>(ds, smem, smem + TILE, 32 * sub, qf, df, bias_row, kb * KT + 32 * sub, s.V, a.logit_scale,
-                                   m, l, delta, (uint32_t)(live >> (32 * sub)));
+                                   m, l, minus_delta, (uint32_t)(live >> (32 * sub)));
       sum[sub] += ds;
     }
   }

@@ -61,14 +61,15 @@ __device__ __forceinline__ void store4_at(T* p, const f32x4& v, int left) {
 }
 
 // A row's biases of the keys that a lane holds of a half tile, 8 q + 4 g + (0 .. 3) from `key0` on, on their way while
-// the products run: where the half tile is whole, no load is in a branch. Keys past V: zeros.
+// the products run: where the half tile is known to be WHOLE, no load is in a branch. Keys past V: zeros.
 template <typename T>
 struct HalfBias {
   typedef typename TypeOps<T>::V4 V4;
   V4 f[4];
+  template <bool WHOLE>
   __device__ __forceinline__ void load(const T* row, int key0, int V, int g) {
     typedef V4 VU __attribute__((aligned(sizeof(T))));
-    if (key0 + 32 <= V) {  // uniform
+    if (WHOLE || key0 + 32 <= V) {  // uniform
 #pragma unroll
       for (int q = 0; q < 4; ++q) f[q] = *(const __attribute__((address_space(1))) VU*)(row + key0 + 8 * q + 4 * g);
       return;
@@ -259,10 +260,11 @@ __device__ __forceinline__ typename TypeOps<T>::V8 acc_frag(const f32x16& a, int
                    a[8 * kk + 4], a[8 * kk + 5], a[8 * kk + 6], a[8 * kk + 7]};
   return TypeOps<T>::from_f32(x);
 }
-__device__ __forceinline__ void clear(f32x16& a) {
+__device__ __forceinline__ void fill(f32x16& a, float x) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) a[i] = 0.f;
+  for (int i = 0; i < 16; ++i) a[i] = x;
 }
+__device__ __forceinline__ void clear(f32x16& a) { fill(a, 0.f); }
 // maximum and sum over the lane pair (l, l ^ 32) without a trip through LDS
 __device__ __forceinline__ float pair_top(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);

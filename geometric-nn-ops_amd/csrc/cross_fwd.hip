@@ -169,9 +169,8 @@ __global__ __launch_bounds__(NT, (Cfg<T, DP, WK, QW>::WGS)) void cross_fwd_kerne
 #pragma unroll
       for (int sub = 0; sub < C::SUBS; ++sub)
 #pragma unroll
-        for (int i = 0; i < QW; ++i) bias[sub][i].load(bp[i], t * C::KT + r0 + 32 * sub, s.V, g);
+        for (int i = 0; i < QW; ++i) bias[sub][i].template load<false>(bp[i], t * C::KT + r0 + 32 * sub, s.V, g);
     f32x16 sc[C::SUBS][QW];
-    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int sub = 0; sub < C::SUBS; ++sub) {
 #pragma unroll
@@ -183,7 +182,6 @@ __global__ __launch_bounds__(NT, (Cfg<T, DP, WK, QW>::WGS)) void cross_fwd_kerne
         for (int i = 0; i < QW; ++i) Mma<T, PREC>::step(sc[sub][i], kf, qf[i][kk]);
       }
     }
-    __builtin_amdgcn_s_setprio(0);
     if constexpr (BIAS) {
 #pragma unroll
       for (int sub = 0; sub < C::SUBS; ++sub)
@@ -196,11 +194,14 @@ __global__ __launch_bounds__(NT, (Cfg<T, DP, WK, QW>::WGS)) void cross_fwd_kerne
             for (int e = 0; e < 4; ++e) sc[sub][i][4 * q + e] = __builtin_fmaf(sc[sub][i][4 * q + e], a.scale, bv[e]);
           }
     }
+    bool whole = true;
 #pragma unroll
-    for (int sub = 0; sub < C::SUBS; ++sub) {
-      const int at = r0 + 32 * sub;
-      const uint32_t word = (uint32_t)(live[at / 64] >> (at & 63));
-      if (word != ~0u) {  // uniform
+    for (int i = 0; i < C::WORDS; ++i) whole = whole && live[i] == ~0ull;
+    if (!whole) {  // uniform
+#pragma unroll
+      for (int sub = 0; sub < C::SUBS; ++sub) {
+        const int at = r0 + 32 * sub;
+        const uint32_t word = (uint32_t)(live[at / 64] >> (at & 63));
 #pragma unroll
         for (int i = 0; i < QW; ++i)
 #pragma unroll
@@ -248,7 +249,6 @@ __global__ __launch_bounds__(NT, (Cfg<T, DP, WK, QW>::WGS)) void cross_fwd_kerne
         sum[i] += (part[0] + part[1]) + (part[2] + part[3]);
         p[i][0] = acc_frag<T>(x, 0), p[i][1] = acc_frag<T>(x, 1);
       }
-      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
@@ -257,7 +257,6 @@ __global__ __launch_bounds__(NT, (Cfg<T, DP, WK, QW>::WGS)) void cross_fwd_kerne
 #pragma unroll
           for (int i = 0; i < QW; ++i) Mma<T, PREC>::step(o[i][cc], vf, p[i][kk]);
         }
-      __builtin_amdgcn_s_setprio(0);
     }
     if constexpr (C::NBUF == 1) __syncthreads();
     if (next < t_end) put(C::NBUF == 1 ? 0 : buf ^ 1, next_live);
