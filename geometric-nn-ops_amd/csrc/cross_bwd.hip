@@ -30,7 +30,9 @@ namespace {
 using namespace cross;
 
 constexpr int NT = 256;
-constexpr int KT = 64;   // keys a tile (dq), rows a tile (dk, dv)
+// Keys a tile (dQ, dbias), rows a tile (dK, dV). fp32 with more than 64 columns holds 128 registers of operands and 128 of
+// sums a lane: of 64 rows, 64 more on their way to LDS were spilled.
+constexpr int tile_of(bool f32, int D) { return f32 && D > 64 ? 32 : 64; }
 
 struct BwdArgs {
   Shape s;
@@ -143,6 +145,8 @@ __global__ __launch_bounds__(NT) void cross_delta_kernel(const BwdArgs a) {
 template <typename T, int DP>
 struct Lds {
   static constexpr int NBUF = sizeof(T) == 2 ? 2 : 1;
+  static constexpr int KT = tile_of(sizeof(T) == 4, DP);
+  static constexpr uint64_t ALL = KT == 64 ? ~0ull : ~0u;  // a tile's keys
   static constexpr int TILE = KT * RowTile<T, DP>::PITCH;
   __align__(16) unsigned char tile[NBUF * 2 * TILE];
   __align__(16) float m[NBUF][KT], l[NBUF][KT], minus_delta[NBUF][KT];
@@ -155,7 +159,7 @@ template <typename T, int PREC, int DP, bool BIAS>
 __device__ __forceinline__ void dq_block(const BwdArgs& a, Lds<T, DP>& lds, uint32_t block) {
   typedef RowTile<T, DP> Tile;
   typedef typename TypeOps<T>::V8 V8;
-  constexpr int TILE = Lds<T, DP>::TILE, NBUF = Lds<T, DP>::NBUF;
+  constexpr int TILE = Lds<T, DP>::TILE, NBUF = Lds<T, DP>::NBUF, KT = Lds<T, DP>::KT;
   unsigned char* smem = lds.tile;
   const Shape& s = a.s;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
@@ -194,7 +198,7 @@ __device__ __forceinline__ void dq_block(const BwdArgs& a, Lds<T, DP>& lds, uint
   Staged<T, DP, KT, NT> kreg, vreg;
   auto seek = [&](int t, uint64_t& word) {
     for (; t < t_end; ++t) {
-      word = live_keys(mask, a.ms[1], t * KT, s.V);
+      word = live_keys(mask, a.ms[1], t * KT, s.V) & Lds<T, DP>::ALL;
       if (word || dbias) break;
     }
     return t;
@@ -205,7 +209,7 @@ __device__ __forceinline__ void dq_block(const BwdArgs& a, Lds<T, DP>& lds, uint
   };
   auto put = [&](int buf, uint64_t word) {  // what masked keys hold, NaN too, meets only zeros
     unsigned char* st = smem + buf * 2 * TILE;
-    if (s.D == DP && word == ~0ull) {  // uniform
+    if (s.D == DP && word == Lds<T, DP>::ALL) {  // uniform
       kreg.store(st);
       vreg.store(st + TILE);
       return;
@@ -224,8 +228,9 @@ __device__ __forceinline__ void dq_block(const BwdArgs& a, Lds<T, DP>& lds, uint
     const int next = seek(t + 1, next_live);
     if (next < t_end) load(next);
     const unsigned char* ks = smem + buf * 2 * TILE;
+    if (sizeof(T) == 2 || rb * 128 + wave * 32 < s.rows)  // uniform; a wave without rows only stages (in 16 bits the branch costs more)
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
+    for (int sub = 0; sub < KT / 32; ++sub) {
       f32x16 ds;
       half_tile<T, PREC, DP, BIAS>(ds, ks, ks + TILE, 32 * sub, qf, df, bias_row, t * KT + 32 * sub, s.V, a.logit_scale, m, l,
                                    minus_delta, (uint32_t)(live >> (32 * sub)));
@@ -270,7 +275,7 @@ template <typename T, int PREC, int DP, bool BIAS>
 __device__ __forceinline__ void dkdv_block(const BwdArgs& a, Lds<T, DP>& lds, uint32_t block) {
   typedef RowTile<T, DP> Tile;
   typedef typename TypeOps<T>::V8 V8;
-  constexpr int TILE = Lds<T, DP>::TILE, NBUF = Lds<T, DP>::NBUF;
+  constexpr int TILE = Lds<T, DP>::TILE, NBUF = Lds<T, DP>::NBUF, KT = Lds<T, DP>::KT;
   unsigned char* smem = lds.tile;
   const Shape& s = a.s;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
@@ -343,8 +348,11 @@ __device__ __forceinline__ void dkdv_block(const BwdArgs& a, Lds<T, DP>& lds, ui
     const unsigned char* qs = smem + buf * 2 * TILE;
     const unsigned char* ds = qs + TILE;
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
+    for (int sub = 0; sub < KT / 32; ++sub) {
       const int r0 = 32 * sub;
+      // uniform: no row there (in 16 bits the products cost less than the branch between them: 195 us of 4 x 2048 x 1400,
+      // 208 with it)
+      if (sizeof(T) == 4 && t * KT + r0 >= s.rows) break;
       f32x16 p, dp;  // the sums of dP start from -Delta
       clear(p);
 #pragma unroll
@@ -418,7 +426,7 @@ template <typename T, int PREC, int DP>
 __device__ __forceinline__ void dbias_block(const BwdArgs& a, Lds<T, DP>& lds, uint32_t block) {
   typedef RowTile<T, DP> Tile;
   typedef typename TypeOps<T>::V8 V8;
-  constexpr int TILE = Lds<T, DP>::TILE;
+  constexpr int TILE = Lds<T, DP>::TILE, KT = Lds<T, DP>::KT;
   unsigned char* smem = lds.tile;
   const Shape& s = a.s;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
@@ -430,10 +438,11 @@ __device__ __forceinline__ void dbias_block(const BwdArgs& a, Lds<T, DP>& lds, u
   const int row = rb * 128 + wave * 32 + l32;
   const int safe = min(row, s.rows - 1), u = safe / s.G, h = hk * s.G + safe % s.G;
   const T* bias_row = (const T*)a.bias + h * a.bs[1] + u * a.bs[2];
-  f32x16 sum[2];
-  clear(sum[0]), clear(sum[1]);
+  f32x16 sum[KT / 32];
+#pragma unroll
+  for (int sub = 0; sub < KT / 32; ++sub) clear(sum[sub]);
   for (int b = 0; b < s.B; ++b) {
-    const uint64_t live = live_keys(a.mask ? a.mask + b * a.ms[0] : nullptr, a.ms[1], kb * KT, s.V);
+    const uint64_t live = live_keys(a.mask ? a.mask + b * a.ms[0] : nullptr, a.ms[1], kb * KT, s.V) & Lds<T, DP>::ALL;
     if (!live) continue;  // the same for the whole workgroup
     const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
     const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
@@ -453,7 +462,7 @@ __device__ __forceinline__ void dbias_block(const BwdArgs& a, Lds<T, DP>& lds, u
     vreg.store(smem + TILE, s.D, [&](int r) { return (live >> r & 1) != 0; });
     __syncthreads();
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
+    for (int sub = 0; sub < KT / 32; ++sub) {
       f32x16 ds;
       half_tile<T, PREC, DP, true>(ds, smem, smem + TILE, 32 * sub, qf, df, bias_row, kb * KT + 32 * sub, s.V, a.logit_scale,
                                    m, l, minus_delta, (uint32_t)(live >> (32 * sub)));
@@ -463,7 +472,7 @@ __device__ __forceinline__ void dbias_block(const BwdArgs& a, Lds<T, DP>& lds, u
   if (row >= s.rows) return;
   T* out = (T*)a.dbias + ((int64_t)h * s.U + u) * s.V;
 #pragma unroll
-  for (int sub = 0; sub < 2; ++sub)
+  for (int sub = 0; sub < KT / 32; ++sub)
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int key = kb * KT + 32 * sub + 8 * q + 4 * g;
@@ -487,6 +496,12 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 || (DKDV && DP > 64) ? 1 : 2) vo
   }
 }
 
+template <typename E>
+__global__ __launch_bounds__(NT) void zeros_kernel(E* p, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x;
+  if (i < n) p[i] = 0;
+}
+
 struct Plan {
   int64_t q_blocks, q_splits, q_tiles, k_blocks, k_splits, k_tiles;
 };
@@ -495,6 +510,7 @@ struct Plan {
 // of dK and dV costs four products, one of dQ three.
 Plan plan(const gnn_cross_attn_bwd_args& g) {
   Plan p{};
+  const int KT = tile_of(g.dtype == GNN_F32, (int)g.D);
   const int64_t rows = g.U * (g.H / g.Hk), heads = g.B * g.Hk, cus = compute_units();
   const int64_t places = g.dtype == GNN_F32 || g.D > 64 ? cus : 2 * cus;
   const int64_t qb = (rows + 127) / 128 * heads, kb = g.dk ? (g.V + 127) / 128 * heads : 0;
@@ -566,9 +582,11 @@ size_t cross_attn_bwd_workspace_bytes(const gnn_cross_attn_bwd_args& g) {
 
 int cross_attn_bwd(const gnn_cross_attn_bwd_args& g, hipStream_t st) {
   const Plan p = plan(g);
+  const bool one_key = g.V == 1;
+  const int KT = tile_of(g.dtype == GNN_F32, (int)g.D);
   const bool shared_bias = g.bias && g.shared_bias && g.B > 1;
   const int64_t rows = g.U * (g.H / g.Hk);
-  const int64_t b_blocks = shared_bias && g.dbias ? (rows + 127) / 128 * ((g.V + KT - 1) / KT) * g.Hk : 0;
+  const int64_t b_blocks = shared_bias && g.dbias && !one_key ? (rows + 127) / 128 * ((g.V + KT - 1) / KT) * g.Hk : 0;
   if (p.q_blocks + p.k_blocks + b_blocks >= ((int64_t)1 << 31) || g.B * g.U * g.H >= ((int64_t)1 << 31))
     return set_error(GNN_ERR_UNSUPPORTED, "cross_attention: grid too large");
   if (!g.workspace || g.workspace_bytes < cross_attn_bwd_workspace_bytes(g))
@@ -583,7 +601,19 @@ int cross_attn_bwd(const gnn_cross_attn_bwd_args& g, hipStream_t st) {
   }
   for (int i = 0; i < 2; ++i) a.ms[i] = g.mask_stride[i];
   a.scale = g.scale, a.logit_scale = g.bias ? g.scale : g.scale * LOG2E;
+  // One key has probability 1 whatever its logit: the logits' gradients are zeros, where P (dP - Delta) would leave the
+  // rounding errors of two sums of the same products.
+  if (one_key) a.scale = a.logit_scale = 0.f, a.bias = nullptr, a.dbias = nullptr;
   a.q_splits = (int)p.q_splits, a.q_tiles = (int)p.q_tiles, a.k_splits = (int)p.k_splits, a.k_tiles = (int)p.k_tiles;
+  if (one_key && g.dbias) {
+    const int64_t n = (g.shared_bias ? 1 : g.B) * g.H * g.U;
+    const dim3 grid((uint32_t)((n + NT - 1) / NT));
+    if (g.dtype == GNN_F32)
+      hipLaunchKernelGGL(zeros_kernel<uint32_t>, grid, dim3(NT), 0, st, (uint32_t*)g.dbias, n);
+    else
+      hipLaunchKernelGGL(zeros_kernel<uint16_t>, grid, dim3(NT), 0, st, (uint16_t*)g.dbias, n);
+    if (int rc = (int)hipGetLastError()) return rc;
+  }
   int64_t nq, nk;
   partial_sums(g, p, nq, nk);
   a.delta = (float*)g.workspace;

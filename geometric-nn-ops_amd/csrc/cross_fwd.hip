@@ -115,7 +115,8 @@ __global__ __launch_bounds__(NT, (Cfg<T, DP, WK, QW>::WGS)) void cross_fwd_kerne
     for (int kk = 0; kk < DP / 16; ++kk) {
       const int d = 16 * kk + 8 * g;
       qf[i][kk] = load8_at(qp + (d < s.D ? d : 0));
-      if (d >= s.D) qf[i][kk] = zero8<T>();
+      // one key has probability 1 whatever its logit: 0 here, which leaves the sum an exact 1
+      if (d >= s.D || s.V == 1) qf[i][kk] = zero8<T>();
     }
 #pragma unroll
     for (int cc = 0; cc < DP / 32; ++cc) clear(o[i][cc]);
@@ -342,15 +343,29 @@ __global__ __launch_bounds__(NT) void cross_join_kernel(const FwdArgs a) {
   if (head >= heads) return;
   const int d = (int)(i - head * per) * 4, h = (int)(head % s.H);
   const int64_t bu = head / s.H, b = bu / s.U, u = bu - b * s.U, stat = (b * s.H + h) * s.U + u;
-  float m = -INFINITY;
-  for (int k = 0; k < a.splits; ++k) m = fmaxf(m, a.part_ml[(k * heads + stat) * 2]);
-  float sum = 0.f;
+  // 8 splits at a time, no load in a branch: past the last one its copies, with no weight
+  float m = -INFINITY, sum = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < a.splits; ++k) {
-    const float* ml = a.part_ml + (k * heads + stat) * 2;
-    const float f = fast_exp2(m == -INFINITY ? 0.f : (ml[0] - m) * unit<BIAS>());
-    sum += f * ml[1];
-    o += f * *reinterpret_cast<const f32x4*>(a.part_o + (k * heads + head) * s.D + d);
+  for (int k0 = 0; k0 < a.splits; k0 += 8) {
+    float mk[8], lk[8];
+    f32x4 ok[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int k = min(k0 + i, a.splits - 1);
+      mk[i] = a.part_ml[(k * heads + stat) * 2], lk[i] = a.part_ml[(k * heads + stat) * 2 + 1];
+      ok[i] = *reinterpret_cast<const f32x4*>(a.part_o + (k * heads + head) * s.D + d);
+    }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, mk[i]);
+    const float old = fast_exp2(top == -INFINITY ? 0.f : (m - top) * unit<BIAS>());
+    sum *= old, o *= old, m = top;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float f = k0 + i < a.splits ? fast_exp2(top == -INFINITY ? 0.f : (mk[i] - top) * unit<BIAS>()) : 0.f;
+      sum += f * lk[i];
+      o += f * ok[i];
+    }
   }
   const float inv = sum > 0.f ? 1.0f / sum : sum == 0.f ? 0.f : sum;
   store4((T*)a.o + head * s.D + d, TypeOps<T>::from_f32(o * inv));
@@ -438,6 +453,7 @@ int cross_attn_fwd(const gnn_cross_attn_args& g, hipStream_t st) {
   for (int i = 0; i < 3; ++i) a.qs[i] = g.q_stride[i], a.ks[i] = g.k_stride[i], a.vs[i] = g.v_stride[i], a.bs[i] = g.bias_stride[i];
   for (int i = 0; i < 2; ++i) a.ms[i] = g.mask_stride[i];
   a.scale = g.bias ? g.scale : g.scale * LOG2E;
+  if (g.V == 1) a.bias = nullptr, a.scale = g.scale * LOG2E;
   a.splits = (int)p.splits, a.tiles_per_split = (int)p.tiles_per_split;
   if (p.splits > 1) {
     if (!g.workspace || g.workspace_bytes < cross_attn_workspace_bytes(g))

@@ -240,6 +240,24 @@ def test_the_lowest_value_is_a_logit_like_any_other(u, dtype):
     assert_within("dbias", grads[3], dbias, (2 * half_step(dtype) + 64 * U) * lost.sum(0, keepdim=True))
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("u", [1, 52])
+@pytest.mark.parametrize("bias", [0, 1, 2])
+def test_one_key(bias, u, dtype):
+    """Its probability is 1 whatever its logit: the output is the value and the logits' gradients are zeros, exactly."""
+    tensors, _, dout = _inputs((3, u, 1, 4, 2, 128, bias, False), dtype, seed=18, scale=3.0)
+    mask = torch.tensor([[True], [False], [True]], device=DEV)
+    for m in (None, mask):
+        leaves = [t.clone().requires_grad_() for t in tensors if t is not None]
+        o = cross_attention(*leaves, *([] if bias else [None]), m)
+        grads = torch.autograd.grad(o, leaves, dout)
+        keep = torch.ones(3, 1, 1, 1, device=DEV, dtype=dtype) if m is None else m[:, :, None, None].to(dtype)
+        assert torch.equal(o, (tensors[2] * keep).repeat_interleave(2, 2).expand(3, u, 4, 128))
+        assert not grads[0].any() and not grads[1].any() and (not bias or not grads[3].any())
+        want = (dout.double() * keep.double()).view(3, u, 2, 2, 128)
+        assert_within("dv", grads[2], want.sum((1, 3))[:, None], _sum_error(2 * u) * want.abs().sum((1, 3))[:, None])
+
+
 def test_no_keys_no_queries():
     for b, u, v, h, hk in ((0, 3, 4, 2, 2), (2, 0, 4, 2, 1), (2, 3, 0, 2, 2), (1, 3, 4, 0, 1)):
         q, k, val = (torch.randn(b, n, m, 32, device=DEV).half().requires_grad_() for n, m in ((u, h), (v, hk), (v, hk)))
