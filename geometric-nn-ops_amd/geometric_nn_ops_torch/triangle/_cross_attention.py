@@ -51,19 +51,20 @@ def _check(q, k, v, bias, mask, scale) -> None:
                          f"{q.shape[2]} heads, got {tuple(k.shape)}")
     if v.shape != k.shape:
         raise ValueError(f"v must have k's shape {tuple(k.shape)}, got {tuple(v.shape)}")
-    (B, U, H), V = q.shape[:3], k.shape[1]
-    if bias is not None and tuple(bias.shape) not in ((B, H, U, V), (1, H, U, V)):
+    (B, U, H), V, dtype, device = q.shape[:3], k.shape[1], q.dtype, q.device
+    if bias is not None and bias.shape not in ((B, H, U, V), (1, H, U, V)):
         raise ValueError(f"bias must have shape {(B, H, U, V)} or {(1, H, U, V)}, got {tuple(bias.shape)}")
     for name, t in (("k", k), ("v", v), ("bias", bias)):
-        if t is not None and t.dtype != q.dtype:
-            raise ValueError(f"{name} must be {q.dtype} like q, got {t.dtype}")
-    if mask is not None and mask.dtype != torch.bool:
-        raise ValueError(f"mask must be bool, got {mask.dtype}")
-    if mask is not None and tuple(mask.shape) != (B, V):
-        raise ValueError(f"mask must have shape {(B, V)}, got {tuple(mask.shape)}")
-    for name, t in (("k", k), ("v", v), ("bias", bias), ("mask", mask)):
-        if t is not None and t.device != q.device:
-            raise ValueError(f"{name} is on {t.device}, q on {q.device}")
+        if t is not None and (t.dtype is not dtype or t.device != device):
+            raise ValueError(f"{name} must be {dtype} like q, got {t.dtype}" if t.dtype is not dtype else
+                             f"{name} is on {t.device}, q on {device}")
+    if mask is not None:
+        if mask.dtype is not torch.bool:
+            raise ValueError(f"mask must be bool, got {mask.dtype}")
+        if mask.shape != (B, V):
+            raise ValueError(f"mask must have shape {(B, V)}, got {tuple(mask.shape)}")
+        if mask.device != device:
+            raise ValueError(f"mask is on {mask.device}, q on {device}")
     if scale is not None and not 0 < scale < 3e38:
         raise ValueError(f"scale must be positive, got {scale}")
 
@@ -101,7 +102,8 @@ def cross_attention(
     tensors = (q, k, v, bias)
     if not q.is_cuda or q.dtype not in _KERNEL_DTYPES or not _hip.supports(q, k) or _ops.carries_tangent(*tensors):
         return cross_attention_torch(q, k, v, bias, mask, scale)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                    or (bias is not None and bias.requires_grad)):
         return _CrossAttentionHip.apply(q, k, v, bias, mask, scale)
     if _ops.eager_ok(q, k, v, bias, mask):
         precision = _precision.matmul_precision(fp32_operands=q.dtype == torch.float32)

@@ -44,9 +44,12 @@ def _args(q, k, q_pos, k_pos, q_weight, k_weight, eps, frequencies, interleaved,
     qp = kp = qs = ks = 0
     pos_bytes = 4
     if q_pos is not None:
+        shared = k_pos is q_pos
         q_pos, qs = _pos(q_pos)
         qp, pos_bytes = q_pos.data_ptr(), q_pos.element_size()
-    if k_pos is not None:
+        if shared:
+            k_pos, kp, ks = q_pos, qp, qs
+    if k_pos is not None and not kp:
         k_pos, ks = _pos(k_pos)
         kp, pos_bytes = k_pos.data_ptr(), k_pos.element_size()
     qw = kw = 0
@@ -58,14 +61,13 @@ def _args(q, k, q_pos, k_pos, q_weight, k_weight, eps, frequencies, interleaved,
         k_weight = k_weight.contiguous()
         kw, param = k_weight.data_ptr(), _lib.DTYPE_CODE[k_weight.dtype]
     host = _host(frequencies)
-    dq, dk = dys
+    (dq, dk), (oq, ok) = dys, outs
     a = _lib.QkRotaryArgs()
     _lib.pack_qk_rotary(
         a, 0, q.data_ptr(), k.data_ptr(), 0 if dq is None else dq.data_ptr(), 0 if dk is None else dk.data_ptr(), qw, kw, qp,
-        kp, 0 if outs[0] is None else outs[0].data_ptr(), 0 if outs[1] is None else outs[1].data_ptr(), 0, 0,
-        ctypes.addressof(host), 0, B, U, V, H, Hk, D, 2 * len(frequencies), *q.stride()[:3], *k.stride()[:3],
-        *((0, 0, 0) if dq is None else dq.stride()[:3]), *((0, 0, 0) if dk is None else dk.stride()[:3]), qs, ks, 1, 1,
-        0.0 if eps is None else eps, eps is not None, interleaved, pos_bytes, dtype, param)
+        kp, 0 if oq is None else oq.data_ptr(), 0 if ok is None else ok.data_ptr(), 0, 0, ctypes.addressof(host), 0, B, U, V,
+        H, Hk, D, 2 * len(frequencies), *q.stride()[:3], *k.stride()[:3], *((0, 0, 0) if dq is None else dq.stride()[:3]),
+        *((0, 0, 0) if dk is None else dk.stride()[:3]), qs, ks, 1, 1, 0.0 if eps is None else eps, eps is not None, interleaved, pos_bytes, dtype, param)
     return a, (q_pos, k_pos, q_weight, k_weight, host)
 
 

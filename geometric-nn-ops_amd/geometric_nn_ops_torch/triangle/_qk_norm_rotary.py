@@ -55,29 +55,30 @@ def _check(q, k, q_pos, k_pos, q_weight, k_weight, eps) -> None:
                          f"{tuple(q.shape)} and {tuple(k.shape)}")
     if k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3] or not q.shape[3]:
         raise ValueError(f"k must have q's batch and head dim {(q.shape[0], q.shape[3])}, got {tuple(k.shape)}")
-    if k.dtype != q.dtype or k.device != q.device:
-        raise ValueError(f"k must be {q.dtype} on {q.device} like q, got {k.dtype} on {k.device}")
+    dtype, device, d = q.dtype, q.device, q.shape[3]
+    if k.dtype is not dtype or k.device != device:
+        raise ValueError(f"k must be {dtype} on {device} like q, got {k.dtype} on {k.device}")
     for name, t, x in (("q_pos", q_pos, q), ("k_pos", k_pos, k)):
-        if t is None:
+        if t is None or (t is q_pos and name == "k_pos" and k.shape[1] == q.shape[1]):
             continue
         if t.dtype not in _POSITION_DTYPES:
             raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
-        if t.dim() not in (1, 2) or t.shape[-1] != x.shape[1] or (t.dim() == 2 and t.shape[0] not in (1, x.shape[0])):
-            raise ValueError(f"{name} must have shape [{x.shape[1]}] or [{x.shape[0]}, {x.shape[1]}], got "
-                             f"{tuple(t.shape)}")
-        if t.device != q.device:
-            raise ValueError(f"{name} is on {t.device}, q on {q.device}")
+        b, n = x.shape[:2]
+        if t.shape not in ((b, n), (n,), (1, n)):
+            raise ValueError(f"{name} must have shape [{n}] or [{b}, {n}], got {tuple(t.shape)}")
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, q on {device}")
     for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
         if t is None:
             continue
         if eps is None:
             raise ValueError(f"{name} goes with a norm: eps must not be None")
-        if tuple(t.shape) != (q.shape[3],):
-            raise ValueError(f"{name} must have shape {(q.shape[3],)}, got {tuple(t.shape)}")
-        if t.dtype not in (q.dtype, torch.float32):
-            raise ValueError(f"{name} must be {q.dtype} like q, or torch.float32, got {t.dtype}")
-        if t.device != q.device:
-            raise ValueError(f"{name} is on {t.device}, q on {q.device}")
+        if t.shape != (d,):
+            raise ValueError(f"{name} must have shape {(d,)}, got {tuple(t.shape)}")
+        if t.dtype is not dtype and t.dtype is not torch.float32:
+            raise ValueError(f"{name} must be {dtype} like q, or torch.float32, got {t.dtype}")
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, q on {device}")
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         raise ValueError(f"q_weight and k_weight must have one dtype, got {q_weight.dtype} and {k_weight.dtype}")
 
@@ -137,7 +138,10 @@ def qk_norm_rotary(
         if not base > 0:
             raise ValueError(f"base must be positive, got {base}")
         how = _frequencies(base, r)
-    q_pos, k_pos = (t if t is None or t.dim() == 2 else t[None] for t in (q_pos, k_pos))
+    if q_pos is not None and q_pos.dim() == 1:
+        q_pos = q_pos[None]
+    if k_pos is not None and k_pos.dim() == 1:
+        k_pos = k_pos[None]
     if q_pos is not None and k_pos is not None and q_pos.dtype != k_pos.dtype:
         q_pos, k_pos = q_pos.to(torch.int64), k_pos.to(torch.int64)
     args = (q, k, q_pos, k_pos, q_weight, k_weight)
@@ -146,7 +150,8 @@ def qk_norm_rotary(
     if (not q.is_cuda or q.dtype not in _KERNEL_DTYPES or not _hip.supports(q, k, 2 * len(how[1]))
             or _ops.carries_tangent(*tensors)):
         return qk_norm_rotary_torch(*args, *how)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad
+                                    or any(t is not None and t.requires_grad for t in (q_weight, k_weight))):
         return _QkNormRotaryHip.apply(*args, how)
     if _ops.eager_ok(*args):
         return _hip.qk_norm_rotary_hip(*args, *how)
