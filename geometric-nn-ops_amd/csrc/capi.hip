@@ -766,6 +766,12 @@ int gnn_qk_rotary_bwd(const gnn_qk_rotary_args* args, void* stream) {
 }
 
 extern "C++" {
+// Whether the kernels' 32-bit offsets reach 64 rows of a product, tokens of `group` heads each
+static bool within_reach(const int64_t* stride, int64_t tokens, int64_t group, size_t element) {
+  const int64_t most = ((int64_t)1 << 31) / (int64_t)element, token = tokens > 1 ? stride[1] : 0;
+  const int64_t head = group > 1 ? stride[2] : 0;
+  return token >= 0 && token < most / 64 && head >= 0 && head < most / group && 64 * token + (group - 1) * head < most;
+}
 // Shapes and types that the attention's two directions share
 template <typename Args>
 static int check_cross_attn(const Args* args) {
@@ -785,6 +791,8 @@ static int check_cross_attn(const Args* args) {
   const size_t e = a.dtype == GNN_F32 ? 4 : 2;
   if (!aligned(a.q, e) || !aligned(a.k, e) || !aligned(a.v, e) || !aligned(a.bias, e) || !aligned(a.stats, 4))
     return set_error(GNN_ERR_ARG, "cross_attention: tensors must be aligned to their elements");
+  if (!within_reach(a.q_stride, a.U, a.H / a.Hk, e) || !within_reach(a.k_stride, a.V, 1, e) || !within_reach(a.v_stride, a.V, 1, e))
+    return set_error(GNN_ERR_UNSUPPORTED, "cross_attention: 64 tokens must span less than 2^31 bytes");
   return GNN_OK;
 }
 }  // extern "C++"
@@ -817,6 +825,8 @@ int gnn_cross_attn_bwd(const gnn_cross_attn_bwd_args* args, void* stream) {
   if (!aligned(a.o, e) || !aligned(a.dout, e) || !aligned(a.dbias, e) || !aligned(a.dq, 16) || !aligned(a.dk, 16) ||
       !aligned(a.dv, 16) || !aligned(a.workspace, 16))
     return set_error(GNN_ERR_ARG, "cross_attention backward: o, dout and dbias must be aligned to their elements, dq, dk, dv and the workspace to 16 bytes");
+  if (!within_reach(a.o_stride, a.U, a.H / a.Hk, e) || !within_reach(a.do_stride, a.U, a.H / a.Hk, e))
+    return set_error(GNN_ERR_UNSUPPORTED, "cross_attention backward: 64 tokens must span less than 2^31 bytes");
   int rc = cross_attn_bwd(a, (hipStream_t)stream);
   if (rc < 0) return rc;
   return hip_status((hipError_t)rc, "cross_attention backward");

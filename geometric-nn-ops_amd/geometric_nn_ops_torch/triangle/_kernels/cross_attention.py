@@ -8,6 +8,7 @@ import torch
 from ... import _lib
 
 MAX_HEAD_DIM = 128
+_FAR = 1 << 31  # bytes
 
 
 def supports(q, k) -> bool:
@@ -18,13 +19,17 @@ def supports(q, k) -> bool:
     # rows, keys and workgroups are numbered in 31 bits
     (V, Hk) = k.shape[1:3]
     row_blocks, key_blocks = Hk * ((U * H // Hk + 127) // 128), Hk * ((V + 127) // 128)
-    return (B * U * H < 1 << 30 and V <= 1 << 29 and B * max(row_blocks, key_blocks) < 1 << 30
+    return (H * D < 1 << 22 and B * U * H < 1 << 30 and V <= 1 << 29 and B * max(row_blocks, key_blocks) < 1 << 30
             and row_blocks * ((V + 63) // 64) < 1 << 31)
 
 
-def _heads(t):
-    """Unit stride over the head dim, the other strides as they are."""
-    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+def _heads(t, group=1):
+    """Unit stride over the head dim, the other strides as they are; a copy too where 64 rows of one product, tokens of
+    ``group`` heads each, lie 2 GiB apart: the kernels count them in 32 bits."""
+    s = t.stride()
+    if s[3] == 1 and 64 * s[1] + (group - 1) * s[2] < _FAR // t.element_size():
+        return t
+    return t.contiguous()
 
 
 def _bias(t, batch):
@@ -46,7 +51,7 @@ def cross_attention_hip(q, k, v, bias, mask, scale, *, precision, keep=False):
     if not out.numel() or not V:
         out.zero_()
         return (out, stats) if keep else out
-    q, k, v = _heads(q), _heads(k), _heads(v)
+    q, k, v = _heads(q, H // Hk), _heads(k), _heads(v)
     bias, bs = _bias(bias, B)
     a = _lib.CrossAttnArgs()
     _lib.pack_cross_attn(
@@ -73,7 +78,8 @@ def cross_attention_bwd_hip(q, k, v, bias, mask, out, stats, dout, scale, *, pre
             if t is not None:
                 t.zero_()
         return dq, dk, dv, dbias
-    q, k, v, out, dout = (_heads(t) for t in (q, k, v, out, dout))
+    k, v = _heads(k), _heads(v)
+    q, out, dout = (_heads(t, H // Hk) for t in (q, out, dout))
     stats = stats.contiguous()  # in whatever layout saved-tensor hooks return it
     bias, bs = _bias(bias, B)
     a = _lib.CrossAttnBwdArgs()

@@ -834,6 +834,7 @@ int gnn_qk_rotary_bwd(const gnn_qk_rotary_args* args, void* stream);
  * stride over D (a multiple of 8 up to 128), any alignment of their elements; o: dense [B,U,H,D], 16-byte aligned.
  * bias: strides of batch (0 where one goes with every sequence), head and query, unit stride over the keys, or NULL;
  * mask: bytes [B,V] with strides, nonzero = keep, or NULL: what masked keys hold, in bias, k or v, has no effect.
+ * 64 tokens of q, k, v (and o, dout below) span less than 2^31 bytes.
  * scale is positive. stats: fp32 [B,H,U,2], written where not NULL, what the backward needs of each row's sum (a
  * reference maximum, +inf where no key is kept, and the log2 of the sum). workspace: gnn_cross_attn_workspace_bytes(args) bytes, 16-byte aligned (NULL when 0), used during the call.
  * The reference's attention has one length and as many key heads as query heads (triangle/_triattn.py:23-106). */

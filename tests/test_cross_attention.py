@@ -126,6 +126,19 @@ def test_what_the_kernels_take():
     for d in (4, 12, 136, 256):
         assert not _hip.supports(t(1, 1, 1, d), t(1, 1, 1, d))
     assert not _hip.supports(t(1, 1, 1, 8), t(1, 1 << 30, 1, 8))
+    assert not _hip.supports(t(1, 1, 1 << 16, 64), t(1, 1, 1, 64))
+
+
+def test_tokens_far_apart_are_copied():
+    def t(shape, stride, dtype=torch.bfloat16):
+        return torch.empty_strided(shape, stride, dtype=dtype, device="meta")
+
+    near = (2, 9, 4, 64), (1 << 40, (1 << 24) - 1, 64, 1)
+    far = (2, 9, 4, 64), (1 << 40, 1 << 24, 64, 1)
+    assert _hip._heads(t(*near)).stride() == near[1]
+    assert _hip._heads(t(*far)).is_contiguous() and _hip._heads(t(*near, torch.float32)).is_contiguous()
+    turned = (2, 9, 4, 64), (1 << 40, 64, 1 << 30, 1)  # heads before tokens: apart only where rows count them
+    assert _hip._heads(t(*turned)).stride() == turned[1] and _hip._heads(t(*turned), 2).is_contiguous()
 
 
 @pytest.mark.parametrize("cls,name", [(_lib.CrossAttnArgs, "gnn_cross_attn_fwd"), (_lib.CrossAttnBwdArgs, "gnn_cross_attn_bwd")])
@@ -161,7 +174,14 @@ def test_argument_errors(cls, name):
     refused(b"required")
     a.k = 4097
     refused(b"aligned")
-    a.k, a.o = 4096, 4096
+    a.k = 4096
+    for field, at, far in (("q", 1, 1 << 24), ("k", 1, 1 << 24), ("v", 1, -1), ("q", 2, 1 << 29), ("q", 1, 1 << 62)):
+        strides = getattr(a, field + "_stride")
+        strides[at] = far
+        refused(b"2^31", _lib.GNN_ERR_UNSUPPORTED)
+        assert size(ctypes.byref(a)) == 0
+        strides[at] = 0
+    a.o = 4096
     if cls is _lib.CrossAttnArgs:
         a.o = 4104
         refused(b"16-byte")
@@ -179,6 +199,10 @@ def test_argument_errors(cls, name):
     a.bias_stride[0], a.dv = 0, 4104
     refused(b"16 bytes")
     a.dv = 4096
+    for strides in (a.o_stride, a.do_stride):
+        strides[1] = 1 << 24
+        refused(b"2^31", _lib.GNN_ERR_UNSUPPORTED)
+        strides[1] = 0
     assert size(ctypes.byref(a)) >= 4 * 6 * 4
     refused(b"workspace", _lib.GNN_ERR_WORKSPACE)
 
