@@ -803,8 +803,8 @@ size_t gnn_cross_attn_workspace_bytes(const gnn_cross_attn_args* args) {
 
 int gnn_cross_attn_fwd(const gnn_cross_attn_args* args, void* stream) {
   if (int rc = check_cross_attn(args)) return rc;
-  if (!args->o || !aligned(args->o, 16) || !aligned(args->workspace, 16))
-    return set_error(GNN_ERR_ARG, "cross_attention: o is required, o and the workspace 16-byte aligned");
+  if (!args->o || !aligned(args->o, 16) || !aligned(args->o_low, 16) || !aligned(args->workspace, 16))
+    return set_error(GNN_ERR_ARG, "cross_attention: o is required, o, o_low and the workspace 16-byte aligned");
   int rc = cross_attn_fwd(*args, (hipStream_t)stream);
   if (rc < 0) return rc;
   return hip_status((hipError_t)rc, "cross_attention");
@@ -822,7 +822,7 @@ int gnn_cross_attn_bwd(const gnn_cross_attn_bwd_args* args, void* stream) {
   if (a.shared_bias && a.bias_stride[0] != 0)
     return set_error(GNN_ERR_ARG, "cross_attention backward: a shared bias has batch stride 0");
   const size_t e = a.dtype == GNN_F32 ? 4 : 2;
-  if (!aligned(a.o, e) || !aligned(a.dout, e) || !aligned(a.dbias, e) || !aligned(a.dq, 16) || !aligned(a.dk, 16) ||
+  if (!aligned(a.o, e) || !aligned(a.o_low, e) || !aligned(a.dout, e) || !aligned(a.dbias, e) || !aligned(a.dq, 16) || !aligned(a.dk, 16) ||
       !aligned(a.dv, 16) || !aligned(a.workspace, 16))
     return set_error(GNN_ERR_ARG, "cross_attention backward: o, dout and dbias must be aligned to their elements, dq, dk, dv and the workspace to 16 bytes");
   if (!within_reach(a.o_stride, a.U, a.H / a.Hk, e) || !within_reach(a.do_stride, a.U, a.H / a.Hk, e))

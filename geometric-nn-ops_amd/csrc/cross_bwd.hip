@@ -40,6 +40,7 @@ struct BwdArgs {
   const void* k;
   const void* v;
   const void* o;
+  const void* o_low;  // dense, or NULL
   const void* dout;
   const void* bias;
   const uint8_t* mask;
@@ -132,8 +133,9 @@ __global__ __launch_bounds__(NT) void cross_delta_kernel(const BwdArgs a) {
   const int64_t bu = head / s.H, b = bu / s.U, u = bu - b * s.U;
   float sum = 0.f;
   if (d < s.D) {
-    const f32x8 x = TypeOps<T>::to_f32(load8_at((const T*)a.o + b * a.os[0] + u * a.os[1] + h * a.os[2] + d)) *
-                    TypeOps<T>::to_f32(load8_at((const T*)a.dout + b * a.ds[0] + u * a.ds[1] + h * a.ds[2] + d));
+    f32x8 o = TypeOps<T>::to_f32(load8_at((const T*)a.o + b * a.os[0] + u * a.os[1] + h * a.os[2] + d));
+    if (a.o_low) o += TypeOps<T>::to_f32(load8_at((const T*)a.o_low + head * s.D + d));
+    const f32x8 x = o * TypeOps<T>::to_f32(load8_at((const T*)a.dout + b * a.ds[0] + u * a.ds[1] + h * a.ds[2] + d));
     sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
   }
 #pragma unroll
@@ -155,7 +157,8 @@ struct Lds {
 };
 
 // -------------------------------------------------------------------------------------- dQ
-template <typename T, int PREC, int DP, bool BIAS>
+// FINER: dS in two parts
+template <typename T, int PREC, int DP, bool BIAS, bool FINER>
 __device__ __forceinline__ void dq_block(const BwdArgs& a, Lds<T, DP>& lds, uint32_t block) {
   typedef RowTile<T, DP> Tile;
   typedef typename TypeOps<T>::V8 V8;
@@ -237,8 +240,14 @@ __device__ __forceinline__ void dq_block(const BwdArgs& a, Lds<T, DP>& lds, uint
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         const V8 f = acc_frag<T>(ds, kk);
+        V8 low;
+        if constexpr (FINER) low = low_frag<T>(ds, kk, f);
 #pragma unroll
-        for (int cc = 0; cc < DP / 32; ++cc) Mma<T, PREC>::step(dq[cc], Tile::turned8(ks, 32 * sub, kk, cc, lane), f);
+        for (int cc = 0; cc < DP / 32; ++cc) {
+          const V8 kf = Tile::turned8(ks, 32 * sub, kk, cc, lane);
+          Mma<T, PREC>::step(dq[cc], kf, f);
+          if constexpr (FINER) Mma<T, PREC>::step(dq[cc], kf, low);
+        }
       }
       if constexpr (BIAS) {
         if (dbias && row_ok)
@@ -482,7 +491,7 @@ __device__ __forceinline__ void dbias_block(const BwdArgs& a, Lds<T, DP>& lds, u
 }
 
 // The workgroups of DKDV, then those of dQ, then those of a shared dbias
-template <typename T, int PREC, int DP, bool BIAS, bool DKDV, bool DQ>
+template <typename T, int PREC, int DP, bool BIAS, bool DKDV, bool DQ, bool FINER>
 __global__ __launch_bounds__(NT, sizeof(T) == 4 || (DKDV && DP > 64) ? 1 : 2) void cross_bwd_kernel(const BwdArgs a) {
   __shared__ Lds<T, DP> lds;
   uint32_t block = blockIdx.x;
@@ -491,7 +500,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 || (DKDV && DP > 64) ? 1 : 2) vo
     block -= a.k_blocks;
   }
   if constexpr (DQ) {
-    if (!BIAS || block < a.q_blocks) return dq_block<T, PREC, DP, BIAS>(a, lds, block);
+    if (!BIAS || block < a.q_blocks) return dq_block<T, PREC, DP, BIAS, FINER>(a, lds, block);
     if constexpr (BIAS) dbias_block<T, PREC, DP>(a, lds, block - a.q_blocks);
   }
 }
@@ -505,9 +514,10 @@ __global__ __launch_bounds__(NT) void zeros_kernel(E* p, int64_t n) {
 struct Plan {
   int64_t q_blocks, q_splits, q_tiles, k_blocks, k_splits, k_tiles;
 };
-// One workgroup of 4 waves a CU in fp32 and for the products of more than 64 columns, two otherwise. Where those of dQ
-// and of dK, dV are fewer than that, each is split so that every workgroup has about an equal part of all tiles: a tile
-// of dK and dV costs four products, one of dQ three.
+// One workgroup of 4 waves a CU in fp32 and for the products of more than 64 columns, two otherwise. Those of dQ
+// and of dK, dV are split so that none has more than about an equal part of all tiles (the queries of a few tokens walk
+// over all keys, while each of many workgroups of dK and dV has one tile: 2 x 9 x 4391, 20 heads of 128 over 10, fp32:
+// 178 us, 985 with dQ in one walk): a tile of dK and dV costs four products, one of dQ three.
 Plan plan(const gnn_cross_attn_bwd_args& g) {
   Plan p{};
   const int KT = tile_of(g.dtype == GNN_F32, (int)g.D);
@@ -518,12 +528,12 @@ Plan plan(const gnn_cross_attn_bwd_args& g) {
   auto divide = [](int64_t tiles, int64_t most, int64_t& splits, int64_t& each) {
     splits = (tiles + most - 1) / most, each = (tiles + splits - 1) / splits;
   };
-  int64_t part = qb + kb < places ? (3 * qb * qt + 4 * kb * kt + places - 1) / places : 4 * std::max(qt, kt);
+  int64_t part = (3 * qb * qt + 4 * kb * kt + places - 1) / places;
   const int64_t least = g.dtype == GNN_F32 ? 2 : 4;  // tiles a workgroup, beside its start and its sums
   for (;; part += part / 16 + 1) {  // until rounding up leaves no second round
     divide(qt, std::max(least, (part + 2) / 3), p.q_splits, p.q_tiles);
     divide(kt, std::max(least, (part + 3) / 4), p.k_splits, p.k_tiles);
-    if (qb * p.q_splits + kb * p.k_splits <= places || (p.q_splits == 1 && p.k_splits == 1)) break;
+    if (qb + kb >= places || qb * p.q_splits + kb * p.k_splits <= places || (p.q_splits == 1 && p.k_splits == 1)) break;
   }
   p.q_blocks = qb * p.q_splits;
   p.k_blocks = kb * p.k_splits;
@@ -542,12 +552,27 @@ int launch(const BwdArgs& a, hipStream_t st) {
   constexpr int LOG = DP <= 32 ? 2 : DP <= 64 ? 3 : 4;
   if (int rc = delta<T, LOG>(a, st)) return rc;
   const uint32_t rest = a.q_blocks + a.b_blocks;
-  if constexpr (DP <= 64 || sizeof(T) == 4) {
-    hipLaunchKernelGGL((cross_bwd_kernel<T, PREC, DP, BIAS, true, true>), dim3(a.k_blocks + rest), dim3(NT), 0, st, a);
+  auto go = [&](auto finer) {
+    constexpr bool FINER = decltype(finer)::value;
+    if constexpr (DP <= 64 || sizeof(T) == 4) {
+      hipLaunchKernelGGL((cross_bwd_kernel<T, PREC, DP, BIAS, true, true, FINER>), dim3(a.k_blocks + rest), dim3(NT), 0, st, a);
+    } else {
+      if (a.k_blocks)
+        hipLaunchKernelGGL((cross_bwd_kernel<T, PREC, DP, BIAS, true, false, false>), dim3(a.k_blocks), dim3(NT), 0, st, a);
+      hipLaunchKernelGGL((cross_bwd_kernel<T, PREC, DP, BIAS, false, true, FINER>), dim3(rest), dim3(NT), 0, st, a);
+    }
+  };
+  // dS in two parts: few keys, and heads so short that a query's pull on its keys shows in their sum: |K|^2 is D + 1 where
+  // their spread is D. A variant of its own: a branch among the products cost 4 x 2048 x 1400 10% (209 us, 190 without).
+  if constexpr (sizeof(T) == 4) {
+    go(std::false_type{});
+  } else if constexpr (DP == 32) {
+    go(std::true_type{});
   } else {
-    if (a.k_blocks)
-      hipLaunchKernelGGL((cross_bwd_kernel<T, PREC, DP, BIAS, true, false>), dim3(a.k_blocks), dim3(NT), 0, st, a);
-    hipLaunchKernelGGL((cross_bwd_kernel<T, PREC, DP, BIAS, false, true>), dim3(rest), dim3(NT), 0, st, a);
+    if (a.s.V <= FINE)
+      go(std::true_type{});
+    else
+      go(std::false_type{});
   }
   return (int)hipGetLastError();
 }
@@ -593,7 +618,7 @@ int cross_attn_bwd(const gnn_cross_attn_bwd_args& g, hipStream_t st) {
     return set_error(GNN_ERR_WORKSPACE, "cross_attention: workspace missing or too small");
   BwdArgs a{};
   a.s = {(int)g.B, (int)g.U, (int)g.V, (int)g.H, (int)g.Hk, (int)(g.H / g.Hk), (int)g.D, (int)(g.U * (g.H / g.Hk))};
-  a.q = g.q, a.k = g.k, a.v = g.v, a.o = g.o, a.dout = g.dout, a.bias = g.bias, a.mask = g.mask, a.stats = g.stats;
+  a.q = g.q, a.k = g.k, a.v = g.v, a.o = g.o, a.o_low = g.o_low, a.dout = g.dout, a.bias = g.bias, a.mask = g.mask, a.stats = g.stats;
   a.dq = g.dq, a.dk = g.dk, a.dv = g.dv, a.dbias = g.dbias;
   for (int i = 0; i < 3; ++i) {
     a.qs[i] = g.q_stride[i], a.ks[i] = g.k_stride[i], a.vs[i] = g.v_stride[i];

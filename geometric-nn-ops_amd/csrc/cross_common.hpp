@@ -13,6 +13,11 @@ namespace cross {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
+// Up to so many keys 16-bit operands made here, p and dS, are multiplied in two parts, 2^-17 exact: few terms cancel, and
+// their roundings do not: of 3 keys, where P (dP - Delta) is a small difference, gradients were off by 2.5 times the one
+// rounding at the end, of 64 and more by 1.4. One tile of keys costs nothing that shows.
+constexpr int FINE = 64;
+
 struct Shape {
   int B, U, V, H, Hk, G, D;
   int rows;  // U G
@@ -259,6 +264,13 @@ __device__ __forceinline__ typename TypeOps<T>::V8 acc_frag(const f32x16& a, int
   const f32x8 x = {a[8 * kk + 0], a[8 * kk + 1], a[8 * kk + 2], a[8 * kk + 3],
                    a[8 * kk + 4], a[8 * kk + 5], a[8 * kk + 6], a[8 * kk + 7]};
   return TypeOps<T>::from_f32(x);
+}
+// what its rounding to f left
+template <typename T>
+__device__ __forceinline__ typename TypeOps<T>::V8 low_frag(const f32x16& a, int kk, const typename TypeOps<T>::V8& f) {
+  const f32x8 x = {a[8 * kk + 0], a[8 * kk + 1], a[8 * kk + 2], a[8 * kk + 3],
+                   a[8 * kk + 4], a[8 * kk + 5], a[8 * kk + 6], a[8 * kk + 7]};
+  return TypeOps<T>::from_f32(x - TypeOps<T>::to_f32(f));
 }
 __device__ __forceinline__ void fill(f32x16& a, float x) {
 #pragma unroll

@@ -43,12 +43,14 @@ struct FwdArgs {
   const void* bias;
   const uint8_t* mask;
   void* o;
+  void* o_low;     // dense like o, what o's rounding left; or NULL
   float* stats;    // [B][H][U][2]: the reference maximum (+inf where no key is kept) and the log2 of the sum; or NULL
   float* part_o;   // [splits][B][U][H][D]
   float* part_ml;  // [splits][B][H][U][2]
   int64_t qs[3], ks[3], vs[3], bs[3], ms[2];
   float scale;  // of the scores: with a bias the caller's, otherwise times log2(e)
   int splits, tiles_per_split;
+  bool fine;  // p in two parts
 };
 
 // WK waves share rows and divide keys (1 or 4); a wave has QW times 32 rows
@@ -67,12 +69,21 @@ struct Cfg {
   static constexpr int WGS = (sizeof(T) == 4 && DP == 128) || (QW == 2 && DP > 64) ? 1 : 2;  // workgroups a CU
 };
 
+template <typename T>
+__device__ __forceinline__ void store_out(const FwdArgs& a, int64_t at, const f32x4& x) {
+  const auto y = TypeOps<T>::from_f32(x);
+  store4((T*)a.o + at, y);
+  if constexpr (sizeof(T) == 2)
+    if (a.o_low) store4((T*)a.o_low + at, TypeOps<T>::from_f32(x - TypeOps<T>::to_f32(y)));
+}
+
 template <typename T, int PREC, int DP, int WK, int QW, bool BIAS>
 __global__ __launch_bounds__(NT, (Cfg<T, DP, WK, QW>::WGS)) void cross_fwd_kernel(const FwdArgs a) {
   typedef Cfg<T, DP, WK, QW> C;
   typedef typename C::KTile KTile;
   typedef typename C::VTile VTile;
   typedef typename TypeOps<T>::V8 V8;
+  constexpr bool FINER = sizeof(T) == 2 && QW == 1;
   __shared__ __align__(16) unsigned char smem[C::LDS];
   __shared__ int found[2];
   const Shape& s = a.s;
@@ -258,6 +269,15 @@ __global__ __launch_bounds__(NT, (Cfg<T, DP, WK, QW>::WGS)) void cross_fwd_kerne
 #pragma unroll
           for (int i = 0; i < QW; ++i) Mma<T, PREC>::step(o[i][cc], vf, p[i][kk]);
         }
+      if constexpr (FINER)
+        if (a.fine)  // uniform; behind the products, not among them: 4096 x 8192, 32 heads of 128, took 582 us then, 563 so
+#pragma unroll
+          for (int kk = 0; kk < 2; ++kk) {
+            const V8 low = low_frag<T>(sc[sub][0], kk, p[0][kk]);
+#pragma unroll
+            for (int cc = 0; cc < DP / 32; ++cc)
+              Mma<T, PREC>::step(o[0][cc], VTile::turned8(vs, r0 + 32 * sub, kk, cc, lane), low);
+          }
     }
     if constexpr (C::NBUF == 1) __syncthreads();
     if (next < t_end) put(C::NBUF == 1 ? 0 : buf ^ 1, next_live);
@@ -327,7 +347,7 @@ __global__ __launch_bounds__(NT, (Cfg<T, DP, WK, QW>::WGS)) void cross_fwd_kerne
         if (a.splits > 1)
           *reinterpret_cast<f32x4*>(a.part_o + split * each + head * s.D + d) = x;
         else
-          store4((T*)a.o + head * s.D + d, TypeOps<T>::from_f32(x));
+          store_out<T>(a, head * s.D + d, x);
       }
     }
   }
@@ -368,7 +388,7 @@ __global__ __launch_bounds__(NT) void cross_join_kernel(const FwdArgs a) {
     }
   }
   const float inv = sum > 0.f ? 1.0f / sum : sum == 0.f ? 0.f : sum;
-  store4((T*)a.o + head * s.D + d, TypeOps<T>::from_f32(o * inv));
+  store_out<T>(a, head * s.D + d, o * inv);
   if (a.stats && d == 0)
     a.stats[2 * stat] = sum == 0.f ? INFINITY : m, a.stats[2 * stat + 1] = sum == 0.f ? 0.f : log2f(sum);
 }
@@ -382,7 +402,7 @@ Plan plan(const gnn_cross_attn_args& g) {
   Plan p{};
   const int64_t rows = g.U * (g.H / g.Hk);
   p.few = rows <= 32;
-  p.wide = g.dtype != GNN_F32 && g.D <= 64 && (rows + 255) / 256 * g.B * g.Hk >= 2 * (int64_t)compute_units();
+  p.wide = g.dtype != GNN_F32 && g.D <= 64 && g.V > FINE && (rows + 255) / 256 * g.B * g.Hk >= 2 * (int64_t)compute_units();
   const int64_t per = p.wide ? 256 : 128, base = (p.few ? 1 : (rows + per - 1) / per) * g.B * g.Hk, kt = p.few ? 128 : 64, tiles = (g.V + kt - 1) / kt;
   // two workgroups a CU where the keys allow it, of 4 tiles at least (2 in fp32, whose products take longer)
   const int64_t want = std::max<int64_t>(1, 2 * (int64_t)compute_units() / base);
@@ -449,11 +469,12 @@ int cross_attn_fwd(const gnn_cross_attn_args& g, hipStream_t st) {
     return set_error(GNN_ERR_UNSUPPORTED, "cross_attention: grid too large");
   FwdArgs a{};
   a.s = {(int)g.B, (int)g.U, (int)g.V, (int)g.H, (int)g.Hk, (int)(g.H / g.Hk), (int)g.D, (int)(g.U * (g.H / g.Hk))};
-  a.q = g.q, a.k = g.k, a.v = g.v, a.bias = g.bias, a.mask = g.mask, a.o = g.o, a.stats = g.stats;
+  a.q = g.q, a.k = g.k, a.v = g.v, a.bias = g.bias, a.mask = g.mask, a.o = g.o, a.o_low = g.o_low, a.stats = g.stats;
   for (int i = 0; i < 3; ++i) a.qs[i] = g.q_stride[i], a.ks[i] = g.k_stride[i], a.vs[i] = g.v_stride[i], a.bs[i] = g.bias_stride[i];
   for (int i = 0; i < 2; ++i) a.ms[i] = g.mask_stride[i];
   a.scale = g.bias ? g.scale : g.scale * LOG2E;
   if (g.V == 1) a.bias = nullptr, a.scale = g.scale * LOG2E;
+  a.fine = g.V <= FINE;
   a.splits = (int)p.splits, a.tiles_per_split = (int)p.tiles_per_split;
   if (p.splits > 1) {
     if (!g.workspace || g.workspace_bytes < cross_attn_workspace_bytes(g))

@@ -695,6 +695,7 @@ class CrossAttnArgs(ctypes.Structure):
         ("bias", ctypes.c_void_p),
         ("mask", ctypes.c_void_p),
         ("o", ctypes.c_void_p),
+        ("o_low", ctypes.c_void_p),
         ("stats", ctypes.c_void_p),
         ("workspace", ctypes.c_void_p),
         ("workspace_bytes", ctypes.c_size_t),
@@ -727,6 +728,7 @@ class CrossAttnBwdArgs(ctypes.Structure):
         ("k", ctypes.c_void_p),
         ("v", ctypes.c_void_p),
         ("o", ctypes.c_void_p),
+        ("o_low", ctypes.c_void_p),
         ("dout", ctypes.c_void_p),
         ("bias", ctypes.c_void_p),
         ("mask", ctypes.c_void_p),

@@ -23,15 +23,15 @@ _KERNEL_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 class _CrossAttentionHip(torch.autograd.Function):
-    """HIP forward that keeps its output and each row's sum, HIP backward that forms the probabilities again with the
+    """HIP forward that keeps its output, what the rounding left of it, and each row's sum, HIP backward that forms the probabilities again with the
     precision that the forward resolved. The backward records no graph: a second derivative raises."""
 
     @staticmethod
     def forward(ctx, q, k, v, bias, mask, scale):
         ctx.precision = _precision.matmul_precision(fp32_operands=q.dtype == torch.float32)
         ctx.scale = scale
-        out, stats = _hip.cross_attention_hip(q, k, v, bias, mask, scale, precision=ctx.precision, keep=True)
-        ctx.save_for_backward(q, k, v, bias, mask, out, stats)
+        out, low, stats = _hip.cross_attention_hip(q, k, v, bias, mask, scale, precision=ctx.precision, keep=True)
+        ctx.save_for_backward(q, k, v, bias, mask, out, low, stats)
         return out
 
     @staticmethod

@@ -43,20 +43,22 @@ def _bias(t, batch):
 
 
 def cross_attention_hip(q, k, v, bias, mask, scale, *, precision, keep=False):
-    """``[B, U, H, D]``, fresh and contiguous; with ``keep`` ``(out, stats)`` with what the backward needs of
-    the rows' sums, fp32 ``[B, H, U, 2]``."""
+    """``[B, U, H, D]``, fresh and contiguous; with ``keep`` ``(out, low, stats)``: what the rounding of a
+    16-bit output left (``None`` in fp32) and what the backward needs of the rows' sums, fp32 ``[B, H, U, 2]``."""
     (B, U, H, D), (V, Hk) = q.shape, k.shape[1:3]
     out = torch.empty((B, U, H, D), device=q.device, dtype=q.dtype)
+    low = torch.empty_like(out) if keep and q.dtype is not torch.float32 else None
     stats = torch.empty((B, H, U, 2), device=q.device, dtype=torch.float32) if keep else None
     if not out.numel() or not V:
         out.zero_()
-        return (out, stats) if keep else out
+        return (out, low, stats) if keep else out
     q, k, v = _heads(q, H // Hk), _heads(k), _heads(v)
     bias, bs = _bias(bias, B)
     a = _lib.CrossAttnArgs()
     _lib.pack_cross_attn(
         a, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if bias is None else bias.data_ptr(),
-        0 if mask is None else mask.data_ptr(), out.data_ptr(), 0 if stats is None else stats.data_ptr(), 0, 0, B, U, V, H, Hk, D,
+        0 if mask is None else mask.data_ptr(), out.data_ptr(), 0 if low is None else low.data_ptr(),
+        0 if stats is None else stats.data_ptr(), 0, 0, B, U, V, H, Hk, D,
         *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *bs, *((0, 0) if mask is None else mask.stride()), scale,
         _lib.DTYPE_CODE[q.dtype], _lib.PRECISION_CODE[precision], 0)
     size = (_lib._lib or _lib.load()).gnn_cross_attn_workspace_bytes(ctypes.byref(a))
@@ -64,10 +66,10 @@ def cross_attention_hip(q, k, v, bias, mask, scale, *, precision, keep=False):
         ws = torch.empty(size, device=q.device, dtype=torch.uint8)
         a.workspace, a.workspace_bytes = ws.data_ptr(), size
     _lib.call("gnn_cross_attn_fwd", a, q.device)
-    return (out, stats) if keep else out
+    return (out, low, stats) if keep else out
 
 
-def cross_attention_bwd_hip(q, k, v, bias, mask, out, stats, dout, scale, *, precision, need_kv=True, need_bias=True):
+def cross_attention_bwd_hip(q, k, v, bias, mask, out, low, stats, dout, scale, *, precision, need_kv=True, need_bias=True):
     """``(dq, dk, dv, dbias)``; dk and dv None unless ``need_kv``, dbias unless ``need_bias``."""
     (B, U, H, D), (V, Hk) = q.shape, k.shape[1:3]
     dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
@@ -80,11 +82,11 @@ def cross_attention_bwd_hip(q, k, v, bias, mask, out, stats, dout, scale, *, pre
         return dq, dk, dv, dbias
     k, v = _heads(k), _heads(v)
     q, out, dout = (_heads(t, H // Hk) for t in (q, out, dout))
-    stats = stats.contiguous()  # in whatever layout saved-tensor hooks return it
+    stats, low = stats.contiguous(), None if low is None else low.contiguous()  # in whatever layout saved-tensor hooks return them
     bias, bs = _bias(bias, B)
     a = _lib.CrossAttnBwdArgs()
     _lib.pack_cross_attn_bwd(
-        a, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(),
+        a, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if low is None else low.data_ptr(), dout.data_ptr(),
         0 if bias is None else bias.data_ptr(), 0 if mask is None else mask.data_ptr(), stats.data_ptr(), dq.data_ptr(),
         0 if dk is None else dk.data_ptr(), 0 if dv is None else dv.data_ptr(), 0 if dbias is None else dbias.data_ptr(), 0,
         0, B, U, V, H, Hk, D, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *dout.stride()[:3], *bs,

@@ -835,7 +835,8 @@ int gnn_qk_rotary_bwd(const gnn_qk_rotary_args* args, void* stream);
  * bias: strides of batch (0 where one goes with every sequence), head and query, unit stride over the keys, or NULL;
  * mask: bytes [B,V] with strides, nonzero = keep, or NULL: what masked keys hold, in bias, k or v, has no effect.
  * 64 tokens of q, k, v (and o, dout below) span less than 2^31 bytes.
- * scale is positive. stats: fp32 [B,H,U,2], written where not NULL, what the backward needs of each row's sum (a
+ * scale is positive. o_low: dense like o, written where not NULL, what the rounding of 16-bit outputs left (of fp32
+ * ones nothing is: NULL). stats: fp32 [B,H,U,2], written where not NULL, what the backward needs of each row's sum (a
  * reference maximum, +inf where no key is kept, and the log2 of the sum). workspace: gnn_cross_attn_workspace_bytes(args) bytes, 16-byte aligned (NULL when 0), used during the call.
  * The reference's attention has one length and as many key heads as query heads (triangle/_triattn.py:23-106). */
 typedef struct gnn_cross_attn_args {
@@ -845,6 +846,7 @@ typedef struct gnn_cross_attn_args {
   const void* bias;
   const uint8_t* mask;
   void* o;
+  void* o_low;
   float* stats;
   void* workspace;
   size_t workspace_bytes;
@@ -862,7 +864,8 @@ typedef struct gnn_cross_attn_args {
 size_t gnn_cross_attn_workspace_bytes(const gnn_cross_attn_args* args);
 int gnn_cross_attn_fwd(const gnn_cross_attn_args* args, void* stream);
 
-/* Its backward from the forward's inputs, output o and stats and the output gradient dout (o and dout: strides as q's).
+/* Its backward from the forward's inputs, output o, o_low (or NULL: the row sums
+ * of dO o carry o's rounding then) and stats and the output gradient dout (o and dout: strides as q's).
  * dq, dk, dv: dense like q, k and v, 16-byte aligned; dk and dv both or neither. dbias: dense [B,H,U,V] (any alignment
  * of its elements), with shared_bias (bias_stride[0] is 0 then) [1,H,U,V] summed over the batch; or NULL. */
 typedef struct gnn_cross_attn_bwd_args {
@@ -870,6 +873,7 @@ typedef struct gnn_cross_attn_bwd_args {
   const void* k;
   const void* v;
   const void* o;
+  const void* o_low;
   const void* dout;
   const void* bias;
   const uint8_t* mask;

@@ -185,7 +185,9 @@ def test_argument_errors(cls, name):
     if cls is _lib.CrossAttnArgs:
         a.o = 4104
         refused(b"16-byte")
-        a.o, a.U, a.Hk, a.V = 4096, 1, 1, 1 << 16  # keys split over workgroups
+        a.o, a.o_low = 4096, 4104
+        refused(b"16-byte")
+        a.o_low, a.U, a.Hk, a.V = None, 1, 1, 1 << 16  # keys split over workgroups
         assert size(ctypes.byref(a)) % 4 == 0 and size(ctypes.byref(a)) > 0
         refused(b"workspace", _lib.GNN_ERR_WORKSPACE)
         return

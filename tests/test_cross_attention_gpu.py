@@ -478,3 +478,33 @@ def test_rows_behind_the_output_stay_as_they_were():
         _lib.call("gnn_cross_attn_fwd", a, q.device)
         assert torch.equal(buf[:q.numel()].view_as(q), cross_attention(q, k, val, scale=0.125))
         assert (buf[q.numel():] == 7).all()
+
+
+@pytest.mark.parametrize("v", [2, 5, 33, 64])
+@pytest.mark.parametrize("masked", [False, True])
+def test_few_keys_lose_no_bits(v, masked):
+    """With up to 64 keys P (dP - Delta) is a small difference, whose terms are held to 2^-16 (two parts of 8 bits):
+    P and dS as operands, and o in Delta, which P's two parts enter as well. fp32 arithmetic, E(D) U at most, is below
+    another 2^-16. Three roundings of operands to one part would be off by 2^-8 each."""
+    B, Uq, H, D = 2, 37, 4, 64
+    (q, k, val, _), _, dout = _inputs((B, Uq, v, H, 2, D, 0, False), torch.bfloat16, seed=v)
+    mask = None
+    if masked:
+        mask = torch.ones(B, v, dtype=torch.bool, device=DEV)
+        mask[0, 1:] = False  # one key: no gradient
+        mask[1, v // 2] = False
+    leaves = [t.clone().requires_grad_() for t in (q, k, val)]
+    got = torch.autograd.grad(cross_attention(*leaves, mask=mask), leaves, dout)
+
+    q, k, val, dout = (t.double().transpose(1, 2) for t in (q, k, val, dout))
+    k, val = (t.repeat_interleave(H // 2, 1) for t in (k, val))
+    x = q @ k.transpose(2, 3).contiguous() * D ** -0.5
+    keep = torch.ones(B, v, dtype=torch.bool, device=DEV) if mask is None else mask
+    p = torch.softmax(x.masked_fill(~keep[:, None, None], float("-inf")), -1)
+    dp = dout @ val.transpose(2, 3).contiguous()
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    most = (dout.abs() * (p @ val.abs())).sum(-1, keepdim=True)
+    slack = 2.0 ** -15 * (ds.abs() + p * (dp.abs() + 2 * most)) * D ** -0.5
+    assert_within("dq", got[0].transpose(1, 2), ds @ k * D ** -0.5, slack @ k.abs())
+    if masked:
+        assert (got[0][0].double().abs() <= (slack @ k.abs())[0].transpose(0, 1)).all()
