@@ -393,22 +393,37 @@ __global__ __launch_bounds__(NT) void cross_join_kernel(const FwdArgs a) {
     a.stats[2 * stat] = sum == 0.f ? INFINITY : m, a.stats[2 * stat + 1] = sum == 0.f ? 0.f : log2f(sum);
 }
 
+// Few: up to 32 rows (8 x 1 x 4096, 32 heads of 64 over 8, bf16: 13.2 us, in the other form 19.0).
+// Wide: 64 rows a wave, so that a fragment of K and V serves two products, where the registers hold them: up to 64 columns,
+// with a bias 32 (4 x 2048 x 1400, 16 heads, bf16: of 64 59 us and 67, with a bias 112 and 107; of 32 46 and 47, with a bias
+// 80 and 93; of 128 twice as long), and two workgroups a CU are left (half the batch of 64: 49 and 36).
 struct Plan {
-  bool few;   // up to 32 rows
-  bool wide;  // 64 rows a wave
+  bool few;
+  bool wide;
   int64_t blocks, splits, tiles_per_split;
 };
 Plan plan(const gnn_cross_attn_args& g) {
   Plan p{};
   const int64_t rows = g.U * (g.H / g.Hk);
   p.few = rows <= 32;
-  p.wide = g.dtype != GNN_F32 && g.D <= 64 && g.V > FINE && (rows + 255) / 256 * g.B * g.Hk >= 2 * (int64_t)compute_units();
+  p.wide = g.dtype != GNN_F32 && g.D <= (g.bias ? 32 : 64) && g.V > FINE && (rows + 255) / 256 * g.B * g.Hk >= 2 * (int64_t)compute_units();
   const int64_t per = p.wide ? 256 : 128, base = (p.few ? 1 : (rows + per - 1) / per) * g.B * g.Hk, kt = p.few ? 128 : 64, tiles = (g.V + kt - 1) / kt;
-  // two workgroups a CU where the keys allow it, of 4 tiles at least (2 in fp32, whose products take longer)
-  const int64_t want = std::max<int64_t>(1, 2 * (int64_t)compute_units() / base);
-  const int64_t most = std::max<int64_t>(1, tiles / (g.dtype == GNN_F32 ? 2 : 4));
-  p.tiles_per_split = (tiles + std::min(want, most) - 1) / std::min(want, most);
-  p.splits = (tiles + p.tiles_per_split - 1) / p.tiles_per_split;
+  // The split of the keys that ends first, in us: rounds of workgroups (two a CU; in fp32, which the products bound, one),
+  // each a start and its tiles, and with several splits the second kernel, its launch and each split's sums written and
+  // read. One query of 2048 keys, 2 sequences, 8 heads of 64, bf16: 8.9 us with two tiles a split, with four
+  // 10.6; 300 queries of 8192 keys, 4 heads of 128: 25.2 with eight, with four 28.9.
+  const bool f32 = g.dtype == GNN_F32;
+  const int64_t places = (f32 ? 1 : 2) * (int64_t)compute_units();
+  const double start = 3, tile = f32 ? 3.4 * (g.D <= 64 ? 1 : 2) / (p.few ? 2 : 1) : 0.7, launch = 4;
+  const double sums = 0.1 + (double)g.B * g.U * g.H * g.D * 8 / 5e6;
+  double best = 0;
+  for (int64_t s = 1; s <= std::min<int64_t>(tiles, 256); ++s) {
+    const int64_t each = (tiles + s - 1) / s, splits = (tiles + each - 1) / each;
+    if (splits != s) continue;
+    const double rounds = (double)((base * s + places - 1) / places);
+    const double time = rounds * (start + each * tile) + (s > 1 ? launch + s * sums : 0);
+    if (s == 1 || time < best) best = time, p.splits = s, p.tiles_per_split = each;
+  }
   p.blocks = base * p.splits;
   return p;
 }
@@ -422,7 +437,7 @@ int launch(const FwdArgs& a, const Plan& p, hipStream_t st) {
       hipLaunchKernelGGL((cross_fwd_kernel<T, PREC, DP, 4, 1, BIAS>), grid, blk, 0, st, a);
       return;
     }
-    if constexpr (sizeof(T) == 2 && DP <= 64)
+    if constexpr (sizeof(T) == 2 && DP <= (BIAS ? 32 : 64))
       if (p.wide) {
         hipLaunchKernelGGL((cross_fwd_kernel<T, PREC, DP, 1, 2, BIAS>), grid, blk, 0, st, a);
         return;

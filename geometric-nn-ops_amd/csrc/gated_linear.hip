@@ -166,7 +166,7 @@ int launch(const GatedArgs& a, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
-// ---- few tiles ------------------------------------------------------------------------------
+// ---- few tiles, fp32 ------------------------------------------------------------------------
 // Single tokens and short sequences, as linear_few_kernel: 32 rows x 32 outputs of both products a workgroup, whose
 // 8 waves split the contraction; the partial sums are added in wave order.
 constexpr int GF_NW = 8, GF_NT = 64 * GF_NW, GF_AHEAD = 4;
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(GR_NT, GR_NT / 256) void gated_rows_kernel(const Ga
   float* const bias = (float*)(weight + 2 * 32 * nb * ROWB);
   // LDS row r: output n0 + 32 (r / 64) + tile_output(r % 32) of matrix r / 32 % 2, zeros past I and O
   for (int e0 = wave * 64; e0 < 64 * nb * 2 * KS; e0 += GR_NT) {  // 1 KB an instruction
-    const uint32_t e = e0 + lane, r = e / (2 * KS), c = (e % (2 * KS)) ^ chunk_swizzle<(ROWB < 256 ? ROWB : 256)>(r);
+    const uint32_t e = e0 + lane, r = e / (2 * KS), c = (e % (2 * KS)) ^ chunk_swizzle<ROWB>(r);
     const int n = n0 + 32 * (r / 64) + tile_output(r & 31);
     const T* row = r & 32 ? (const T*)a.wu + (int64_t)n * a.wu_ld : (const T*)a.wg + (int64_t)n * a.wg_ld;
     __builtin_amdgcn_global_load_lds(n < a.O && 8 * (int)c < a.I ? (const void*)(row + 8 * c) : (const void*)zero_chunk,
@@ -288,8 +288,8 @@ __global__ __launch_bounds__(GR_NT, GR_NT / 256) void gated_rows_kernel(const Ga
   const unsigned char* wrow[KS];
 #pragma unroll
   for (int kk = 0; kk < KS; ++kk)
-    wrow[kk] = weight + l32 * ROWB + (((2 * kk + g) ^ chunk_swizzle<(ROWB < 256 ? ROWB : 256)>(l32)) << 4);
-  // rows of 16 steps take 64 registers: theirs are not loaded ahead
+    wrow[kk] = weight + l32 * ROWB + (((2 * kk + g) ^ chunk_swizzle<ROWB>(l32)) << 4);
+  // the backward's rows of 8 steps, beside twice the sums, are not loaded ahead
   constexpr bool AHEAD = KS <= (BWD ? 4 : 8);
   u32x4_t next[KS / 2][2], x[KS / 2][2];
   auto turn_rows = [&]() {
@@ -386,13 +386,15 @@ struct RowsForm {
   int ks, cols, parts;
   size_t lds;
 };
+// Rows of up to 128 inputs: of 256 half as many outputs fit, each workgroup's rows are read by twice as many, and tiles are
+// as fast or faster (147456 x 256 -> 512, bf16: 119 us both, the backward's first kernel 225 here, 202 in tiles).
 RowsForm rows_form(const GatedArgs& a, int bytes) {
   auto rows16 = [](const void* p, int64_t ld) { return ((uintptr_t)p % 16) == 0 && ld % 8 == 0 && ld < (1 << 24); };
-  if (bytes != 2 || a.M < RS_MIN_ROWS || a.I > 256 || a.O % 8 || a.x_ld >= (1 << 24) || !rows16(a.out, a.out_ld) ||
+  if (bytes != 2 || a.M < RS_MIN_ROWS || a.I > 128 || a.O % 8 || a.x_ld >= (1 << 24) || !rows16(a.out, a.out_ld) ||
       (a.dy && !rows16(a.dy, a.dy_ld)))
     return {};
   RowsForm f{};
-  f.ks = a.I <= 64 ? 4 : a.I <= 128 ? 8 : 16;
+  f.ks = a.I <= 64 ? 4 : 8;
   const int each = 2 * (32 * f.ks + 4), most = RS_LDS / each / 64 * 64;
   f.parts = (a.O + most - 1) / most;
   f.cols = ((a.O + f.parts - 1) / f.parts + 63) / 64 * 64;
@@ -419,32 +421,36 @@ int launch_rows(const GatedArgs& a, const RowsForm& f, hipStream_t st) {
 template <typename T>
 int launch_rows(const GatedArgs& a, const RowsForm& f, hipStream_t st) {
   if (f.ks == 4) return a.dy ? launch_rows<T, 4, true>(a, f, st) : launch_rows<T, 4, false>(a, f, st);
-  if (f.ks == 8) return a.dy ? launch_rows<T, 8, true>(a, f, st) : launch_rows<T, 8, false>(a, f, st);
-  return a.dy ? launch_rows<T, 16, true>(a, f, st) : launch_rows<T, 16, false>(a, f, st);
+  return a.dy ? launch_rows<T, 8, true>(a, f, st) : launch_rows<T, 8, false>(a, f, st);
 }
 
+// The form of a call. Resident weights for many short rows, up to 4 parts of which read the same rows (262144 x 128 ->
+// 1024, bf16: 223 us; 65536 rows 52, in tiles 83; 32768 x 128 -> 512 19.5 and 24.9, 16384 17.1 and 14.2).
+// Tiles of 256 x 128 where they fill the CUs and leave no second round half empty (x 1024 -> 2048, 256 tiles 36 us, of
+// 128 x 64 42; 288 tiles 62 and 54; 384 tiles 62 both; 512 tiles 69 and 82), of 128 x 64 where those fill them
+// (1024 x 1024 -> 2048: 15.0 us, of 64 x 32 17.9; 1024 x 1024 -> 1024: 13.9 and 10.0). fp32: one size of tiles, as larger
+// ones are no faster (8192 x 2048 -> 2048: 1054 us, of 128 x 128 1061), and below half a tile a CU few rows' form (512 x
+// 512 -> 512: 12 us, in tiles 24; 1024 x 512 -> 1024: 34 and 26).
 template <typename T, int PREC>
 int run(const GatedArgs& a, hipStream_t st) {
   const int64_t cus = compute_units();
-  if constexpr (sizeof(T) == 2) {
-    const RowsForm f = rows_form(a, sizeof(T));
-    if (f.parts && f.parts <= 4) return launch_rows<T>(a, f, st);
-  }
   if constexpr (sizeof(T) == 4) {
     typedef Tile<T, 2, 2, 1, 2, 128, 2> Small;
     if (tiles_of<Small>(a) >= cus / 2) return launch<T, PREC, Small>(a, st);
+    const int64_t few = (a.M + 31) / 32 * ((a.O + 31) / 32);
+    hipLaunchKernelGGL((gated_few_kernel<T, PREC>), dim3((uint32_t)few), dim3(GF_NT), 0, st, a);
+    return (int)hipGetLastError();
   } else {
+    const RowsForm f = rows_form(a, sizeof(T));
+    if (f.parts && f.parts <= 4) return launch_rows<T>(a, f, st);
     typedef Tile<T, 2, 4, 4, 2, 128, 2> Large;
     typedef Tile<T, 2, 2, 2, 2, 128, 2> Medium;
     typedef Tile<T, 2, 1, 1, 2, 128, 4> Small;
-    if (tiles_of<Large>(a) >= cus) return launch<T, PREC, Large>(a, st);
+    const int64_t large = tiles_of<Large>(a);
+    if ((16 * large >= 15 * cus && large <= cus) || 2 * large >= 3 * cus) return launch<T, PREC, Large>(a, st);
     if (tiles_of<Medium>(a) >= cus) return launch<T, PREC, Medium>(a, st);
-    if (tiles_of<Small>(a) >= cus / 2) return launch<T, PREC, Small>(a, st);
+    return launch<T, PREC, Small>(a, st);
   }
-  const int64_t few = (a.M + 31) / 32 * ((a.O + 31) / 32);
-  if (few >= ((int64_t)1 << 31)) return set_error(GNN_ERR_UNSUPPORTED, "gated_linear: grid too large");
-  hipLaunchKernelGGL((gated_few_kernel<T, PREC>), dim3((uint32_t)few), dim3(GF_NT), 0, st, a);
-  return (int)hipGetLastError();
 }
 
 // ---- the weights as dx reads them ---------------------------------------------------------------
