@@ -16,8 +16,13 @@
 // whose ends fill each other's: 16 heads, 4 x 2048 x 1400, 64 columns. With more columns dk and dv take all of a CU's
 // registers and go alone. Where one of the first two leaves CUs idle its loop is split over workgroups, whose fp32 sums
 // are added in order.
-// P and dS are rounded to the operands' type for the products behind them. fp16: P is held 2^10 times as large for dV,
-// or a row spread over 10^5 keys would fall below fp16's normal range.
+// P and dS are rounded to the operands' type for the products behind them (dS in two parts for dQ of few keys and short
+// heads), and Delta takes what the rounding of O left with it. fp16: P is held 2^10 times as large for dV, or a row
+// spread over 10^5 keys would fall below fp16's normal range.
+//
+// 4 x 2048 x 1400, 16 heads of 64, bf16: 191 us for five products of 19 GFLOP (77 at a large product's rate), of which S
+// and dP are formed twice. The matrix units are busy 31% of the time, the vector units 41%, LDS 42%: 212 registers leave
+// two waves a SIMD, too few to keep all three busy at once.
 #include <algorithm>
 #include <type_traits>
 

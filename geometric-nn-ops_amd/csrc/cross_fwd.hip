@@ -19,6 +19,9 @@
 //   up to 32 rows (a decoded token): 4 waves that share the 32 rows and take 32 keys each of tiles of 128; their
 //   maxima, sums and outputs meet in LDS at the end.
 // Where these leave CUs idle the keys are split over workgroups, whose fp32 outputs a second kernel joins.
+//
+// 4096 x 8192, 32 heads of 128, bf16: 563 us of 550 GFLOP (441 at a large product's rate), the softmax's vector work beside
+// the products. One query of 8191 keys, 8 sequences, 32 heads of 128 over 8: 40 us, K and V at 5 TB/s, and 4 for the joining.
 #include <algorithm>
 #include <type_traits>
 

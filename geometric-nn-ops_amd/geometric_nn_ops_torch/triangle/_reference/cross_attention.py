@@ -7,7 +7,8 @@ def cross_attention_torch(q, k, v, bias, mask, scale):
     (B, U, H, D), (V, Hk) = q.shape, k.shape[1:3]
     wide = torch.promote_types(q.dtype, torch.float32)
     if not V:
-        return q * 0 if bias is None else q * 0 + (bias.sum() * 0).to(q.dtype)
+        empty = [t.sum() for t in (k, v, bias) if t is not None]  # zeros, which keep these in the graph
+        return q.masked_fill(torch.ones((), dtype=torch.bool, device=q.device), 0.0) + sum(empty)
     # rows: the queries of all heads that share a key head
     rows = q.to(wide).reshape(B, U, Hk, H // Hk, D).permute(0, 2, 3, 1, 4).reshape(B, Hk, H // Hk * U, D)
     k, v = (t.to(wide).transpose(1, 2) for t in (k, v))

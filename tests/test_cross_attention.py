@@ -87,6 +87,14 @@ def test_no_keys():
         assert t.shape == x.shape and not t.any()
 
 
+def test_no_keys_whatever_the_queries_hold():
+    q, k, v = (torch.full((1, 2, 2, 8), float("nan"), requires_grad=True), *(torch.ones(1, 0, 1, 8, requires_grad=True) for _ in "kv"))
+    out = cross_attention(q, k, v)
+    assert out.shape == q.shape and not out.any()
+    for t, x in zip(torch.autograd.grad(out.sum(), [q, k, v]), (q, k, v)):
+        assert t.shape == x.shape and not t.any()
+
+
 def test_refusals():
     q, k, bias = torch.zeros(2, 3, 4, 8), torch.zeros(2, 5, 2, 8), torch.zeros(2, 4, 3, 5)
     with pytest.raises(ValueError, match=r"\[batch, queries, heads, head_dim\]"):
