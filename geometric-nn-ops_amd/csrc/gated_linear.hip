@@ -428,14 +428,18 @@ int launch_rows(const GatedArgs& a, const RowsForm& f, hipStream_t st) {
 // 1024, bf16: 223 us; 65536 rows 52, in tiles 83; 32768 x 128 -> 512 19.5 and 24.9, 16384 17.1 and 14.2).
 // Tiles of 256 x 128 where they fill the CUs and leave no second round half empty (x 1024 -> 2048, 256 tiles 36 us, of
 // 128 x 64 42; 288 tiles 62 and 54; 384 tiles 62 both; 512 tiles 69 and 82), of 128 x 64 where those fill them
-// (1024 x 1024 -> 2048: 15.0 us, of 64 x 32 17.9; 1024 x 1024 -> 1024: 13.9 and 10.0). fp32: one size of tiles, as larger
-// ones are no faster (8192 x 2048 -> 2048: 1054 us, of 128 x 128 1061), and below half a tile a CU few rows' form (512 x
+// (1024 x 1024 -> 2048: 15.0 us, of 64 x 32 17.9; 1024 x 1024 -> 1024: 13.9 and 10.0). fp32: tiles of 128 x 64 where
+// their last round is full enough (4099 x 336 -> 883, 0.9 of a round: 55 us, of 64 x 64 63; 3000 x 256 -> 2048, 1.5 rounds:
+// 61 and 65; x 1024 -> 1024, 1.03 rounds: 207 and 178), of 64 x 64, and below half a tile of those a CU few rows' form (512 x
 // 512 -> 512: 12 us, in tiles 24; 1024 x 512 -> 1024: 34 and 26).
 template <typename T, int PREC>
 int run(const GatedArgs& a, hipStream_t st) {
   const int64_t cus = compute_units();
   if constexpr (sizeof(T) == 4) {
     typedef Tile<T, 2, 2, 1, 2, 128, 2> Small;
+    typedef Tile<T, 4, 2, 1, 2, 128, 2> Large;
+    const int64_t large = tiles_of<Large>(a), rounds = (large + 2 * cus - 1) / (2 * cus);  // two workgroups a CU
+    if (10 * large >= 7 * rounds * 2 * cus) return launch<T, PREC, Large>(a, st);
     if (tiles_of<Small>(a) >= cus / 2) return launch<T, PREC, Small>(a, st);
     const int64_t few = (a.M + 31) / 32 * ((a.O + 31) / 32);
     hipLaunchKernelGGL((gated_few_kernel<T, PREC>), dim3((uint32_t)few), dim3(GF_NT), 0, st, a);
