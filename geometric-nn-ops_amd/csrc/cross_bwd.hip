@@ -588,11 +588,9 @@ int run(const BwdArgs& a, hipStream_t st) {
     constexpr int DP = decltype(dp)::value;
     return a.bias ? launch<T, PREC, DP, true>(a, st) : launch<T, PREC, DP, false>(a, st);
   };
-  if constexpr (sizeof(T) == 2) {
-    if (a.s.D <= 32) return go(std::integral_constant<int, 32>{});
-    if (a.s.D > 64 && a.s.D <= 96) return go(std::integral_constant<int, 96>{});
-  }
+  if (a.s.D <= 32) return go(std::integral_constant<int, 32>{});
   if (a.s.D <= 64) return go(std::integral_constant<int, 64>{});
+  if (a.s.D <= 96) return go(std::integral_constant<int, 96>{});
   return go(std::integral_constant<int, 128>{});
 }
 

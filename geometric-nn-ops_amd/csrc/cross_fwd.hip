@@ -69,7 +69,7 @@ struct Cfg {
   static constexpr int KBYTES = KT * KTile::PITCH, TILE = KBYTES + KT * VTile::PITCH;
   static constexpr int MERGE = WK == 1 ? 0 : 4 * 64 * (16 * (DP / 32) + 4) * 4;  // of the waves' results
   static constexpr int LDS = NBUF * TILE > MERGE ? NBUF * TILE : MERGE;
-  static constexpr int WGS = (sizeof(T) == 4 && DP == 128) || (QW == 2 && DP > 64) ? 1 : 2;  // workgroups a CU
+  static constexpr int WGS = sizeof(T) == 4 && DP > 64 ? 1 : 2;  // workgroups a CU
 };
 
 template <typename T>
@@ -411,13 +411,13 @@ Plan plan(const gnn_cross_attn_args& g) {
   p.few = rows <= 32;
   p.wide = g.dtype != GNN_F32 && g.D <= (g.bias ? 32 : 64) && g.V > FINE && (rows + 255) / 256 * g.B * g.Hk >= 2 * (int64_t)compute_units();
   const int64_t per = p.wide ? 256 : 128, base = (p.few ? 1 : (rows + per - 1) / per) * g.B * g.Hk, kt = p.few ? 128 : 64, tiles = (g.V + kt - 1) / kt;
-  // The split of the keys that ends first, in us: rounds of workgroups (two a CU; in fp32, which the products bound, one),
-  // each a start and its tiles, and with several splits the second kernel, its launch and each split's sums written and
+  // The split of the keys that ends first, in us: rounds of workgroups (two a CU; in fp32 one where the products bound
+  // it or LDS holds one), each a start and its tiles, and with several splits the second kernel, its launch and each split's sums written and
   // read. One query of 2048 keys, 2 sequences, 8 heads of 64, bf16: 8.9 us with two tiles a split, with four
   // 10.6; 300 queries of 8192 keys, 4 heads of 128: 25.2 with eight, with four 28.9.
   const bool f32 = g.dtype == GNN_F32;
-  const int64_t places = (f32 ? 1 : 2) * (int64_t)compute_units();
-  const double start = 3, tile = f32 ? 3.4 * (g.D <= 64 ? 1 : 2) / (p.few ? 2 : 1) : 0.7, launch = 4;
+  const int64_t places = (f32 && (!p.few || g.D > 64) ? 1 : 2) * (int64_t)compute_units();
+  const double start = 3, tile = f32 ? 1.7 * ((g.D + 31) / 32) / (p.few ? 2 : 1) : 0.7, launch = 4;
   const double sums = 0.1 + (double)g.B * g.U * g.H * g.D * 8 / 5e6;
   double best = 0;
   for (int64_t s = 1; s <= std::min<int64_t>(tiles, 256); ++s) {
@@ -466,11 +466,9 @@ int launch(const FwdArgs& a, const Plan& p, hipStream_t st) {
 
 template <typename T, int PREC>
 int run(const FwdArgs& a, const Plan& p, hipStream_t st) {
-  if constexpr (sizeof(T) == 2) {
-    if (a.s.D <= 32) return launch<T, PREC, 32>(a, p, st);
-    if (a.s.D > 64 && a.s.D <= 96) return launch<T, PREC, 96>(a, p, st);
-  }
+  if (a.s.D <= 32) return launch<T, PREC, 32>(a, p, st);
   if (a.s.D <= 64) return launch<T, PREC, 64>(a, p, st);
+  if (a.s.D <= 96) return launch<T, PREC, 96>(a, p, st);
   return launch<T, PREC, 128>(a, p, st);
 }
 
