@@ -23,6 +23,7 @@
 // 4096 x 8192, 32 heads of 128, bf16: 563 us of 550 GFLOP (441 at a large product's rate), the softmax's vector work beside
 // the products. One query of 8191 keys, 8 sequences, 32 heads of 128 over 8: 40 us, K and V at 5 TB/s, and 4 for the joining.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "cross_common.hpp"
@@ -412,20 +413,22 @@ Plan plan(const gnn_cross_attn_args& g) {
   p.wide = g.dtype != GNN_F32 && g.D <= (g.bias ? 32 : 64) && g.V > FINE && (rows + 255) / 256 * g.B * g.Hk >= 2 * (int64_t)compute_units();
   const int64_t per = p.wide ? 256 : 128, base = (p.few ? 1 : (rows + per - 1) / per) * g.B * g.Hk, kt = p.few ? 128 : 64, tiles = (g.V + kt - 1) / kt;
   // The split of the keys that ends first, in us: rounds of workgroups (two a CU; in fp32 one where the products bound
-  // it or LDS holds one), each a start and its tiles, and with several splits the second kernel, its launch and each split's sums written and
-  // read. One query of 2048 keys, 2 sequences, 8 heads of 64, bf16: 8.9 us with two tiles a split, with four
-  // 10.6; 300 queries of 8192 keys, 4 heads of 128: 25.2 with eight, with four 28.9.
+  // it or LDS holds one), each a start and its tiles, and with several splits the second kernel, its launch and each
+  // split's sums written and read. One query of 2048 keys, 2 sequences, 8 heads of 64, bf16: 8.9 us with two tiles a
+  // split, with four 10.6; 300 queries of 8192 keys, 4 heads of 128: 25.2 with eight, with four 28.9.
   const bool f32 = g.dtype == GNN_F32;
   const int64_t places = (f32 && (!p.few || g.D > 64) ? 1 : 2) * (int64_t)compute_units();
   const double start = 3, tile = f32 ? 1.7 * ((g.D + 31) / 32) / (p.few ? 2 : 1) : 0.7, launch = 4;
   const double sums = 0.1 + (double)g.B * g.U * g.H * g.D * 8 / 5e6;
+  // none, whole rounds, and where the tiles' and the sums' time are balanced
+  const int64_t tries[] = {1, places / base, 2 * places / base, 3 * places / base, (int64_t)std::sqrt((double)tiles * tile / sums)};
   double best = 0;
-  for (int64_t s = 1; s <= std::min<int64_t>(tiles, 256); ++s) {
-    const int64_t each = (tiles + s - 1) / s, splits = (tiles + each - 1) / each;
-    if (splits != s) continue;
-    const double rounds = (double)((base * s + places - 1) / places);
-    const double time = rounds * (start + each * tile) + (s > 1 ? launch + s * sums : 0);
-    if (s == 1 || time < best) best = time, p.splits = s, p.tiles_per_split = each;
+  for (const int64_t want : tries) {
+    const int64_t most = std::max<int64_t>(1, std::min(want, tiles));
+    const int64_t each = (tiles + most - 1) / most, splits = (tiles + each - 1) / each;
+    const double rounds = (double)((base * splits + places - 1) / places);
+    const double time = rounds * (start + (double)each * tile) + (splits > 1 ? launch + (double)splits * sums : 0);
+    if (best == 0 || time < best) best = time, p.splits = splits, p.tiles_per_split = each;
   }
   p.blocks = base * p.splits;
   return p;
