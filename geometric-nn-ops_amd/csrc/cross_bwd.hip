@@ -514,10 +514,17 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 || (DKDV && DP > 64) ? 1 : 2) vo
   }
 }
 
-template <typename E>
-__global__ __launch_bounds__(NT) void zeros_kernel(E* p, int64_t n) {
-  const int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x;
-  if (i < n) p[i] = 0;
+// dbias of one key, [B or 1][H][U]: 0, and NaN where a row's probability or output gradient has it
+template <typename T>
+__global__ __launch_bounds__(NT) void one_key_dbias_kernel(const BwdArgs a, T* dbias, int sequences) {
+  const int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x, each = (int64_t)a.s.H * a.s.U, n = a.s.B / sequences * each;
+  if (i >= n) return;
+  float sum = 0.f;
+  for (int b = 0; b < sequences; ++b) {
+    const int64_t stat = b * each + i;
+    if (a.stats[2 * stat] != INFINITY) sum += 0.f * (a.stats[2 * stat + 1] + a.delta[stat]);
+  }
+  dbias[i] = (T)sum;
 }
 
 struct Plan {
@@ -633,19 +640,11 @@ int cross_attn_bwd(const gnn_cross_attn_bwd_args& g, hipStream_t st) {
   }
   for (int i = 0; i < 2; ++i) a.ms[i] = g.mask_stride[i];
   a.scale = g.scale, a.logit_scale = g.bias ? g.scale : g.scale * LOG2E;
-  // One key has probability 1 whatever its logit: the logits' gradients are zeros, where P (dP - Delta) would leave the
-  // rounding errors of two sums of the same products.
+  // One key has probability 1, or 0 where its bias leaves nothing, whatever its logit: P comes from the row's statistics
+  // alone (store_stats), and the logits' gradients are zeros, where P (dP - Delta) would leave the rounding errors of two
+  // sums of the same products.
   if (one_key) a.scale = a.logit_scale = 0.f, a.bias = nullptr, a.dbias = nullptr;
   a.q_splits = (int)p.q_splits, a.q_tiles = (int)p.q_tiles, a.k_splits = (int)p.k_splits, a.k_tiles = (int)p.k_tiles;
-  if (one_key && g.dbias) {
-    const int64_t n = (g.shared_bias ? 1 : g.B) * g.H * g.U;
-    const dim3 grid((uint32_t)((n + NT - 1) / NT));
-    if (g.dtype == GNN_F32)
-      hipLaunchKernelGGL(zeros_kernel<uint32_t>, grid, dim3(NT), 0, st, (uint32_t*)g.dbias, n);
-    else
-      hipLaunchKernelGGL(zeros_kernel<uint16_t>, grid, dim3(NT), 0, st, (uint16_t*)g.dbias, n);
-    if (int rc = (int)hipGetLastError()) return rc;
-  }
   int64_t nq, nk;
   partial_sums(g, p, nq, nk);
   a.delta = (float*)g.workspace;
@@ -660,6 +659,16 @@ int cross_attn_bwd(const gnn_cross_attn_bwd_args& g, hipStream_t st) {
     case GNN_BF16: rc = run<bf16, PREC_NATIVE>(a, st); break;
     case GNN_F16: rc = run<f16, PREC_NATIVE>(a, st); break;
     default: rc = g.precision == GNN_PREC_BF16X3 ? run<float, PREC_BF16X3>(a, st) : run<float, PREC_IEEE>(a, st);
+  }
+  if (rc == 0 && one_key && g.dbias) {
+    const int sequences = g.shared_bias ? a.s.B : 1;  // summed
+    const dim3 grid((uint32_t)((g.B / sequences * g.H * g.U + NT - 1) / NT));
+    switch (g.dtype) {
+      case GNN_BF16: hipLaunchKernelGGL(one_key_dbias_kernel<bf16>, grid, dim3(NT), 0, st, a, (bf16*)g.dbias, sequences); break;
+      case GNN_F16: hipLaunchKernelGGL(one_key_dbias_kernel<f16>, grid, dim3(NT), 0, st, a, (f16*)g.dbias, sequences); break;
+      default: hipLaunchKernelGGL(one_key_dbias_kernel<float>, grid, dim3(NT), 0, st, a, (float*)g.dbias, sequences);
+    }
+    rc = (int)hipGetLastError();
   }
   if (rc || (!nq && !nk)) return rc;
   gnn_reduce_args r{};

@@ -48,7 +48,7 @@ struct FwdArgs {
   const uint8_t* mask;
   void* o;
   void* o_low;     // dense like o, what o's rounding left; or NULL
-  float* stats;    // [B][H][U][2]: the reference maximum (+inf where no key is kept) and the log2 of the sum; or NULL
+  float* stats;    // [B][H][U][2], what store_stats leaves of a row; or NULL
   float* part_o;   // [splits][B][U][H][D]
   float* part_ml;  // [splits][B][H][U][2]
   int64_t qs[3], ks[3], vs[3], bs[3], ms[2];
@@ -79,6 +79,14 @@ __device__ __forceinline__ void store_out(const FwdArgs& a, int64_t at, const f3
   store4((T*)a.o + at, y);
   if constexpr (sizeof(T) == 2)
     if (a.o_low) store4((T*)a.o_low + at, TypeOps<T>::from_f32(x - TypeOps<T>::to_f32(y)));
+}
+
+// What the backward needs of a row whose probabilities sum to `sum` beside the maximum m: m and the log2 of the sum; +inf
+// and 0 where nothing is left; NaN twice where the row holds one. Of one key, whose logit the backward does not
+// form, 0 and 0.
+__device__ __forceinline__ void store_stats(const FwdArgs& a, int64_t at, float m, float sum) {
+  a.stats[2 * at] = sum > 0.f ? (a.s.V == 1 ? 0.f : m) : sum == 0.f ? INFINITY : sum;
+  a.stats[2 * at + 1] = sum == 0.f ? 0.f : log2f(sum);
 }
 
 template <typename T, int PREC, int DP, int WK, int QW, bool BIAS>
@@ -130,8 +138,7 @@ __global__ __launch_bounds__(NT, (Cfg<T, DP, WK, QW>::WGS)) void cross_fwd_kerne
     for (int kk = 0; kk < DP / 16; ++kk) {
       const int d = 16 * kk + 8 * g;
       qf[i][kk] = load8_at(qp + (d < s.D ? d : 0));
-      // one key has probability 1 whatever its logit: 0 here, which leaves the sum an exact 1
-      if (d >= s.D || s.V == 1) qf[i][kk] = zero8<T>();
+      if (d >= s.D) qf[i][kk] = zero8<T>();
     }
 #pragma unroll
     for (int cc = 0; cc < DP / 32; ++cc) clear(o[i][cc]);
@@ -337,7 +344,7 @@ __global__ __launch_bounds__(NT, (Cfg<T, DP, WK, QW>::WGS)) void cross_fwd_kerne
         ml[0] = m[i], ml[1] = sum[i];
       }
     } else if (first && a.stats) {
-      a.stats[2 * stat] = sum[i] == 0.f ? INFINITY : m[i], a.stats[2 * stat + 1] = sum[i] == 0.f ? 0.f : log2f(sum[i]);
+      store_stats(a, stat, m[i], sum[i]);
     }
 #pragma unroll
     for (int k = 0; k < (WK == 1 ? DP / 32 : 1); ++k) {
@@ -393,8 +400,7 @@ __global__ __launch_bounds__(NT) void cross_join_kernel(const FwdArgs a) {
   }
   const float inv = sum > 0.f ? 1.0f / sum : sum == 0.f ? 0.f : sum;
   store_out<T>(a, head * s.D + d, o * inv);
-  if (a.stats && d == 0)
-    a.stats[2 * stat] = sum == 0.f ? INFINITY : m, a.stats[2 * stat + 1] = sum == 0.f ? 0.f : log2f(sum);
+  if (a.stats && d == 0) store_stats(a, stat, m, sum);
 }
 
 // Few: up to 32 rows (8 x 1 x 4096, 32 heads of 64 over 8, bf16: 13.2 us, in the other form 19.0).
@@ -491,8 +497,8 @@ int cross_attn_fwd(const gnn_cross_attn_args& g, hipStream_t st) {
   a.q = g.q, a.k = g.k, a.v = g.v, a.bias = g.bias, a.mask = g.mask, a.o = g.o, a.o_low = g.o_low, a.stats = g.stats;
   for (int i = 0; i < 3; ++i) a.qs[i] = g.q_stride[i], a.ks[i] = g.k_stride[i], a.vs[i] = g.v_stride[i], a.bs[i] = g.bias_stride[i];
   for (int i = 0; i < 2; ++i) a.ms[i] = g.mask_stride[i];
-  a.scale = g.bias ? g.scale : g.scale * LOG2E;
-  if (g.V == 1) a.bias = nullptr, a.scale = g.scale * LOG2E;
+  // One key has the weight 1 at any scale: at 1 its score less the maximum is an exact 0
+  a.scale = g.bias ? g.scale : g.V == 1 ? 1.f : g.scale * LOG2E;
   a.fine = g.V <= FINE;
   a.splits = (int)p.splits, a.tiles_per_split = (int)p.tiles_per_split;
   if (p.splits > 1) {

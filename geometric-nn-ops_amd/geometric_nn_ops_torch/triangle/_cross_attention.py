@@ -93,8 +93,8 @@ def cross_attention(
     follow ``torch.backends.cuda.matmul.fp32_precision``.
 
     Returns:
-        A fresh contiguous ``[B, U, H, D]`` tensor of q's dtype: zeros, with zero gradients, for queries that no key
-        is left to. Differentiable in q, k, v and bias (a shared bias's gradient is summed over the batch, in fp32);
+        A fresh contiguous ``[B, U, H, D]`` tensor of q's dtype: zeros, with zero gradients, for queries to which the
+        mask, or a bias of -inf, leaves no key. Differentiable in q, k, v and bias (a shared bias's gradient is summed over the batch, in fp32);
         repeated calls give the same bits.
     """
     _check(q, k, v, bias, mask, scale)

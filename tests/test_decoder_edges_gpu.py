@@ -1,0 +1,90 @@
+"""cross_attention where little is left of a row: one key under a bias, infinities and NaN."""
+
+import pytest
+import torch
+
+from geometric_nn_ops_torch.triangle import cross_attention
+from op_helpers import DTYPES, IDS, U, assert_within
+from test_cross_attention_gpu import NAMES, _inputs
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+INF, NAN = float("inf"), float("nan")
+
+
+def _train(tensors, mask, dout, scale=None):
+    """The output and the gradients of q, k, v and, where there is one, the bias."""
+    leaves = [t.detach().clone().requires_grad_() for t in tensors if t is not None]
+    o = cross_attention(*leaves, *([] if len(leaves) == 4 else [None]), mask, scale)
+    return [o.detach(), *torch.autograd.grad(o, leaves, dout)]
+
+
+def _torch_path(tensors, mask, dout):
+    wide = [None if t is None else t.cpu().double() for t in tensors]
+    return _train(wide, None if mask is None else mask.cpu(), dout.cpu().double())
+
+
+# ---- one key
+def _one_key(u, bias, dtype, masked):
+    """Three sequences of one key, and the gradients that stock torch has in float64."""
+    tensors, _, dout = _inputs((3, u, 1, 4, 2, 128, bias, False), dtype, seed=40)
+    mask = torch.tensor([[True], [False], [True]], device=DEV) if masked else None
+    return tensors, mask, dout
+
+
+def _same(got, want, dtype, sums):
+    """NaN where stock torch has it. o holds one value or none and dq, dk, dbias are zeros: equal; dv adds ``sums``
+    output gradients, each below 6, in fp32."""
+    for name, a, e in zip(NAMES, got, want):
+        a = a.cpu()
+        assert torch.equal(a.isnan(), e.isnan()), name
+        a, e = a.double().nan_to_num(nan=0.0), e.nan_to_num(nan=0.0)
+        if name != "dv":
+            assert torch.equal(a, e), name
+        else:
+            assert_within(name, a.to(dtype), e, min(sums, 16 + 4 * sums ** 0.5) * U * 6 * sums * torch.ones_like(e))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("u", [1, 52])
+@pytest.mark.parametrize("bias", [1, 2])
+def test_one_key_that_a_bias_takes_away(bias, u, masked, dtype):
+    """A bias of -inf leaves its query nothing: zeros, and nothing of its output gradient in dv."""
+    tensors, mask, dout = _one_key(u, bias, dtype, masked)
+    tensors[3][:, 1, ::3] = -INF
+    got = _train(tensors, mask, dout)
+    assert not got[0][:, ::3, 1].any() and got[0][0, :, 0].any()
+    _same(got, _torch_path(tensors, mask, dout), dtype, 2 * u)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("u", [1, 52])
+@pytest.mark.parametrize("bias", [1, 2])
+@pytest.mark.parametrize("what", [INF, NAN])
+def test_one_key_whose_bias_is_no_number(what, bias, u, dtype):
+    tensors, mask, dout = _one_key(u, bias, dtype, True)
+    tensors[3][0, 2, u // 2, 0] = what
+    got = _train(tensors, mask, dout)
+    assert got[0][0, u // 2, 2].isnan().all() and not got[0][0, u // 2, 0].isnan().any()
+    _same(got, _torch_path(tensors, mask, dout), dtype, 2 * u)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("bias", [0, 1, 2])
+def test_one_key_and_a_query_that_is_no_number(bias, dtype):
+    tensors, mask, dout = _one_key(52, bias, dtype, True)
+    tensors[0][2, 7, 3, 5] = NAN
+    got = _train(tensors, mask, dout)
+    assert got[0][2, 7, 3].isnan().all() and not got[0][2, 7, 2].isnan().any()
+    _same(got, _torch_path(tensors, mask, dout), dtype, 104)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("bias", [0, 2])
+def test_one_key_of_a_large_logit(bias, dtype):
+    """The weight is an exact 1 beside logits of some thousand."""
+    tensors, _, dout = _inputs((3, 52, 1, 4, 2, 128, bias, False), dtype, seed=41, scale=30.0)
+    o = cross_attention(*tensors)
+    assert torch.equal(o, tensors[2].repeat_interleave(2, 2).expand_as(o))
+    _same(_train(tensors, None, dout / 30), _torch_path(tensors, None, dout / 30), dtype, 104)
