@@ -424,8 +424,9 @@ __device__ __forceinline__ void dkdv_block(const BwdArgs& a, Lds<T, DP>& lds, ui
     for (int q = 0; q < 4; ++q) {
       const int d = 32 * cc + 8 * q + 4 * g;
       if (d >= s.D) continue;
-      const f32x4 x = f32x4{dk[cc][4 * q], dk[cc][4 * q + 1], dk[cc][4 * q + 2], dk[cc][4 * q + 3]} * a.scale;
-      const f32x4 y = f32x4{dv[cc][4 * q], dv[cc][4 * q + 1], dv[cc][4 * q + 2], dv[cc][4 * q + 3]} * (1.f / p_scale<T>());
+      f32x4 x = f32x4{dk[cc][4 * q], dk[cc][4 * q + 1], dk[cc][4 * q + 2], dk[cc][4 * q + 3]} * a.scale;
+      f32x4 y = f32x4{dv[cc][4 * q], dv[cc][4 * q + 1], dv[cc][4 * q + 2], dv[cc][4 * q + 3]} * (1.f / p_scale<T>());
+      if (!kept) x = y = f32x4{0.f, 0.f, 0.f, 0.f};  // zeros so far, but where Q or dO hold infinities or NaN
       if (a.part_k) {
         *reinterpret_cast<f32x4*>(a.part_k + 2 * split * each + at + d) = x;
         *reinterpret_cast<f32x4*>(a.part_k + (2 * split + 1) * each + at + d) = y;

@@ -88,3 +88,25 @@ def test_one_key_of_a_large_logit(bias, dtype):
     o = cross_attention(*tensors)
     assert torch.equal(o, tensors[2].repeat_interleave(2, 2).expand_as(o))
     _same(_train(tensors, None, dout / 30), _torch_path(tensors, None, dout / 30), dtype, 104)
+
+
+# ---- output gradients that are no numbers
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("what", [INF, NAN])
+@pytest.mark.parametrize("shape", [(3, 70, 333, 4, 2, 64, 1, True), (2, 5, 200, 4, 2, 128, 2, True),
+                                   (1, 2300, 40, 4, 2, 32, 0, True), (2, 300, 90, 4, 2, 96, 0, True)], ids=str)
+def test_an_infinite_output_gradient_stays_with_the_kept_keys(shape, what, dtype):
+    """It reaches every kept key of its key head, and no masked one."""
+    tensors, mask, dout = _inputs(shape, dtype, seed=42)
+    plain = _train(tensors, mask, dout)
+    dout[0, 3, 2, 7] = what
+    got = _train(tensors, mask, dout)
+    for t in got[2:4]:
+        assert not t[~mask].any() and not t[0, mask[0], 1].isfinite().all(-1).any()
+    if shape[6]:
+        kept = mask.any(0, keepdim=True) if shape[6] == 1 else mask  # of a shared bias: by some sequence
+        assert not got[4].masked_fill(kept[:, None, None].expand_as(got[4]), 0.0).any()
+    for a, e in zip(got[2:4], plain[2:4]):
+        assert torch.equal(a[0, :, 0], e[0, :, 0]) and torch.equal(a[1:], e[1:])
+    got[1][0, 3, 2] = plain[1][0, 3, 2]
+    assert torch.equal(got[1], plain[1])
