@@ -93,13 +93,14 @@ __device__ __forceinline__ void row_stats(const float* stats, float& m, float& l
   if constexpr (!BIAS) m += l;
 }
 
-// dS^T = P (dP - Delta) of one half tile of 32 keys for the lane's row.
-// `word`: the kept keys of the half tile.
+// dS^T = P (dP - Delta) of one half tile of 32 keys for the lane's row. `word`: the kept keys of the half tile; `dead`:
+// some row of the wave has none (m is +inf): zeros there, whatever its output gradient holds.
 template <typename T, int PREC, int DP, bool BIAS>
 __device__ __forceinline__ void half_tile(f32x16& dp, const unsigned char* ks, const unsigned char* vs, int at,
                                           const typename TypeOps<T>::V8 (&qf)[DP / 16],
                                           const typename TypeOps<T>::V8 (&df)[DP / 16], const T* bias_row, int key0, int V,
-                                          float scale, float m, float l, const f32x16& minus_delta, uint32_t word) {
+                                          float scale, float m, float l, const f32x16& minus_delta, uint32_t word,
+                                          bool dead) {
   typedef RowTile<T, DP> Tile;
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   HalfBias<T> bias;
@@ -122,9 +123,10 @@ __device__ __forceinline__ void half_tile(f32x16& dp, const unsigned char* ks, c
       dp[i] *= probability<BIAS>(sc[i], scale, add[e], m, l);
     }
   }
-  if (word != ~0u) {  // uniform
+  if (word != ~0u || dead) {  // uniform
+    const uint32_t kept = m == INFINITY ? 0u : word;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) dp[i] = word >> acc_row(i, g) & 1 ? dp[i] : 0.f;
+    for (int i = 0; i < 16; ++i) dp[i] = kept >> acc_row(i, g) & 1 ? dp[i] : 0.f;
   }
 }
 
@@ -193,6 +195,7 @@ __device__ __forceinline__ void dq_block(const BwdArgs& a, Lds<T, DP>& lds, uint
   load_row<T, DP>(df, (const T*)a.dout + b * a.ds[0] + u * a.ds[1] + h * a.ds[2], s.D, g);
   float m, l;
   row_stats<BIAS>(a.stats + 2 * stat, m, l);
+  const bool dead = __any(m == INFINITY);
   f32x16 minus_delta;  // what the sums of dP start from
   fill(minus_delta, -a.delta[stat]);
   // own bias: every tile is visited, so that what no row keeps gets its zeros
@@ -242,7 +245,7 @@ __device__ __forceinline__ void dq_block(const BwdArgs& a, Lds<T, DP>& lds, uint
     for (int sub = 0; sub < KT / 32; ++sub) {
       f32x16 ds;
       half_tile<T, PREC, DP, BIAS>(ds, ks, ks + TILE, 32 * sub, qf, df, bias_row, t * KT + 32 * sub, s.V, a.logit_scale, m, l,
-                                   minus_delta, (uint32_t)(live >> (32 * sub)));
+                                   minus_delta, (uint32_t)(live >> (32 * sub)), dead);
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         const V8 f = acc_frag<T>(ds, kk);
@@ -481,7 +484,7 @@ __device__ __forceinline__ void dbias_block(const BwdArgs& a, Lds<T, DP>& lds, u
     for (int sub = 0; sub < KT / 32; ++sub) {
       f32x16 ds;
       half_tile<T, PREC, DP, true>(ds, smem, smem + TILE, 32 * sub, qf, df, bias_row, kb * KT + 32 * sub, s.V, a.logit_scale,
-                                   m, l, minus_delta, (uint32_t)(live >> (32 * sub)));
+                                   m, l, minus_delta, (uint32_t)(live >> (32 * sub)), __any(m == INFINITY));
       sum[sub] += ds;
     }
   }

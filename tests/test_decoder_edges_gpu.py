@@ -110,3 +110,19 @@ def test_an_infinite_output_gradient_stays_with_the_kept_keys(shape, what, dtype
         assert torch.equal(a[0, :, 0], e[0, :, 0]) and torch.equal(a[1:], e[1:])
     got[1][0, 3, 2] = plain[1][0, 3, 2]
     assert torch.equal(got[1], plain[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("what", [INF, NAN])
+@pytest.mark.parametrize("shape", [(2, 70, 333, 4, 2, 64, 1, False), (2, 5, 200, 4, 2, 128, 2, True),
+                                   (1, 40, 5000, 2, 1, 32, 2, False), (2, 33, 1, 4, 2, 64, 1, False)], ids=str)
+def test_rows_without_keys_have_no_gradient(shape, what, dtype):
+    """Whatever their output gradient holds: zeros in dq and dbias, as stock torch has them."""
+    tensors, mask, dout = _inputs(shape, dtype, seed=43)
+    tensors[3][:, 1, 2:5] = -INF
+    plain = _train(tensors, mask, dout)
+    dout[:, 2:5, 1] = what
+    got = _train(tensors, mask, dout)
+    for i in (0, 1, 4):
+        assert torch.equal(got[i], plain[i]), NAMES[i]
+    assert not got[1][:, 2:5, 1].any() and not got[4][:, 1, 2:5].any()
