@@ -17,8 +17,14 @@
 // registers and go alone. Where one of the first two leaves CUs idle its loop is split over workgroups, whose fp32 sums
 // are added in order.
 // P and dS are rounded to the operands' type for the products behind them (dS in two parts for dQ of few keys and short
-// heads), and Delta takes what the rounding of O left with it. fp16: P is held 2^10 times as large for dV, or a row
-// spread over 10^5 keys would fall below fp16's normal range.
+// heads), and Delta takes what the rounding of O left with it.
+//
+// fp16's range: P is held 2^10 times as large for dV, or a row spread over 10^5 keys would fall below the normal range.
+// dS falls sooner, with the output gradient, and as much above 1 it would leave the range upwards. |dS_rj| is at most
+// 2 |dO_r| max_j |v_j|, and dS is held at the power of two that brings this bound into 2^14 .. 2^15: each row's own for dQ,
+// where it goes into the exponent of P and out with the store, the largest of all rows for dK, whose sums go over rows.
+// The lengths |dO_r| come with Delta, the longest v_j from further workgroups of that kernel. (16384 keys, dO of 2^-8:
+// dQ was off by 5.4e-3 unscaled; a factor of one size for all would overflow beside large gradients.)
 //
 // 4 x 2048 x 1400, 16 heads of 64, bf16: 191 us for five products of 19 GFLOP (77 at a large product's rate), of which S
 // and dP are formed twice. The matrix units are busy 31% of the time, the vector units 41%, LDS 42%: 212 registers leave
@@ -51,6 +57,9 @@ struct BwdArgs {
   const uint8_t* mask;
   const float* stats;  // [B][H][U][2]
   float* delta;      // [B][H][U]
+  float* length;     // fp16: |dO| of each row, [B][H][U]
+  float* top;        // fp16: the longest kept v_j of each part of the keys, [B][Hk][v_parts]
+  int v_parts;
   void* dq;
   void* dk;
   void* dv;
@@ -61,13 +70,28 @@ struct BwdArgs {
   float scale, logit_scale;  // the caller's; without a bias times log2(e)
   int q_splits, q_tiles;  // tiles of keys a split
   int k_splits, k_tiles;  // tiles of rows a split
-  uint32_t q_blocks, k_blocks, b_blocks;
+  uint32_t delta_blocks, q_blocks, k_blocks, b_blocks;
   bool shared_bias;
   bool q_first;  // the workgroups of dQ before those of dK and dV
 };
 
-template <typename T> constexpr float p_scale() { return 1.f; }  // of P in dV
-template <> constexpr float p_scale<f16>() { return 0x1p10f; }
+template <typename T> constexpr bool RANGED = false;  // operands held at powers of two
+template <> constexpr bool RANGED<f16> = true;
+constexpr int P_LOG = 10;  // of P in dV, where RANGED
+
+// Of dS below `bound`; 0 where nothing or no number bounds it
+__device__ __forceinline__ int ds_log(float bound) {
+  return bound > 0.f && bound < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(bound) : 0;
+}
+__device__ __forceinline__ float wave_top(float x) {
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) x = fmaxf(x, __shfl_xor(x, k));
+  return x;
+}
+// The longest v_j of a key head
+__device__ __forceinline__ float longest_value(const BwdArgs& a, int b, int hk) {
+  return wave_top(a.top[((int64_t)b * a.s.Hk + hk) * a.v_parts + min((int)(threadIdx.x & 63), a.v_parts - 1)]);
+}
 
 // Fragments of one row of a lane, zeros past D
 template <typename T, int DP>
@@ -131,24 +155,72 @@ __device__ __forceinline__ void half_tile(f32x16& dp, const unsigned char* ks, c
 }
 
 // ------------------------------------------------------------------------------------ Delta
+__device__ __forceinline__ float sum8(const f32x8& x) { return ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])); }
+
+// The longest kept v_j of one part of a key head's keys; 2^LOG lanes of 8 elements a row
+constexpr int KEYS_A_PART = 256, MAX_PARTS = 64;
+template <typename T, int LOG>
+__device__ __forceinline__ void longest_of_part(const BwdArgs& a, uint32_t block) {
+  constexpr int AT_ONCE = 4, ROWS = NT >> LOG;
+  __shared__ float tops[NT / 64];
+  const Shape& s = a.s;
+  const int part = block % a.v_parts, hk = block / a.v_parts % s.Hk, b = block / a.v_parts / s.Hk;
+  const int each = (s.V + a.v_parts - 1) / a.v_parts, end = min(s.V, (part + 1) * each);
+  const int d = (int)(threadIdx.x & ((1 << LOG) - 1)) * 8;
+  const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[2] + (d < s.D ? d : 0);
+  const uint8_t* mask = a.mask ? a.mask + b * a.ms[0] : nullptr;
+  float top = 0.f;
+  for (int k0 = part * each + ((int)threadIdx.x >> LOG); k0 < end; k0 += AT_ONCE * ROWS) {
+    f32x8 x[AT_ONCE];
+    bool kept[AT_ONCE];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int64_t key = min(k0 + i * ROWS, end - 1);
+      x[i] = TypeOps<T>::to_f32(load8_at(vp + key * a.vs[1]));
+      kept[i] = !mask || mask[key * a.ms[1]] != 0;
+    }
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      float sum = d < s.D ? sum8(x[i] * x[i]) : 0.f;
+#pragma unroll
+      for (int k = 1; k < (1 << LOG); k *= 2) sum += __shfl_xor(sum, k);
+      if (kept[i]) top = fmaxf(top, sum);
+    }
+  }
+  top = wave_top(top);
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) a.top[block] = sqrtf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+}
+
 // 2^LOG lanes of 8 elements a row
 template <typename T, int LOG>
 __global__ __launch_bounds__(NT) void cross_delta_kernel(const BwdArgs a) {
   const Shape& s = a.s;
+  if constexpr (RANGED<T>)
+    if (blockIdx.x >= a.delta_blocks) return longest_of_part<T, LOG>(a, blockIdx.x - a.delta_blocks);
   const int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x, heads = (int64_t)s.B * s.U * s.H;
   const int64_t head = min(i >> LOG, heads - 1);
   const int d = (int)(i & ((1 << LOG) - 1)) * 8, h = (int)(head % s.H);
   const int64_t bu = head / s.H, b = bu / s.U, u = bu - b * s.U;
-  float sum = 0.f;
+  float sum = 0.f, square = 0.f;
   if (d < s.D) {
     f32x8 o = TypeOps<T>::to_f32(load8_at((const T*)a.o + b * a.os[0] + u * a.os[1] + h * a.os[2] + d));
     if (a.o_low) o += TypeOps<T>::to_f32(load8_at((const T*)a.o_low + head * s.D + d));
-    const f32x8 x = o * TypeOps<T>::to_f32(load8_at((const T*)a.dout + b * a.ds[0] + u * a.ds[1] + h * a.ds[2] + d));
-    sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+    const f32x8 x = TypeOps<T>::to_f32(load8_at((const T*)a.dout + b * a.ds[0] + u * a.ds[1] + h * a.ds[2] + d));
+    sum = sum8(o * x);
+    if constexpr (RANGED<T>) square = sum8(x * x);
   }
 #pragma unroll
-  for (int k = 1; k < (1 << LOG); k *= 2) sum += __shfl_xor(sum, k);
-  if (d == 0 && i >> LOG < heads) a.delta[(b * s.H + h) * s.U + u] = sum;
+  for (int k = 1; k < (1 << LOG); k *= 2) {
+    sum += __shfl_xor(sum, k);
+    if constexpr (RANGED<T>) square += __shfl_xor(square, k);
+  }
+  if (d == 0 && i >> LOG < heads) {
+    const int64_t stat = (b * s.H + h) * s.U + u;
+    a.delta[stat] = sum;
+    if constexpr (RANGED<T>) a.length[stat] = sqrtf(square);
+  }
 }
 
 // LDS of a workgroup
@@ -196,6 +268,12 @@ __device__ __forceinline__ void dq_block(const BwdArgs& a, Lds<T, DP>& lds, uint
   float m, l;
   row_stats<BIAS>(a.stats + 2 * stat, m, l);
   const bool dead = __any(m == INFINITY);
+  float undo = 1.f;  // of dS's power of two
+  if constexpr (RANGED<T>) {
+    const int log = ds_log(2.f * a.length[stat] * longest_value(a, b, hk));
+    (BIAS ? l : m) -= (float)log;
+    undo = ldexpf(1.f, -log);
+  }
   f32x16 minus_delta;  // what the sums of dP start from
   fill(minus_delta, -a.delta[stat]);
   // own bias: every tile is visited, so that what no row keeps gets its zeros
@@ -263,7 +341,7 @@ __device__ __forceinline__ void dq_block(const BwdArgs& a, Lds<T, DP>& lds, uint
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const int key = t * KT + 32 * sub + 8 * q + 4 * g;
-            if (key < s.V) store4_at(dbias + key, f32x4{ds[4 * q], ds[4 * q + 1], ds[4 * q + 2], ds[4 * q + 3]}, s.V - key);
+            if (key < s.V) store4_at(dbias + key, f32x4{ds[4 * q], ds[4 * q + 1], ds[4 * q + 2], ds[4 * q + 3]} * undo, s.V - key);
           }
       }
     }
@@ -280,7 +358,7 @@ __device__ __forceinline__ void dq_block(const BwdArgs& a, Lds<T, DP>& lds, uint
     for (int q = 0; q < 4; ++q) {
       const int d = 32 * cc + 8 * q + 4 * g;
       if (d >= s.D) continue;
-      const f32x4 x = f32x4{dq[cc][4 * q], dq[cc][4 * q + 1], dq[cc][4 * q + 2], dq[cc][4 * q + 3]} * a.scale;
+      const f32x4 x = f32x4{dq[cc][4 * q], dq[cc][4 * q + 1], dq[cc][4 * q + 2], dq[cc][4 * q + 3]} * (a.scale * undo);
       if (a.part_q)
         *reinterpret_cast<f32x4*>(a.part_q + split * each + head * s.D + d) = x;
       else
@@ -324,6 +402,22 @@ __device__ __forceinline__ void dkdv_block(const BwdArgs& a, Lds<T, DP>& lds, ui
   for (int cc = 0; cc < DP / 32; ++cc) clear(dk[cc]), clear(dv[cc]);
   const int tiles = (s.rows + KT - 1) / KT;
   const int t0 = split * a.k_tiles, t_end = any_kept ? min(tiles, t0 + a.k_tiles) : t0;
+  float hold = 1.f, undo = 1.f;  // dS's power of two over P's, and what undoes it; the same in every split
+  if constexpr (RANGED<T>) {
+    constexpr int AT_ONCE = 8;
+    const float* length = a.length + ((int64_t)b * s.H + hk * s.G) * s.U;  // of the key head's rows
+    if (threadIdx.x == 0) lds.found[0] = 0;
+    __syncthreads();
+    float top = 0.f;
+    for (int i = threadIdx.x; i < s.rows; i += AT_ONCE * NT)
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) top = fmaxf(top, length[min(i + k * NT, s.rows - 1)]);
+    top = wave_top(top);
+    if (lane == 0) atomicMax(&lds.found[0], __float_as_int(top));
+    __syncthreads();
+    const int log = __builtin_amdgcn_readfirstlane(ds_log(2.f * __int_as_float(lds.found[0]) * longest_value(a, b, hk)));
+    hold = ldexpf(1.f, log - P_LOG), undo = ldexpf(1.f, -log);
+  }
   Staged<T, DP, KT, NT> qreg, dreg;
   float next_m = 0.f, next_l = 0.f, next_delta = 0.f;
   int64_t next_bias = 0;
@@ -334,6 +428,7 @@ __device__ __forceinline__ void dkdv_block(const BwdArgs& a, Lds<T, DP>& lds, ui
       const int row = min(t * KT + (int)threadIdx.x, s.rows - 1), u = row / s.G, h = hk * s.G + row % s.G;
       const int64_t stat = ((int64_t)b * s.H + h) * s.U + u;
       row_stats<BIAS>(a.stats + 2 * stat, next_m, next_l);
+      if constexpr (RANGED<T>) (BIAS ? next_l : next_m) -= (float)P_LOG;
       if (t * KT + (int)threadIdx.x >= s.rows) next_m = INFINITY;  // P = 2^-inf, and zeros of Q and dO
       next_delta = a.delta[stat];
       if constexpr (BIAS) next_bias = h * a.bs[1] + u * a.bs[2];
@@ -402,9 +497,9 @@ __device__ __forceinline__ void dkdv_block(const BwdArgs& a, Lds<T, DP>& lds, ui
         for (int i = 0; i < 16; ++i) p[i] = kept ? p[i] : 0.f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) dp[i] *= p[i];
-      if constexpr (p_scale<T>() != 1.f)
+      if constexpr (RANGED<T>)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) p[i] *= p_scale<T>();
+        for (int i = 0; i < 16; ++i) dp[i] *= hold;
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         const V8 pf = acc_frag<T>(p, kk), sf = acc_frag<T>(dp, kk);
@@ -427,8 +522,8 @@ __device__ __forceinline__ void dkdv_block(const BwdArgs& a, Lds<T, DP>& lds, ui
     for (int q = 0; q < 4; ++q) {
       const int d = 32 * cc + 8 * q + 4 * g;
       if (d >= s.D) continue;
-      f32x4 x = f32x4{dk[cc][4 * q], dk[cc][4 * q + 1], dk[cc][4 * q + 2], dk[cc][4 * q + 3]} * a.scale;
-      f32x4 y = f32x4{dv[cc][4 * q], dv[cc][4 * q + 1], dv[cc][4 * q + 2], dv[cc][4 * q + 3]} * (1.f / p_scale<T>());
+      f32x4 x = f32x4{dk[cc][4 * q], dk[cc][4 * q + 1], dk[cc][4 * q + 2], dk[cc][4 * q + 3]} * (a.scale * undo);
+      f32x4 y = f32x4{dv[cc][4 * q], dv[cc][4 * q + 1], dv[cc][4 * q + 2], dv[cc][4 * q + 3]} * (RANGED<T> ? 0x1p-10f : 1.f);
       if (!kept) x = y = f32x4{0.f, 0.f, 0.f, 0.f};  // zeros so far, but where Q or dO hold infinities or NaN
       if (a.part_k) {
         *reinterpret_cast<f32x4*>(a.part_k + 2 * split * each + at + d) = x;
@@ -561,14 +656,15 @@ Plan plan(const gnn_cross_attn_bwd_args& g) {
 }
 
 template <typename T, int LOG>
-int delta(const BwdArgs& a, hipStream_t st) {
-  const int64_t blocks = (((int64_t)a.s.B * a.s.U * a.s.H << LOG) + NT - 1) / NT;
-  hipLaunchKernelGGL((cross_delta_kernel<T, LOG>), dim3((uint32_t)blocks), dim3(NT), 0, st, a);
+int delta(BwdArgs& a, hipStream_t st) {
+  a.delta_blocks = (uint32_t)((((int64_t)a.s.B * a.s.U * a.s.H << LOG) + NT - 1) / NT);
+  const uint32_t more = RANGED<T> ? (uint32_t)(a.s.B * a.s.Hk * a.v_parts) : 0;
+  hipLaunchKernelGGL((cross_delta_kernel<T, LOG>), dim3(a.delta_blocks + more), dim3(NT), 0, st, a);
   return (int)hipGetLastError();
 }
 
 template <typename T, int PREC, int DP, bool BIAS>
-int launch(const BwdArgs& a, hipStream_t st) {
+int launch(BwdArgs& a, hipStream_t st) {
   constexpr int LOG = DP <= 32 ? 2 : DP <= 64 ? 3 : 4;
   if (int rc = delta<T, LOG>(a, st)) return rc;
   const uint32_t rest = a.q_blocks + a.b_blocks;
@@ -598,7 +694,7 @@ int launch(const BwdArgs& a, hipStream_t st) {
 }
 
 template <typename T, int PREC>
-int run(const BwdArgs& a, hipStream_t st) {
+int run(BwdArgs& a, hipStream_t st) {
   auto go = [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
     return a.bias ? launch<T, PREC, DP, true>(a, st) : launch<T, PREC, DP, false>(a, st);
@@ -609,7 +705,21 @@ int run(const BwdArgs& a, hipStream_t st) {
   return go(std::integral_constant<int, 128>{});
 }
 
-// fp32 sums of the splits: dQ's, and behind them dK's and dV's
+// The workspace: Delta, and in fp16 the rows' lengths and the parts' longest values, in whole 16 bytes each; then the fp32
+// sums of the splits, dQ's, and behind them dK's and dV's
+struct Heads {
+  int64_t rows, tops, v_parts;
+  int64_t floats() const { return rows + (tops ? rows + tops : 0); }
+};
+Heads heads_of(const gnn_cross_attn_bwd_args& g) {
+  Heads h{};
+  h.rows = (g.B * g.U * g.H + 3) / 4 * 4;
+  if (g.dtype == GNN_F16) {
+    h.v_parts = std::min<int64_t>(MAX_PARTS, (g.V + KEYS_A_PART - 1) / KEYS_A_PART);
+    h.tops = (g.B * g.Hk * h.v_parts + 3) / 4 * 4;
+  }
+  return h;
+}
 void partial_sums(const gnn_cross_attn_bwd_args& g, const Plan& p, int64_t& q, int64_t& k) {
   q = p.q_splits > 1 ? p.q_splits * g.B * g.U * g.H * g.D : 0;
   k = p.k_splits > 1 && g.dk ? 2 * p.k_splits * g.B * g.V * g.Hk * g.D : 0;
@@ -620,7 +730,7 @@ void partial_sums(const gnn_cross_attn_bwd_args& g, const Plan& p, int64_t& q, i
 size_t cross_attn_bwd_workspace_bytes(const gnn_cross_attn_bwd_args& g) {
   int64_t q, k;
   partial_sums(g, plan(g), q, k);
-  return ((size_t)g.B * g.U * g.H + 3) / 4 * 16 + (size_t)(q + k) * sizeof(float);
+  return (size_t)(heads_of(g).floats() + q + k) * sizeof(float);
 }
 
 int cross_attn_bwd(const gnn_cross_attn_bwd_args& g, hipStream_t st) {
@@ -651,8 +761,10 @@ int cross_attn_bwd(const gnn_cross_attn_bwd_args& g, hipStream_t st) {
   a.q_splits = (int)p.q_splits, a.q_tiles = (int)p.q_tiles, a.k_splits = (int)p.k_splits, a.k_tiles = (int)p.k_tiles;
   int64_t nq, nk;
   partial_sums(g, p, nq, nk);
+  const Heads heads = heads_of(g);
   a.delta = (float*)g.workspace;
-  float* parts = a.delta + (g.B * g.U * g.H + 3) / 4 * 4;
+  if (heads.tops) a.length = a.delta + heads.rows, a.top = a.length + heads.rows, a.v_parts = (int)heads.v_parts;
+  float* parts = a.delta + heads.floats();
   if (nq) a.part_q = parts;
   if (nk) a.part_k = parts + nq;
   a.q_blocks = (uint32_t)p.q_blocks, a.k_blocks = (uint32_t)p.k_blocks, a.b_blocks = (uint32_t)b_blocks;

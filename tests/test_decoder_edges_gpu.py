@@ -1,11 +1,17 @@
-"""cross_attention where little is left of a row: one key under a bias, infinities and NaN."""
+"""cross_attention where little is left of a row: one key under a bias, infinities and NaN, gradients far from one.
+
+Bounds of gradients' digits, in the norm of a row's D elements. Storing one is off by half a step of it, or of fp16's
+smallest. The operands dS are off by half a step each, independently: by half / sqrt(3) sqrt(sum dS^2 k^2) in the
+mean over the row, of which sqrt(3) times is 6 deviations away for 32 elements on. Delta is off by what p's rounding leaves
+in o: one number a row, six deviations are 2 sqrt(3) half sqrt(sum_d dO^2 sum_j p^2 v^2). fp32 arithmetic is off by some U of
+the terms, below 2^-16 of them."""
 
 import pytest
 import torch
 
 from geometric_nn_ops_torch.triangle import cross_attention
-from op_helpers import DTYPES, IDS, U, assert_within
-from test_cross_attention_gpu import NAMES, _inputs
+from op_helpers import DTYPES, IDS, U, assert_within, half_step
+from test_cross_attention_gpu import NAMES, _exact, _inputs
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -126,3 +132,84 @@ def test_rows_without_keys_have_no_gradient(shape, what, dtype):
     for i in (0, 1, 4):
         assert torch.equal(got[i], plain[i]), NAMES[i]
     assert not got[1][:, 2:5, 1].any() and not got[4][:, 1, 2:5].any()
+
+
+# ---- gradients far from one
+def _digits(tensors, mask, dout, dtype):
+    """((value, bound of a row's error), ...) of dq and dk in float64."""
+    (B, Uq, H, D), Hk = tensors[0].shape, tensors[1].shape[2]
+    half, scale = half_step(dtype), D ** -0.5
+    q, k, v, do = (t.double().transpose(1, 2) for t in (*tensors[:3], dout))
+    k, v = (t.repeat_interleave(H // Hk, 1) for t in (k, v))
+    x = q @ k.transpose(2, 3).contiguous() * scale
+    if tensors[3] is not None:
+        x = x + tensors[3].double()
+    if mask is not None:
+        x = x.masked_fill(~mask[:, None, None], -INF)
+    P = torch.softmax(x, -1)
+    dP = do @ v.transpose(2, 3).contiguous()
+    dS = P * (dP - (P * dP).sum(-1, keepdim=True))
+    delta = 2 * 3 ** 0.5 * half * (do.square() * (P.square() @ v.square())).sum(-1, keepdim=True).sqrt()
+    dSt, Pt = (t.transpose(2, 3).contiguous() for t in (dS, P))
+
+    def own(t):  # summed over the heads that share a key head
+        return t.reshape(B, Hk, H // Hk, -1, D).sum(2)
+
+    def bound(value, spread, by_delta):
+        stored = half * value.norm(dim=-1) + (2.0 ** -25 * D ** 0.5 if dtype == torch.float16 else 0.0)
+        return stored + scale * ((half + 2.0 ** -16) * spread.sum(-1).sqrt() + by_delta)
+
+    dq, dk = scale * dS @ k, scale * own(dSt @ q)
+    return ((dq.transpose(1, 2), bound(dq, dS.square() @ k.square(), (delta * (P @ k)).norm(dim=-1)).transpose(1, 2)),
+            (dk.transpose(1, 2), bound(dk, own(dSt.square() @ q.square()),
+                                       own((Pt.square() @ (delta * q).square())).sum(-1).sqrt()).transpose(1, 2)))
+
+
+def _hold_digits(tensors, mask, dout, dtype):
+    got = _train(tensors, mask, dout)
+    for name, a, (want, bound) in zip(("dq", "dk"), got[1:3], _digits(tensors, mask, dout, dtype)):
+        off = (a.double() - want).norm(dim=-1)
+        assert (off <= bound).all(), (name, (off / bound).max().item())
+    return got
+
+
+LONG = [(1, 256, 16384, 2, 1, 64, 0, False), (1, 200, 8000, 2, 2, 128, 0, True), (2, 130, 6000, 2, 2, 64, 2, False),
+        (2, 130, 6000, 2, 1, 32, 1, False), (1, 64, 5000, 4, 2, 96, 0, True), (1, 150, 4000, 2, 2, 128, 2, False)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("size", [8, 10])
+@pytest.mark.parametrize("shape", LONG, ids=str)
+def test_long_rows_of_small_gradients_keep_their_digits(shape, size, dtype):
+    tensors, mask, dout = _inputs(shape, dtype, seed=44)
+    dout = dout * 2.0 ** -size
+    got = _hold_digits(tensors, mask, dout, dtype)
+    if shape[6]:
+        assert_within("dbias", got[4], *_exact(tensors, mask, dout)[4])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_each_row_keeps_its_digits(dtype):
+    """Output gradients of sizes from row to row apart, an all-masked sequence and a row of zeros among them."""
+    tensors, mask, dout = _inputs((3, 140, 3000, 4, 2, 64, 0, True), dtype, seed=45)
+    dout *= (2.0 ** -(torch.arange(140, device=DEV) % 11 - 2.0)).to(dtype)[None, :, None, None]
+    dout[0, 17] = 0.0
+    mask[1] = mask[0]
+    _hold_digits(tensors, mask, dout, dtype)
+    mask[1] = False
+    got = _train(tensors, mask, dout)
+    assert all(torch.isfinite(t).all() for t in got) and not got[1][0, 17].any()
+    assert not any(t[1].any() for t in got)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_large_gradients_stay_finite(d, dtype):
+    """dS beyond fp16's 65504, with queries and keys so small that dq and dk are not."""
+    tensors, mask, dout = _inputs((2, 200, 70, 4, 2, d, 0, True), dtype, seed=46)
+    tensors[0] *= 2.0 ** -6
+    tensors[1] *= 2.0 ** -8
+    tensors[2] *= 2.0 ** 7
+    dout = dout * 2.0 ** 10
+    got = _hold_digits(tensors, mask, dout, dtype)
+    assert all(torch.isfinite(t).all() for t in got)
