@@ -8,8 +8,9 @@
 // whole pairs, so that the rotation needs no exchange, and behind the turned part the two halves of 2 E plain ones
 // (angle 0). A team takes some heads of one token: a lane's E angles are the same for all of them and are made
 // once. The product pos f is formed in 64 bits and reduced to a fraction of a turn there: at position 10^6 fp32
-// would be 0.06 off. The hardware's sine and cosine take turns and are off by 2^-23 at most over half a turn to both
-// sides (measured at 2^20 places), with less than a tenth of the library's instructions.
+// would be 0.06 off. For 16-bit rows the hardware's sine and cosine take the turns, off by 2^-23 at most over half a turn
+// to both sides (measured at 2^20 places), a two-thousandth of fp16's rounding; fp32 rows, whose rounding that is twice of,
+// have polynomials of their own.
 // Workgroups are the queries' or the keys'; in the backward they stay and walk over their tokens, and each leaves
 // one fp32 row of its weight's gradient, added in order afterwards.
 #include <algorithm>
@@ -99,8 +100,28 @@ struct Pairs {
   }
 };
 
+// Of a turn in -1/2 .. 1/2, which is (k + 4 f) quarters with |f| <= 1/8. fp32: sin(2 pi f) = f (2 pi + P(f^2)), cos(2 pi f)
+// = 1 + f^2 Q(f^2) with polynomials fitted in 64 bits (even relative errors of 2^-28 and 2^-33), swapped and signed by
+// k: off by 1.5 units of 2^-24 of themselves at most (3 10^6 places in fp32 arithmetic against 80 bits).
+template <typename T>
+__device__ __forceinline__ void sine_cosine(float turn, float& sn, float& cs) {
+  if constexpr (sizeof(T) == 2) {
+    sn = __builtin_amdgcn_sinf(turn), cs = __builtin_amdgcn_cosf(turn);
+  } else {
+    const float k = rintf(4.f * turn), f = __builtin_fmaf(-0.25f, k, turn), x = f * f;
+    const float p = __builtin_fmaf(x, __builtin_fmaf(x, __builtin_fmaf(x, -75.39356f, 81.592354f), -41.341663f), -1.9519194e-07f);
+    const float q = __builtin_fmaf(x, __builtin_fmaf(x, __builtin_fmaf(x, 59.229218f, -85.44324f), 64.93932f), -19.739208f);
+    const float s = __builtin_fmaf(f, 6.2831855f, f * p), c = __builtin_fmaf(x, q, 1.f);
+    const uint32_t quarter = (uint32_t)(int)k;
+    const bool odd = quarter & 1;
+    sn = __uint_as_float(__float_as_uint(odd ? c : s) ^ (quarter & 2) << 30);
+    cs = __uint_as_float(__float_as_uint(odd ? s : c) ^ (quarter + 1 & 2) << 30);
+  }
+}
+
+// The backward: three waves a SIMD. Of 169 registers, one more than these have, it took up to a fifth longer in fp32.
 template <typename T, int E, bool NEIGHBOURS, bool BWD>
-__global__ __launch_bounds__(QR_NT) void qk_norm_rotary_kernel(const RotaryArgs a) {
+__global__ __launch_bounds__(QR_NT, BWD ? 3 : 1) void qk_norm_rotary_kernel(const RotaryArgs a) {
   typedef Vec<T, E> O;
   typedef typename O::V V;
   typedef typename O::F F;
@@ -144,7 +165,9 @@ __global__ __launch_bounds__(QR_NT) void qk_norm_rotary_kernel(const RotaryArgs 
       for (int e = 0; e < E; ++e) {
         const double t = p * a.turns[E * at + e];
         const float turn = (float)(t - rint(t));
-        sinv[e] = __builtin_amdgcn_sinf(turn), cosv[e] = __builtin_amdgcn_cosf(turn);
+        float sn, cs;
+        sine_cosine<T>(turn, sn, cs);
+        sinv[e] = sn, cosv[e] = cs;
       }
     }
     const T* x = (const T*)s.x + b * s.xs[0] + n * s.xs[1];
