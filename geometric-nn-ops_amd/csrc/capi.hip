@@ -769,8 +769,8 @@ extern "C++" {
 // Whether the kernels' 32-bit offsets reach 64 rows of a product, tokens of `group` heads each
 static bool within_reach(const int64_t* stride, int64_t tokens, int64_t group, size_t element) {
   const int64_t most = ((int64_t)1 << 31) / (int64_t)element, token = tokens > 1 ? stride[1] : 0;
-  const int64_t head = group > 1 ? stride[2] : 0;
-  return token >= 0 && token < most / 64 && head >= 0 && head < most / group && 64 * token + (group - 1) * head < most;
+  if (token < 0 || token >= most / 64) return false;
+  return group == 1 || (stride[2] >= 0 && stride[2] <= (most - 1 - 64 * token) / (group - 1));
 }
 // Shapes and types that the attention's two directions share
 template <typename Args>

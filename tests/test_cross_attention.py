@@ -217,6 +217,24 @@ def test_argument_errors(cls, name):
     refused(b"workspace", _lib.GNN_ERR_WORKSPACE)
 
 
+def test_heads_far_apart_are_taken_or_copied():
+    """What the host side leaves in place the library takes: both count 64 tokens and the heads of one of them."""
+    lib = _lib.load()
+    most = (1 << 31) // 2  # elements of 2 bytes
+    for group in (2, 3, 8):
+        for head in (most // group - 64, most // group + 64, (most - 64 * 64) // (group - 1) - 64, (most - 64 * 64) // (group - 1) + 64):
+            q = torch.empty_strided((1, 3, group, 64), (1 << 40, 64, head, 1), dtype=torch.bfloat16, device="meta")
+            in_place = _hip._heads(q, group).stride() == q.stride()
+            a = _lib.CrossAttnBwdArgs()
+            a.dtype, a.D, a.B, a.U, a.V, a.H, a.Hk, a.scale = _lib.GNN_BF16, 64, 1, 3, 5, group, 1, 1.0
+            a.q = a.k = a.v = 4096
+            a.q_stride = _lib.I64x3(*q.stride()[:3])
+            taken = lib.gnn_cross_attn_bwd_workspace_bytes(ctypes.byref(a)) > 0
+            assert taken == in_place, (group, head)
+    a.q_stride[2] = (1 << 63) - 1  # no overflow on the way
+    assert lib.gnn_cross_attn_bwd_workspace_bytes(ctypes.byref(a)) == 0
+
+
 def test_args_match_the_c_layout(tmp_path):
     root = pathlib.Path(__file__).resolve().parent.parent
     structs = {"gnn_cross_attn_args": _lib.CrossAttnArgs, "gnn_cross_attn_bwd_args": _lib.CrossAttnBwdArgs}

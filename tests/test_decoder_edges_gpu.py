@@ -213,3 +213,17 @@ def test_large_gradients_stay_finite(d, dtype):
     dout = dout * 2.0 ** 10
     got = _hold_digits(tensors, mask, dout, dtype)
     assert all(torch.isfinite(t).all() for t in got)
+
+
+def test_heads_far_apart():
+    """Two query heads a key head, more than 1 GiB between them: read in place."""
+    tensors, mask, dout = _inputs((1, 130, 200, 2, 1, 64, 0, True), torch.bfloat16, seed=47)
+    want = _train(tensors, mask, dout)
+    apart = (1 << 29) + 4096  # elements
+    q = torch.empty(apart + 130 * 64, device=DEV, dtype=torch.bfloat16).as_strided((1, 130, 2, 64), (apart, 64, apart, 1))
+    q.copy_(tensors[0])
+    q.requires_grad_()
+    o = cross_attention(q, *tensors[1:3], None, mask)
+    assert torch.equal(o, want[0])
+    (dq,) = torch.autograd.grad(o, q, dout)
+    assert torch.equal(dq, want[1])
