@@ -786,6 +786,9 @@ static int check_cross_attn(const Args* args) {
   if (a.B < 1 || a.U < 1 || a.V < 1 || a.H < 1 || a.Hk < 1 || a.B > most || a.U > most || a.V > most || a.H > most ||
       a.H % a.Hk || a.U * (a.H / a.Hk) > most)
     return set_error(GNN_ERR_ARG, "cross_attention: B, U, V, H and Hk must be positive, U H / Hk and V at most 2^30, H a multiple of Hk");
+  const int64_t grid = (int64_t)1 << 31;
+  if ((__int128)a.B * a.U * a.H >= grid || (__int128)a.B * a.Hk * ((a.V + 127) / 128) >= grid)
+    return set_error(GNN_ERR_UNSUPPORTED, "cross_attention: grid too large");
   if (!(a.scale > 0.f) || a.scale > 3e38f) return set_error(GNN_ERR_ARG, "cross_attention: scale must be positive");
   if (!a.q || !a.k || !a.v) return set_error(GNN_ERR_ARG, "cross_attention: q, k and v are required");
   const size_t e = a.dtype == GNN_F32 ? 4 : 2;

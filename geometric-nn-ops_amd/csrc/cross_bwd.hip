@@ -740,7 +740,7 @@ int cross_attn_bwd(const gnn_cross_attn_bwd_args& g, hipStream_t st) {
   const bool shared_bias = g.bias && g.shared_bias && g.B > 1;
   const int64_t rows = g.U * (g.H / g.Hk);
   const int64_t b_blocks = shared_bias && g.dbias && !one_key ? (rows + 127) / 128 * ((g.V + KT - 1) / KT) * g.Hk : 0;
-  if (p.q_blocks + p.k_blocks + b_blocks >= ((int64_t)1 << 31) || g.B * g.U * g.H >= ((int64_t)1 << 31))
+  if (p.q_blocks + p.k_blocks + b_blocks >= ((int64_t)1 << 31))
     return set_error(GNN_ERR_UNSUPPORTED, "cross_attention: grid too large");
   if (!g.workspace || g.workspace_bytes < cross_attn_bwd_workspace_bytes(g))
     return set_error(GNN_ERR_WORKSPACE, "cross_attention: workspace missing or too small");

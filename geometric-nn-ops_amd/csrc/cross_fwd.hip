@@ -490,7 +490,7 @@ size_t cross_attn_workspace_bytes(const gnn_cross_attn_args& g) {
 
 int cross_attn_fwd(const gnn_cross_attn_args& g, hipStream_t st) {
   const Plan p = plan(g);
-  if (p.blocks >= ((int64_t)1 << 31) || g.B * g.U * g.H >= ((int64_t)1 << 31))
+  if (p.blocks >= ((int64_t)1 << 31))
     return set_error(GNN_ERR_UNSUPPORTED, "cross_attention: grid too large");
   FwdArgs a{};
   a.s = {(int)g.B, (int)g.U, (int)g.V, (int)g.H, (int)g.Hk, (int)(g.H / g.Hk), (int)g.D, (int)(g.U * (g.H / g.Hk))};

@@ -2,8 +2,10 @@
 argument errors."""
 
 import ctypes
+import os
 import pathlib
 import subprocess
+import sys
 
 import pytest
 import torch
@@ -233,6 +235,31 @@ def test_heads_far_apart_are_taken_or_copied():
             assert taken == in_place, (group, head)
     a.q_stride[2] = (1 << 63) - 1  # no overflow on the way
     assert lib.gnn_cross_attn_bwd_workspace_bytes(ctypes.byref(a)) == 0
+
+
+HUGE = '''
+import ctypes, sys
+from geometric_nn_ops_torch import _lib
+lib = _lib.load()
+for b, u, v, h, hk in ((1 << 30, (1 << 30) - 1, 2, 1 << 30, 1 << 30), (1 << 29, 1 << 20, 127, 1 << 30, 1 << 30),
+                       (1 << 24, 1 << 20, 1, 1 << 29, 1 << 24), (1 << 16, 1, 1 << 30, 1 << 14, 1 << 14)):
+    for cls, name in ((_lib.CrossAttnArgs, "gnn_cross_attn"), (_lib.CrossAttnBwdArgs, "gnn_cross_attn_bwd")):
+        a = cls()
+        a.dtype, a.D, a.B, a.U, a.V, a.H, a.Hk, a.scale = _lib.GNN_BF16, 64, b, u, v, h, hk, 1.0
+        a.q = a.k = a.v = a.o = 4096
+        if "bwd" in name:
+            a.dout = a.dq = a.dk = a.dv = a.stats = 4096
+        assert getattr(lib, name + "_workspace_bytes")(ctypes.byref(a)) == 0
+        fn = getattr(lib, name if "bwd" in name else name + "_fwd")
+        assert fn(ctypes.byref(a), None) == _lib.GNN_ERR_UNSUPPORTED and b"grid" in lib.gnn_last_error()
+'''
+
+
+def test_sizes_beyond_any_grid_are_refused():
+    """Their products pass 64 bits; in a process of its own, which a division by zero would end."""
+    root = pathlib.Path(__file__).resolve().parent.parent / "geometric-nn-ops_amd"
+    run = subprocess.run([sys.executable, "-c", HUGE], env={**os.environ, "PYTHONPATH": str(root)}, capture_output=True, text=True)
+    assert run.returncode == 0, (run.returncode, run.stderr[-500:])
 
 
 def test_args_match_the_c_layout(tmp_path):
