@@ -702,6 +702,13 @@ int gnn_gated_linear_wgrad(const gnn_gated_linear_wgrad_args* args, void* stream
   return hip_status((hipError_t)rc, "gated_linear gradients");
 }
 
+// Whether a side's heads can be counted and numbered
+static bool qk_rotary_rows_fit(const gnn_qk_rotary_args& a, int side) {
+  const int64_t most = (int64_t)1 << 34;
+  const __int128 tokens = (__int128)a.B * a.N[side];
+  return tokens < most && tokens * a.H[side] < most;
+}
+
 static int check_qk_rotary(const gnn_qk_rotary_args* args, bool bwd) {
   if (!args) return set_error(GNN_ERR_ARG, "qk_norm_rotary: args is NULL");
   const gnn_qk_rotary_args& a = *args;
@@ -724,6 +731,7 @@ static int check_qk_rotary(const gnn_qk_rotary_args* args, bool bwd) {
         !aligned(a.dweight[k], we) || !aligned(a.pos[k], a.pos_bytes))
       return set_error(GNN_ERR_ARG, "qk_norm_rotary: tensors must be aligned to their elements");
     if (!a.B || !a.N[k] || !a.H[k]) continue;
+    if (!qk_rotary_rows_fit(a, k)) return set_error(GNN_ERR_UNSUPPORTED, "qk_norm_rotary: B N H must be below 2^34");
     if (!a.x[k] || (bwd ? !a.dy[k] : !a.out[k]))
       return set_error(GNN_ERR_ARG, "qk_norm_rotary: x and out, or in the backward x and dy, are required");
     if (bwd && (a.parts[k] < 1 || a.parts[k] >= ((int64_t)1 << 30)))
@@ -742,7 +750,7 @@ int gnn_qk_rotary_fwd(const gnn_qk_rotary_args* args, void* stream) {
 
 int64_t gnn_qk_rotary_parts(const gnn_qk_rotary_args* args, int32_t side) {
   if (!args || side < 0 || side > 1 || args->D < 8 || args->D > 256 || args->B < 0 || args->N[side] < 0 ||
-      args->H[side] < 1)
+      args->H[side] < 1 || args->H[side] > (1 << 20) || !qk_rotary_rows_fit(*args, side))
     return 0;
   return qk_rotary_parts(*args, side);
 }

@@ -799,7 +799,8 @@ int gnn_gated_linear_wgrad(const gnn_gated_linear_wgrad_args* args, void* stream
  * strides of batch, token and head, unit stride over D, any alignment of their elements; out dense. A side without
  * tokens or heads is left out. weight: [D] in param_dtype (the rows' dtype or GNN_F32), or NULL; pos: int32 or int64
  * (pos_bytes), [N] pos_stride apart a batch, or NULL (no rotation of that side); frequencies: R / 2 doubles on the
- * host, read during the call. D: a multiple of 8 up to 256, R: a multiple of 8 up to D (0: none). norm 0: no norms.
+ * host, read during the call. D: a multiple of 8 up to 256, R: a multiple of 8 up to D (0: none); at most 2^20 heads,
+ * B N H below 2^34. norm 0: no norms.
  * Backward: out is dx (or NULL), and for each side with dweight the weight's gradient ([D] in param_dtype) is summed
  * over parts[side] workgroups (as gnn_qk_rotary_parts returns it; any from 1 on is right) through partial, fp32 rows
  * of D, parts[0] (where dweight[0]) and then parts[1]. The reference has no such op. */

@@ -3,8 +3,10 @@ argument errors."""
 
 import ctypes
 import math
+import os
 import pathlib
 import subprocess
+import sys
 
 import pytest
 import torch
@@ -158,6 +160,31 @@ def test_argument_errors():
     assert lib.gnn_qk_rotary_parts(ctypes.byref(a), 0) == 1 and lib.gnn_qk_rotary_parts(ctypes.byref(a), 2) == 0
     a.N[0] = 0  # nothing to do
     assert lib.gnn_qk_rotary_fwd(ctypes.byref(a), None) == 0
+
+
+HUGE = """
+import ctypes
+from geometric_nn_ops_torch import _lib
+lib = _lib.load()
+for b, n, h in ((1, 3, 1 << 32), (8, 3, 1 << 40), (1 << 30, 1 << 16, 1 << 20), (1 << 62, 1 << 62, 1 << 20), (1, 1 << 34, 1)):
+    a = _lib.QkRotaryArgs()
+    a.D = a.R = 8
+    a.B, a.N[0], a.H[0] = b, n, h
+    assert lib.gnn_qk_rotary_parts(ctypes.byref(a), 0) == 0
+    a.dtype = a.param_dtype = _lib.GNN_BF16
+    a.pos_bytes, a.x[0], a.dy[0], a.out[0], a.parts[0] = 8, 4096, 4096, 4096, 1
+    for fn in (lib.gnn_qk_rotary_fwd, lib.gnn_qk_rotary_bwd):
+        assert fn(ctypes.byref(a), None) < 0, (b, n, h)
+a.B, a.N[0], a.H[0] = 1, 1 << 14, (1 << 20) - 1
+assert lib.gnn_qk_rotary_parts(ctypes.byref(a), 0) > 0
+"""
+
+
+def test_sizes_beyond_any_grid_are_refused():
+    """Heads past 2^31, and products past 64 bits; in a process of its own, which a division by zero would end."""
+    root = pathlib.Path(__file__).resolve().parent.parent / "geometric-nn-ops_amd"
+    run = subprocess.run([sys.executable, "-c", HUGE], env={**os.environ, "PYTHONPATH": str(root)}, capture_output=True, text=True)
+    assert run.returncode == 0, (run.returncode, run.stderr[-500:])
 
 
 def test_args_match_the_c_layout(tmp_path):
