@@ -627,8 +627,8 @@ int gnn_gated_linear(const gnn_gated_linear_args* args, void* stream) {
   if (a.activation < GNN_ACT_NONE || a.activation > GNN_ACT_SIGMOID)
     return set_error(GNN_ERR_ARG, "gated_linear: unknown activation");
   const int64_t most = (int64_t)1 << 29;
-  if (a.M < 1 || a.I < 1 || a.O < 1 || a.I > most || a.O > most || a.out_cols != (a.O + 7) / 8 * 8)
-    return set_error(GNN_ERR_ARG, "gated_linear: M, I and O must be positive, I and O at most 2^29, out_cols O rounded up to 8");
+  if (a.M < 1 || a.M > (int64_t)1 << 40 || a.I < 1 || a.O < 1 || a.I > most || a.O > most || a.out_cols != (a.O + 7) / 8 * 8)
+    return set_error(GNN_ERR_ARG, "gated_linear: M, I and O must be positive, M at most 2^40, I and O 2^29, out_cols O rounded up to 8");
   const int64_t e = a.dtype == GNN_F32 ? 4 : 2;
   if (!aligned(a.x, 16) || !aligned(a.wg, 16) || !aligned(a.wu, 16) || (a.I * e) % 16 || (a.x_ld * e) % 16 ||
       (a.wg_ld * e) % 16 || (a.wu_ld * e) % 16)

@@ -740,7 +740,7 @@ int gnn_column_sums(const gnn_column_sums_args* args, void* stream);
  * side: out[m][n] = dy zu act'(zg) and out[m][out_cols + n] = dy act(zg), zeros for n from O to out_cols. x: rows of I
  * elements, x_ld apart; wg, wu: [O] rows of I; all 16-byte aligned with I and the pitches multiples of 16 bytes (pad
  * with zeros). bg, bu: [O] or NULL. dy: rows of O, any alignment of their elements; out: rows of O (any alignment),
- * with dy of 2 out_cols, out_cols = O rounded up to 8. All in dtype; products and epilogue in fp32, one rounding.
+ * with dy of 2 out_cols, out_cols = O rounded up to 8. M is at most 2^40. All in dtype; products and epilogue in fp32, one rounding.
  * precision: fp32 products (GNN_PREC_IEEE or GNN_PREC_BF16X3). The reference has no such op. */
 typedef struct gnn_gated_linear_args {
   const void* x;

@@ -135,6 +135,19 @@ def test_argument_errors():
     refused(b"aligned", lib.gnn_gated_turn, t)
 
 
+def test_rows_beyond_any_grid_are_refused():
+    """Rounding them up to tiles passes 64 bits: no launch of what is left of the product."""
+    lib = _lib.load()
+    a = _lib.GatedLinearArgs()
+    a.x = a.wg = a.wu = a.out = 4096
+    a.dtype, a.I, a.O, a.out_cols, a.x_ld, a.wg_ld, a.wu_ld, a.out_ld = _lib.GNN_BF16, 16, 8, 8, 16, 16, 16, 8
+    for rows in ((1 << 40) + 1, (1 << 63) - 1):
+        a.M = rows
+        assert lib.gnn_gated_linear(ctypes.byref(a), None) == _lib.GNN_ERR_ARG and b"2^40" in lib.gnn_last_error()
+    a.O, a.out_cols, a.out_ld, a.M = 1 << 29, 1 << 29, 1 << 29, 1 << 40
+    assert lib.gnn_gated_linear(ctypes.byref(a), None) == _lib.GNN_ERR_UNSUPPORTED
+
+
 def test_parameter_gradients_refuse_what_they_cannot_write():
     lib = _lib.load()
     a = _lib.GatedLinearWgradArgs()
