@@ -8,7 +8,7 @@ def cross_attention_torch(q, k, v, bias, mask, scale):
     wide = torch.promote_types(q.dtype, torch.float32)
     if not V:
         empty = [t.sum() for t in (k, v, bias) if t is not None]  # zeros, which keep these in the graph
-        return q.masked_fill(torch.ones((), dtype=torch.bool, device=q.device), 0.0) + sum(empty)
+        return (q.masked_fill(torch.ones((), dtype=torch.bool, device=q.device), 0.0) + sum(empty)).contiguous()
     # rows: the queries of all heads that share a key head
     rows = q.to(wide).reshape(B, U, Hk, H // Hk, D).permute(0, 2, 3, 1, 4).reshape(B, Hk, H // Hk * U, D)
     k, v = (t.to(wide).transpose(1, 2) for t in (k, v))
@@ -22,4 +22,4 @@ def cross_attention_torch(q, k, v, bias, mask, scale):
     dead = s.detach().amax(-1, keepdim=True) == float("-inf")  # nothing is kept
     p = torch.softmax(s.masked_fill(dead, 0.0), -1).masked_fill(dead, 0.0)
     o = (p.view(B, Hk, H // Hk * U, V) @ v).view(B, Hk, H // Hk, U, D)
-    return o.permute(0, 3, 1, 2, 4).reshape(B, U, H, D).to(q.dtype)
+    return o.permute(0, 3, 1, 2, 4).reshape(B, U, H, D).to(q.dtype).contiguous()

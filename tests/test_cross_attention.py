@@ -97,6 +97,15 @@ def test_no_keys_whatever_the_queries_hold():
         assert t.shape == x.shape and not t.any()
 
 
+@pytest.mark.parametrize("heads", [1, 2])
+@pytest.mark.parametrize("keys", [0, 1, 5])
+def test_the_result_is_contiguous(keys, heads):
+    """Whatever the layout of the queries, as the kernels' is."""
+    q, k = torch.randn(2, 4, 3, 8).transpose(1, 2), torch.randn(2, heads, keys, 8).transpose(1, 2)
+    for t in (q, q[:, :1], q.double()):
+        assert cross_attention(t, k.to(t.dtype), k.to(t.dtype)).is_contiguous()
+
+
 def test_refusals():
     q, k, bias = torch.zeros(2, 3, 4, 8), torch.zeros(2, 5, 2, 8), torch.zeros(2, 4, 3, 5)
     with pytest.raises(ValueError, match=r"\[batch, queries, heads, head_dim\]"):
