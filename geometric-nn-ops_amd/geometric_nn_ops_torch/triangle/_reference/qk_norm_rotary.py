@@ -24,7 +24,8 @@ def _one(x, pos, weight, eps, frequencies, interleaved):
     if pos is not None:
         r = 2 * len(frequencies)
         y = torch.cat([_turned(y[..., :r], pos, frequencies, interleaved), y[..., r:]], -1)
-    return y.to(x.dtype)
+    y = y.to(x.dtype).contiguous()
+    return y.clone() if y is x else y
 
 
 def qk_norm_rotary_torch(q, k, q_pos, k_pos, q_weight, k_weight, eps, frequencies, interleaved):

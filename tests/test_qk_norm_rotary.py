@@ -69,6 +69,18 @@ def test_torch_path_gradients(interleaved):
                                           rotary_dim=4, interleaved=interleaved), args)
 
 
+@pytest.mark.parametrize("eps", [None, 1e-6])
+@pytest.mark.parametrize("pos", [None, torch.arange(3)])
+def test_the_results_are_fresh_and_contiguous(pos, eps):
+    """Also where nothing is normed or turned, and whatever the layout of the rows."""
+    for x in (torch.randn(2, 3, 4, 8), torch.randn(2, 4, 3, 8).transpose(1, 2), torch.randn(2, 3, 4, 8).bfloat16()):
+        before = x.clone()
+        for y in qk_norm_rotary(x, x, pos, eps=eps):
+            assert y.is_contiguous()
+            y.zero_()
+        assert torch.equal(x, before)
+
+
 def test_refusals():
     q, k, pos = torch.zeros(2, 3, 4, 8), torch.zeros(2, 5, 2, 8), torch.arange(3)
     with pytest.raises(ValueError, match=r"\[batch, tokens, heads, head_dim\]"):
