@@ -89,8 +89,9 @@ def cross_attention(
         scale: of the logits, positive; ``None`` -> ``D ** -0.5``.
 
     All floating tensors in one dtype. Logits, softmax and sums run in fp32 and results round once; probabilities and
-    the logits' gradients are rounded to the inputs' dtype as operands of the products behind them. fp32 products
-    follow ``torch.backends.cuda.matmul.fp32_precision``.
+    the logits' gradients are rounded to the inputs' dtype as operands of the products behind them (the output's
+    probabilities in two parts, which lose nothing, of up to 64 keys or up to 32 queries and heads a key head). fp32
+    products follow ``torch.backends.cuda.matmul.fp32_precision``.
 
     Returns:
         A fresh contiguous ``[B, U, H, D]`` tensor of q's dtype: zeros, with zero gradients, for queries to which the
