@@ -13,8 +13,8 @@
 //               turned for dV^T += dO^T P and dK^T += Q^T dS.
 //   dbias_block a bias for all sequences: a tile of 128 rows x 64 keys of one head group walks over the batch.
 // Delta comes from a kernel of its own, so that the three are workgroups of one launch (dk and dv, the longest, first)
-// whose ends fill each other's: 16 heads, 4 x 2048 x 1400, 64 columns. With more columns dk and dv take all of a CU's
-// registers and go alone. Where one of the first two leaves CUs idle its loop is split over workgroups, whose fp32 sums
+// whose ends fill each other's: 16 heads, 4 x 2048 x 1400, 64 columns. In 16 bits and more columns dk and dv take all of a
+// CU's registers and go alone, dQ after them. Where one of the first two leaves CUs idle its loop is split over workgroups, whose fp32 sums
 // are added in order.
 // P and dS are rounded to the operands' type for the products behind them (dS in two parts for dQ of few keys and short
 // heads), and Delta takes what the rounding of O left with it.
@@ -26,7 +26,7 @@
 // The lengths |dO_r| come with Delta, the longest v_j from further workgroups of that kernel. (16384 keys, dO of 2^-8:
 // dQ was off by 5.4e-3 unscaled; a factor of one size for all would overflow beside large gradients.)
 //
-// 4 x 2048 x 1400, 16 heads of 64, bf16: 191 us for five products of 19 GFLOP (77 at a large product's rate), of which S
+// 4 x 2048 x 1400, 16 heads of 64, bf16: 191 to 205 us (box by box) for five products of 19 GFLOP (77 at a large product's rate), of which S
 // and dP are formed twice. The matrix units are busy 31% of the time, the vector units 41%, LDS 42%: 212 registers leave
 // two waves a SIMD, too few to keep all three busy at once.
 #include <algorithm>
@@ -237,7 +237,8 @@ struct Lds {
 };
 
 // -------------------------------------------------------------------------------------- dQ
-// FINER: dS in two parts
+// FINER: dS in two parts. 16 bits, 128 columns: the 256 registers of two waves a SIMD do not hold it all, 9 are kept in
+// scratch, with a bias 45 (fp16: 10 and 55).
 template <typename T, int PREC, int DP, bool BIAS, bool FINER>
 __device__ __forceinline__ void dq_block(const BwdArgs& a, Lds<T, DP>& lds, uint32_t block) {
   typedef RowTile<T, DP> Tile;
@@ -633,6 +634,8 @@ struct Plan {
 // and of dK, dV are split so that none has more than about an equal part of all tiles (the queries of a few tokens walk
 // over all keys, while each of many workgroups of dK and dV has one tile: 2 x 9 x 4391, 20 heads of 128 over 10, fp32:
 // 178 us, 985 with dQ in one walk): a tile of dK and dV costs four products, one of dQ three.
+// (The two launches of 16 bits above 64 columns each have the card to themselves and get a part of it: 1 x 1024 x 2048, 8
+// heads of 128, bf16: 53 us on 128 workgroups of dK and dV, then 86 on 128 of dQ.)
 Plan plan(const gnn_cross_attn_bwd_args& g) {
   Plan p{};
   const int KT = tile_of(g.dtype == GNN_F32, (int)g.D);

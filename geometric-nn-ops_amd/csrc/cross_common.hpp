@@ -13,7 +13,7 @@ namespace cross {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-// Up to so many keys 16-bit operands made here, p and dS, are multiplied in two parts, 2^-17 exact: few terms cancel, and
+// Up to so many keys 16-bit operands made here, p and dQ's dS, are multiplied in two parts, 2^-17 exact: few terms cancel, and
 // their roundings do not: of 3 keys, where P (dP - Delta) is a small difference, gradients were off by 2.5 times the one
 // rounding at the end, of 64 and more by 1.4. One tile of keys costs nothing that shows.
 constexpr int FINE = 64;

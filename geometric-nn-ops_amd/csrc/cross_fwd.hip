@@ -20,8 +20,8 @@
 //   maxima, sums and outputs meet in LDS at the end.
 // Where these leave CUs idle the keys are split over workgroups, whose fp32 outputs a second kernel joins.
 //
-// 4096 x 8192, 32 heads of 128, bf16: 563 us of 550 GFLOP (441 at a large product's rate), the softmax's vector work beside
-// the products. One query of 8191 keys, 8 sequences, 32 heads of 128 over 8: 40 us, K and V at 5 TB/s, and 4 for the joining.
+// 4096 x 8192, 32 heads of 128, bf16: 574 us of 550 GFLOP (441 at a large product's rate), the softmax's vector work beside
+// the products. One query of 8191 keys, 8 sequences, 32 heads of 128 over 8: 41 us, K and V at 5 TB/s, and 4 for the joining.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
