@@ -14,8 +14,8 @@
 //   dbias_block a bias for all sequences: a tile of 128 rows x 64 keys of one head group walks over the batch.
 // Delta comes from a kernel of its own, so that the three are workgroups of one launch (dk and dv, the longest, first)
 // whose ends fill each other's: 16 heads, 4 x 2048 x 1400, 64 columns. In 16 bits and more columns dk and dv take all of a
-// CU's registers and go alone, dQ after them. Where one of the first two leaves CUs idle its loop is split over workgroups, whose fp32 sums
-// are added in order.
+// CU's registers and go alone, dQ after them. Where one of the first two leaves CUs idle its loop is split over workgroups,
+// whose fp32 sums are added in order.
 // P and dS are rounded to the operands' type for the products behind them (dS in two parts for dQ of few keys and short
 // heads), and Delta takes what the rounding of O left with it.
 //
@@ -23,11 +23,12 @@
 // dS falls sooner, with the output gradient, and as much above 1 it would leave the range upwards. |dS_rj| is at most
 // 2 |dO_r| max_j |v_j|, and dS is held at the power of two that brings this bound into 2^14 .. 2^15: each row's own for dQ,
 // where it goes into the exponent of P and out with the store, the largest of all rows for dK, whose sums go over rows.
-// The lengths |dO_r| come with Delta, the longest v_j from further workgroups of that kernel. (16384 keys, dO of 2^-8:
-// dQ was off by 5.4e-3 unscaled; a factor of one size for all would overflow beside large gradients.)
+// The lengths |dO_r| come with Delta, the longest v_j from further workgroups of that kernel. (16384 keys, dO of 2^-8: dQ is
+// off by 4.1e-4, 5.4e-3 unscaled, the storing alone by 3.5e-4; one factor for all calls would overflow beside large
+// gradients. 4 x 2048 x 1400, 16 heads of 64: 214 us, 205 unscaled.)
 //
-// 4 x 2048 x 1400, 16 heads of 64, bf16: 191 to 205 us (box by box) for five products of 19 GFLOP (77 at a large product's rate), of which S
-// and dP are formed twice. The matrix units are busy 31% of the time, the vector units 41%, LDS 42%: 212 registers leave
+// 4 x 2048 x 1400, 16 heads of 64, bf16: 191 to 205 us (card by card) for five products of 19 GFLOP (77 at a large product's rate), of
+// which S and dP are formed twice. The matrix units are busy 31% of the time, the vector units 41%, LDS 42%: 212 registers leave
 // two waves a SIMD, too few to keep all three busy at once.
 #include <algorithm>
 #include <type_traits>

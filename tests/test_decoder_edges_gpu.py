@@ -253,3 +253,43 @@ def test_single_queries_round_once(shape, dtype):
     if dtype == torch.float16:
         slack = slack + 2.0 ** -25 * v.abs().sum(2, keepdim=True) * (P.amax(-1, keepdim=True))
     assert_within("o", cross_attention(*tensors, mask), (P @ v).transpose(1, 2), slack.transpose(1, 2))
+
+
+@pytest.mark.parametrize("u,v,bias", [(1, 3000, 0), (90, 700, 1), (300, 65, 2)])
+def test_powers_of_two_follow_the_data_of_each_replay(u, v, bias):
+    """A captured fp16 training call with output gradients of other sizes in its buffer: every replay as the eager call."""
+    tensors, mask, dout = _inputs((2, u, v, 4, 2, 64, bias, True), torch.float16, seed=49)
+    first = dout.clone()
+
+    def block():
+        leaves = [t.detach().requires_grad_() for t in tensors if t is not None]
+        o = cross_attention(*leaves, *([] if len(leaves) == 4 else [None]), mask)
+        return (o.detach(), *torch.autograd.grad(o, leaves, dout))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        block()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = block()
+    for size in (1.0, 2.0 ** -10, 2.0 ** 9, 0.0):
+        dout.copy_(first * size)
+        want = [t.clone() for t in block()]
+        for t in captured:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for name, a, e in zip(NAMES, captured, want):
+            assert torch.equal(a, e), (name, size)
+        torch.cuda.synchronize()
+
+
+def test_only_what_is_needed_in_fp16():
+    tensors, mask, dout = _inputs((2, 50, 300, 4, 2, 128, 1, True), torch.float16, seed=50)
+    every = _train(tensors, mask, dout)
+    for i in range(4):
+        some = [t.clone().requires_grad_(j == i) for j, t in enumerate(tensors)]
+        (got,) = torch.autograd.grad(cross_attention(*some, mask), [some[i]], dout)
+        assert torch.equal(got, every[1 + i]), NAMES[1 + i]
