@@ -95,7 +95,8 @@ def cross_attention(
 
     Returns:
         A fresh contiguous ``[B, U, H, D]`` tensor of q's dtype: zeros, with zero gradients, for queries to which the
-        mask, or a bias of -inf, leaves no key. Differentiable in q, k, v and bias (a shared bias's gradient is summed over the batch, in fp32);
+        mask, or a bias of -inf, leaves no key (an output gradient of infinities or NaN there still reaches k and v
+        where a bias took the keys away). Differentiable in q, k, v and bias (a shared bias's gradient is summed over the batch, in fp32);
         repeated calls give the same bits.
     """
     _check(q, k, v, bias, mask, scale)
